@@ -14,6 +14,7 @@
 #include "analysis.h"
 #include "jit.h"
 #include "launch.h"
+#include "optim.h"
 #include "planner.h"
 #include "profile.h"
 #include "rt_internal.h"
@@ -941,6 +942,47 @@ int32_t arcqml_rt_v2_scaled_copy(const arcqml_c128 *input, size_t batch, size_t 
         scaled_copy_device(reinterpret_cast<const double2 *>(input), batch, uint32_t(num_qubits),
                            factors, reinterpret_cast<double2 *>(output), ctx,
                            pick_stream(ctx, stream));
+    });
+}
+
+// ---------------------------------------------------------------- training over many tensors
+
+size_t arcqml_rt_v2_gradient_workspace(size_t num_tensors) {
+    return tensor_workspace(num_tensors);
+}
+
+int32_t arcqml_rt_v2_gradient_norm(const ArcqmlTensor *gradients, size_t num_tensors,
+                                   double *norm, double *workspace, size_t workspace_len,
+                                   void *stream) {
+    return guarded([&] {
+        if (!norm) fail("norm pointer is null");
+        gradient_norm_device(gradients, num_tensors, norm, workspace, workspace_len,
+                             static_cast<cudaStream_t>(stream));
+    });
+}
+
+int32_t arcqml_rt_v2_clip_gradients(const ArcqmlTensor *gradients, size_t num_tensors,
+                                    double max_norm, const double *given_norm, double *norm,
+                                    double *workspace, size_t workspace_len, void *stream) {
+    return guarded([&] {
+        clip_gradients_device(gradients, num_tensors, max_norm, given_norm, norm, workspace,
+                              workspace_len, static_cast<cudaStream_t>(stream));
+    });
+}
+
+int32_t arcqml_rt_v2_adam_step(const ArcqmlTensor *parameters, const ArcqmlTensor *gradients,
+                               const ArcqmlTensor *first_moments,
+                               const ArcqmlTensor *second_moments, const ArcqmlTensor *copies,
+                               size_t num_tensors, int64_t *step,
+                               const ArcqmlAdamOptions *options, const double *given_norm,
+                               double *norm, double *workspace, size_t workspace_len,
+                               void *stream) {
+    return guarded([&] {
+        if (!step) fail("step counter is null");
+        if (!options) fail("Adam options are null");
+        adam_step_device(parameters, gradients, first_moments, second_moments, copies,
+                         num_tensors, step, *options, given_norm, norm, workspace, workspace_len,
+                         static_cast<cudaStream_t>(stream));
     });
 }
 

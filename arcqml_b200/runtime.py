@@ -131,6 +131,10 @@ SIGNATURES = {
     "arcqml_rt_v2_peer_buffer_close": (_I32, [_P]),
     "arcqml_rt_v2_peer_buffer_destroy": (_I32, [_P]),
     "arcqml_rt_v2_adjoint_backward": (_I32, [_P, _P, _P, _S, _S, _P, _P, _S, _P, _S, _P]),
+    "arcqml_rt_v2_gradient_workspace": (_S, [_S]),
+    "arcqml_rt_v2_gradient_norm": (_I32, [_P, _S, _P, _P, _S, _P]),
+    "arcqml_rt_v2_clip_gradients": (_I32, [_P, _S, _D, _P, _P, _P, _S, _P]),
+    "arcqml_rt_v2_adam_step": (_I32, [_P, _P, _P, _P, _P, _S, _P, _P, _P, _P, _P, _S, _P]),
     "arcqml_rt_v2_norms": (_I32, [_P, _S, _S, _P, _P]),
     "arcqml_rt_v2_norms_noalloc": (_I32, [_P, _S, _S, _P, _P]),
     "arcqml_rt_v2_set_basis_state": (_I32, [_P, _S, _S, C.c_uint64, _P]),
@@ -582,6 +586,263 @@ def small_adam_device(plan: CircuitPlan, observable: "Observable", num_qubits: i
     if state is not None:
         state.step += int(steps)
     return energies, params
+
+
+
+# ------------------------------------------------------------------ training over many tensors
+
+NO_TENSOR = 4
+_TENSOR = np.dtype([("data", np.uint64), ("length", np.uint64), ("dtype", np.uint32),
+                    ("reserved", np.uint32)])  # ArcqmlTensor
+
+
+class AdamOptions(C.Structure):
+    _fields_ = [("learning_rate", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double),
+                ("epsilon", C.c_double), ("weight_decay", C.c_double), ("max_norm", C.c_double),
+                ("decoupled", C.c_int32), ("reserved", C.c_int32)]
+
+
+def _dtype_code(dtype):
+    """(code of the components, components per element) of a torch dtype, or None."""
+    import torch
+    return {torch.float64: (0, 1), torch.float32: (1, 1), torch.bfloat16: (2, 1),
+            torch.float16: (3, 1), torch.complex128: (0, 2), torch.complex64: (1, 2)}.get(dtype)
+
+
+def _layout(t):
+    """None for a contiguous tensor, (shape, strides) for another one that fills its memory without
+    gaps or overlap; anything else is refused."""
+    if t.is_contiguous():
+        return None
+    size = 1
+    for stride, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != size:
+            raise TypeError("tensors must fill their memory without gaps or overlap: got shape "
+                            f"{list(t.shape)} with strides {list(t.stride())}")
+        size *= n
+    return tuple((n, st) for n, st in zip(t.shape, t.stride()) if n != 1)
+
+
+class TensorList:
+    """The tensors of a model, or their gradients, as the calls below take them: floating or complex
+    CUDA tensors of one device; None where a parameter has no gradient. Checking a list and writing
+    it down costs about a microsecond per tensor: a training loop whose tensors stay keeps its lists.
+    Every call reads the tensors' addresses anew, and one that has moved (a new ``.data``) is
+    checked and written down again; a list whose tensors change shape in place is made anew."""
+
+    def __init__(self, tensors):
+        self.tensors = list(tensors)
+        self._present = [t for t in self.tensors if t is not None]
+        self._write_down()
+
+    def __len__(self) -> int:
+        return len(self.tensors)
+
+    def _write_down(self) -> None:
+        import torch
+        table = np.zeros(max(1, len(self.tensors)), dtype=_TENSOR)
+        layouts, devices = [], set()
+        for i, t in enumerate(self.tensors):
+            if t is None:
+                table[i] = (0, 0, NO_TENSOR, 0)
+                layouts.append(None)
+                continue
+            kind = _dtype_code(t.dtype) if isinstance(t, torch.Tensor) else None
+            if kind is None or not t.is_cuda or t.layout != torch.strided or t.is_conj() or \
+                    t.is_neg():
+                raise TypeError("a tensor list takes dense float64, float32, bfloat16, float16 and "
+                                f"complex CUDA tensors or None: place {i} holds "
+                                + (f"{t.dtype} on {t.device}" if isinstance(t, torch.Tensor)
+                                   else type(t).__name__))
+            layouts.append(_layout(t))
+            devices.add(t.device.index)
+            table[i] = (t.data_ptr(), t.numel() * kind[1], kind[0], 0)
+        if len(devices) > 1:
+            raise TypeError("the tensors of a list must be on one device")
+        self.device_index = devices.pop() if devices else None
+        self._table, self._layouts = table, layouts
+        self._shapes = [None if t is None else t.shape for t in self.tensors]
+        self._pointers = [t.data_ptr() for t in self._present]
+        self._apart = None
+
+    def _current(self) -> int:
+        """Address of the table, after a look at the tensors' addresses and the current device."""
+        import torch
+        if list(map(torch.Tensor.data_ptr, self._present)) != self._pointers:
+            self._write_down()
+        if self.device_index is not None and self.device_index != torch.cuda.current_device():
+            raise RuntimeError(f"the tensors are on cuda:{self.device_index} and the current device "
+                               f"is cuda:{torch.cuda.current_device()}")
+        return self._table.ctypes.data
+
+    def _check_apart(self, name: str) -> None:
+        """Refuses a list that is written to when two of its tensors share memory."""
+        if self._apart is None:
+            self._apart = _tables_apart([self._table])
+        if not self._apart:
+            raise RuntimeError(f"{name} share memory: each may be in the list once")
+
+    def _written(self) -> None:
+        """Tells autograd that the tensors changed."""
+        import torch
+        torch.autograd.graph.increment_version(self._present)
+
+
+def _tables_apart(tables) -> bool:
+    t = np.concatenate(tables)
+    t = t[(t["dtype"] != NO_TENSOR) & (t["length"] > 0)]
+    t = t[np.argsort(t["data"], kind="stable")]
+    size = np.array([8, 4, 2, 2], dtype=np.uint64)[t["dtype"]]
+    return bool(np.all(t["data"][:-1] + t["length"][:-1] * size[:-1] <= t["data"][1:]))
+
+
+def _tensor_list(tensors) -> TensorList:
+    return tensors if isinstance(tensors, TensorList) else TensorList(tensors)
+
+
+class _TensorCall:
+    """Stream, scratch and norm of one call. All of it is allocated for the call alone, on its
+    stream, so calls on other streams and captured graphs share nothing."""
+
+    def __init__(self, count: int, stream, norm_wanted: bool = True):
+        import torch
+        words = load().arcqml_rt_v2_gradient_workspace(count)
+        if stream is None:
+            self.stream = torch.cuda.current_stream().cuda_stream
+            self._allocate(words, norm_wanted)
+        else:
+            self.stream = int(stream)
+            with torch.cuda.stream(torch.cuda.ExternalStream(self.stream)):
+                self._allocate(words, norm_wanted)
+
+    def _allocate(self, words: int, norm_wanted: bool) -> None:
+        import torch
+        self.words = words
+        self.workspace = torch.empty(words, dtype=torch.float64, device="cuda")
+        self.norm = torch.empty((), dtype=torch.float64, device="cuda") if norm_wanted else None
+
+    def arguments(self, given):
+        """(given norm, norm, workspace, its length, stream) as the entry points take them."""
+        return (None if given is None else _scalar_ptr(given),
+                None if self.norm is None else self.norm.data_ptr(), self.workspace.data_ptr(),
+                self.words, self.stream)
+
+
+def _scalar_ptr(t) -> int:
+    import torch
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == torch.float64
+            and t.numel() == 1 and t.get_device() == torch.cuda.current_device()):
+        raise TypeError("a given norm must be one float64 on the current CUDA device")
+    return t.data_ptr()
+
+
+def gradient_norm_device(gradients, stream=None):
+    """The 2-norm over every element of every tensor of `gradients` (a TensorList, or a sequence of
+    CUDA tensors and None) as a float64 CUDA scalar (arcqml_rt_v2_gradient_norm). Nothing is read
+    back: the norm can go into the calls below, or its square into an all-reduce."""
+    g = _tensor_list(gradients)
+    table = g._current()
+    call = _TensorCall(len(g), stream)
+    _status(load().arcqml_rt_v2_gradient_norm(table, len(g), *call.arguments(None)[1:]))
+    return call.norm
+
+
+def clip_gradients_device(gradients, max_norm: float, norm=None, stream=None):
+    """Scales `gradients` in place by min(1, max_norm / (n + 1e-6)) with n their global norm, or
+    `norm` (a float64 CUDA scalar: over several lists, or over ranks), and returns n
+    (arcqml_rt_v2_clip_gradients)."""
+    g = _tensor_list(gradients)
+    table = g._current()
+    g._check_apart("the gradients")
+    call = _TensorCall(len(g), stream)
+    _status(load().arcqml_rt_v2_clip_gradients(table, len(g), float(max_norm),
+                                               *call.arguments(norm)))
+    g._written()
+    return call.norm
+
+
+class DeviceAdamState:
+    """Moments and step count of Adam over device tensors (``adam_step_device``): ``m`` and ``v``
+    hold one tensor per parameter, of its shape and strides, in float32 (float64 or complex128 for
+    float64 and complex128 parameters, complex64 for complex64 ones); ``step`` is an int64 CUDA
+    scalar with the steps taken. They start at zero, or continue the ones given."""
+
+    def __init__(self, parameters, m=None, v=None, step=0):
+        import torch
+        p = _tensor_list(parameters)
+        if len(p._present) != len(p):
+            raise TypeError("a parameter list has no empty places")
+        self.m = self._zeros(p) if m is None else list(m)
+        self.v = self._zeros(p) if v is None else list(v)
+        device = torch.device("cuda", torch.cuda.current_device() if p.device_index is None
+                              else p.device_index)
+        if isinstance(step, torch.Tensor):
+            if step.dtype != torch.int64 or step.numel() != 1 or step.device != device:
+                raise TypeError(f"the step count must be one int64 on {device}")
+            self.step = step
+        else:
+            if int(step) < 0:
+                raise ValueError("the step count must not be negative")
+            self.step = torch.full((), int(step), dtype=torch.int64, device=device)
+        self._m, self._v = TensorList(self.m), TensorList(self.v)
+        for name, other in (("first", self._m), ("second", self._v)):
+            if other._shapes != p._shapes or other._layouts != p._layouts:
+                raise ValueError(f"the {name} moments must have the parameters' shapes and strides")
+
+    @staticmethod
+    def _zeros(p: TensorList):
+        import torch
+        wide = {torch.bfloat16: torch.float32, torch.float16: torch.float32}
+        return [torch.zeros_like(t, dtype=wide.get(t.dtype, t.dtype)) for t in p.tensors]
+
+
+def adam_step_device(parameters, gradients, state: DeviceAdamState, lr: float = 0.05,
+                     betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.0,
+                     decoupled: bool = False, max_norm: float = None, norm=None, copies=None,
+                     stream=None):
+    """One Adam step over `parameters` (arcqml_rt_v2_adam_step), in place, with the update of
+    ``AdamState.update``: coupled L2 weight decay, or with `decoupled` the decay applied to the
+    parameter itself. With `max_norm` the gradients enter the step scaled as
+    ``clip_gradients_device`` scales them (they stay as they are) and their global norm is returned;
+    `norm` gives that norm instead. A parameter whose gradient is None is left as it is. `copies`
+    (bfloat16 or float16 tensors, or None, one per parameter) receive the new values of float32
+    parameters. The step count is on the device: a captured step counts on when it is replayed
+    (`lr` and the other numbers stay those of the capture)."""
+    p, g = _tensor_list(parameters), _tensor_list(gradients)
+    c = None if copies is None else _tensor_list(copies)
+    if max_norm is None and norm is not None:
+        raise ValueError("a given norm needs max_norm")
+    if max_norm is not None and not float(max_norm) >= 0.0:
+        raise ValueError("max_norm must be finite and not negative")
+    if len(p._present) != len(p):
+        raise TypeError("a parameter list has no empty places")
+    lists = [p, g, state._m, state._v] + ([] if c is None else [c])
+    tables = [x._current() for x in lists]
+    for name, other in (("gradients", g), ("moments", state._m), ("moments", state._v),
+                        ("copies", c)):
+        if other is None:
+            continue
+        if len(other) != len(p):
+            raise ValueError(f"{len(p)} parameters and {len(other)} {name}")
+        if other._layouts != p._layouts or other._shapes != p._shapes:
+            for i, t in enumerate(other.tensors):
+                if t is not None and (other._layouts[i] != p._layouts[i]
+                                      or other._shapes[i] != p._shapes[i]):
+                    raise ValueError(f"{name} and parameters differ in shape or strides at place {i}")
+    for name, other in (("the parameters", p), ("the moments", state._m),
+                        ("the moments", state._v), ("the copies", c)):
+        if other is not None:
+            other._check_apart(name)
+    options = AdamOptions(float(lr), float(betas[0]), float(betas[1]), float(eps),
+                          float(weight_decay), -1.0 if max_norm is None else float(max_norm),
+                          int(bool(decoupled)), 0)
+    call = _TensorCall(len(p), stream, norm_wanted=max_norm is not None)
+    _status(load().arcqml_rt_v2_adam_step(
+        *tables[:4], None if c is None else tables[4], len(p), state.step.data_ptr(),
+        C.byref(options), *call.arguments(norm)))
+    for x in lists[:1] + lists[2:]:
+        x._written()
+    return call.norm
 
 
 def norms_device(state, num_qubits: int, stream=None) -> np.ndarray:

@@ -193,6 +193,79 @@ int32_t arcqml_rt_v2_small_adam(const CircuitPlanHandle *plan,
                                 double beta1, double beta2, double epsilon, double weight_decay,
                                 double *energies, void *stream);
 
+/* Training over many device tensors: the global norm of a model's gradients, clipping by that
+ * norm, and the Adam step (no reference counterpart on the device: the update is the Adam of
+ * crates/arcqml-optim/src/adam.rs:190-240). They serve models whose trained values live on the
+ * device beside a circuit's parameters: the tensors of a classical half, trained input states.
+ * Every tensor is the memory of `length` elements without gaps (any order of its dimensions); a
+ * complex tensor is passed as its 2 x length components. Nothing is read back and no call waits:
+ * norms, factors and the step count stay on the device, so the calls can be captured into a CUDA
+ * graph. The tables are copied into the launches; they may be freed when a call returns. */
+enum {
+    ARCQML_F64 = 0,
+    ARCQML_F32 = 1,
+    ARCQML_BF16 = 2,
+    ARCQML_F16 = 3,
+    ARCQML_NO_TENSOR = 4 /* this place of the list holds no tensor (a parameter without gradient) */
+};
+typedef struct ArcqmlTensor {
+    void *data;       /* device pointer, aligned to the element's size; ignored when length is 0 */
+    uint64_t length;  /* elements */
+    uint32_t dtype;
+    uint32_t reserved; /* 0 */
+} ArcqmlTensor;
+
+/* Doubles of device scratch that the three calls below take for lists of num_tensors tensors. The
+ * scratch belongs to one call at a time: calls that can overlap (other streams, replayed graphs)
+ * need their own. */
+size_t arcqml_rt_v2_gradient_workspace(size_t num_tensors);
+
+/* *norm <- sqrt of the sum of squares over every element of every tensor (device). The sum is
+ * kept in f64 and its order is fixed by the lengths, types and the GPU, so equal inputs give equal
+ * bits. A NaN or an infinity in a gradient gives a NaN or infinite norm; squares leave the f64
+ * range for elements above 1e154. No tensors, or empty ones: 0. */
+int32_t arcqml_rt_v2_gradient_norm(const ArcqmlTensor *gradients, size_t num_tensors,
+                                   double *norm, double *workspace, size_t workspace_len,
+                                   void *stream);
+
+/* Scales every gradient in place by min(1, max_norm / (n + 1e-6)), n the global norm of the list,
+ * or *given_norm (device) when given_norm is not null: a norm over several lists, or over the
+ * ranks of a sharded model. *norm (device, may be null) <- n. A factor of 1 leaves the gradients
+ * unwritten; a NaN norm makes every gradient NaN and an infinite one makes the finite gradients 0,
+ * the others NaN. Products are f64 for f64 tensors and f32 otherwise, rounded once to the type.
+ * The tensors must not overlap. max_norm must be finite and not negative. */
+int32_t arcqml_rt_v2_clip_gradients(const ArcqmlTensor *gradients, size_t num_tensors,
+                                    double max_norm, const double *given_norm, double *norm,
+                                    double *workspace, size_t workspace_len, void *stream);
+
+typedef struct ArcqmlAdamOptions {
+    double learning_rate, beta1, beta2, epsilon, weight_decay;
+    double max_norm;   /* negative: no clipping */
+    int32_t decoupled; /* 0: decay joins the gradient (the reference's); 1: it scales the parameter */
+    int32_t reserved;  /* 0 */
+} ArcqmlAdamOptions;
+
+/* One Adam step over every tensor, t = *step + 1 (step: device, steps taken so far; the call adds
+ * one). With f the clip factor of the gradients' global norm (1 when max_norm is negative; the
+ * gradients themselves stay as they are):
+ *   a = f g, plus weight_decay p unless decoupled
+ *   m <- beta1 m + (1 - beta1) a;   v <- beta2 v + (1 - beta2) a^2
+ *   p <- p (scaled by 1 - learning_rate weight_decay when decoupled)
+ *        - learning_rate (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + epsilon)
+ * f64 parameters take f64 gradients and moments and are computed in f64, each operation rounded
+ * on its own in the order of the host's and the optimizer loop's Adam. Parameters of the other
+ * types take gradients of any of those types and f32 moments, and are computed in f32. A place
+ * whose gradient is ARCQML_NO_TENSOR is left as it is. copies (may be null; places may be
+ * ARCQML_NO_TENSOR) receive the new values of f32 parameters rounded to bf16 or f16. given_norm,
+ * norm: as above, used with max_norm >= 0 only. Parameters, moments and copies must not overlap. */
+int32_t arcqml_rt_v2_adam_step(const ArcqmlTensor *parameters, const ArcqmlTensor *gradients,
+                               const ArcqmlTensor *first_moments,
+                               const ArcqmlTensor *second_moments, const ArcqmlTensor *copies,
+                               size_t num_tensors, int64_t *step,
+                               const ArcqmlAdamOptions *options, const double *given_norm,
+                               double *norm, double *workspace, size_t workspace_len,
+                               void *stream);
+
 /* State analysis (crates/arcqml-analysis/src/statevector), on every row of a device state.
  * probabilities: probabilities[row][i] = |psi_row[i]|^2 (device, [batch, 2^n];
  *   probabilities.rs:22-25).
