@@ -947,8 +947,8 @@ int32_t arcqml_rt_v2_scaled_copy(const arcqml_c128 *input, size_t batch, size_t 
 
 // ---------------------------------------------------------------- training over many tensors
 
-size_t arcqml_rt_v2_gradient_workspace(size_t num_tensors) {
-    return tensor_workspace(num_tensors);
+size_t arcqml_rt_v2_gradient_workspace(const ArcqmlTensor *tensors, size_t num_tensors) {
+    return tensor_workspace(tensors, num_tensors);
 }
 
 int32_t arcqml_rt_v2_gradient_norm(const ArcqmlTensor *gradients, size_t num_tensors,

@@ -8,14 +8,17 @@
 // corrections pass between the launches in device scratch that the caller gives, so nothing is
 // shared between calls and no sum depends on the order in which blocks finish.
 //
-//   k_square_sums   per block the f64 sum of squares of its chunks
-//   k_scalars       one block: the sums in order -> norm, clip factor, step count, bias corrections
-//   k_clip, k_adam  the list scaled, or updated
+//   k_square_sums      per block the f64 sum of squares of its chunks
+//   k_scalars          one block: the sums in order -> norm, clip factor, step, bias corrections
+//   k_clip, k_adam     the list scaled, or updated
+//   k_short_*          all of it for a short list, in one launch of one cluster
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <sstream>
 #include <string>
@@ -24,14 +27,24 @@
 #include "optim.h"
 #include "profile.h"
 
+namespace cg = cooperative_groups;
+
 namespace arcqml {
 namespace {
 
 constexpr int kOT = 256;                 // threads per block
 constexpr uint32_t kMaxBlocks = 148 * 8; // blocks of one launch
 constexpr uint32_t kMaxTensors = 512;    // tensors of one launch
-constexpr uint32_t kVectors = 2048;      // 16-byte vectors of one chunk (k_square_sums, k_clip)
-constexpr uint32_t kGroups = 2048;       // groups of 4 elements of one chunk (k_adam)
+constexpr uint32_t kChunk = 2048;        // 16-byte vectors (k_square_sums, k_clip) or groups of 4
+                                         // elements (k_adam) of one chunk
+// Short lists: one cluster, a warp per chunk.
+constexpr uint32_t kShortTensors = 64;
+#ifndef ARCQML_SHORT_ELEMENTS
+#define ARCQML_SHORT_ELEMENTS (1u << 18)
+#endif
+constexpr uint64_t kShortElements = ARCQML_SHORT_ELEMENTS;
+constexpr uint32_t kCluster = 16, kShortThreads = 512;
+constexpr uint32_t kShortVectors = 256, kShortGroups = 64;
 
 // What k_scalars leaves for the launches behind it (the head of the scratch).
 struct Scalars {
@@ -40,26 +53,26 @@ struct Scalars {
 constexpr size_t kScalarDoubles = sizeof(Scalars) / sizeof(double);
 
 // The tensors of one launch. first[i]: the number of chunks before tensor i; first[count]: of all.
-struct TensorTable {
-    void *data[kMaxTensors];
-    uint64_t length[kMaxTensors];
-    uint32_t first[kMaxTensors + 1];
-    uint8_t dtype[kMaxTensors];
+template <uint32_t CAP> struct TensorTable {
+    void *data[CAP];
+    uint64_t length[CAP];
+    uint32_t first[CAP + 1];
+    uint8_t dtype[CAP];
     uint32_t count;
 };
 
-struct AdamTable {
-    void *p[kMaxTensors], *m[kMaxTensors], *v[kMaxTensors], *copy[kMaxTensors];
-    const void *g[kMaxTensors];
-    uint64_t length[kMaxTensors];
-    uint32_t first[kMaxTensors + 1];
-    uint8_t types[kMaxTensors];   // of the parameter, the gradient (<< 2) and the copy (<< 4)
-    uint8_t aligned[kMaxTensors]; // kAligned*: arrays whose groups start on their own size
-    uint8_t head[kMaxTensors];    // elements before the first group
+template <uint32_t CAP> struct AdamTable {
+    void *p[CAP], *m[CAP], *v[CAP], *copy[CAP];
+    const void *g[CAP];
+    uint64_t length[CAP];
+    uint32_t first[CAP + 1];
+    uint8_t types[CAP];   // of the parameter, the gradient (<< 2) and the copy (<< 4)
+    uint8_t aligned[CAP]; // kAligned*: arrays whose groups start on their own size
+    uint8_t head[CAP];    // elements before the first group
     uint32_t count;
 };
 enum { kAlignedG = 1, kAlignedM = 2, kAlignedV = 4, kAlignedCopy = 8, kHasCopy = 16 };
-static_assert(sizeof(AdamTable) < 32000, "kernel parameters hold 32764 bytes");
+static_assert(sizeof(AdamTable<kMaxTensors>) < 32000, "kernel parameters hold 32764 bytes");
 
 // The tensor of chunk c: the last i with first[i] <= c (tensors without chunks are not listed).
 template <class T>
@@ -150,22 +163,24 @@ template <class T> __device__ __forceinline__ uint32_t head_of(const T *p, uint6
 }
 
 // Sum over the block in a fixed order; valid in thread 0.
-__device__ __forceinline__ double o_block_sum(double v) {
-    __shared__ double red[kOT / 32];
+template <int THREADS> __device__ __forceinline__ double o_block_sum(double v) {
+    __shared__ double red[THREADS / 32];
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
     double r = 0.0;
     if (threadIdx.x == 0)
-        for (int w = 0; w < kOT / 32; ++w) r += red[w];
+        for (int w = 0; w < THREADS / 32; ++w) r += red[w];
     return r;
 }
 
+// A chunk is taken by LANES threads, of which this is `lane`, and holds PER vectors or groups.
+//
 // Squares of one chunk, added to acc in f64: the squares of f32 values leave the range of f32, and a
 // norm that comes back in f64 is wanted to its precision.
-template <uint32_t DTYPE>
+template <uint32_t DTYPE, uint32_t LANES, uint32_t PER>
 __device__ __forceinline__ void square_chunk(const void *data, uint64_t length, uint32_t chunk,
-                                             double (&acc)[4]) {
+                                             uint32_t lane, double (&acc)[4]) {
     using T = typename Elem<DTYPE>::type;
     using W = typename Elem<DTYPE>::wide;
     constexpr int N = 16 / sizeof(T), U = 8;
@@ -173,8 +188,8 @@ __device__ __forceinline__ void square_chunk(const void *data, uint64_t length, 
     const uint32_t head = head_of(p, length);
     const uint64_t vectors = (length - head) / N;
     const auto *q = reinterpret_cast<const Words<DTYPE, N> *>(p + head);
-    const uint64_t v0 = uint64_t(chunk) * kVectors;
-    const uint32_t n = uint32_t(min(uint64_t(kVectors), vectors - min(v0, vectors)));
+    const uint64_t v0 = uint64_t(chunk) * PER;
+    const uint32_t n = uint32_t(min(uint64_t(PER), vectors - min(v0, vectors)));
     const auto add = [&](const Words<DTYPE, N> &raw) {
         W x[N];
         raw.unpack(x);
@@ -184,77 +199,90 @@ __device__ __forceinline__ void square_chunk(const void *data, uint64_t length, 
             acc[j % 4] = fma(d, d, acc[j % 4]);
         }
     };
-    uint32_t v = threadIdx.x;
-    for (; v + (U - 1) * kOT < n; v += U * kOT) {
+    uint32_t v = lane;
+    for (; v + (U - 1) * LANES < n; v += U * LANES) {
         Words<DTYPE, N> x[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) x[u] = q[v0 + v + u * kOT];
+        for (int u = 0; u < U; ++u) x[u] = q[v0 + v + u * LANES];
 #pragma unroll
         for (int u = 0; u < U; ++u) add(x[u]);
     }
-    for (; v < n; v += kOT) add(q[v0 + v]);
+    for (; v < n; v += LANES) add(q[v0 + v]);
     // the elements before the first vector (chunk 0) and behind the last one (the last chunk)
-    if (chunk == 0 && threadIdx.x < head) {
-        const double d = double(widen(p[threadIdx.x]));
+    if (chunk == 0 && lane < head) {
+        const double d = double(widen(p[lane]));
         acc[0] = fma(d, d, acc[0]);
     }
     const uint64_t done = head + vectors * N;
-    if (v0 + kVectors >= vectors && threadIdx.x < length - done) {
-        const double d = double(widen(p[done + threadIdx.x]));
+    if (v0 + PER >= vectors && lane < length - done) {
+        const double d = double(widen(p[done + lane]));
         acc[1] = fma(d, d, acc[1]);
     }
 }
 
+// The squares of one chunk of tensor k of a table.
+template <uint32_t LANES, uint32_t PER, class Table>
+__device__ __forceinline__ void square_chunk_of(const Table &t, uint32_t k, uint32_t chunk,
+                                                uint32_t lane, double (&acc)[4]) {
+    const void *g = t.data[k];
+    const uint64_t n = t.length[k];
+    switch (t.dtype[k]) {
+    case ARCQML_F64: square_chunk<ARCQML_F64, LANES, PER>(g, n, chunk, lane, acc); break;
+    case ARCQML_F32: square_chunk<ARCQML_F32, LANES, PER>(g, n, chunk, lane, acc); break;
+    case ARCQML_BF16: square_chunk<ARCQML_BF16, LANES, PER>(g, n, chunk, lane, acc); break;
+    default: square_chunk<ARCQML_F16, LANES, PER>(g, n, chunk, lane, acc);
+    }
+}
+
 __global__ void __launch_bounds__(kOT)
-    k_square_sums(const __grid_constant__ TensorTable t, double *__restrict__ sums) {
+    k_square_sums(const __grid_constant__ TensorTable<kMaxTensors> t, double *__restrict__ sums) {
     double acc[4] = {0.0, 0.0, 0.0, 0.0};
     for (uint32_t c = blockIdx.x; c < t.first[t.count]; c += gridDim.x) {
-        const uint32_t k = tensor_of(t, c), chunk = c - t.first[k];
-        const void *g = t.data[k];
-        const uint64_t n = t.length[k];
-        switch (t.dtype[k]) {
-        case ARCQML_F64: square_chunk<ARCQML_F64>(g, n, chunk, acc); break;
-        case ARCQML_F32: square_chunk<ARCQML_F32>(g, n, chunk, acc); break;
-        case ARCQML_BF16: square_chunk<ARCQML_BF16>(g, n, chunk, acc); break;
-        default: square_chunk<ARCQML_F16>(g, n, chunk, acc);
-        }
+        const uint32_t k = tensor_of(t, c);
+        square_chunk_of<kOT, kChunk>(t, k, c - t.first[k], threadIdx.x, acc);
     }
-    const double sum = o_block_sum((acc[0] + acc[1]) + (acc[2] + acc[3]));
+    const double sum = o_block_sum<kOT>((acc[0] + acc[1]) + (acc[2] + acc[3]));
     if (threadIdx.x == 0) sums[blockIdx.x] = sum;
 }
 
-// One block. given != null: n = *given; else the root of the count sums. factor: 1 without
-// clipping (max_norm < 0); a NaN norm stays a NaN factor. step != null: one more step is counted.
+// min(1, max_norm / (norm + 1e-6)), 1 without clipping (max_norm < 0). A NaN norm gives NaN.
+__device__ __forceinline__ double clip_factor(double norm, double max_norm) {
+    if (!(max_norm >= 0.0)) return 1.0;
+    const double f = max_norm / (norm + 1e-6);
+    return f > 1.0 ? 1.0 : f;
+}
+
+__device__ __forceinline__ double bias_correction(double beta, int64_t t) {
+    return 1.0 - pow(beta, double(t));
+}
+
+// One block. given != null: n = *given; else the root of the count sums. step != null: one more
+// step is counted.
 __global__ void __launch_bounds__(kOT)
     k_scalars(const double *__restrict__ sums, uint32_t count, const double *given,
               double max_norm, int64_t *step, double beta1, double beta2, double *norm,
               Scalars *out) {
     double acc = 0.0;
     for (uint32_t i = threadIdx.x; i < count; i += kOT) acc += sums[i];
-    acc = o_block_sum(acc);
+    acc = o_block_sum<kOT>(acc);
     if (threadIdx.x != 0) return;
     const double n = given ? *given : sqrt(acc);
     if (norm) *norm = n;
-    double factor = 1.0;
-    if (max_norm >= 0.0) {
-        factor = max_norm / (n + 1e-6);
-        if (factor > 1.0) factor = 1.0;
-    }
-    Scalars r{n, factor, 1.0, 1.0};
+    Scalars r{n, clip_factor(n, max_norm), 1.0, 1.0};
     if (step) {
         const int64_t now = *step + 1;
         *step = now;
-        r.bc1 = 1.0 - pow(beta1, double(now));
-        r.bc2 = 1.0 - pow(beta2, double(now));
+        r.bc1 = bias_correction(beta1, now);
+        r.bc2 = bias_correction(beta2, now);
     }
     *out = r;
 }
 
 // One chunk times the factor: the product in the type of the arithmetic (f32 for 16-bit types, the
 // factor rounded to it), rounded once to the element's type.
-template <uint32_t DTYPE>
+template <uint32_t DTYPE, uint32_t LANES, uint32_t PER>
 __device__ __forceinline__ void clip_chunk(void *data, uint64_t length, uint32_t chunk,
-                                           double factor) {
+                                           uint32_t lane, double factor) {
     using T = typename Elem<DTYPE>::type;
     using W = typename Elem<DTYPE>::wide;
     constexpr int N = 16 / sizeof(T), U = 4;
@@ -263,8 +291,8 @@ __device__ __forceinline__ void clip_chunk(void *data, uint64_t length, uint32_t
     const uint32_t head = head_of(p, length);
     const uint64_t vectors = (length - head) / N;
     auto *q = reinterpret_cast<Words<DTYPE, N> *>(p + head);
-    const uint64_t v0 = uint64_t(chunk) * kVectors;
-    const uint32_t n = uint32_t(min(uint64_t(kVectors), vectors - min(v0, vectors)));
+    const uint64_t v0 = uint64_t(chunk) * PER;
+    const uint32_t n = uint32_t(min(uint64_t(PER), vectors - min(v0, vectors)));
     const auto scale = [&](Words<DTYPE, N> &raw) {
         W x[N];
         raw.unpack(x);
@@ -272,42 +300,48 @@ __device__ __forceinline__ void clip_chunk(void *data, uint64_t length, uint32_t
         for (int j = 0; j < N; ++j) x[j] *= f;
         raw.pack(x);
     };
-    uint32_t v = threadIdx.x;
-    for (; v + (U - 1) * kOT < n; v += U * kOT) {
+    uint32_t v = lane;
+    for (; v + (U - 1) * LANES < n; v += U * LANES) {
         Words<DTYPE, N> x[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) x[u] = q[v0 + v + u * kOT];
+        for (int u = 0; u < U; ++u) x[u] = q[v0 + v + u * LANES];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             scale(x[u]);
-            q[v0 + v + u * kOT] = x[u];
+            q[v0 + v + u * LANES] = x[u];
         }
     }
-    for (; v < n; v += kOT) {
+    for (; v < n; v += LANES) {
         Words<DTYPE, N> x = q[v0 + v];
         scale(x);
         q[v0 + v] = x;
     }
-    if (chunk == 0 && threadIdx.x < head) narrow(widen(p[threadIdx.x]) * f, p[threadIdx.x]);
+    if (chunk == 0 && lane < head) narrow(widen(p[lane]) * f, p[lane]);
     const uint64_t done = head + vectors * N;
-    if (v0 + kVectors >= vectors && threadIdx.x < length - done)
-        narrow(widen(p[done + threadIdx.x]) * f, p[done + threadIdx.x]);
+    if (v0 + PER >= vectors && lane < length - done)
+        narrow(widen(p[done + lane]) * f, p[done + lane]);
+}
+
+template <uint32_t LANES, uint32_t PER, class Table>
+__device__ __forceinline__ void clip_chunk_of(const Table &t, uint32_t k, uint32_t chunk,
+                                              uint32_t lane, double factor) {
+    void *g = t.data[k];
+    const uint64_t n = t.length[k];
+    switch (t.dtype[k]) {
+    case ARCQML_F64: clip_chunk<ARCQML_F64, LANES, PER>(g, n, chunk, lane, factor); break;
+    case ARCQML_F32: clip_chunk<ARCQML_F32, LANES, PER>(g, n, chunk, lane, factor); break;
+    case ARCQML_BF16: clip_chunk<ARCQML_BF16, LANES, PER>(g, n, chunk, lane, factor); break;
+    default: clip_chunk<ARCQML_F16, LANES, PER>(g, n, chunk, lane, factor);
+    }
 }
 
 __global__ void __launch_bounds__(kOT, 4)
-    k_clip(const __grid_constant__ TensorTable t, const Scalars *__restrict__ sc) {
+    k_clip(const __grid_constant__ TensorTable<kMaxTensors> t, const Scalars *__restrict__ sc) {
     const double factor = sc->factor;
     if (factor == 1.0) return;
     for (uint32_t c = blockIdx.x; c < t.first[t.count]; c += gridDim.x) {
-        const uint32_t k = tensor_of(t, c), chunk = c - t.first[k];
-        void *g = t.data[k];
-        const uint64_t n = t.length[k];
-        switch (t.dtype[k]) {
-        case ARCQML_F64: clip_chunk<ARCQML_F64>(g, n, chunk, factor); break;
-        case ARCQML_F32: clip_chunk<ARCQML_F32>(g, n, chunk, factor); break;
-        case ARCQML_BF16: clip_chunk<ARCQML_BF16>(g, n, chunk, factor); break;
-        default: clip_chunk<ARCQML_F16>(g, n, chunk, factor);
-        }
+        const uint32_t k = tensor_of(t, c);
+        clip_chunk_of<kOT, kChunk>(t, k, c - t.first[k], threadIdx.x, factor);
     }
 }
 
@@ -332,7 +366,19 @@ struct AdamScalars32 {
     float b1, b2, nb1, nb2, eps, wd, down, rate, root, factor;
 };
 
+__device__ __forceinline__ AdamScalars64 scalars64(const ArcqmlAdamOptions &o, double bc1,
+                                                   double bc2, double factor) {
+    return AdamScalars64{o.learning_rate, o.beta1, o.beta2, 1.0 - o.beta1, 1.0 - o.beta2,
+                         o.epsilon, o.weight_decay, 1.0 - o.learning_rate * o.weight_decay, bc1,
+                         bc2, factor};
+}
+
 // f32: rate = lr / (1 - beta1^t) and root = 1 / (1 - beta2^t) are formed in f64 and rounded once.
+__device__ __forceinline__ AdamScalars32 scalars32(const AdamScalars64 &h) {
+    return AdamScalars32{float(h.b1), float(h.b2), float(h.nb1), float(h.nb2), float(h.eps),
+                         float(h.wd), float(h.down), float(h.lr / h.bc1), float(1.0 / h.bc2),
+                         float(h.factor)};
+}
 __device__ __forceinline__ void adam_update(float &p, float &m, float &v, float g,
                                             const AdamScalars32 &h, bool decoupled) {
     float a = g * h.factor;
@@ -370,9 +416,9 @@ __device__ __forceinline__ void store4(void *p, uint64_t e, bool aligned,
     }
 }
 
-template <uint32_t PT, uint32_t GT, class H>
-__device__ __forceinline__ void adam_chunk(const AdamTable &t, uint32_t k, uint32_t chunk,
-                                           const H &h, bool decoupled) {
+template <uint32_t PT, uint32_t GT, uint32_t LANES, uint32_t PER, class Table, class H>
+__device__ __forceinline__ void adam_chunk(const Table &t, uint32_t k, uint32_t chunk,
+                                           uint32_t lane, const H &h, bool decoupled) {
     using P = typename Elem<PT>::type;
     using G = typename Elem<GT>::type;
     using W = typename Elem<PT>::wide;
@@ -383,8 +429,8 @@ __device__ __forceinline__ void adam_chunk(const AdamTable &t, uint32_t k, uint3
     void *p = t.p[k], *m = t.m[k], *v = t.v[k], *copy = t.copy[k];
     const void *g = t.g[k];
     const uint64_t groups = (length - head) / 4;
-    const uint64_t i0 = uint64_t(chunk) * kGroups;
-    const uint32_t n = uint32_t(min(uint64_t(kGroups), groups - min(i0, groups)));
+    const uint64_t i0 = uint64_t(chunk) * PER;
+    const uint32_t n = uint32_t(min(uint64_t(PER), groups - min(i0, groups)));
     const uint64_t e0 = head + 4 * i0;
     const auto update = [&](uint64_t e, const Words<PT, 4> &rp, const Words<GT, 4> &rg,
                             const Words<WT, 4> &rm, const Words<WT, 4> &rv) {
@@ -405,24 +451,24 @@ __device__ __forceinline__ void adam_chunk(const AdamTable &t, uint32_t k, uint3
             }
         }
     };
-    uint32_t i = threadIdx.x;
-    for (; i + (U - 1) * kOT < n; i += U * kOT) {
+    uint32_t i = lane;
+    for (; i + (U - 1) * LANES < n; i += U * LANES) {
         Words<PT, 4> xp[U];
         Words<GT, 4> xg[U];
         Words<WT, 4> xm[U], xv[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const uint64_t e = e0 + 4 * (i + u * kOT);
+            const uint64_t e = e0 + 4 * (i + u * LANES);
             xp[u] = load4<PT>(p, e, true);
             xg[u] = load4<GT>(g, e, aligned & kAlignedG);
             xm[u] = load4<WT>(m, e, aligned & kAlignedM);
             xv[u] = load4<WT>(v, e, aligned & kAlignedV);
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) update(e0 + 4 * (i + u * kOT), xp[u], xg[u], xm[u], xv[u]);
+        for (int u = 0; u < U; ++u) update(e0 + 4 * (i + u * LANES), xp[u], xg[u], xm[u], xv[u]);
     }
     if constexpr (U > 1) {
-        for (; i < n; i += kOT) {
+        for (; i < n; i += LANES) {
             const uint64_t e = e0 + 4 * i;
             update(e, load4<PT>(p, e, true), load4<GT>(g, e, aligned & kAlignedG),
                    load4<WT>(m, e, aligned & kAlignedM), load4<WT>(v, e, aligned & kAlignedV));
@@ -430,10 +476,10 @@ __device__ __forceinline__ void adam_chunk(const AdamTable &t, uint32_t k, uint3
     }
     // the elements before the first group (chunk 0) and behind the last one (the last chunk)
     const uint64_t done = head + groups * 4;
-    const uint32_t tail = i0 + kGroups >= groups ? uint32_t(length - done) : 0;
+    const uint32_t tail = i0 + PER >= groups ? uint32_t(length - done) : 0;
     const uint32_t first = chunk == 0 ? head : 0;
-    if (threadIdx.x < first + tail) {
-        const uint64_t e = threadIdx.x < first ? threadIdx.x : done + threadIdx.x - first;
+    if (lane < first + tail) {
+        const uint64_t e = lane < first ? lane : done + lane - first;
         P &rp = static_cast<P *>(p)[e];
         W x = widen(rp);
         adam_update(x, static_cast<W *>(m)[e], static_cast<W *>(v)[e],
@@ -448,13 +494,25 @@ __device__ __forceinline__ void adam_chunk(const AdamTable &t, uint32_t k, uint3
     }
 }
 
-template <uint32_t PT>
-__device__ __forceinline__ void adam_chunk_of(const AdamTable &t, uint32_t k, uint32_t chunk,
-                                              const AdamScalars32 &h, bool decoupled) {
+template <uint32_t PT, uint32_t LANES, uint32_t PER, class Table>
+__device__ __forceinline__ void adam_chunk_g(const Table &t, uint32_t k, uint32_t chunk,
+                                             uint32_t lane, const AdamScalars32 &h,
+                                             bool decoupled) {
     switch (t.types[k] >> 2 & 3) {
-    case ARCQML_F32: adam_chunk<PT, ARCQML_F32>(t, k, chunk, h, decoupled); break;
-    case ARCQML_BF16: adam_chunk<PT, ARCQML_BF16>(t, k, chunk, h, decoupled); break;
-    default: adam_chunk<PT, ARCQML_F16>(t, k, chunk, h, decoupled);
+    case ARCQML_F32: adam_chunk<PT, ARCQML_F32, LANES, PER>(t, k, chunk, lane, h, decoupled); break;
+    case ARCQML_BF16: adam_chunk<PT, ARCQML_BF16, LANES, PER>(t, k, chunk, lane, h, decoupled); break;
+    default: adam_chunk<PT, ARCQML_F16, LANES, PER>(t, k, chunk, lane, h, decoupled);
+    }
+}
+
+template <uint32_t LANES, uint32_t PER, class Table>
+__device__ __forceinline__ void adam_chunk_of(const Table &t, uint32_t k, uint32_t chunk,
+                                              uint32_t lane, const AdamScalars32 &h,
+                                              bool decoupled) {
+    switch (t.types[k] & 3) {
+    case ARCQML_F32: adam_chunk_g<ARCQML_F32, LANES, PER>(t, k, chunk, lane, h, decoupled); break;
+    case ARCQML_BF16: adam_chunk_g<ARCQML_BF16, LANES, PER>(t, k, chunk, lane, h, decoupled); break;
+    default: adam_chunk_g<ARCQML_F16, LANES, PER>(t, k, chunk, lane, h, decoupled);
     }
 }
 
@@ -462,28 +520,134 @@ __device__ __forceinline__ void adam_chunk_of(const AdamTable &t, uint32_t k, ui
 // (two or three divisions and a root per element) takes twice the registers.
 template <bool F64>
 __global__ void __launch_bounds__(kOT, F64 ? 2 : 4)
-    k_adam(const __grid_constant__ AdamTable t, const __grid_constant__ ArcqmlAdamOptions o,
-           const Scalars *__restrict__ sc) {
-    const double factor = sc->factor, bc1 = sc->bc1, bc2 = sc->bc2;
+    k_adam(const __grid_constant__ AdamTable<kMaxTensors> t,
+           const __grid_constant__ ArcqmlAdamOptions o, const Scalars *__restrict__ sc) {
     const bool decoupled = o.decoupled != 0;
-    const double lr = o.learning_rate, down = 1.0 - lr * o.weight_decay;
-    const AdamScalars64 h{lr, o.beta1, o.beta2, 1.0 - o.beta1, 1.0 - o.beta2, o.epsilon,
-                          o.weight_decay, down, bc1, bc2, factor};
-    const AdamScalars32 hf{float(h.b1), float(h.b2), float(h.nb1), float(h.nb2), float(h.eps),
-                           float(h.wd), float(down), float(lr / bc1), float(1.0 / bc2),
-                           float(factor)};
+    const AdamScalars64 h = scalars64(o, sc->bc1, sc->bc2, sc->factor);
+    const AdamScalars32 hf = scalars32(h);
     for (uint32_t c = blockIdx.x; c < t.first[t.count]; c += gridDim.x) {
         const uint32_t k = tensor_of(t, c), chunk = c - t.first[k];
-        if constexpr (F64) {
-            adam_chunk<ARCQML_F64, ARCQML_F64>(t, k, chunk, h, decoupled);
-        } else {
-            switch (t.types[k] & 3) {
-            case ARCQML_F32: adam_chunk_of<ARCQML_F32>(t, k, chunk, hf, decoupled); break;
-            case ARCQML_BF16: adam_chunk_of<ARCQML_BF16>(t, k, chunk, hf, decoupled); break;
-            default: adam_chunk_of<ARCQML_F16>(t, k, chunk, hf, decoupled);
+        if constexpr (F64)
+            adam_chunk<ARCQML_F64, ARCQML_F64, kOT, kChunk>(t, k, chunk, threadIdx.x, h, decoupled);
+        else adam_chunk_of<kOT, kChunk>(t, k, chunk, threadIdx.x, hf, decoupled);
+    }
+}
+
+// ------------------------------------------------------------------ short lists
+
+// The sum of v over the cluster, in rank order, in every thread. The blocks' sums are read from
+// their shared memory: no block may end before the cluster has met again (cluster_left).
+__device__ __forceinline__ double cluster_sum(double v, cg::cluster_group &cluster) {
+    __shared__ double mine;
+    const double sum = o_block_sum<kShortThreads>(v);
+    if (threadIdx.x == 0) mine = sum;
+    cluster.sync();
+    double r = 0.0;
+    for (uint32_t b = 0; b < cluster.num_blocks(); ++b) r += *cluster.map_shared_rank(&mine, b);
+    return r;
+}
+
+// Norm (or the given one) and clip of a short list: clips when max_norm >= 0.
+__global__ void __launch_bounds__(kShortThreads, 1)
+    k_short_clip(const __grid_constant__ TensorTable<kShortTensors> t, const double *given,
+                 double max_norm, double *norm) {
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t lane = threadIdx.x & 31, chunks = t.first[t.count];
+    const uint32_t warp = cluster.block_rank() * (kShortThreads / 32) + (threadIdx.x >> 5);
+    const uint32_t warps = cluster.num_blocks() * (kShortThreads / 32);
+    double acc[4] = {0.0, 0.0, 0.0, 0.0};
+    double n;
+    if (given) {
+        n = *given;
+    } else {
+        for (uint32_t c = warp; c < chunks; c += warps) {
+            const uint32_t k = tensor_of(t, c);
+            square_chunk_of<32, kShortVectors>(t, k, c - t.first[k], lane, acc);
+        }
+        n = sqrt(cluster_sum((acc[0] + acc[1]) + (acc[2] + acc[3]), cluster));
+    }
+    if (warp == 0 && lane == 0 && norm) *norm = n;
+    const double factor = clip_factor(n, max_norm);
+    if (factor != 1.0)
+        for (uint32_t c = warp; c < chunks; c += warps) {
+            const uint32_t k = tensor_of(t, c);
+            clip_chunk_of<32, kShortVectors>(t, k, c - t.first[k], lane, factor);
+        }
+    cluster.sync();
+}
+
+// The squares of a chunk's gradients, over the same elements that adam_chunk takes.
+template <uint32_t GT, uint32_t LANES, uint32_t PER, class Table>
+__device__ __forceinline__ void square_groups(const Table &t, uint32_t k, uint32_t chunk,
+                                              uint32_t lane, double (&acc)[4]) {
+    using G = typename Elem<GT>::type;
+    const uint32_t head = t.head[k];
+    const uint64_t length = t.length[k], groups = (length - head) / 4, i0 = uint64_t(chunk) * PER;
+    const uint32_t n = uint32_t(min(uint64_t(PER), groups - min(i0, groups)));
+    const void *g = t.g[k];
+#pragma unroll 2
+    for (uint32_t i = lane; i < n; i += LANES) {
+        typename Elem<GT>::wide x[4];
+        load4<GT>(g, head + 4 * (i0 + i), t.aligned[k] & kAlignedG).unpack(x);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j] = fma(double(x[j]), double(x[j]), acc[j]);
+    }
+    const uint64_t done = head + groups * 4;
+    const uint32_t tail = i0 + PER >= groups ? uint32_t(length - done) : 0;
+    const uint32_t first = chunk == 0 ? head : 0;
+    if (lane < first + tail) {
+        const double x =
+            double(widen(static_cast<const G *>(g)[lane < first ? lane : done + lane - first]));
+        acc[0] = fma(x, x, acc[0]);
+    }
+}
+
+// One Adam step of a short list. Every block reads the step count before the cluster first meets;
+// the first block writes the new one after that.
+__global__ void __launch_bounds__(kShortThreads, 1)
+    k_short_adam(const __grid_constant__ AdamTable<kShortTensors> t,
+                 const __grid_constant__ ArcqmlAdamOptions o, int64_t *step, const double *given,
+                 double *norm) {
+    __shared__ double bc[2];
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t lane = threadIdx.x & 31, chunks = t.first[t.count];
+    const uint32_t warp = cluster.block_rank() * (kShortThreads / 32) + (threadIdx.x >> 5);
+    const uint32_t warps = cluster.num_blocks() * (kShortThreads / 32);
+    const int64_t now = *step + 1;
+    // the last warp has the fewest chunks
+    if (threadIdx.x == kShortThreads - 1) bc[0] = bias_correction(o.beta1, now);
+    if (threadIdx.x == kShortThreads - 2) bc[1] = bias_correction(o.beta2, now);
+    double n = 0.0;
+    if (o.max_norm >= 0.0 && !given) {
+        double acc[4] = {0.0, 0.0, 0.0, 0.0};
+        for (uint32_t c = warp; c < chunks; c += warps) {
+            const uint32_t k = tensor_of(t, c), chunk = c - t.first[k];
+            switch (t.types[k] >> 2 & 3) {
+            case ARCQML_F64: square_groups<ARCQML_F64, 32, kShortGroups>(t, k, chunk, lane, acc); break;
+            case ARCQML_F32: square_groups<ARCQML_F32, 32, kShortGroups>(t, k, chunk, lane, acc); break;
+            case ARCQML_BF16: square_groups<ARCQML_BF16, 32, kShortGroups>(t, k, chunk, lane, acc); break;
+            default: square_groups<ARCQML_F16, 32, kShortGroups>(t, k, chunk, lane, acc);
             }
         }
+        n = sqrt(cluster_sum((acc[0] + acc[1]) + (acc[2] + acc[3]), cluster));
+    } else {
+        if (given) n = *given;
+        cluster.sync();
     }
+    if (warp == 0 && lane == 0) {
+        if (norm) *norm = n;
+        *step = now;
+    }
+    const bool decoupled = o.decoupled != 0;
+    const AdamScalars64 h = scalars64(o, bc[0], bc[1], clip_factor(n, o.max_norm));
+    const AdamScalars32 hf = scalars32(h);
+    for (uint32_t c = warp; c < chunks; c += warps) {
+        const uint32_t k = tensor_of(t, c), chunk = c - t.first[k];
+        if ((t.types[k] & 3) == ARCQML_F64)
+            adam_chunk<ARCQML_F64, ARCQML_F64, 32, kShortGroups>(t, k, chunk, lane, h, decoupled);
+        else adam_chunk_of<32, kShortGroups>(t, k, chunk, lane, hf, decoupled);
+    }
+    cluster.sync();
 }
 
 // ------------------------------------------------------------------ host side
@@ -512,27 +676,22 @@ bool check_tensor(const ArcqmlTensor &t, const char *list, size_t i) {
     return true;
 }
 
-void check_workspace(const double *ws, size_t len, size_t count) {
+void check_workspace(const double *ws, size_t len, size_t need) {
     if (!ws) fail("workspace is null");
     if (reinterpret_cast<uintptr_t>(ws) % 16) fail("workspace is not aligned to 16 bytes");
-    if (len < tensor_workspace(count)) {
+    if (len < need) {
         std::ostringstream m;
-        m << "workspace of " << len << " doubles is too small for " << count << " tensors: needs "
-          << tensor_workspace(count);
+        m << "workspace of " << len << " doubles is too small: the list needs " << need;
         fail(m.str());
     }
 }
 
-uint32_t blocks_for(uint64_t chunks) {
-    return uint32_t(std::max<uint64_t>(1, std::min<uint64_t>(chunks, kMaxBlocks)));
-}
-
-// Chunks of a tensor in k_square_sums and k_clip: at least one, for the elements outside vectors.
-uint64_t chunks_of(const ArcqmlTensor &t) {
+// Chunks of `per` vectors of a tensor: at least one, for the elements outside vectors.
+uint64_t chunks_of(const ArcqmlTensor &t, uint32_t per) {
     const uint32_t size = element_size(t.dtype);
     const uint64_t head = (-reinterpret_cast<uintptr_t>(t.data) & 15) / size;
     const uint64_t vectors = t.length > head ? (t.length - head) / (16 / size) : 0;
-    return std::max<uint64_t>(1, (vectors + kVectors - 1) / kVectors);
+    return std::max<uint64_t>(1, (vectors + per - 1) / per);
 }
 
 // The whole list is checked before anything is launched. Chunks are counted in 32 bits.
@@ -540,49 +699,148 @@ void check_tensors(const ArcqmlTensor *list, size_t count, const char *name) {
     if (count && !list) fail(std::string(name) + " list is null");
     uint64_t chunks = 0;
     for (size_t i = 0; i < count; ++i)
-        if (check_tensor(list[i], name, i)) chunks += list[i].length / kVectors + 1;
+        if (check_tensor(list[i], name, i)) chunks += list[i].length / kChunk + 1;
     if (chunks >> 31) fail(std::string(name) + " list holds too many elements");
 }
 
-// Calls launch(table, blocks, bytes) for every launch that the (checked) list takes.
-template <class F>
-void for_tensor_launches(const ArcqmlTensor *list, size_t count, F &&launch) {
-    TensorTable t;
+// Whether one cluster takes the list in one launch.
+bool is_short(const ArcqmlTensor *list, size_t count) {
+    uint64_t elements = 0;
+    uint32_t tensors = 0;
+    for (size_t i = 0; i < count; ++i) {
+        if (!present(list[i])) continue;
+        elements += list[i].length;
+        if (++tensors > kShortTensors || elements > kShortElements) return false;
+    }
+    return true;
+}
+
+// Fills tables with a list's (checked) tensors in chunks of `per` vectors and calls
+// launch(table, bytes) for each full one and the last.
+template <uint32_t CAP, class F>
+void for_tensor_tables(const ArcqmlTensor *list, size_t count, uint32_t per, F &&launch) {
+    TensorTable<CAP> t;
     t.count = 0;
     uint64_t chunks = 0;
     double bytes = 0.0;
-    auto flush = [&] {
-        if (!t.count) return;
+    const auto flush = [&] {
         t.first[t.count] = uint32_t(chunks);
-        launch(t, blocks_for(chunks), bytes);
+        launch(t, bytes);
         t.count = 0;
         chunks = 0;
         bytes = 0.0;
     };
     for (size_t i = 0; i < count; ++i) {
         if (!present(list[i])) continue;
-        const uint64_t n = chunks_of(list[i]);
-        if (t.count == kMaxTensors) flush();
+        if (t.count == CAP) flush();
         t.data[t.count] = list[i].data;
         t.length[t.count] = list[i].length;
         t.dtype[t.count] = uint8_t(list[i].dtype);
         t.first[t.count++] = uint32_t(chunks);
-        chunks += n;
+        chunks += chunks_of(list[i], per);
         bytes += double(list[i].length) * element_size(list[i].dtype);
     }
     flush();
 }
 
+// The same for a (checked) Adam step, over the tensors of the given class: the f64 parameters, the
+// others, or all.
+enum AdamClass { ADAM_OTHERS, ADAM_F64, ADAM_ALL };
+struct AdamLists {
+    const ArcqmlTensor *params, *grads, *m, *v, *copies;
+    size_t count;
+};
+template <uint32_t CAP, class F>
+void for_adam_tables(const AdamLists &l, AdamClass which, uint32_t per, F &&launch) {
+    AdamTable<CAP> t;
+    t.count = 0;
+    uint64_t chunks = 0;
+    double bytes = 0.0;
+    const auto flush = [&] {
+        t.first[t.count] = uint32_t(chunks);
+        launch(t, bytes);
+        t.count = 0;
+        chunks = 0;
+        bytes = 0.0;
+    };
+    // groups of 4 elements from the first place on where the parameter's start on their size
+    const auto apart = [](const ArcqmlTensor &x) {
+        return (reinterpret_cast<uintptr_t>(x.data) / element_size(x.dtype)) & 3;
+    };
+    for (size_t i = 0; i < l.count; ++i) {
+        const ArcqmlTensor &p = l.params[i], &g = l.grads[i];
+        if (!present(p) || g.dtype == ARCQML_NO_TENSOR ||
+            (which != ADAM_ALL && (p.dtype == ARCQML_F64) != (which == ADAM_F64)))
+            continue;
+        if (t.count == CAP) flush();
+        const bool copy = l.copies && l.copies[i].dtype != ARCQML_NO_TENSOR;
+        const uint64_t at = apart(p), head = std::min<uint64_t>(-at & 3, p.length);
+        const uint32_t k = t.count++;
+        t.p[k] = p.data;
+        t.g[k] = g.data;
+        t.m[k] = l.m[i].data;
+        t.v[k] = l.v[i].data;
+        t.copy[k] = copy ? l.copies[i].data : nullptr;
+        t.length[k] = p.length;
+        t.first[k] = uint32_t(chunks);
+        t.types[k] = uint8_t(p.dtype | g.dtype << 2 | (copy ? l.copies[i].dtype << 4 : 0));
+        t.aligned[k] = uint8_t((apart(g) == at ? kAlignedG : 0) |
+                               (apart(l.m[i]) == at ? kAlignedM : 0) |
+                               (apart(l.v[i]) == at ? kAlignedV : 0) |
+                               (copy && apart(l.copies[i]) == at ? kAlignedCopy : 0) |
+                               (copy ? kHasCopy : 0));
+        t.head[k] = uint8_t(head);
+        chunks += std::max<uint64_t>(1, ((p.length - head) / 4 + per - 1) / per);
+        bytes += double(p.length) *
+                 (2.0 * element_size(p.dtype) + element_size(g.dtype) +
+                  4.0 * element_size(l.m[i].dtype) +
+                  (copy ? element_size(l.copies[i].dtype) : 0.0));
+    }
+    if (t.count) flush();
+}
+
+// A launch of one cluster.
+template <auto KERNEL, class... Args>
+void launch_cluster(double bytes, cudaStream_t s, const char *what, Args... args) {
+    // above 8 blocks a cluster's size has to be allowed, once per kernel and device
+    static std::atomic<uint64_t> allowed{0};
+    int dev = 0;
+    check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
+    const uint64_t bit = uint64_t(1) << (dev & 63);
+    if (dev > 63 || !(allowed.load(std::memory_order_relaxed) & bit)) {
+        check_cuda(cudaFuncSetAttribute(reinterpret_cast<const void *>(KERNEL),
+                                        cudaFuncAttributeNonPortableClusterSizeAllowed, 1),
+                   what);
+        allowed.fetch_or(bit, std::memory_order_relaxed);
+    }
+    cudaLaunchConfig_t c{};
+    cudaLaunchAttribute a{};
+    a.id = cudaLaunchAttributeClusterDimension;
+    a.val.clusterDim.x = kCluster;
+    a.val.clusterDim.y = a.val.clusterDim.z = 1;
+    c.gridDim = dim3(kCluster);
+    c.blockDim = dim3(kShortThreads);
+    c.stream = s;
+    c.attrs = &a;
+    c.numAttrs = 1;
+    const ProfToken tok = prof_begin(PROF_OTHER, s);
+    check_cuda(cudaLaunchKernelEx(&c, KERNEL, args...), what);
+    prof_end(tok, s, bytes);
+}
+
 // Sums of squares of the list into ws; returns their count.
 uint32_t square_sums(const ArcqmlTensor *grads, size_t count, double *ws, cudaStream_t s) {
     uint32_t sums = 0;
-    for_tensor_launches(grads, count, [&](const TensorTable &t, uint32_t blocks, double bytes) {
-        const ProfToken tok = prof_begin(PROF_OTHER, s);
-        k_square_sums<<<blocks, kOT, 0, s>>>(t, ws + kScalarDoubles + sums);
-        prof_end(tok, s, bytes);
-        check_cuda(cudaGetLastError(), "gradient norm kernel launch");
-        sums += blocks;
-    });
+    for_tensor_tables<kMaxTensors>(
+        grads, count, kChunk, [&](const TensorTable<kMaxTensors> &t, double bytes) {
+            if (!t.count) return;
+            const uint32_t blocks = std::min(t.first[t.count], kMaxBlocks);
+            const ProfToken tok = prof_begin(PROF_OTHER, s);
+            k_square_sums<<<blocks, kOT, 0, s>>>(t, ws + kScalarDoubles + sums);
+            prof_end(tok, s, bytes);
+            check_cuda(cudaGetLastError(), "gradient norm kernel launch");
+            sums += blocks;
+        });
     return sums;
 }
 
@@ -597,16 +855,28 @@ Scalars *scalars(uint32_t sums, const double *given, double max_norm, int64_t *s
     return out;
 }
 
+// The norm of a short list, or its clipping (max_norm >= 0).
+void short_clip(const ArcqmlTensor *grads, size_t count, const double *given, double max_norm,
+                double *norm, cudaStream_t s) {
+    for_tensor_tables<kShortTensors>(
+        grads, count, kShortVectors, [&](const TensorTable<kShortTensors> &t, double bytes) {
+            launch_cluster<k_short_clip>(max_norm >= 0.0 ? 2.0 * bytes : bytes, s,
+                                         "gradient norm kernel launch", t, given, max_norm, norm);
+        });
+}
+
 }  // namespace
 
-size_t tensor_workspace(size_t num_tensors) {
-    return kScalarDoubles + (num_tensors / kMaxTensors + 1) * size_t(kMaxBlocks);
+size_t tensor_workspace(const ArcqmlTensor *list, size_t count) {
+    if (!list || is_short(list, count)) return 0;
+    return kScalarDoubles + (count / kMaxTensors + 1) * size_t(kMaxBlocks);
 }
 
 void gradient_norm_device(const ArcqmlTensor *grads, size_t count, double *norm, double *ws,
                           size_t ws_len, cudaStream_t s) {
     check_tensors(grads, count, "gradient");
-    check_workspace(ws, ws_len, count);
+    if (is_short(grads, count)) return short_clip(grads, count, nullptr, -1.0, norm, s);
+    check_workspace(ws, ws_len, tensor_workspace(grads, count));
     const uint32_t sums = square_sums(grads, count, ws, s);
     scalars(sums, nullptr, -1.0, nullptr, 0.0, 0.0, norm, ws, s);
 }
@@ -617,15 +887,18 @@ void clip_gradients_device(const ArcqmlTensor *grads, size_t count, double max_n
     check_tensors(grads, count, "gradient");
     if (!std::isfinite(max_norm) || max_norm < 0.0)
         fail("the maximum norm must be finite and not negative");
-    check_workspace(ws, ws_len, count);
+    if (is_short(grads, count)) return short_clip(grads, count, given, max_norm, norm, s);
+    check_workspace(ws, ws_len, tensor_workspace(grads, count));
     const uint32_t sums = given ? 0 : square_sums(grads, count, ws, s);
     const Scalars *sc = scalars(sums, given, max_norm, nullptr, 0.0, 0.0, norm, ws, s);
-    for_tensor_launches(grads, count, [&](const TensorTable &t, uint32_t blocks, double bytes) {
-        const ProfToken tok = prof_begin(PROF_OTHER, s);
-        k_clip<<<blocks, kOT, 0, s>>>(t, sc);
-        prof_end(tok, s, 2.0 * bytes);
-        check_cuda(cudaGetLastError(), "clip kernel launch");
-    });
+    for_tensor_tables<kMaxTensors>(
+        grads, count, kChunk, [&](const TensorTable<kMaxTensors> &t, double bytes) {
+            if (!t.count) return;
+            const ProfToken tok = prof_begin(PROF_OTHER, s);
+            k_clip<<<std::min(t.first[t.count], kMaxBlocks), kOT, 0, s>>>(t, sc);
+            prof_end(tok, s, 2.0 * bytes);
+            check_cuda(cudaGetLastError(), "clip kernel launch");
+        });
 }
 
 void adam_step_device(const ArcqmlTensor *params, const ArcqmlTensor *grads,
@@ -644,7 +917,8 @@ void adam_step_device(const ArcqmlTensor *params, const ArcqmlTensor *grads,
         fail("invalid Adam hyperparameters (finite lr and weight decay, 0 <= beta < 1, eps >= 0)");
     if (!std::isfinite(o.max_norm)) fail("the maximum norm must be finite");
     if (o.reserved != 0 || (o.decoupled != 0 && o.decoupled != 1)) fail("invalid Adam options");
-    check_workspace(ws, ws_len, count);
+    const bool one = is_short(params, count);
+    if (!one) check_workspace(ws, ws_len, tensor_workspace(params, count));
     for (size_t i = 0; i < count; ++i) {
         const uint32_t pt = params[i].dtype, wide = pt == ARCQML_F64 ? ARCQML_F64 : ARCQML_F32;
         const uint64_t n = params[i].length;
@@ -663,66 +937,36 @@ void adam_step_device(const ArcqmlTensor *params, const ArcqmlTensor *grads,
         if (copies[i].length != n) fail_at("copy", i, "differs in length from its parameter");
     }
     const bool clips = o.max_norm >= 0.0;
-    const uint32_t sums = clips && !given ? square_sums(grads, count, ws, s) : 0;
-    const Scalars *sc = scalars(sums, clips ? given : nullptr, clips ? o.max_norm : -1.0, step,
-                                o.beta1, o.beta2, clips ? norm : nullptr, ws, s);
-    AdamTable t;
-    t.count = 0;
-    uint64_t chunks = 0;
-    double bytes = 0.0;
-    bool f64 = false;
-    auto flush = [&] {
-        if (!t.count) return;
-        t.first[t.count] = uint32_t(chunks);
-        const ProfToken tok = prof_begin(PROF_OTHER, s);
-        if (f64) k_adam<true><<<blocks_for(chunks), kOT, 0, s>>>(t, o, sc);
-        else k_adam<false><<<blocks_for(chunks), kOT, 0, s>>>(t, o, sc);
-        prof_end(tok, s, bytes);
-        check_cuda(cudaGetLastError(), "Adam kernel launch");
-        t.count = 0;
-        chunks = 0;
-        bytes = 0.0;
-    };
-    for (size_t j = 0; j < 2 * count; ++j) {  // the others, then the f64 tensors
-        const size_t i = j < count ? j : j - count;
-        if (j == count) {
-            flush();
-            f64 = true;
-        }
-        if (!present(params[i]) || grads[i].dtype == ARCQML_NO_TENSOR ||
-            (params[i].dtype == ARCQML_F64) != f64)
-            continue;
-        if (t.count == kMaxTensors) flush();
-        const uint32_t k = t.count++;
-        const uint32_t ct = copies ? copies[i].dtype : uint32_t(ARCQML_NO_TENSOR);
-        const bool copy = ct != ARCQML_NO_TENSOR;
-        const uint64_t length = params[i].length;
-        // groups of 4 elements from the first place on where the parameter's start on their size
-        const auto apart = [&](const ArcqmlTensor &x) {
-            return (reinterpret_cast<uintptr_t>(x.data) / element_size(x.dtype)) & 3;
+    if (!clips) given = nullptr;
+    if (!clips) norm = nullptr;
+    const AdamLists lists{params, grads, m, v, copies, count};
+    if (one) {
+        bool launched = false;
+        const auto launch = [&](const AdamTable<kShortTensors> &t, double bytes) {
+            launch_cluster<k_short_adam>(bytes, s, "Adam kernel launch", t, o, step, given, norm);
+            launched = true;
         };
-        const uint64_t at = apart(params[i]), head = std::min<uint64_t>(-at & 3, length);
-        t.p[k] = params[i].data;
-        t.g[k] = grads[i].data;
-        t.m[k] = m[i].data;
-        t.v[k] = v[i].data;
-        t.copy[k] = copy ? copies[i].data : nullptr;
-        t.length[k] = length;
-        t.first[k] = uint32_t(chunks);
-        t.types[k] = uint8_t(params[i].dtype | grads[i].dtype << 2 | (copy ? ct << 4 : 0));
-        t.aligned[k] = uint8_t((apart(grads[i]) == at ? kAlignedG : 0) |
-                               (apart(m[i]) == at ? kAlignedM : 0) |
-                               (apart(v[i]) == at ? kAlignedV : 0) |
-                               (copy && apart(copies[i]) == at ? kAlignedCopy : 0) |
-                               (copy ? kHasCopy : 0));
-        t.head[k] = uint8_t(head);
-        chunks += std::max<uint64_t>(1, ((length - head) / 4 + kGroups - 1) / kGroups);
-        bytes += double(params[i].length) *
-                 (2.0 * element_size(params[i].dtype) + element_size(grads[i].dtype) +
-                  4.0 * element_size(m[i].dtype) +
-                  (ct == ARCQML_NO_TENSOR ? 0.0 : element_size(ct)));
+        for_adam_tables<kShortTensors>(lists, ADAM_ALL, kShortGroups, launch);
+        if (!launched) {  // nothing to update: the step counts all the same
+            AdamTable<kShortTensors> none;
+            none.count = none.first[0] = 0;
+            launch(none, 0.0);
+        }
+        return;
     }
-    flush();
+    const uint32_t sums = clips && !given ? square_sums(grads, count, ws, s) : 0;
+    const Scalars *sc = scalars(sums, given, clips ? o.max_norm : -1.0, step, o.beta1, o.beta2,
+                                norm, ws, s);
+    for (const AdamClass which : {ADAM_OTHERS, ADAM_F64})
+        for_adam_tables<kMaxTensors>(
+            lists, which, kChunk, [&](const AdamTable<kMaxTensors> &t, double bytes) {
+                const uint32_t blocks = std::min(t.first[t.count], kMaxBlocks);
+                const ProfToken tok = prof_begin(PROF_OTHER, s);
+                if (which == ADAM_F64) k_adam<true><<<blocks, kOT, 0, s>>>(t, o, sc);
+                else k_adam<false><<<blocks, kOT, 0, s>>>(t, o, sc);
+                prof_end(tok, s, bytes);
+                check_cuda(cudaGetLastError(), "Adam kernel launch");
+            });
 }
 
 }  // namespace arcqml

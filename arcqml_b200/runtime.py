@@ -131,7 +131,7 @@ SIGNATURES = {
     "arcqml_rt_v2_peer_buffer_close": (_I32, [_P]),
     "arcqml_rt_v2_peer_buffer_destroy": (_I32, [_P]),
     "arcqml_rt_v2_adjoint_backward": (_I32, [_P, _P, _P, _S, _S, _P, _P, _S, _P, _S, _P]),
-    "arcqml_rt_v2_gradient_workspace": (_S, [_S]),
+    "arcqml_rt_v2_gradient_workspace": (_S, [_P, _S]),
     "arcqml_rt_v2_gradient_norm": (_I32, [_P, _S, _P, _P, _S, _P]),
     "arcqml_rt_v2_clip_gradients": (_I32, [_P, _S, _D, _P, _P, _P, _S, _P]),
     "arcqml_rt_v2_adam_step": (_I32, [_P, _P, _P, _P, _P, _S, _P, _P, _P, _P, _P, _S, _P]),
@@ -661,19 +661,20 @@ class TensorList:
             raise TypeError("the tensors of a list must be on one device")
         self.device_index = devices.pop() if devices else None
         self._table, self._layouts = table, layouts
+        self._address = table.ctypes.data
+        self._words = load().arcqml_rt_v2_gradient_workspace(self._address, len(self.tensors))
         self._shapes = [None if t is None else t.shape for t in self.tensors]
         self._pointers = [t.data_ptr() for t in self._present]
         self._apart = None
 
-    def _current(self) -> int:
+    def _current(self, torch) -> int:
         """Address of the table, after a look at the tensors' addresses and the current device."""
-        import torch
         if list(map(torch.Tensor.data_ptr, self._present)) != self._pointers:
             self._write_down()
         if self.device_index is not None and self.device_index != torch.cuda.current_device():
             raise RuntimeError(f"the tensors are on cuda:{self.device_index} and the current device "
                                f"is cuda:{torch.cuda.current_device()}")
-        return self._table.ctypes.data
+        return self._address
 
     def _check_apart(self, name: str) -> None:
         """Refuses a list that is written to when two of its tensors share memory."""
@@ -682,9 +683,8 @@ class TensorList:
         if not self._apart:
             raise RuntimeError(f"{name} share memory: each may be in the list once")
 
-    def _written(self) -> None:
+    def _written(self, torch) -> None:
         """Tells autograd that the tensors changed."""
-        import torch
         torch.autograd.graph.increment_version(self._present)
 
 
@@ -700,36 +700,20 @@ def _tensor_list(tensors) -> TensorList:
     return tensors if isinstance(tensors, TensorList) else TensorList(tensors)
 
 
-class _TensorCall:
-    """Stream, scratch and norm of one call. All of it is allocated for the call alone, on its
-    stream, so calls on other streams and captured graphs share nothing."""
-
-    def __init__(self, count: int, stream, norm_wanted: bool = True):
-        import torch
-        words = load().arcqml_rt_v2_gradient_workspace(count)
-        if stream is None:
-            self.stream = torch.cuda.current_stream().cuda_stream
-            self._allocate(words, norm_wanted)
-        else:
-            self.stream = int(stream)
-            with torch.cuda.stream(torch.cuda.ExternalStream(self.stream)):
-                self._allocate(words, norm_wanted)
-
-    def _allocate(self, words: int, norm_wanted: bool) -> None:
-        import torch
-        self.words = words
-        self.workspace = torch.empty(words, dtype=torch.float64, device="cuda")
-        self.norm = torch.empty((), dtype=torch.float64, device="cuda") if norm_wanted else None
-
-    def arguments(self, given):
-        """(given norm, norm, workspace, its length, stream) as the entry points take them."""
-        return (None if given is None else _scalar_ptr(given),
-                None if self.norm is None else self.norm.data_ptr(), self.workspace.data_ptr(),
-                self.words, self.stream)
+def _call_memory(torch, stream, words: int, norm: bool):
+    """(stream, norm, scratch) of one call. All of it is allocated for the call alone, on its stream,
+    so calls on other streams and captured graphs share nothing."""
+    if stream is not None:
+        with torch.cuda.stream(torch.cuda.ExternalStream(int(stream))):
+            return (int(stream),) + _call_memory(torch, None, words, norm)[1:]
+    device = torch.cuda.current_device()
+    # the raw handle: a Stream object costs as much as the launch
+    raw = torch._C._cuda_getCurrentRawStream(device)
+    return (raw, torch.empty((), dtype=torch.float64, device=device) if norm else None,
+            torch.empty(words, dtype=torch.float64, device=device) if words else None)
 
 
-def _scalar_ptr(t) -> int:
-    import torch
+def _scalar_ptr(torch, t) -> int:
     if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == torch.float64
             and t.numel() == 1 and t.get_device() == torch.cuda.current_device()):
         raise TypeError("a given norm must be one float64 on the current CUDA device")
@@ -740,25 +724,30 @@ def gradient_norm_device(gradients, stream=None):
     """The 2-norm over every element of every tensor of `gradients` (a TensorList, or a sequence of
     CUDA tensors and None) as a float64 CUDA scalar (arcqml_rt_v2_gradient_norm). Nothing is read
     back: the norm can go into the calls below, or its square into an all-reduce."""
+    import torch
     g = _tensor_list(gradients)
-    table = g._current()
-    call = _TensorCall(len(g), stream)
-    _status(load().arcqml_rt_v2_gradient_norm(table, len(g), *call.arguments(None)[1:]))
-    return call.norm
+    table = g._current(torch)
+    on, out, ws = _call_memory(torch, stream, g._words, True)
+    _status(load().arcqml_rt_v2_gradient_norm(table, len(g), out.data_ptr(),
+                                              None if ws is None else ws.data_ptr(), g._words, on))
+    return out
 
 
 def clip_gradients_device(gradients, max_norm: float, norm=None, stream=None):
     """Scales `gradients` in place by min(1, max_norm / (n + 1e-6)) with n their global norm, or
     `norm` (a float64 CUDA scalar: over several lists, or over ranks), and returns n
     (arcqml_rt_v2_clip_gradients)."""
+    import torch
     g = _tensor_list(gradients)
-    table = g._current()
+    table = g._current(torch)
     g._check_apart("the gradients")
-    call = _TensorCall(len(g), stream)
-    _status(load().arcqml_rt_v2_clip_gradients(table, len(g), float(max_norm),
-                                               *call.arguments(norm)))
-    g._written()
-    return call.norm
+    given = None if norm is None else _scalar_ptr(torch, norm)
+    on, out, ws = _call_memory(torch, stream, g._words, True)
+    _status(load().arcqml_rt_v2_clip_gradients(table, len(g), float(max_norm), given,
+                                               out.data_ptr(),
+                                               None if ws is None else ws.data_ptr(), g._words, on))
+    g._written(torch)
+    return out
 
 
 class DeviceAdamState:
@@ -808,41 +797,47 @@ def adam_step_device(parameters, gradients, state: DeviceAdamState, lr: float = 
     (bfloat16 or float16 tensors, or None, one per parameter) receive the new values of float32
     parameters. The step count is on the device: a captured step counts on when it is replayed
     (`lr` and the other numbers stay those of the capture)."""
-    p, g = _tensor_list(parameters), _tensor_list(gradients)
+    import torch
+    p, g, m, v = _tensor_list(parameters), _tensor_list(gradients), state._m, state._v
     c = None if copies is None else _tensor_list(copies)
-    if max_norm is None and norm is not None:
-        raise ValueError("a given norm needs max_norm")
-    if max_norm is not None and not float(max_norm) >= 0.0:
-        raise ValueError("max_norm must be finite and not negative")
     if len(p._present) != len(p):
         raise TypeError("a parameter list has no empty places")
-    lists = [p, g, state._m, state._v] + ([] if c is None else [c])
-    tables = [x._current() for x in lists]
-    for name, other in (("gradients", g), ("moments", state._m), ("moments", state._v),
-                        ("copies", c)):
-        if other is None:
-            continue
-        if len(other) != len(p):
-            raise ValueError(f"{len(p)} parameters and {len(other)} {name}")
-        if other._layouts != p._layouts or other._shapes != p._shapes:
-            for i, t in enumerate(other.tensors):
-                if t is not None and (other._layouts[i] != p._layouts[i]
-                                      or other._shapes[i] != p._shapes[i]):
-                    raise ValueError(f"{name} and parameters differ in shape or strides at place {i}")
-    for name, other in (("the parameters", p), ("the moments", state._m),
-                        ("the moments", state._v), ("the copies", c)):
-        if other is not None:
-            other._check_apart(name)
-    options = AdamOptions(float(lr), float(betas[0]), float(betas[1]), float(eps),
-                          float(weight_decay), -1.0 if max_norm is None else float(max_norm),
-                          int(bool(decoupled)), 0)
-    call = _TensorCall(len(p), stream, norm_wanted=max_norm is not None)
+    if max_norm is None:
+        if norm is not None:
+            raise ValueError("a given norm needs max_norm")
+        max_norm, given = -1.0, None
+    else:
+        max_norm, given = float(max_norm), None if norm is None else _scalar_ptr(torch, norm)
+        if not max_norm >= 0.0:
+            raise ValueError("the maximum norm must be finite and not negative")
+    tables = [x._current(torch) for x in (p, g, m, v)]
+    tables.append(None if c is None else c._current(torch))
+    for name, x in (("gradients", g), ("moments", m), ("moments", v), ("copies", c)):
+        if x is not None and (x._shapes != p._shapes or x._layouts != p._layouts):
+            _check_places(name, x, p)
+    p._check_apart("the parameters")
+    m._check_apart("the moments")
+    v._check_apart("the moments")
+    if c is not None:
+        c._check_apart("the copies")
+    options = AdamOptions(lr, betas[0], betas[1], eps, weight_decay, max_norm, bool(decoupled), 0)
+    on, out, ws = _call_memory(torch, stream, p._words, max_norm >= 0.0)
     _status(load().arcqml_rt_v2_adam_step(
-        *tables[:4], None if c is None else tables[4], len(p), state.step.data_ptr(),
-        C.byref(options), *call.arguments(norm)))
-    for x in lists[:1] + lists[2:]:
-        x._written()
-    return call.norm
+        *tables, len(p), state.step.data_ptr(), C.byref(options), given,
+        None if out is None else out.data_ptr(), None if ws is None else ws.data_ptr(), p._words,
+        on))
+    for x in (p, m, v) if c is None else (p, m, v, c):
+        x._written(torch)
+    return out
+
+
+def _check_places(name: str, x: TensorList, p: TensorList) -> None:
+    """x has one place per parameter, and its tensors have the parameters' shapes and strides."""
+    if len(x) != len(p):
+        raise ValueError(f"{len(p)} parameters and {len(x)} {name}")
+    for i, t in enumerate(x.tensors):
+        if t is not None and (x._layouts[i], x._shapes[i]) != (p._layouts[i], p._shapes[i]):
+            raise ValueError(f"{name} and parameters differ in shape or strides at place {i}")
 
 
 def norms_device(state, num_qubits: int, stream=None) -> np.ndarray:

@@ -63,9 +63,13 @@ def test_malformed_lists(runtime, call):
     call.message(call.norm_of(table(runtime, (64, 1 << 41, 1, 0))), "too long")
     call.message(call.norm_of(table(runtime, *[(64, (1 << 40) - 1, 1, 0)] * 40)), "too many elements")
     call.message(call.norm_of(table(runtime, ok), norm=False), "norm pointer is null")
-    call.message(call.norm_of(table(runtime, ok), ws=False), "workspace is null")
-    need = runtime.load().arcqml_rt_v2_gradient_workspace(1)
-    call.message(call.norm_of(table(runtime, ok), words=need - 1), "too small")
+    # a list that one launch does not take needs scratch
+    for long in (table(runtime, *[ok] * 2000), table(runtime, (64, 1 << 30, 1, 0))):
+        need = runtime.load().arcqml_rt_v2_gradient_workspace(long.ctypes.data, len(long))
+        assert need > 0
+        call.message(call.norm_of(long, ws=False), "workspace is null")
+        call.message(call.norm_of(long, words=need - 1), "too small")
+    assert runtime.load().arcqml_rt_v2_gradient_workspace(table(runtime, ok).ctypes.data, 1) == 0
     call.message(call.clip(table(runtime, ok), -1.0), "finite and not negative")
     call.message(call.clip(table(runtime, ok), float("nan")), "finite and not negative")
     call.message(call.clip(table(runtime, ok), float("inf")), "finite and not negative")
