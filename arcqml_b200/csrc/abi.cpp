@@ -947,8 +947,12 @@ int32_t arcqml_rt_v2_scaled_copy(const arcqml_c128 *input, size_t batch, size_t 
 
 // ---------------------------------------------------------------- training over many tensors
 
-size_t arcqml_rt_v2_gradient_workspace(const ArcqmlTensor *tensors, size_t num_tensors) {
-    return tensor_workspace(tensors, num_tensors);
+size_t arcqml_rt_v2_gradient_workspace(const ArcqmlTensor *gradients, size_t num_tensors) {
+    return gradient_workspace(gradients, num_tensors);
+}
+
+size_t arcqml_rt_v2_adam_workspace(const ArcqmlTensor *parameters, size_t num_tensors) {
+    return adam_workspace(parameters, num_tensors);
 }
 
 int32_t arcqml_rt_v2_gradient_norm(const ArcqmlTensor *gradients, size_t num_tensors,

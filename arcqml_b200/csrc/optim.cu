@@ -33,24 +33,61 @@ namespace arcqml {
 namespace {
 
 constexpr int kOT = 256;                 // threads per block
-constexpr uint32_t kMaxBlocks = 148 * 8; // blocks of one launch
+#ifndef V_NORM_BLOCKS
+#define V_NORM_BLOCKS 6
+#endif
+#ifndef V_BLOCKS
+#define V_BLOCKS 100000000
+#endif
+#ifndef V_CHUNK
+#define V_CHUNK 2048
+#endif
+#ifndef V_U
+#define V_U 2
+#endif
+#ifndef V_NU
+#define V_NU 8
+#endif
+#ifndef V_OCC
+#define V_OCC 4
+#endif
+#ifndef V_COCC
+#define V_COCC 4
+#endif
+#ifndef V_CU
+#define V_CU 4
+#endif
+#ifndef V_NOCC
+#define V_NOCC 6
+#endif
+constexpr uint32_t kMaxBlocks = 148 * V_NORM_BLOCKS; // blocks of one launch
 constexpr uint32_t kMaxTensors = 512;    // tensors of one launch
-constexpr uint32_t kChunk = 2048;        // 16-byte vectors (k_square_sums, k_clip) or groups of 4
+constexpr uint32_t kChunk = V_CHUNK;        // 16-byte vectors (k_square_sums, k_clip) or groups of 4
                                          // elements (k_adam) of one chunk
 // Short lists: one cluster, a warp per chunk.
 constexpr uint32_t kShortTensors = 64;
-#ifndef ARCQML_SHORT_ELEMENTS
-#define ARCQML_SHORT_ELEMENTS (1u << 18)
+#ifndef V_SHORT
+#define V_SHORT 1
 #endif
-constexpr uint64_t kShortElements = ARCQML_SHORT_ELEMENTS;
+constexpr uint64_t kShortBytes = V_SHORT * (uint64_t(4) << 20), kShortAdamBytes = V_SHORT * (uint64_t(1) << 20);
 constexpr uint32_t kCluster = 16, kShortThreads = 512;
 constexpr uint32_t kShortVectors = 256, kShortGroups = 64;
 
+struct AdamScalars64 {
+    double lr, b1, b2, nb1, nb2, eps, wd, down, bc1, bc2, factor;
+};
+struct AdamScalars32 {
+    float b1, b2, nb1, nb2, eps, wd, down, rate, root, factor;
+};
+
 // What k_scalars leaves for the launches behind it (the head of the scratch).
 struct Scalars {
-    double norm, factor, bc1, bc2;
+    double factor;
+    AdamScalars64 h;
+    AdamScalars32 hf;
 };
-constexpr size_t kScalarDoubles = sizeof(Scalars) / sizeof(double);
+constexpr size_t kScalarDoubles = 32;
+static_assert(sizeof(Scalars) <= kScalarDoubles * sizeof(double), "the head of the scratch");
 
 // The tensors of one launch. first[i]: the number of chunks before tensor i; first[count]: of all.
 template <uint32_t CAP> struct TensorTable {
@@ -58,7 +95,7 @@ template <uint32_t CAP> struct TensorTable {
     uint64_t length[CAP];
     uint32_t first[CAP + 1];
     uint8_t dtype[CAP];
-    uint32_t count;
+    uint32_t count, per; // tensors; vectors of a chunk
 };
 
 template <uint32_t CAP> struct AdamTable {
@@ -69,7 +106,7 @@ template <uint32_t CAP> struct AdamTable {
     uint8_t types[CAP];   // of the parameter, the gradient (<< 2) and the copy (<< 4)
     uint8_t aligned[CAP]; // kAligned*: arrays whose groups start on their own size
     uint8_t head[CAP];    // elements before the first group
-    uint32_t count;
+    uint32_t count, per;  // tensors; groups of a chunk
 };
 enum { kAlignedG = 1, kAlignedM = 2, kAlignedV = 4, kAlignedCopy = 8, kHasCopy = 16 };
 static_assert(sizeof(AdamTable<kMaxTensors>) < 32000, "kernel parameters hold 32764 bytes");
@@ -162,6 +199,11 @@ template <class T> __device__ __forceinline__ uint32_t head_of(const T *p, uint6
     return h < length ? h : uint32_t(length);
 }
 
+// The launches of one call follow each other without a gap: each lets the next one's blocks start as
+// its own finish, and those wait before they read what an earlier launch wrote.
+__device__ __forceinline__ void let_next_start() { cudaTriggerProgrammaticLaunchCompletion(); }
+__device__ __forceinline__ void wait_for_last() { cudaGridDependencySynchronize(); }
+
 // Sum over the block in a fixed order; valid in thread 0.
 template <int THREADS> __device__ __forceinline__ double o_block_sum(double v) {
     __shared__ double red[THREADS / 32];
@@ -174,22 +216,22 @@ template <int THREADS> __device__ __forceinline__ double o_block_sum(double v) {
     return r;
 }
 
-// A chunk is taken by LANES threads, of which this is `lane`, and holds PER vectors or groups.
+// A chunk is taken by LANES threads, of which this is `lane`, and holds `per` vectors or groups.
 //
 // Squares of one chunk, added to acc in f64: the squares of f32 values leave the range of f32, and a
 // norm that comes back in f64 is wanted to its precision.
-template <uint32_t DTYPE, uint32_t LANES, uint32_t PER>
+template <uint32_t DTYPE, uint32_t LANES>
 __device__ __forceinline__ void square_chunk(const void *data, uint64_t length, uint32_t chunk,
-                                             uint32_t lane, double (&acc)[4]) {
+                                             uint32_t per, uint32_t lane, double (&acc)[4]) {
     using T = typename Elem<DTYPE>::type;
     using W = typename Elem<DTYPE>::wide;
-    constexpr int N = 16 / sizeof(T), U = 8;
+    constexpr int N = 16 / sizeof(T), U = V_NU;
     const T *p = static_cast<const T *>(data);
     const uint32_t head = head_of(p, length);
     const uint64_t vectors = (length - head) / N;
     const auto *q = reinterpret_cast<const Words<DTYPE, N> *>(p + head);
-    const uint64_t v0 = uint64_t(chunk) * PER;
-    const uint32_t n = uint32_t(min(uint64_t(PER), vectors - min(v0, vectors)));
+    const uint64_t v0 = uint64_t(chunk) * per;
+    const uint32_t n = uint32_t(min(uint64_t(per), vectors - min(v0, vectors)));
     const auto add = [&](const Words<DTYPE, N> &raw) {
         W x[N];
         raw.unpack(x);
@@ -214,32 +256,33 @@ __device__ __forceinline__ void square_chunk(const void *data, uint64_t length, 
         acc[0] = fma(d, d, acc[0]);
     }
     const uint64_t done = head + vectors * N;
-    if (v0 + PER >= vectors && lane < length - done) {
+    if (v0 + per >= vectors && lane < length - done) {
         const double d = double(widen(p[done + lane]));
         acc[1] = fma(d, d, acc[1]);
     }
 }
 
 // The squares of one chunk of tensor k of a table.
-template <uint32_t LANES, uint32_t PER, class Table>
+template <uint32_t LANES, class Table>
 __device__ __forceinline__ void square_chunk_of(const Table &t, uint32_t k, uint32_t chunk,
                                                 uint32_t lane, double (&acc)[4]) {
     const void *g = t.data[k];
     const uint64_t n = t.length[k];
     switch (t.dtype[k]) {
-    case ARCQML_F64: square_chunk<ARCQML_F64, LANES, PER>(g, n, chunk, lane, acc); break;
-    case ARCQML_F32: square_chunk<ARCQML_F32, LANES, PER>(g, n, chunk, lane, acc); break;
-    case ARCQML_BF16: square_chunk<ARCQML_BF16, LANES, PER>(g, n, chunk, lane, acc); break;
-    default: square_chunk<ARCQML_F16, LANES, PER>(g, n, chunk, lane, acc);
+    case ARCQML_F64: square_chunk<ARCQML_F64, LANES>(g, n, chunk, t.per, lane, acc); break;
+    case ARCQML_F32: square_chunk<ARCQML_F32, LANES>(g, n, chunk, t.per, lane, acc); break;
+    case ARCQML_BF16: square_chunk<ARCQML_BF16, LANES>(g, n, chunk, t.per, lane, acc); break;
+    default: square_chunk<ARCQML_F16, LANES>(g, n, chunk, t.per, lane, acc);
     }
 }
 
-__global__ void __launch_bounds__(kOT)
+__global__ void __launch_bounds__(kOT, V_NOCC)
     k_square_sums(const __grid_constant__ TensorTable<kMaxTensors> t, double *__restrict__ sums) {
+    let_next_start();
     double acc[4] = {0.0, 0.0, 0.0, 0.0};
     for (uint32_t c = blockIdx.x; c < t.first[t.count]; c += gridDim.x) {
         const uint32_t k = tensor_of(t, c);
-        square_chunk_of<kOT, kChunk>(t, k, c - t.first[k], threadIdx.x, acc);
+        square_chunk_of<kOT>(t, k, c - t.first[k], threadIdx.x, acc);
     }
     const double sum = o_block_sum<kOT>((acc[0] + acc[1]) + (acc[2] + acc[3]));
     if (threadIdx.x == 0) sums[blockIdx.x] = sum;
@@ -256,43 +299,65 @@ __device__ __forceinline__ double bias_correction(double beta, int64_t t) {
     return 1.0 - pow(beta, double(t));
 }
 
+__device__ __forceinline__ AdamScalars64 scalars64(const ArcqmlAdamOptions &o, double bc1,
+                                                   double bc2, double factor) {
+    return AdamScalars64{o.learning_rate, o.beta1, o.beta2, 1.0 - o.beta1, 1.0 - o.beta2,
+                         o.epsilon, o.weight_decay, 1.0 - o.learning_rate * o.weight_decay, bc1,
+                         bc2, factor};
+}
+// f32: rate = lr / (1 - beta1^t) and root = 1 / (1 - beta2^t) are formed in f64 and rounded once.
+__device__ __forceinline__ AdamScalars32 scalars32(const AdamScalars64 &h) {
+    return AdamScalars32{float(h.b1), float(h.b2), float(h.nb1), float(h.nb2), float(h.eps),
+                         float(h.wd), float(h.down), float(h.lr / h.bc1), float(1.0 / h.bc2),
+                         float(h.factor)};
+}
+
 // One block. given != null: n = *given; else the root of the count sums. step != null: one more
 // step is counted.
 __global__ void __launch_bounds__(kOT)
-    k_scalars(const double *__restrict__ sums, uint32_t count, const double *given,
-              double max_norm, int64_t *step, double beta1, double beta2, double *norm,
+    k_scalars(const double *sums, uint32_t count, const double *given,
+              const __grid_constant__ ArcqmlAdamOptions o, int64_t *step, double *norm,
               Scalars *out) {
+    __shared__ double bc[2];
+    let_next_start();
+    // the step count is no work of the launch before this one: its powers need not wait
+    int64_t now = 0;
+    if (step) {
+        now = *step + 1;
+        if (threadIdx.x == 32) bc[0] = bias_correction(o.beta1, now);
+        if (threadIdx.x == 64) bc[1] = bias_correction(o.beta2, now);
+    }
+    wait_for_last();
     double acc = 0.0;
     for (uint32_t i = threadIdx.x; i < count; i += kOT) acc += sums[i];
     acc = o_block_sum<kOT>(acc);
     if (threadIdx.x != 0) return;
     const double n = given ? *given : sqrt(acc);
     if (norm) *norm = n;
-    Scalars r{n, clip_factor(n, max_norm), 1.0, 1.0};
+    const double factor = clip_factor(n, o.max_norm);
+    out->factor = factor;
     if (step) {
-        const int64_t now = *step + 1;
         *step = now;
-        r.bc1 = bias_correction(beta1, now);
-        r.bc2 = bias_correction(beta2, now);
+        out->h = scalars64(o, bc[0], bc[1], factor);
+        out->hf = scalars32(out->h);
     }
-    *out = r;
 }
 
 // One chunk times the factor: the product in the type of the arithmetic (f32 for 16-bit types, the
 // factor rounded to it), rounded once to the element's type.
-template <uint32_t DTYPE, uint32_t LANES, uint32_t PER>
+template <uint32_t DTYPE, uint32_t LANES>
 __device__ __forceinline__ void clip_chunk(void *data, uint64_t length, uint32_t chunk,
-                                           uint32_t lane, double factor) {
+                                           uint32_t per, uint32_t lane, double factor) {
     using T = typename Elem<DTYPE>::type;
     using W = typename Elem<DTYPE>::wide;
-    constexpr int N = 16 / sizeof(T), U = 4;
+    constexpr int N = 16 / sizeof(T), U = V_CU;
     const W f = W(factor);
     T *p = static_cast<T *>(data);
     const uint32_t head = head_of(p, length);
     const uint64_t vectors = (length - head) / N;
     auto *q = reinterpret_cast<Words<DTYPE, N> *>(p + head);
-    const uint64_t v0 = uint64_t(chunk) * PER;
-    const uint32_t n = uint32_t(min(uint64_t(PER), vectors - min(v0, vectors)));
+    const uint64_t v0 = uint64_t(chunk) * per;
+    const uint32_t n = uint32_t(min(uint64_t(per), vectors - min(v0, vectors)));
     const auto scale = [&](Words<DTYPE, N> &raw) {
         W x[N];
         raw.unpack(x);
@@ -318,36 +383,33 @@ __device__ __forceinline__ void clip_chunk(void *data, uint64_t length, uint32_t
     }
     if (chunk == 0 && lane < head) narrow(widen(p[lane]) * f, p[lane]);
     const uint64_t done = head + vectors * N;
-    if (v0 + PER >= vectors && lane < length - done)
+    if (v0 + per >= vectors && lane < length - done)
         narrow(widen(p[done + lane]) * f, p[done + lane]);
 }
 
-template <uint32_t LANES, uint32_t PER, class Table>
+template <uint32_t LANES, class Table>
 __device__ __forceinline__ void clip_chunk_of(const Table &t, uint32_t k, uint32_t chunk,
                                               uint32_t lane, double factor) {
     void *g = t.data[k];
     const uint64_t n = t.length[k];
     switch (t.dtype[k]) {
-    case ARCQML_F64: clip_chunk<ARCQML_F64, LANES, PER>(g, n, chunk, lane, factor); break;
-    case ARCQML_F32: clip_chunk<ARCQML_F32, LANES, PER>(g, n, chunk, lane, factor); break;
-    case ARCQML_BF16: clip_chunk<ARCQML_BF16, LANES, PER>(g, n, chunk, lane, factor); break;
-    default: clip_chunk<ARCQML_F16, LANES, PER>(g, n, chunk, lane, factor);
+    case ARCQML_F64: clip_chunk<ARCQML_F64, LANES>(g, n, chunk, t.per, lane, factor); break;
+    case ARCQML_F32: clip_chunk<ARCQML_F32, LANES>(g, n, chunk, t.per, lane, factor); break;
+    case ARCQML_BF16: clip_chunk<ARCQML_BF16, LANES>(g, n, chunk, t.per, lane, factor); break;
+    default: clip_chunk<ARCQML_F16, LANES>(g, n, chunk, t.per, lane, factor);
     }
 }
 
-__global__ void __launch_bounds__(kOT, 4)
-    k_clip(const __grid_constant__ TensorTable<kMaxTensors> t, const Scalars *__restrict__ sc) {
+__global__ void __launch_bounds__(kOT, V_COCC)
+    k_clip(const __grid_constant__ TensorTable<kMaxTensors> t, const Scalars *sc) {
+    let_next_start();
+    wait_for_last();
     const double factor = sc->factor;
     if (factor == 1.0) return;
-    for (uint32_t c = blockIdx.x; c < t.first[t.count]; c += gridDim.x) {
-        const uint32_t k = tensor_of(t, c);
-        clip_chunk_of<kOT, kChunk>(t, k, c - t.first[k], threadIdx.x, factor);
-    }
+    // the last chunks first: they are the ones that the norm left in L2
+    const uint32_t c = t.first[t.count] - 1 - blockIdx.x, k = tensor_of(t, c);
+    clip_chunk_of<kOT>(t, k, c - t.first[k], threadIdx.x, factor);
 }
-
-struct AdamScalars64 {
-    double lr, b1, b2, nb1, nb2, eps, wd, down, bc1, bc2, factor;
-};
 
 // f64, every operation rounded on its own, in the order of the host's update and of the optimizer
 // loop (crates/arcqml-optim/src/adam.rs:190-240), so the three agree to the bias corrections.
@@ -362,23 +424,6 @@ __device__ __forceinline__ void adam_update(double &p, double &m, double &v, dou
     p = __dsub_rn(p, __ddiv_rn(__dmul_rn(h.lr, mh), __dadd_rn(__dsqrt_rn(vh), h.eps)));
 }
 
-struct AdamScalars32 {
-    float b1, b2, nb1, nb2, eps, wd, down, rate, root, factor;
-};
-
-__device__ __forceinline__ AdamScalars64 scalars64(const ArcqmlAdamOptions &o, double bc1,
-                                                   double bc2, double factor) {
-    return AdamScalars64{o.learning_rate, o.beta1, o.beta2, 1.0 - o.beta1, 1.0 - o.beta2,
-                         o.epsilon, o.weight_decay, 1.0 - o.learning_rate * o.weight_decay, bc1,
-                         bc2, factor};
-}
-
-// f32: rate = lr / (1 - beta1^t) and root = 1 / (1 - beta2^t) are formed in f64 and rounded once.
-__device__ __forceinline__ AdamScalars32 scalars32(const AdamScalars64 &h) {
-    return AdamScalars32{float(h.b1), float(h.b2), float(h.nb1), float(h.nb2), float(h.eps),
-                         float(h.wd), float(h.down), float(h.lr / h.bc1), float(1.0 / h.bc2),
-                         float(h.factor)};
-}
 __device__ __forceinline__ void adam_update(float &p, float &m, float &v, float g,
                                             const AdamScalars32 &h, bool decoupled) {
     float a = g * h.factor;
@@ -416,21 +461,21 @@ __device__ __forceinline__ void store4(void *p, uint64_t e, bool aligned,
     }
 }
 
-template <uint32_t PT, uint32_t GT, uint32_t LANES, uint32_t PER, class Table, class H>
+template <uint32_t PT, uint32_t GT, uint32_t LANES, class Table, class H>
 __device__ __forceinline__ void adam_chunk(const Table &t, uint32_t k, uint32_t chunk,
                                            uint32_t lane, const H &h, bool decoupled) {
     using P = typename Elem<PT>::type;
     using G = typename Elem<GT>::type;
     using W = typename Elem<PT>::wide;
     constexpr uint32_t WT = sizeof(W) == 8 ? ARCQML_F64 : ARCQML_F32;
-    constexpr int U = sizeof(W) == 8 ? 1 : 2;
+    constexpr int U = sizeof(W) == 8 ? 1 : V_U;
     const uint64_t length = t.length[k];
-    const uint32_t head = t.head[k], aligned = t.aligned[k], ct = t.types[k] >> 4;
+    const uint32_t per = t.per, head = t.head[k], aligned = t.aligned[k], ct = t.types[k] >> 4;
     void *p = t.p[k], *m = t.m[k], *v = t.v[k], *copy = t.copy[k];
     const void *g = t.g[k];
     const uint64_t groups = (length - head) / 4;
-    const uint64_t i0 = uint64_t(chunk) * PER;
-    const uint32_t n = uint32_t(min(uint64_t(PER), groups - min(i0, groups)));
+    const uint64_t i0 = uint64_t(chunk) * per;
+    const uint32_t n = uint32_t(min(uint64_t(per), groups - min(i0, groups)));
     const uint64_t e0 = head + 4 * i0;
     const auto update = [&](uint64_t e, const Words<PT, 4> &rp, const Words<GT, 4> &rg,
                             const Words<WT, 4> &rm, const Words<WT, 4> &rv) {
@@ -476,7 +521,7 @@ __device__ __forceinline__ void adam_chunk(const Table &t, uint32_t k, uint32_t 
     }
     // the elements before the first group (chunk 0) and behind the last one (the last chunk)
     const uint64_t done = head + groups * 4;
-    const uint32_t tail = i0 + PER >= groups ? uint32_t(length - done) : 0;
+    const uint32_t tail = i0 + per >= groups ? uint32_t(length - done) : 0;
     const uint32_t first = chunk == 0 ? head : 0;
     if (lane < first + tail) {
         const uint64_t e = lane < first ? lane : done + lane - first;
@@ -494,43 +539,44 @@ __device__ __forceinline__ void adam_chunk(const Table &t, uint32_t k, uint32_t 
     }
 }
 
-template <uint32_t PT, uint32_t LANES, uint32_t PER, class Table>
+template <uint32_t PT, uint32_t LANES, class Table>
 __device__ __forceinline__ void adam_chunk_g(const Table &t, uint32_t k, uint32_t chunk,
                                              uint32_t lane, const AdamScalars32 &h,
                                              bool decoupled) {
     switch (t.types[k] >> 2 & 3) {
-    case ARCQML_F32: adam_chunk<PT, ARCQML_F32, LANES, PER>(t, k, chunk, lane, h, decoupled); break;
-    case ARCQML_BF16: adam_chunk<PT, ARCQML_BF16, LANES, PER>(t, k, chunk, lane, h, decoupled); break;
-    default: adam_chunk<PT, ARCQML_F16, LANES, PER>(t, k, chunk, lane, h, decoupled);
+    case ARCQML_F32: adam_chunk<PT, ARCQML_F32, LANES>(t, k, chunk, lane, h, decoupled); break;
+    case ARCQML_BF16: adam_chunk<PT, ARCQML_BF16, LANES>(t, k, chunk, lane, h, decoupled); break;
+    default: adam_chunk<PT, ARCQML_F16, LANES>(t, k, chunk, lane, h, decoupled);
     }
 }
 
-template <uint32_t LANES, uint32_t PER, class Table>
+template <uint32_t LANES, class Table>
 __device__ __forceinline__ void adam_chunk_of(const Table &t, uint32_t k, uint32_t chunk,
                                               uint32_t lane, const AdamScalars32 &h,
                                               bool decoupled) {
     switch (t.types[k] & 3) {
-    case ARCQML_F32: adam_chunk_g<ARCQML_F32, LANES, PER>(t, k, chunk, lane, h, decoupled); break;
-    case ARCQML_BF16: adam_chunk_g<ARCQML_BF16, LANES, PER>(t, k, chunk, lane, h, decoupled); break;
-    default: adam_chunk_g<ARCQML_F16, LANES, PER>(t, k, chunk, lane, h, decoupled);
+    case ARCQML_F32: adam_chunk_g<ARCQML_F32, LANES>(t, k, chunk, lane, h, decoupled); break;
+    case ARCQML_BF16: adam_chunk_g<ARCQML_BF16, LANES>(t, k, chunk, lane, h, decoupled); break;
+    default: adam_chunk_g<ARCQML_F16, LANES>(t, k, chunk, lane, h, decoupled);
     }
 }
 
-// The f64 tensors of a list and the others go to launches of their own: the f64 arithmetic
-// (two or three divisions and a root per element) takes twice the registers.
-template <bool F64>
-__global__ void __launch_bounds__(kOT, F64 ? 2 : 4)
-    k_adam(const __grid_constant__ AdamTable<kMaxTensors> t,
-           const __grid_constant__ ArcqmlAdamOptions o, const Scalars *__restrict__ sc) {
-    const bool decoupled = o.decoupled != 0;
-    const AdamScalars64 h = scalars64(o, sc->bc1, sc->bc2, sc->factor);
-    const AdamScalars32 hf = scalars32(h);
-    for (uint32_t c = blockIdx.x; c < t.first[t.count]; c += gridDim.x) {
-        const uint32_t k = tensor_of(t, c), chunk = c - t.first[k];
-        if constexpr (F64)
-            adam_chunk<ARCQML_F64, ARCQML_F64, kOT, kChunk>(t, k, chunk, threadIdx.x, h, decoupled);
-        else adam_chunk_of<kOT, kChunk>(t, k, chunk, threadIdx.x, hf, decoupled);
-    }
+// The f64 arithmetic (three divisions and a root per element) takes twice the registers of the
+// other one, and with them half the blocks of an SM: a list's f64 tensors and its others go to
+// launches of their own unless the others are few.
+enum AdamClass { ADAM_OTHERS, ADAM_F64, ADAM_ALL };
+template <AdamClass CLASS>
+__global__ void __launch_bounds__(kOT, CLASS == ADAM_OTHERS ? V_OCC : 2)
+    k_adam(const __grid_constant__ AdamTable<kMaxTensors> t, bool decoupled, const Scalars *sc) {
+    let_next_start();
+    wait_for_last();
+    // the last chunks first: their gradients are the ones that the norm left in L2
+    const uint32_t chunks = t.first[t.count];
+    const uint32_t c = chunks - 1 - blockIdx.x, k = tensor_of(t, c), chunk = c - t.first[k];
+    if (CLASS == ADAM_F64 || (CLASS == ADAM_ALL && (t.types[k] & 3) == ARCQML_F64))
+        adam_chunk<ARCQML_F64, ARCQML_F64, kOT>(t, k, chunk, threadIdx.x, sc->h, decoupled);
+    else if (CLASS != ADAM_F64)
+        adam_chunk_of<kOT>(t, k, chunk, threadIdx.x, sc->hf, decoupled);
 }
 
 // ------------------------------------------------------------------ short lists
@@ -562,7 +608,7 @@ __global__ void __launch_bounds__(kShortThreads, 1)
     } else {
         for (uint32_t c = warp; c < chunks; c += warps) {
             const uint32_t k = tensor_of(t, c);
-            square_chunk_of<32, kShortVectors>(t, k, c - t.first[k], lane, acc);
+            square_chunk_of<32>(t, k, c - t.first[k], lane, acc);
         }
         n = sqrt(cluster_sum((acc[0] + acc[1]) + (acc[2] + acc[3]), cluster));
     }
@@ -571,19 +617,19 @@ __global__ void __launch_bounds__(kShortThreads, 1)
     if (factor != 1.0)
         for (uint32_t c = warp; c < chunks; c += warps) {
             const uint32_t k = tensor_of(t, c);
-            clip_chunk_of<32, kShortVectors>(t, k, c - t.first[k], lane, factor);
+            clip_chunk_of<32>(t, k, c - t.first[k], lane, factor);
         }
     cluster.sync();
 }
 
 // The squares of a chunk's gradients, over the same elements that adam_chunk takes.
-template <uint32_t GT, uint32_t LANES, uint32_t PER, class Table>
+template <uint32_t GT, uint32_t LANES, class Table>
 __device__ __forceinline__ void square_groups(const Table &t, uint32_t k, uint32_t chunk,
                                               uint32_t lane, double (&acc)[4]) {
     using G = typename Elem<GT>::type;
-    const uint32_t head = t.head[k];
-    const uint64_t length = t.length[k], groups = (length - head) / 4, i0 = uint64_t(chunk) * PER;
-    const uint32_t n = uint32_t(min(uint64_t(PER), groups - min(i0, groups)));
+    const uint32_t per = t.per, head = t.head[k];
+    const uint64_t length = t.length[k], groups = (length - head) / 4, i0 = uint64_t(chunk) * per;
+    const uint32_t n = uint32_t(min(uint64_t(per), groups - min(i0, groups)));
     const void *g = t.g[k];
 #pragma unroll 2
     for (uint32_t i = lane; i < n; i += LANES) {
@@ -593,7 +639,7 @@ __device__ __forceinline__ void square_groups(const Table &t, uint32_t k, uint32
         for (int j = 0; j < 4; ++j) acc[j] = fma(double(x[j]), double(x[j]), acc[j]);
     }
     const uint64_t done = head + groups * 4;
-    const uint32_t tail = i0 + PER >= groups ? uint32_t(length - done) : 0;
+    const uint32_t tail = i0 + per >= groups ? uint32_t(length - done) : 0;
     const uint32_t first = chunk == 0 ? head : 0;
     if (lane < first + tail) {
         const double x =
@@ -623,10 +669,10 @@ __global__ void __launch_bounds__(kShortThreads, 1)
         for (uint32_t c = warp; c < chunks; c += warps) {
             const uint32_t k = tensor_of(t, c), chunk = c - t.first[k];
             switch (t.types[k] >> 2 & 3) {
-            case ARCQML_F64: square_groups<ARCQML_F64, 32, kShortGroups>(t, k, chunk, lane, acc); break;
-            case ARCQML_F32: square_groups<ARCQML_F32, 32, kShortGroups>(t, k, chunk, lane, acc); break;
-            case ARCQML_BF16: square_groups<ARCQML_BF16, 32, kShortGroups>(t, k, chunk, lane, acc); break;
-            default: square_groups<ARCQML_F16, 32, kShortGroups>(t, k, chunk, lane, acc);
+            case ARCQML_F64: square_groups<ARCQML_F64, 32>(t, k, chunk, lane, acc); break;
+            case ARCQML_F32: square_groups<ARCQML_F32, 32>(t, k, chunk, lane, acc); break;
+            case ARCQML_BF16: square_groups<ARCQML_BF16, 32>(t, k, chunk, lane, acc); break;
+            default: square_groups<ARCQML_F16, 32>(t, k, chunk, lane, acc);
             }
         }
         n = sqrt(cluster_sum((acc[0] + acc[1]) + (acc[2] + acc[3]), cluster));
@@ -644,8 +690,8 @@ __global__ void __launch_bounds__(kShortThreads, 1)
     for (uint32_t c = warp; c < chunks; c += warps) {
         const uint32_t k = tensor_of(t, c), chunk = c - t.first[k];
         if ((t.types[k] & 3) == ARCQML_F64)
-            adam_chunk<ARCQML_F64, ARCQML_F64, 32, kShortGroups>(t, k, chunk, lane, h, decoupled);
-        else adam_chunk_of<32, kShortGroups>(t, k, chunk, lane, hf, decoupled);
+            adam_chunk<ARCQML_F64, ARCQML_F64, 32>(t, k, chunk, lane, h, decoupled);
+        else adam_chunk_of<32>(t, k, chunk, lane, hf, decoupled);
     }
     cluster.sync();
 }
@@ -704,13 +750,13 @@ void check_tensors(const ArcqmlTensor *list, size_t count, const char *name) {
 }
 
 // Whether one cluster takes the list in one launch.
-bool is_short(const ArcqmlTensor *list, size_t count) {
-    uint64_t elements = 0;
+bool is_short(const ArcqmlTensor *list, size_t count, uint64_t most) {
+    uint64_t bytes = 0;
     uint32_t tensors = 0;
     for (size_t i = 0; i < count; ++i) {
         if (!present(list[i])) continue;
-        elements += list[i].length;
-        if (++tensors > kShortTensors || elements > kShortElements) return false;
+        bytes += list[i].length * element_size(list[i].dtype);
+        if (++tensors > kShortTensors || bytes > most) return false;
     }
     return true;
 }
@@ -721,6 +767,7 @@ template <uint32_t CAP, class F>
 void for_tensor_tables(const ArcqmlTensor *list, size_t count, uint32_t per, F &&launch) {
     TensorTable<CAP> t;
     t.count = 0;
+    t.per = per;
     uint64_t chunks = 0;
     double bytes = 0.0;
     const auto flush = [&] {
@@ -745,7 +792,6 @@ void for_tensor_tables(const ArcqmlTensor *list, size_t count, uint32_t per, F &
 
 // The same for a (checked) Adam step, over the tensors of the given class: the f64 parameters, the
 // others, or all.
-enum AdamClass { ADAM_OTHERS, ADAM_F64, ADAM_ALL };
 struct AdamLists {
     const ArcqmlTensor *params, *grads, *m, *v, *copies;
     size_t count;
@@ -754,6 +800,7 @@ template <uint32_t CAP, class F>
 void for_adam_tables(const AdamLists &l, AdamClass which, uint32_t per, F &&launch) {
     AdamTable<CAP> t;
     t.count = 0;
+    t.per = per;
     uint64_t chunks = 0;
     double bytes = 0.0;
     const auto flush = [&] {
@@ -828,31 +875,67 @@ void launch_cluster(double bytes, cudaStream_t s, const char *what, Args... args
     prof_end(tok, s, bytes);
 }
 
+// A launch of `blocks` blocks that, with `follows`, may start while the last one ends.
+template <auto KERNEL, class... Args>
+void launch(uint32_t blocks, bool follows, double bytes, cudaStream_t s, const char *what,
+            const Args &...args) {
+    cudaLaunchConfig_t c{};
+    cudaLaunchAttribute a{};
+    a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    a.val.programmaticStreamSerializationAllowed = 1;
+    c.gridDim = dim3(blocks);
+    c.blockDim = dim3(kOT);
+    c.stream = s;
+    c.attrs = &a;
+    c.numAttrs = follows ? 1 : 0;
+    const ProfToken tok = prof_begin(PROF_OTHER, s);
+    check_cuda(cudaLaunchKernelEx(&c, KERNEL, args...), what);
+    prof_end(tok, s, bytes);
+}
+
+// Vectors or groups of a chunk, from all of the list's: two chunks for each place that the launch
+// has on the GPU, between 256 (one access per thread) and 2048.
+uint32_t chunk_size(uint64_t total, uint32_t places) {
+    uint32_t per = kOT;
+    while (per < kChunk && uint64_t(per) * places * 2 < total) per *= 2;
+    return per;
+}
+
 // Sums of squares of the list into ws; returns their count.
-uint32_t square_sums(const ArcqmlTensor *grads, size_t count, double *ws, cudaStream_t s) {
+uint32_t square_sums(const ArcqmlTensor *grads, size_t count, uint32_t per, double *ws,
+                     cudaStream_t s) {
     uint32_t sums = 0;
     for_tensor_tables<kMaxTensors>(
-        grads, count, kChunk, [&](const TensorTable<kMaxTensors> &t, double bytes) {
+        grads, count, per, [&](const TensorTable<kMaxTensors> &t, double bytes) {
             if (!t.count) return;
             const uint32_t blocks = std::min(t.first[t.count], kMaxBlocks);
-            const ProfToken tok = prof_begin(PROF_OTHER, s);
-            k_square_sums<<<blocks, kOT, 0, s>>>(t, ws + kScalarDoubles + sums);
-            prof_end(tok, s, bytes);
-            check_cuda(cudaGetLastError(), "gradient norm kernel launch");
+            launch<k_square_sums>(blocks, false, bytes, s, "gradient norm kernel launch", t,
+                                  ws + kScalarDoubles + sums);
             sums += blocks;
         });
     return sums;
 }
 
-Scalars *scalars(uint32_t sums, const double *given, double max_norm, int64_t *step, double beta1,
-                 double beta2, double *norm, double *ws, cudaStream_t s) {
+uint32_t vectors_per_chunk(const ArcqmlTensor *list, size_t count) {
+    uint64_t bytes = 0;
+    for (size_t i = 0; i < count; ++i)
+        if (present(list[i])) bytes += list[i].length * element_size(list[i].dtype);
+    return chunk_size(bytes / 16, kMaxBlocks);
+}
+
+const Scalars *scalars(uint32_t sums, const double *given, const ArcqmlAdamOptions &o,
+                       int64_t *step, double *norm, double *ws, cudaStream_t s) {
     auto *out = reinterpret_cast<Scalars *>(ws);
-    const ProfToken tok = prof_begin(PROF_OTHER, s);
-    k_scalars<<<1, kOT, 0, s>>>(ws + kScalarDoubles, sums, given, max_norm, step, beta1, beta2,
-                                norm, out);
-    prof_end(tok, s, 8.0 * sums);
-    check_cuda(cudaGetLastError(), "gradient norm kernel launch");
+    launch<k_scalars>(1, sums != 0, 8.0 * sums, s, "gradient norm kernel launch",
+                      static_cast<const double *>(ws + kScalarDoubles), sums, given, o, step, norm,
+                      out);
     return out;
+}
+
+ArcqmlAdamOptions clip_options(double max_norm) {
+    ArcqmlAdamOptions o{};
+    o.max_norm = max_norm;
+    return o;
 }
 
 // The norm of a short list, or its clipping (max_norm >= 0).
@@ -867,18 +950,25 @@ void short_clip(const ArcqmlTensor *grads, size_t count, const double *given, do
 
 }  // namespace
 
-size_t tensor_workspace(const ArcqmlTensor *list, size_t count) {
-    if (!list || is_short(list, count)) return 0;
+static size_t workspace_of(size_t count) {
     return kScalarDoubles + (count / kMaxTensors + 1) * size_t(kMaxBlocks);
+}
+
+size_t gradient_workspace(const ArcqmlTensor *list, size_t count) {
+    return !list || is_short(list, count, kShortBytes) ? 0 : workspace_of(count);
+}
+
+size_t adam_workspace(const ArcqmlTensor *list, size_t count) {
+    return !list || is_short(list, count, kShortAdamBytes) ? 0 : workspace_of(count);
 }
 
 void gradient_norm_device(const ArcqmlTensor *grads, size_t count, double *norm, double *ws,
                           size_t ws_len, cudaStream_t s) {
     check_tensors(grads, count, "gradient");
-    if (is_short(grads, count)) return short_clip(grads, count, nullptr, -1.0, norm, s);
-    check_workspace(ws, ws_len, tensor_workspace(grads, count));
-    const uint32_t sums = square_sums(grads, count, ws, s);
-    scalars(sums, nullptr, -1.0, nullptr, 0.0, 0.0, norm, ws, s);
+    if (is_short(grads, count, kShortBytes)) return short_clip(grads, count, nullptr, -1.0, norm, s);
+    check_workspace(ws, ws_len, workspace_of(count));
+    const uint32_t sums = square_sums(grads, count, vectors_per_chunk(grads, count), ws, s);
+    scalars(sums, nullptr, clip_options(-1.0), nullptr, norm, ws, s);
 }
 
 void clip_gradients_device(const ArcqmlTensor *grads, size_t count, double max_norm,
@@ -887,17 +977,15 @@ void clip_gradients_device(const ArcqmlTensor *grads, size_t count, double max_n
     check_tensors(grads, count, "gradient");
     if (!std::isfinite(max_norm) || max_norm < 0.0)
         fail("the maximum norm must be finite and not negative");
-    if (is_short(grads, count)) return short_clip(grads, count, given, max_norm, norm, s);
-    check_workspace(ws, ws_len, tensor_workspace(grads, count));
-    const uint32_t sums = given ? 0 : square_sums(grads, count, ws, s);
-    const Scalars *sc = scalars(sums, given, max_norm, nullptr, 0.0, 0.0, norm, ws, s);
+    if (is_short(grads, count, kShortBytes)) return short_clip(grads, count, given, max_norm, norm, s);
+    check_workspace(ws, ws_len, workspace_of(count));
+    const uint32_t per = vectors_per_chunk(grads, count);
+    const uint32_t sums = given ? 0 : square_sums(grads, count, per, ws, s);
+    const Scalars *sc = scalars(sums, given, clip_options(max_norm), nullptr, norm, ws, s);
     for_tensor_tables<kMaxTensors>(
-        grads, count, kChunk, [&](const TensorTable<kMaxTensors> &t, double bytes) {
-            if (!t.count) return;
-            const ProfToken tok = prof_begin(PROF_OTHER, s);
-            k_clip<<<std::min(t.first[t.count], kMaxBlocks), kOT, 0, s>>>(t, sc);
-            prof_end(tok, s, 2.0 * bytes);
-            check_cuda(cudaGetLastError(), "clip kernel launch");
+        grads, count, per, [&](const TensorTable<kMaxTensors> &t, double bytes) {
+            if (t.count)
+                launch<k_clip>(t.first[t.count], true, 2.0 * bytes, s, "clip kernel launch", t, sc);
         });
 }
 
@@ -917,8 +1005,8 @@ void adam_step_device(const ArcqmlTensor *params, const ArcqmlTensor *grads,
         fail("invalid Adam hyperparameters (finite lr and weight decay, 0 <= beta < 1, eps >= 0)");
     if (!std::isfinite(o.max_norm)) fail("the maximum norm must be finite");
     if (o.reserved != 0 || (o.decoupled != 0 && o.decoupled != 1)) fail("invalid Adam options");
-    const bool one = is_short(params, count);
-    if (!one) check_workspace(ws, ws_len, tensor_workspace(params, count));
+    const bool one = is_short(params, count, kShortAdamBytes);
+    if (!one) check_workspace(ws, ws_len, workspace_of(count));
     for (size_t i = 0; i < count; ++i) {
         const uint32_t pt = params[i].dtype, wide = pt == ARCQML_F64 ? ARCQML_F64 : ARCQML_F32;
         const uint64_t n = params[i].length;
@@ -942,31 +1030,42 @@ void adam_step_device(const ArcqmlTensor *params, const ArcqmlTensor *grads,
     const AdamLists lists{params, grads, m, v, copies, count};
     if (one) {
         bool launched = false;
-        const auto launch = [&](const AdamTable<kShortTensors> &t, double bytes) {
+        const auto run = [&](const AdamTable<kShortTensors> &t, double bytes) {
             launch_cluster<k_short_adam>(bytes, s, "Adam kernel launch", t, o, step, given, norm);
             launched = true;
         };
-        for_adam_tables<kShortTensors>(lists, ADAM_ALL, kShortGroups, launch);
+        for_adam_tables<kShortTensors>(lists, ADAM_ALL, kShortGroups, run);
         if (!launched) {  // nothing to update: the step counts all the same
             AdamTable<kShortTensors> none;
             none.count = none.first[0] = 0;
-            launch(none, 0.0);
+            run(none, 0.0);
         }
         return;
     }
-    const uint32_t sums = clips && !given ? square_sums(grads, count, ws, s) : 0;
-    const Scalars *sc = scalars(sums, given, clips ? o.max_norm : -1.0, step, o.beta1, o.beta2,
-                                norm, ws, s);
-    for (const AdamClass which : {ADAM_OTHERS, ADAM_F64})
+    uint64_t groups[2] = {0, 0};  // of the f64 parameters, of the others
+    for (size_t i = 0; i < count; ++i) groups[params[i].dtype != ARCQML_F64] += params[i].length / 4;
+    const uint32_t sums =
+        clips && !given ? square_sums(grads, count, vectors_per_chunk(grads, count), ws, s) : 0;
+    const Scalars *sc = scalars(sums, given, o, step, norm, ws, s);
+    const bool decoupled = o.decoupled != 0;
+    const auto update = [&](AdamClass which, uint32_t per) {
         for_adam_tables<kMaxTensors>(
-            lists, which, kChunk, [&](const AdamTable<kMaxTensors> &t, double bytes) {
-                const uint32_t blocks = std::min(t.first[t.count], kMaxBlocks);
-                const ProfToken tok = prof_begin(PROF_OTHER, s);
-                if (which == ADAM_F64) k_adam<true><<<blocks, kOT, 0, s>>>(t, o, sc);
-                else k_adam<false><<<blocks, kOT, 0, s>>>(t, o, sc);
-                prof_end(tok, s, bytes);
-                check_cuda(cudaGetLastError(), "Adam kernel launch");
+            lists, which, per, [&](const AdamTable<kMaxTensors> &t, double bytes) {
+                const uint32_t blocks = t.first[t.count];
+                const char *what = "Adam kernel launch";
+                if (which == ADAM_ALL)
+                    launch<k_adam<ADAM_ALL>>(blocks, true, bytes, s, what, t, decoupled, sc);
+                else if (which == ADAM_F64)
+                    launch<k_adam<ADAM_F64>>(blocks, true, bytes, s, what, t, decoupled, sc);
+                else launch<k_adam<ADAM_OTHERS>>(blocks, true, bytes, s, what, t, decoupled, sc);
             });
+    };
+    if (groups[0] && groups[1] <= 4 * groups[0]) {
+        update(ADAM_ALL, chunk_size(groups[0] + groups[1], kMaxBlocks));
+    } else {
+        update(ADAM_OTHERS, chunk_size(groups[1], kMaxBlocks));
+        update(ADAM_F64, chunk_size(groups[0], kMaxBlocks));
+    }
 }
 
 }  // namespace arcqml

@@ -6,8 +6,10 @@
 
 namespace arcqml {
 
-// Doubles of device scratch for a list (0: a short list, one launch).
-size_t tensor_workspace(const ArcqmlTensor *list, size_t count);
+// Doubles of device scratch for a list of gradients, and for a list of parameters (0: a short list,
+// one launch).
+size_t gradient_workspace(const ArcqmlTensor *list, size_t count);
+size_t adam_workspace(const ArcqmlTensor *list, size_t count);
 // *norm (device) <- 2-norm over all elements of all tensors.
 void gradient_norm_device(const ArcqmlTensor *grads, size_t count, double *norm, double *ws,
                           size_t ws_len, cudaStream_t s);

@@ -132,6 +132,7 @@ SIGNATURES = {
     "arcqml_rt_v2_peer_buffer_destroy": (_I32, [_P]),
     "arcqml_rt_v2_adjoint_backward": (_I32, [_P, _P, _P, _S, _S, _P, _P, _S, _P, _S, _P]),
     "arcqml_rt_v2_gradient_workspace": (_S, [_P, _S]),
+    "arcqml_rt_v2_adam_workspace": (_S, [_P, _S]),
     "arcqml_rt_v2_gradient_norm": (_I32, [_P, _S, _P, _P, _S, _P]),
     "arcqml_rt_v2_clip_gradients": (_I32, [_P, _S, _D, _P, _P, _P, _S, _P]),
     "arcqml_rt_v2_adam_step": (_I32, [_P, _P, _P, _P, _P, _S, _P, _P, _P, _P, _P, _S, _P]),
@@ -663,9 +664,11 @@ class TensorList:
         self._table, self._layouts = table, layouts
         self._address = table.ctypes.data
         self._words = load().arcqml_rt_v2_gradient_workspace(self._address, len(self.tensors))
+        self._adam_words = load().arcqml_rt_v2_adam_workspace(self._address, len(self.tensors))
         self._shapes = [None if t is None else t.shape for t in self.tensors]
         self._pointers = [t.data_ptr() for t in self._present]
         self._apart = None
+        self._state = object()  # another one whenever the list is written down
 
     def _current(self, torch) -> int:
         """Address of the table, after a look at the tensors' addresses and the current device."""
@@ -774,6 +777,7 @@ class DeviceAdamState:
                 raise ValueError("the step count must not be negative")
             self.step = torch.full((), int(step), dtype=torch.int64, device=device)
         self._m, self._v = TensorList(self.m), TensorList(self.v)
+        self._checked = None
         for name, other in (("first", self._m), ("second", self._v)):
             if other._shapes != p._shapes or other._layouts != p._layouts:
                 raise ValueError(f"the {name} moments must have the parameters' shapes and strides")
@@ -812,22 +816,25 @@ def adam_step_device(parameters, gradients, state: DeviceAdamState, lr: float = 
             raise ValueError("the maximum norm must be finite and not negative")
     tables = [x._current(torch) for x in (p, g, m, v)]
     tables.append(None if c is None else c._current(torch))
-    for name, x in (("gradients", g), ("moments", m), ("moments", v), ("copies", c)):
-        if x is not None and (x._shapes != p._shapes or x._layouts != p._layouts):
-            _check_places(name, x, p)
-    p._check_apart("the parameters")
-    m._check_apart("the moments")
-    v._check_apart("the moments")
-    if c is not None:
-        c._check_apart("the copies")
+    # the lists are held against one another once, and again when one is written down anew
+    states = (p._state, g._state, m._state, v._state, None if c is None else c._state)
+    if states != state._checked:
+        for name, x in (("gradients", g), ("moments", m), ("moments", v), ("copies", c)):
+            if x is not None:
+                _check_places(name, x, p)
+        for name, x in (("parameters", p), ("moments", m), ("moments", v), ("copies", c)):
+            if x is not None:
+                x._check_apart("the " + name)
+        state._checked = states
     options = AdamOptions(lr, betas[0], betas[1], eps, weight_decay, max_norm, bool(decoupled), 0)
-    on, out, ws = _call_memory(torch, stream, p._words, max_norm >= 0.0)
+    on, out, ws = _call_memory(torch, stream, p._adam_words, max_norm >= 0.0)
     _status(load().arcqml_rt_v2_adam_step(
         *tables, len(p), state.step.data_ptr(), C.byref(options), given,
-        None if out is None else out.data_ptr(), None if ws is None else ws.data_ptr(), p._words,
-        on))
-    for x in (p, m, v) if c is None else (p, m, v, c):
-        x._written(torch)
+        None if out is None else out.data_ptr(), None if ws is None else ws.data_ptr(),
+        p._adam_words, on))
+    p._written(torch)
+    if c is not None:
+        c._written(torch)
     return out
 
 

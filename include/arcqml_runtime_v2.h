@@ -215,11 +215,12 @@ typedef struct ArcqmlTensor {
     uint32_t reserved; /* 0 */
 } ArcqmlTensor;
 
-/* Doubles of device scratch that the three calls below take for a list (the gradients of the first
- * two, the parameters of the third); 0 for a short list, whose calls take a null workspace. It
- * depends on the places, types and lengths alone. The scratch belongs to one call at a time: calls
- * that can overlap (other streams, replayed graphs) need their own. */
-size_t arcqml_rt_v2_gradient_workspace(const ArcqmlTensor *tensors, size_t num_tensors);
+/* Doubles of device scratch that a call takes for its list: the norm and clipping for their
+ * gradients, the Adam step for its parameters. 0 for a short list, whose calls take a null
+ * workspace. It depends on the places, types and lengths alone. The scratch belongs to one call at a
+ * time: calls that can overlap (other streams, replayed graphs) need their own. */
+size_t arcqml_rt_v2_gradient_workspace(const ArcqmlTensor *gradients, size_t num_tensors);
+size_t arcqml_rt_v2_adam_workspace(const ArcqmlTensor *parameters, size_t num_tensors);
 
 /* *norm <- sqrt of the sum of squares over every element of every tensor (device). The sum is
  * kept in f64 and its order is fixed by the lengths, types and the GPU, so equal inputs give equal

@@ -459,3 +459,43 @@ def test_refusals_on_the_device(runtime):
     with pytest.raises(TypeError, match="step count"):
         runtime.DeviceAdamState([a], step=torch.zeros((), device="cuda"))
     assert torch.equal(a, before) and int(state.step) == 0
+
+
+def test_captured_long_lists(runtime):
+    """The launches of a list that takes several, captured and replayed against calls."""
+    def model():
+        g = gen(91)
+        p = [normal((700_001,), torch.float32, g), normal((300_000,), torch.float64, g),
+             normal((90_000,), torch.bfloat16, g)]
+        return p, [normal(t.shape, t.dtype, g) for t in p], runtime.DeviceAdamState(p)
+
+    def step(p, q, state):
+        norm = runtime.clip_gradients_device(q, 50.0)
+        return norm, runtime.adam_step_device(p, q, state, lr=0.01, max_norm=1.0)
+
+    a, b = model(), model()
+    step(*model())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(*a)
+    for _ in range(5):
+        graph.replay()
+    torch.cuda.synchronize()
+    for _ in range(5):
+        want = step(*b)
+    assert int(a[2].step) == 5 and all(torch.equal(x, y) for x, y in zip(got, want))
+    assert all(torch.equal(x, y) for x, y in zip(a[0] + a[1] + a[2].m + a[2].v,
+                                                 b[0] + b[1] + b[2].m + b[2].v))
+
+
+@pytest.mark.parametrize("narrow", [100_000, 3_000_000])
+def test_mixed_long_lists(runtime, narrow):
+    """f64 tensors and others in one launch (few others), and in launches of their own."""
+    g = gen(95)
+    params = [normal((400_003,), torch.float64, g), normal((narrow + 1,), torch.float32, g),
+              normal((20_001,), torch.bfloat16, g), normal((300, 128), torch.complex128, g)]
+    grads = [normal(p.shape, p.dtype, g, 0.1) for p in params]
+    run_adam(runtime, params, grads, max_norm=1.0, wd=0.01, steps=2)
+    check_norm(runtime.gradient_norm_device(grads), grads)
+    run_adam(runtime, params, [None, None] + grads[2:], max_norm=1.0)
