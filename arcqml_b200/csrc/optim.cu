@@ -22,6 +22,7 @@
 #include <cmath>
 #include <sstream>
 #include <string>
+#include <type_traits>
 
 #include "launch.h"
 #include "optim.h"
@@ -33,43 +34,14 @@ namespace arcqml {
 namespace {
 
 constexpr int kOT = 256;                 // threads per block
-#ifndef V_NORM_BLOCKS
-#define V_NORM_BLOCKS 6
-#endif
-#ifndef V_BLOCKS
-#define V_BLOCKS 100000000
-#endif
-#ifndef V_CHUNK
-#define V_CHUNK 2048
-#endif
-#ifndef V_U
-#define V_U 2
-#endif
-#ifndef V_NU
-#define V_NU 8
-#endif
-#ifndef V_OCC
-#define V_OCC 4
-#endif
-#ifndef V_COCC
-#define V_COCC 4
-#endif
-#ifndef V_CU
-#define V_CU 4
-#endif
-#ifndef V_NOCC
-#define V_NOCC 6
-#endif
-constexpr uint32_t kMaxBlocks = 148 * V_NORM_BLOCKS; // blocks of one launch
-constexpr uint32_t kMaxTensors = 512;    // tensors of one launch
-constexpr uint32_t kChunk = V_CHUNK;        // 16-byte vectors (k_square_sums, k_clip) or groups of 4
-                                         // elements (k_adam) of one chunk
+constexpr uint32_t kMaxBlocks = 148 * 6; // blocks of k_square_sums: what is resident at once
+constexpr uint32_t kChunk = 2048;        // most 16-byte vectors (k_square_sums, k_clip) or groups
+                                         // (k_adam) of one chunk
+// Tensors of one launch. A launch costs the host 2.3 us more with 28 KB of parameters than with 3 KB.
+constexpr uint32_t kFewTensors = 64, kMaxTensors = 1500, kMaxAdamTensors = 512;
 // Short lists: one cluster, a warp per chunk.
-constexpr uint32_t kShortTensors = 64;
-#ifndef V_SHORT
-#define V_SHORT 1
-#endif
-constexpr uint64_t kShortBytes = V_SHORT * (uint64_t(4) << 20), kShortAdamBytes = V_SHORT * (uint64_t(1) << 20);
+constexpr uint32_t kShortTensors = kFewTensors;
+constexpr uint64_t kShortBytes = uint64_t(4) << 20, kShortAdamBytes = uint64_t(1) << 20;
 constexpr uint32_t kCluster = 16, kShortThreads = 512;
 constexpr uint32_t kShortVectors = 256, kShortGroups = 64;
 
@@ -109,7 +81,7 @@ template <uint32_t CAP> struct AdamTable {
     uint32_t count, per;  // tensors; groups of a chunk
 };
 enum { kAlignedG = 1, kAlignedM = 2, kAlignedV = 4, kAlignedCopy = 8, kHasCopy = 16 };
-static_assert(sizeof(AdamTable<kMaxTensors>) < 32000, "kernel parameters hold 32764 bytes");
+static_assert(sizeof(TensorTable<kMaxTensors>) < 32600 && sizeof(AdamTable<kMaxAdamTensors>) < 32600, "kernel parameters hold 32764 bytes");
 
 // The tensor of chunk c: the last i with first[i] <= c (tensors without chunks are not listed).
 template <class T>
@@ -225,7 +197,7 @@ __device__ __forceinline__ void square_chunk(const void *data, uint64_t length, 
                                              uint32_t per, uint32_t lane, double (&acc)[4]) {
     using T = typename Elem<DTYPE>::type;
     using W = typename Elem<DTYPE>::wide;
-    constexpr int N = 16 / sizeof(T), U = V_NU;
+    constexpr int N = 16 / sizeof(T), U = 8;
     const T *p = static_cast<const T *>(data);
     const uint32_t head = head_of(p, length);
     const uint64_t vectors = (length - head) / N;
@@ -276,8 +248,9 @@ __device__ __forceinline__ void square_chunk_of(const Table &t, uint32_t k, uint
     }
 }
 
-__global__ void __launch_bounds__(kOT, V_NOCC)
-    k_square_sums(const __grid_constant__ TensorTable<kMaxTensors> t, double *__restrict__ sums) {
+template <uint32_t CAP>
+__global__ void __launch_bounds__(kOT, 6)
+    k_square_sums(const __grid_constant__ TensorTable<CAP> t, double *__restrict__ sums) {
     let_next_start();
     double acc[4] = {0.0, 0.0, 0.0, 0.0};
     for (uint32_t c = blockIdx.x; c < t.first[t.count]; c += gridDim.x) {
@@ -350,7 +323,7 @@ __device__ __forceinline__ void clip_chunk(void *data, uint64_t length, uint32_t
                                            uint32_t per, uint32_t lane, double factor) {
     using T = typename Elem<DTYPE>::type;
     using W = typename Elem<DTYPE>::wide;
-    constexpr int N = 16 / sizeof(T), U = V_CU;
+    constexpr int N = 16 / sizeof(T), U = 4;
     const W f = W(factor);
     T *p = static_cast<T *>(data);
     const uint32_t head = head_of(p, length);
@@ -400,8 +373,9 @@ __device__ __forceinline__ void clip_chunk_of(const Table &t, uint32_t k, uint32
     }
 }
 
-__global__ void __launch_bounds__(kOT, V_COCC)
-    k_clip(const __grid_constant__ TensorTable<kMaxTensors> t, const Scalars *sc) {
+template <uint32_t CAP>
+__global__ void __launch_bounds__(kOT, 4)
+    k_clip(const __grid_constant__ TensorTable<CAP> t, const Scalars *sc) {
     let_next_start();
     wait_for_last();
     const double factor = sc->factor;
@@ -435,29 +409,34 @@ __device__ __forceinline__ void adam_update(float &p, float &m, float &v, float 
     p = fmaf(-h.rate, u, p);
 }
 
-// A group (4 elements from element e on) of an array: one access, or one per element.
+// The elements of a group of k_adam: one 16-byte access to the f64 or f32 arrays.
+template <uint32_t DTYPE> constexpr int kGroup = DTYPE == ARCQML_F64 ? 2 : 4;
+
+// A group (from element e on) of an array: one access, or one per element.
 template <uint32_t DTYPE>
-__device__ __forceinline__ Words<DTYPE, 4> load4(const void *p, uint64_t e, bool aligned) {
+__device__ __forceinline__ Words<DTYPE, kGroup<DTYPE>> load_group(const void *p, uint64_t e, bool aligned) {
+    constexpr int N = kGroup<DTYPE>;
     using T = typename Elem<DTYPE>::type;
     const T *q = static_cast<const T *>(p) + e;
-    if (aligned) return *reinterpret_cast<const Words<DTYPE, 4> *>(q);
-    typename Elem<DTYPE>::wide x[4];
-    for (int j = 0; j < 4; ++j) x[j] = widen(q[j]);
-    Words<DTYPE, 4> raw;
+    if (aligned) return *reinterpret_cast<const Words<DTYPE, N> *>(q);
+    typename Elem<DTYPE>::wide x[N];
+    for (int j = 0; j < N; ++j) x[j] = widen(q[j]);
+    Words<DTYPE, N> raw;
     raw.pack(x);
     return raw;
 }
 template <uint32_t DTYPE>
-__device__ __forceinline__ void store4(void *p, uint64_t e, bool aligned,
-                                       const typename Elem<DTYPE>::wide (&x)[4]) {
+__device__ __forceinline__ void store_group(void *p, uint64_t e, bool aligned,
+                                       const typename Elem<DTYPE>::wide (&x)[kGroup<DTYPE>]) {
+    constexpr int N = kGroup<DTYPE>;
     using T = typename Elem<DTYPE>::type;
     T *q = static_cast<T *>(p) + e;
     if (aligned) {
-        Words<DTYPE, 4> raw;
+        Words<DTYPE, N> raw;
         raw.pack(x);
-        *reinterpret_cast<Words<DTYPE, 4> *>(q) = raw;
+        *reinterpret_cast<Words<DTYPE, N> *>(q) = raw;
     } else {
-        for (int j = 0; j < 4; ++j) narrow(x[j], q[j]);
+        for (int j = 0; j < N; ++j) narrow(x[j], q[j]);
     }
 }
 
@@ -468,59 +447,57 @@ __device__ __forceinline__ void adam_chunk(const Table &t, uint32_t k, uint32_t 
     using G = typename Elem<GT>::type;
     using W = typename Elem<PT>::wide;
     constexpr uint32_t WT = sizeof(W) == 8 ? ARCQML_F64 : ARCQML_F32;
-    constexpr int U = sizeof(W) == 8 ? 1 : V_U;
+    constexpr int U = 2, N = kGroup<PT>;
     const uint64_t length = t.length[k];
     const uint32_t per = t.per, head = t.head[k], aligned = t.aligned[k], ct = t.types[k] >> 4;
     void *p = t.p[k], *m = t.m[k], *v = t.v[k], *copy = t.copy[k];
     const void *g = t.g[k];
-    const uint64_t groups = (length - head) / 4;
+    const uint64_t groups = (length - head) / N;
     const uint64_t i0 = uint64_t(chunk) * per;
     const uint32_t n = uint32_t(min(uint64_t(per), groups - min(i0, groups)));
-    const uint64_t e0 = head + 4 * i0;
-    const auto update = [&](uint64_t e, const Words<PT, 4> &rp, const Words<GT, 4> &rg,
-                            const Words<WT, 4> &rm, const Words<WT, 4> &rv) {
-        W x[4], y[4], mm[4], vv[4];
+    const uint64_t e0 = head + N * i0;
+    const auto update = [&](uint64_t e, const Words<PT, N> &rp, const Words<GT, N> &rg,
+                            const Words<WT, N> &rm, const Words<WT, N> &rv) {
+        W x[N], y[N], mm[N], vv[N];
         rp.unpack(x);
         rg.unpack(y);
         rm.unpack(mm);
         rv.unpack(vv);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) adam_update(x[j], mm[j], vv[j], y[j], h, decoupled);
-        store4<PT>(p, e, true, x);
-        store4<WT>(m, e, aligned & kAlignedM, mm);
-        store4<WT>(v, e, aligned & kAlignedV, vv);
+        for (int j = 0; j < N; ++j) adam_update(x[j], mm[j], vv[j], y[j], h, decoupled);
+        store_group<PT>(p, e, true, x);
+        store_group<WT>(m, e, aligned & kAlignedM, mm);
+        store_group<WT>(v, e, aligned & kAlignedV, vv);
         if constexpr (PT == ARCQML_F32) {
             if (aligned & kHasCopy) {
-                if (ct == ARCQML_BF16) store4<ARCQML_BF16>(copy, e, aligned & kAlignedCopy, x);
-                else store4<ARCQML_F16>(copy, e, aligned & kAlignedCopy, x);
+                if (ct == ARCQML_BF16) store_group<ARCQML_BF16>(copy, e, aligned & kAlignedCopy, x);
+                else store_group<ARCQML_F16>(copy, e, aligned & kAlignedCopy, x);
             }
         }
     };
     uint32_t i = lane;
     for (; i + (U - 1) * LANES < n; i += U * LANES) {
-        Words<PT, 4> xp[U];
-        Words<GT, 4> xg[U];
-        Words<WT, 4> xm[U], xv[U];
+        Words<PT, N> xp[U];
+        Words<GT, N> xg[U];
+        Words<WT, N> xm[U], xv[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const uint64_t e = e0 + 4 * (i + u * LANES);
-            xp[u] = load4<PT>(p, e, true);
-            xg[u] = load4<GT>(g, e, aligned & kAlignedG);
-            xm[u] = load4<WT>(m, e, aligned & kAlignedM);
-            xv[u] = load4<WT>(v, e, aligned & kAlignedV);
+            const uint64_t e = e0 + N * (i + u * LANES);
+            xp[u] = load_group<PT>(p, e, true);
+            xg[u] = load_group<GT>(g, e, aligned & kAlignedG);
+            xm[u] = load_group<WT>(m, e, aligned & kAlignedM);
+            xv[u] = load_group<WT>(v, e, aligned & kAlignedV);
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) update(e0 + 4 * (i + u * LANES), xp[u], xg[u], xm[u], xv[u]);
+        for (int u = 0; u < U; ++u) update(e0 + N * (i + u * LANES), xp[u], xg[u], xm[u], xv[u]);
     }
-    if constexpr (U > 1) {
-        for (; i < n; i += LANES) {
-            const uint64_t e = e0 + 4 * i;
-            update(e, load4<PT>(p, e, true), load4<GT>(g, e, aligned & kAlignedG),
-                   load4<WT>(m, e, aligned & kAlignedM), load4<WT>(v, e, aligned & kAlignedV));
-        }
+    for (; i < n; i += LANES) {
+        const uint64_t e = e0 + N * i;
+        update(e, load_group<PT>(p, e, true), load_group<GT>(g, e, aligned & kAlignedG),
+               load_group<WT>(m, e, aligned & kAlignedM), load_group<WT>(v, e, aligned & kAlignedV));
     }
     // the elements before the first group (chunk 0) and behind the last one (the last chunk)
-    const uint64_t done = head + groups * 4;
+    const uint64_t done = head + groups * N;
     const uint32_t tail = i0 + per >= groups ? uint32_t(length - done) : 0;
     const uint32_t first = chunk == 0 ? head : 0;
     if (lane < first + tail) {
@@ -561,22 +538,24 @@ __device__ __forceinline__ void adam_chunk_of(const Table &t, uint32_t k, uint32
     }
 }
 
-// The f64 arithmetic (three divisions and a root per element) takes twice the registers of the
-// other one, and with them half the blocks of an SM: a list's f64 tensors and its others go to
-// launches of their own unless the others are few.
-enum AdamClass { ADAM_OTHERS, ADAM_F64, ADAM_ALL };
-template <AdamClass CLASS>
-__global__ void __launch_bounds__(kOT, CLASS == ADAM_OTHERS ? V_OCC : 2)
-    k_adam(const __grid_constant__ AdamTable<kMaxTensors> t, bool decoupled, const Scalars *sc) {
+// One launch for every type: at 4 blocks (64 registers) the f64 arithmetic, three divisions and a
+// root per element, spills a little and still runs as fast as in a launch of its own.
+template <uint32_t CAP>
+__global__ void __launch_bounds__(kOT, 4)
+    k_adam(const __grid_constant__ AdamTable<CAP> t, bool decoupled, const Scalars *sc) {
     let_next_start();
     wait_for_last();
     // the last chunks first: their gradients are the ones that the norm left in L2
     const uint32_t chunks = t.first[t.count];
     const uint32_t c = chunks - 1 - blockIdx.x, k = tensor_of(t, c), chunk = c - t.first[k];
-    if (CLASS == ADAM_F64 || (CLASS == ADAM_ALL && (t.types[k] & 3) == ARCQML_F64))
-        adam_chunk<ARCQML_F64, ARCQML_F64, kOT>(t, k, chunk, threadIdx.x, sc->h, decoupled);
-    else if (CLASS != ADAM_F64)
-        adam_chunk_of<kOT>(t, k, chunk, threadIdx.x, sc->hf, decoupled);
+    // copies of the scalars: for all the compiler knows the stores change what sc points to
+    if ((t.types[k] & 3) == ARCQML_F64) {
+        const AdamScalars64 h = sc->h;
+        adam_chunk<ARCQML_F64, ARCQML_F64, kOT>(t, k, chunk, threadIdx.x, h, decoupled);
+    } else {
+        const AdamScalars32 h = sc->hf;
+        adam_chunk_of<kOT>(t, k, chunk, threadIdx.x, h, decoupled);
+    }
 }
 
 // ------------------------------------------------------------------ short lists
@@ -627,18 +606,19 @@ template <uint32_t GT, uint32_t LANES, class Table>
 __device__ __forceinline__ void square_groups(const Table &t, uint32_t k, uint32_t chunk,
                                               uint32_t lane, double (&acc)[4]) {
     using G = typename Elem<GT>::type;
+    constexpr int N = kGroup<GT>;  // f64 gradients belong to f64 parameters
     const uint32_t per = t.per, head = t.head[k];
-    const uint64_t length = t.length[k], groups = (length - head) / 4, i0 = uint64_t(chunk) * per;
+    const uint64_t length = t.length[k], groups = (length - head) / N, i0 = uint64_t(chunk) * per;
     const uint32_t n = uint32_t(min(uint64_t(per), groups - min(i0, groups)));
     const void *g = t.g[k];
 #pragma unroll 2
     for (uint32_t i = lane; i < n; i += LANES) {
-        typename Elem<GT>::wide x[4];
-        load4<GT>(g, head + 4 * (i0 + i), t.aligned[k] & kAlignedG).unpack(x);
+        typename Elem<GT>::wide x[N];
+        load_group<GT>(g, head + N * (i0 + i), t.aligned[k] & kAlignedG).unpack(x);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[j] = fma(double(x[j]), double(x[j]), acc[j]);
+        for (int j = 0; j < N; ++j) acc[j] = fma(double(x[j]), double(x[j]), acc[j]);
     }
-    const uint64_t done = head + groups * 4;
+    const uint64_t done = head + groups * N;
     const uint32_t tail = i0 + per >= groups ? uint32_t(length - done) : 0;
     const uint32_t first = chunk == 0 ? head : 0;
     if (lane < first + tail) {
@@ -701,6 +681,9 @@ __global__ void __launch_bounds__(kShortThreads, 1)
 uint32_t element_size(uint32_t dtype) {
     return dtype == ARCQML_F64 ? 8 : dtype == ARCQML_F32 ? 4 : 2;
 }
+
+// Elements of a group of k_adam (kGroup).
+uint32_t group_size(const ArcqmlTensor &t) { return t.dtype == ARCQML_F64 ? 2 : 4; }
 
 [[noreturn]] void fail_at(const char *list, size_t i, const char *what) {
     std::ostringstream m;
@@ -790,14 +773,13 @@ void for_tensor_tables(const ArcqmlTensor *list, size_t count, uint32_t per, F &
     flush();
 }
 
-// The same for a (checked) Adam step, over the tensors of the given class: the f64 parameters, the
-// others, or all.
+// The same for a (checked) Adam step. Calls launch for no empty table.
 struct AdamLists {
     const ArcqmlTensor *params, *grads, *m, *v, *copies;
     size_t count;
 };
 template <uint32_t CAP, class F>
-void for_adam_tables(const AdamLists &l, AdamClass which, uint32_t per, F &&launch) {
+void for_adam_tables(const AdamLists &l, uint32_t per, F &&launch) {
     AdamTable<CAP> t;
     t.count = 0;
     t.per = per;
@@ -810,18 +792,16 @@ void for_adam_tables(const AdamLists &l, AdamClass which, uint32_t per, F &&laun
         chunks = 0;
         bytes = 0.0;
     };
-    // groups of 4 elements from the first place on where the parameter's start on their size
+    // groups from the first place on where the parameter's start on their size
     const auto apart = [](const ArcqmlTensor &x) {
-        return (reinterpret_cast<uintptr_t>(x.data) / element_size(x.dtype)) & 3;
+        return (reinterpret_cast<uintptr_t>(x.data) / element_size(x.dtype)) & (group_size(x) - 1);
     };
     for (size_t i = 0; i < l.count; ++i) {
         const ArcqmlTensor &p = l.params[i], &g = l.grads[i];
-        if (!present(p) || g.dtype == ARCQML_NO_TENSOR ||
-            (which != ADAM_ALL && (p.dtype == ARCQML_F64) != (which == ADAM_F64)))
-            continue;
+        if (!present(p) || g.dtype == ARCQML_NO_TENSOR) continue;
         if (t.count == CAP) flush();
         const bool copy = l.copies && l.copies[i].dtype != ARCQML_NO_TENSOR;
-        const uint64_t at = apart(p), head = std::min<uint64_t>(-at & 3, p.length);
+        const uint64_t at = apart(p), head = std::min<uint64_t>(-at & (group_size(p) - 1), p.length);
         const uint32_t k = t.count++;
         t.p[k] = p.data;
         t.g[k] = g.data;
@@ -837,7 +817,7 @@ void for_adam_tables(const AdamLists &l, AdamClass which, uint32_t per, F &&laun
                                (copy && apart(l.copies[i]) == at ? kAlignedCopy : 0) |
                                (copy ? kHasCopy : 0));
         t.head[k] = uint8_t(head);
-        chunks += std::max<uint64_t>(1, ((p.length - head) / 4 + per - 1) / per);
+        chunks += std::max<uint64_t>(1, ((p.length - head) / group_size(p) + per - 1) / per);
         bytes += double(p.length) *
                  (2.0 * element_size(p.dtype) + element_size(g.dtype) +
                   4.0 * element_size(l.m[i].dtype) +
@@ -888,8 +868,10 @@ void launch(uint32_t blocks, bool follows, double bytes, cudaStream_t s, const c
     c.stream = s;
     c.attrs = &a;
     c.numAttrs = follows ? 1 : 0;
+    static_assert(std::is_same_v<decltype(KERNEL), void (*)(Args...)>);
+    void *params[] = {const_cast<void *>(static_cast<const void *>(&args))...};
     const ProfToken tok = prof_begin(PROF_OTHER, s);
-    check_cuda(cudaLaunchKernelEx(&c, KERNEL, args...), what);
+    check_cuda(cudaLaunchKernelExC(&c, reinterpret_cast<const void *>(KERNEL), params), what);
     prof_end(tok, s, bytes);
 }
 
@@ -901,19 +883,50 @@ uint32_t chunk_size(uint64_t total, uint32_t places) {
     return per;
 }
 
+bool are_few(const ArcqmlTensor *list, size_t count) {
+    if (count <= kFewTensors) return true;
+    size_t tensors = 0;
+    for (size_t i = 0; i < count; ++i) tensors += present(list[i]);
+    return tensors <= kFewTensors;
+}
+
 // Sums of squares of the list into ws; returns their count.
+template <uint32_t CAP>
+uint32_t square_sums_in(const ArcqmlTensor *grads, size_t count, uint32_t per, double *ws,
+                        cudaStream_t s) {
+    uint32_t sums = 0;
+    for_tensor_tables<CAP>(grads, count, per, [&](const TensorTable<CAP> &t, double bytes) {
+        if (!t.count) return;
+        const uint32_t blocks = std::min(t.first[t.count], kMaxBlocks);
+        launch<k_square_sums<CAP>>(blocks, false, bytes, s, "gradient norm kernel launch", t,
+                                   ws + kScalarDoubles + sums);
+        sums += blocks;
+    });
+    return sums;
+}
+
 uint32_t square_sums(const ArcqmlTensor *grads, size_t count, uint32_t per, double *ws,
                      cudaStream_t s) {
-    uint32_t sums = 0;
-    for_tensor_tables<kMaxTensors>(
-        grads, count, per, [&](const TensorTable<kMaxTensors> &t, double bytes) {
-            if (!t.count) return;
-            const uint32_t blocks = std::min(t.first[t.count], kMaxBlocks);
-            launch<k_square_sums>(blocks, false, bytes, s, "gradient norm kernel launch", t,
-                                  ws + kScalarDoubles + sums);
-            sums += blocks;
-        });
-    return sums;
+    return are_few(grads, count) ? square_sums_in<kFewTensors>(grads, count, per, ws, s)
+                                 : square_sums_in<kMaxTensors>(grads, count, per, ws, s);
+}
+
+template <uint32_t CAP>
+void clip_in(const ArcqmlTensor *grads, size_t count, uint32_t per, const Scalars *sc,
+             cudaStream_t s) {
+    for_tensor_tables<CAP>(grads, count, per, [&](const TensorTable<CAP> &t, double bytes) {
+        if (t.count)
+            launch<k_clip<CAP>>(t.first[t.count], true, 2.0 * bytes, s, "clip kernel launch", t, sc);
+    });
+}
+
+template <uint32_t CAP>
+void adam_in(const AdamLists &lists, uint32_t per, bool decoupled, const Scalars *sc,
+             cudaStream_t s) {
+    for_adam_tables<CAP>(lists, per, [&](const AdamTable<CAP> &t, double bytes) {
+        launch<k_adam<CAP>>(t.first[t.count], true, bytes, s, "Adam kernel launch", t, decoupled,
+                            sc);
+    });
 }
 
 uint32_t vectors_per_chunk(const ArcqmlTensor *list, size_t count) {
@@ -982,11 +995,8 @@ void clip_gradients_device(const ArcqmlTensor *grads, size_t count, double max_n
     const uint32_t per = vectors_per_chunk(grads, count);
     const uint32_t sums = given ? 0 : square_sums(grads, count, per, ws, s);
     const Scalars *sc = scalars(sums, given, clip_options(max_norm), nullptr, norm, ws, s);
-    for_tensor_tables<kMaxTensors>(
-        grads, count, per, [&](const TensorTable<kMaxTensors> &t, double bytes) {
-            if (t.count)
-                launch<k_clip>(t.first[t.count], true, 2.0 * bytes, s, "clip kernel launch", t, sc);
-        });
+    if (are_few(grads, count)) clip_in<kFewTensors>(grads, count, per, sc, s);
+    else clip_in<kMaxTensors>(grads, count, per, sc, s);
 }
 
 void adam_step_device(const ArcqmlTensor *params, const ArcqmlTensor *grads,
@@ -1034,7 +1044,7 @@ void adam_step_device(const ArcqmlTensor *params, const ArcqmlTensor *grads,
             launch_cluster<k_short_adam>(bytes, s, "Adam kernel launch", t, o, step, given, norm);
             launched = true;
         };
-        for_adam_tables<kShortTensors>(lists, ADAM_ALL, kShortGroups, run);
+        for_adam_tables<kShortTensors>(lists, kShortGroups, run);
         if (!launched) {  // nothing to update: the step counts all the same
             AdamTable<kShortTensors> none;
             none.count = none.first[0] = 0;
@@ -1042,30 +1052,14 @@ void adam_step_device(const ArcqmlTensor *params, const ArcqmlTensor *grads,
         }
         return;
     }
-    uint64_t groups[2] = {0, 0};  // of the f64 parameters, of the others
-    for (size_t i = 0; i < count; ++i) groups[params[i].dtype != ARCQML_F64] += params[i].length / 4;
     const uint32_t sums =
         clips && !given ? square_sums(grads, count, vectors_per_chunk(grads, count), ws, s) : 0;
     const Scalars *sc = scalars(sums, given, o, step, norm, ws, s);
-    const bool decoupled = o.decoupled != 0;
-    const auto update = [&](AdamClass which, uint32_t per) {
-        for_adam_tables<kMaxTensors>(
-            lists, which, per, [&](const AdamTable<kMaxTensors> &t, double bytes) {
-                const uint32_t blocks = t.first[t.count];
-                const char *what = "Adam kernel launch";
-                if (which == ADAM_ALL)
-                    launch<k_adam<ADAM_ALL>>(blocks, true, bytes, s, what, t, decoupled, sc);
-                else if (which == ADAM_F64)
-                    launch<k_adam<ADAM_F64>>(blocks, true, bytes, s, what, t, decoupled, sc);
-                else launch<k_adam<ADAM_OTHERS>>(blocks, true, bytes, s, what, t, decoupled, sc);
-            });
-    };
-    if (groups[0] && groups[1] <= 4 * groups[0]) {
-        update(ADAM_ALL, chunk_size(groups[0] + groups[1], kMaxBlocks));
-    } else {
-        update(ADAM_OTHERS, chunk_size(groups[1], kMaxBlocks));
-        update(ADAM_F64, chunk_size(groups[0], kMaxBlocks));
-    }
+    uint64_t groups = 0;
+    for (size_t i = 0; i < count; ++i) groups += params[i].length / group_size(params[i]);
+    const uint32_t per = chunk_size(groups, kMaxBlocks);
+    if (are_few(params, count)) adam_in<kFewTensors>(lists, per, o.decoupled != 0, sc, s);
+    else adam_in<kMaxAdamTensors>(lists, per, o.decoupled != 0, sc, s);
 }
 
 }  // namespace arcqml

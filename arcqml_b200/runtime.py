@@ -667,16 +667,19 @@ class TensorList:
         self._adam_words = load().arcqml_rt_v2_adam_workspace(self._address, len(self.tensors))
         self._shapes = [None if t is None else t.shape for t in self.tensors]
         self._pointers = [t.data_ptr() for t in self._present]
+        # the tensors whose version counters stand for all: views share their base's
+        roots = [t._base if t._is_view() else t for t in self._present]
+        self._roots = list({id(t): t for t in roots}.values())
         self._apart = None
         self._state = object()  # another one whenever the list is written down
 
-    def _current(self, torch) -> int:
+    def _current(self, torch, device: int) -> int:
         """Address of the table, after a look at the tensors' addresses and the current device."""
         if list(map(torch.Tensor.data_ptr, self._present)) != self._pointers:
             self._write_down()
-        if self.device_index is not None and self.device_index != torch.cuda.current_device():
+        if self.device_index != device and self.device_index is not None:
             raise RuntimeError(f"the tensors are on cuda:{self.device_index} and the current device "
-                               f"is cuda:{torch.cuda.current_device()}")
+                               f"is cuda:{device}")
         return self._address
 
     def _check_apart(self, name: str) -> None:
@@ -688,7 +691,7 @@ class TensorList:
 
     def _written(self, torch) -> None:
         """Tells autograd that the tensors changed."""
-        torch.autograd.graph.increment_version(self._present)
+        torch.autograd.graph.increment_version(self._roots)
 
 
 def _tables_apart(tables) -> bool:
@@ -703,22 +706,21 @@ def _tensor_list(tensors) -> TensorList:
     return tensors if isinstance(tensors, TensorList) else TensorList(tensors)
 
 
-def _call_memory(torch, stream, words: int, norm: bool):
+def _call_memory(torch, device: int, stream, words: int, norm: bool):
     """(stream, norm, scratch) of one call. All of it is allocated for the call alone, on its stream,
     so calls on other streams and captured graphs share nothing."""
     if stream is not None:
         with torch.cuda.stream(torch.cuda.ExternalStream(int(stream))):
-            return (int(stream),) + _call_memory(torch, None, words, norm)[1:]
-    device = torch.cuda.current_device()
+            return (int(stream),) + _call_memory(torch, device, None, words, norm)[1:]
     # the raw handle: a Stream object costs as much as the launch
     raw = torch._C._cuda_getCurrentRawStream(device)
     return (raw, torch.empty((), dtype=torch.float64, device=device) if norm else None,
             torch.empty(words, dtype=torch.float64, device=device) if words else None)
 
 
-def _scalar_ptr(torch, t) -> int:
+def _scalar_ptr(torch, device: int, t) -> int:
     if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == torch.float64
-            and t.numel() == 1 and t.get_device() == torch.cuda.current_device()):
+            and t.numel() == 1 and t.get_device() == device):
         raise TypeError("a given norm must be one float64 on the current CUDA device")
     return t.data_ptr()
 
@@ -729,8 +731,9 @@ def gradient_norm_device(gradients, stream=None):
     back: the norm can go into the calls below, or its square into an all-reduce."""
     import torch
     g = _tensor_list(gradients)
-    table = g._current(torch)
-    on, out, ws = _call_memory(torch, stream, g._words, True)
+    device = torch.cuda.current_device()
+    table = g._current(torch, device)
+    on, out, ws = _call_memory(torch, device, stream, g._words, True)
     _status(load().arcqml_rt_v2_gradient_norm(table, len(g), out.data_ptr(),
                                               None if ws is None else ws.data_ptr(), g._words, on))
     return out
@@ -742,10 +745,11 @@ def clip_gradients_device(gradients, max_norm: float, norm=None, stream=None):
     (arcqml_rt_v2_clip_gradients)."""
     import torch
     g = _tensor_list(gradients)
-    table = g._current(torch)
+    device = torch.cuda.current_device()
+    table = g._current(torch, device)
     g._check_apart("the gradients")
-    given = None if norm is None else _scalar_ptr(torch, norm)
-    on, out, ws = _call_memory(torch, stream, g._words, True)
+    given = None if norm is None else _scalar_ptr(torch, device, norm)
+    on, out, ws = _call_memory(torch, device, stream, g._words, True)
     _status(load().arcqml_rt_v2_clip_gradients(table, len(g), float(max_norm), given,
                                                out.data_ptr(),
                                                None if ws is None else ws.data_ptr(), g._words, on))
@@ -806,16 +810,17 @@ def adam_step_device(parameters, gradients, state: DeviceAdamState, lr: float = 
     c = None if copies is None else _tensor_list(copies)
     if len(p._present) != len(p):
         raise TypeError("a parameter list has no empty places")
+    device = torch.cuda.current_device()
     if max_norm is None:
         if norm is not None:
             raise ValueError("a given norm needs max_norm")
         max_norm, given = -1.0, None
     else:
-        max_norm, given = float(max_norm), None if norm is None else _scalar_ptr(torch, norm)
+        max_norm, given = float(max_norm), None if norm is None else _scalar_ptr(torch, device, norm)
         if not max_norm >= 0.0:
             raise ValueError("the maximum norm must be finite and not negative")
-    tables = [x._current(torch) for x in (p, g, m, v)]
-    tables.append(None if c is None else c._current(torch))
+    tables = [x._current(torch, device) for x in (p, g, m, v)]
+    tables.append(None if c is None else c._current(torch, device))
     # the lists are held against one another once, and again when one is written down anew
     states = (p._state, g._state, m._state, v._state, None if c is None else c._state)
     if states != state._checked:
@@ -827,7 +832,7 @@ def adam_step_device(parameters, gradients, state: DeviceAdamState, lr: float = 
                 x._check_apart("the " + name)
         state._checked = states
     options = AdamOptions(lr, betas[0], betas[1], eps, weight_decay, max_norm, bool(decoupled), 0)
-    on, out, ws = _call_memory(torch, stream, p._adam_words, max_norm >= 0.0)
+    on, out, ws = _call_memory(torch, device, stream, p._adam_words, max_norm >= 0.0)
     _status(load().arcqml_rt_v2_adam_step(
         *tables, len(p), state.step.data_ptr(), C.byref(options), given,
         None if out is None else out.data_ptr(), None if ws is None else ws.data_ptr(),

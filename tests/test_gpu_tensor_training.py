@@ -100,7 +100,7 @@ def test_norm_of_mixed_types_strides_and_empty_places(runtime):
         assert float(runtime.clip_gradients_device(nothing, 1.0)) == 0.0
 
 
-@pytest.mark.parametrize("tensors", [511, 512, 513, 1100, 1700])
+@pytest.mark.parametrize("tensors", [64, 65, 511, 512, 513, 1100, 1500, 1501])
 def test_lists_longer_than_one_launch(runtime, tensors):
     g = gen(tensors)
     lengths = [1 + (i * 37) % 201 for i in range(tensors)]
@@ -491,7 +491,7 @@ def test_captured_long_lists(runtime):
 
 @pytest.mark.parametrize("narrow", [100_000, 3_000_000])
 def test_mixed_long_lists(runtime, narrow):
-    """f64 tensors and others in one launch (few others), and in launches of their own."""
+    """f64 tensors and others in one launch."""
     g = gen(95)
     params = [normal((400_003,), torch.float64, g), normal((narrow + 1,), torch.float32, g),
               normal((20_001,), torch.bfloat16, g), normal((300, 128), torch.complex128, g)]
