@@ -38,7 +38,7 @@ constexpr uint32_t kMaxBlocks = 148 * 6; // blocks of k_square_sums: what is res
 constexpr uint32_t kChunk = 2048;        // most 16-byte vectors (k_square_sums, k_clip) or groups
                                          // (k_adam) of one chunk
 // Tensors of one launch. A launch costs the host 2.3 us more with 28 KB of parameters than with 3 KB.
-constexpr uint32_t kFewTensors = 64, kMaxTensors = 1500, kMaxAdamTensors = 512;
+constexpr uint32_t kFewTensors = 64, kSomeTensors = 512, kMaxTensors = 1500;
 // Short lists: one cluster, a warp per chunk.
 constexpr uint32_t kShortTensors = kFewTensors;
 constexpr uint64_t kShortBytes = uint64_t(4) << 20, kShortAdamBytes = uint64_t(1) << 20;
@@ -81,7 +81,7 @@ template <uint32_t CAP> struct AdamTable {
     uint32_t count, per;  // tensors; groups of a chunk
 };
 enum { kAlignedG = 1, kAlignedM = 2, kAlignedV = 4, kAlignedCopy = 8, kHasCopy = 16 };
-static_assert(sizeof(TensorTable<kMaxTensors>) < 32600 && sizeof(AdamTable<kMaxAdamTensors>) < 32600, "kernel parameters hold 32764 bytes");
+static_assert(sizeof(TensorTable<kMaxTensors>) < 32600 && sizeof(AdamTable<kSomeTensors>) < 32600, "kernel parameters hold 32764 bytes");
 
 // The tensor of chunk c: the last i with first[i] <= c (tensors without chunks are not listed).
 template <class T>
@@ -221,7 +221,14 @@ __device__ __forceinline__ void square_chunk(const void *data, uint64_t length, 
 #pragma unroll
         for (int u = 0; u < U; ++u) add(x[u]);
     }
-    for (; v < n; v += LANES) add(q[v0 + v]);
+    if (v < n) {  // less than a batch is left
+        Words<DTYPE, N> x[U] = {};
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (v + u * LANES < n) x[u] = q[v0 + v + u * LANES];
+#pragma unroll
+        for (int u = 0; u < U; ++u) add(x[u]);
+    }
     // the elements before the first vector (chunk 0) and behind the last one (the last chunk)
     if (chunk == 0 && lane < head) {
         const double d = double(widen(p[lane]));
@@ -349,10 +356,17 @@ __device__ __forceinline__ void clip_chunk(void *data, uint64_t length, uint32_t
             q[v0 + v + u * LANES] = x[u];
         }
     }
-    for (; v < n; v += LANES) {
-        Words<DTYPE, N> x = q[v0 + v];
-        scale(x);
-        q[v0 + v] = x;
+    if (v < n) {  // less than a batch is left
+        Words<DTYPE, N> x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (v + u * LANES < n) x[u] = q[v0 + v + u * LANES];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (v + u * LANES < n) {
+                scale(x[u]);
+                q[v0 + v + u * LANES] = x[u];
+            }
     }
     if (chunk == 0 && lane < head) narrow(widen(p[lane]) * f, p[lane]);
     const uint64_t done = head + vectors * N;
@@ -826,32 +840,40 @@ void for_adam_tables(const AdamLists &l, uint32_t per, F &&launch) {
     if (t.count) flush();
 }
 
-// A launch of one cluster.
+// A launch of one cluster of no more blocks than the list's chunks give warps to work, at most 16: a
+// small list takes few SMs (its time is the launch's either way).
 template <auto KERNEL, class... Args>
-void launch_cluster(double bytes, cudaStream_t s, const char *what, Args... args) {
-    // above 8 blocks a cluster's size has to be allowed, once per kernel and device
-    static std::atomic<uint64_t> allowed{0};
-    int dev = 0;
-    check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
-    const uint64_t bit = uint64_t(1) << (dev & 63);
-    if (dev > 63 || !(allowed.load(std::memory_order_relaxed) & bit)) {
-        check_cuda(cudaFuncSetAttribute(reinterpret_cast<const void *>(KERNEL),
-                                        cudaFuncAttributeNonPortableClusterSizeAllowed, 1),
-                   what);
-        allowed.fetch_or(bit, std::memory_order_relaxed);
+void launch_cluster(uint32_t chunks, double bytes, cudaStream_t s, const char *what,
+                    const Args &...args) {
+    static_assert(std::is_same_v<decltype(KERNEL), void (*)(Args...)>);
+    uint32_t blocks = 1;
+    while (blocks < kCluster && blocks * (kShortThreads / 32) < chunks) blocks *= 2;
+    if (blocks > 8) {
+        // above 8 blocks a cluster's size has to be allowed, once per kernel and device
+        static std::atomic<uint64_t> allowed{0};
+        int dev = 0;
+        check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
+        const uint64_t bit = uint64_t(1) << (dev & 63);
+        if (dev > 63 || !(allowed.load(std::memory_order_relaxed) & bit)) {
+            check_cuda(cudaFuncSetAttribute(reinterpret_cast<const void *>(KERNEL),
+                                            cudaFuncAttributeNonPortableClusterSizeAllowed, 1),
+                       what);
+            allowed.fetch_or(bit, std::memory_order_relaxed);
+        }
     }
     cudaLaunchConfig_t c{};
     cudaLaunchAttribute a{};
     a.id = cudaLaunchAttributeClusterDimension;
-    a.val.clusterDim.x = kCluster;
+    a.val.clusterDim.x = blocks;
     a.val.clusterDim.y = a.val.clusterDim.z = 1;
-    c.gridDim = dim3(kCluster);
+    c.gridDim = dim3(blocks);
     c.blockDim = dim3(kShortThreads);
     c.stream = s;
     c.attrs = &a;
-    c.numAttrs = 1;
+    c.numAttrs = blocks > 1 ? 1 : 0;
+    void *params[] = {const_cast<void *>(static_cast<const void *>(&args))...};
     const ProfToken tok = prof_begin(PROF_OTHER, s);
-    check_cuda(cudaLaunchKernelEx(&c, KERNEL, args...), what);
+    check_cuda(cudaLaunchKernelExC(&c, reinterpret_cast<const void *>(KERNEL), params), what);
     prof_end(tok, s, bytes);
 }
 
@@ -883,50 +905,34 @@ uint32_t chunk_size(uint64_t total, uint32_t places) {
     return per;
 }
 
-bool are_few(const ArcqmlTensor *list, size_t count) {
-    if (count <= kFewTensors) return true;
-    size_t tensors = 0;
-    for (size_t i = 0; i < count; ++i) tensors += present(list[i]);
-    return tensors <= kFewTensors;
+// Calls f(capacity) with the smallest table that holds the list's tensors, or else the largest.
+template <class F> void for_table_size(const ArcqmlTensor *list, size_t count, F &&f) {
+    size_t tensors = count;
+    if (count > kFewTensors)
+        tensors = size_t(std::count_if(list, list + count, [](auto &t) { return present(t); }));
+    if (tensors <= kFewTensors) f(std::integral_constant<uint32_t, kFewTensors>{});
+    else if (tensors <= kSomeTensors) f(std::integral_constant<uint32_t, kSomeTensors>{});
+    else f(std::integral_constant<uint32_t, kMaxTensors>{});
 }
 
 // Sums of squares of the list into ws; returns their count.
 template <uint32_t CAP>
-uint32_t square_sums_in(const ArcqmlTensor *grads, size_t count, uint32_t per, double *ws,
-                        cudaStream_t s) {
-    uint32_t sums = 0;
-    for_tensor_tables<CAP>(grads, count, per, [&](const TensorTable<CAP> &t, double bytes) {
-        if (!t.count) return;
-        const uint32_t blocks = std::min(t.first[t.count], kMaxBlocks);
-        launch<k_square_sums<CAP>>(blocks, false, bytes, s, "gradient norm kernel launch", t,
-                                   ws + kScalarDoubles + sums);
-        sums += blocks;
-    });
-    return sums;
+uint32_t square_sums(const TensorTable<CAP> &t, double bytes, double *sums, cudaStream_t s) {
+    if (!t.count) return 0;
+    const uint32_t blocks = std::min(t.first[t.count], kMaxBlocks);
+    launch<k_square_sums<CAP>>(blocks, false, bytes, s, "gradient norm kernel launch", t, sums);
+    return blocks;
 }
 
 uint32_t square_sums(const ArcqmlTensor *grads, size_t count, uint32_t per, double *ws,
                      cudaStream_t s) {
-    return are_few(grads, count) ? square_sums_in<kFewTensors>(grads, count, per, ws, s)
-                                 : square_sums_in<kMaxTensors>(grads, count, per, ws, s);
-}
-
-template <uint32_t CAP>
-void clip_in(const ArcqmlTensor *grads, size_t count, uint32_t per, const Scalars *sc,
-             cudaStream_t s) {
-    for_tensor_tables<CAP>(grads, count, per, [&](const TensorTable<CAP> &t, double bytes) {
-        if (t.count)
-            launch<k_clip<CAP>>(t.first[t.count], true, 2.0 * bytes, s, "clip kernel launch", t, sc);
+    uint32_t sums = 0;
+    for_table_size(grads, count, [&](auto capacity) {
+        for_tensor_tables<capacity>(grads, count, per, [&](const auto &t, double bytes) {
+            sums += square_sums(t, bytes, ws + kScalarDoubles + sums, s);
+        });
     });
-}
-
-template <uint32_t CAP>
-void adam_in(const AdamLists &lists, uint32_t per, bool decoupled, const Scalars *sc,
-             cudaStream_t s) {
-    for_adam_tables<CAP>(lists, per, [&](const AdamTable<CAP> &t, double bytes) {
-        launch<k_adam<CAP>>(t.first[t.count], true, bytes, s, "Adam kernel launch", t, decoupled,
-                            sc);
-    });
+    return sums;
 }
 
 uint32_t vectors_per_chunk(const ArcqmlTensor *list, size_t count) {
@@ -956,7 +962,7 @@ void short_clip(const ArcqmlTensor *grads, size_t count, const double *given, do
                 double *norm, cudaStream_t s) {
     for_tensor_tables<kShortTensors>(
         grads, count, kShortVectors, [&](const TensorTable<kShortTensors> &t, double bytes) {
-            launch_cluster<k_short_clip>(max_norm >= 0.0 ? 2.0 * bytes : bytes, s,
+            launch_cluster<k_short_clip>(t.first[t.count], max_norm >= 0.0 ? 2.0 * bytes : bytes, s,
                                          "gradient norm kernel launch", t, given, max_norm, norm);
         });
 }
@@ -993,10 +999,28 @@ void clip_gradients_device(const ArcqmlTensor *grads, size_t count, double max_n
     if (is_short(grads, count, kShortBytes)) return short_clip(grads, count, given, max_norm, norm, s);
     check_workspace(ws, ws_len, workspace_of(count));
     const uint32_t per = vectors_per_chunk(grads, count);
-    const uint32_t sums = given ? 0 : square_sums(grads, count, per, ws, s);
-    const Scalars *sc = scalars(sums, given, clip_options(max_norm), nullptr, norm, ws, s);
-    if (are_few(grads, count)) clip_in<kFewTensors>(grads, count, per, sc, s);
-    else clip_in<kMaxTensors>(grads, count, per, sc, s);
+    const auto o = clip_options(max_norm);
+    for_table_size(grads, count, [&](auto capacity) {
+        constexpr uint32_t CAP = capacity;
+        const auto clip = [&](const TensorTable<CAP> &t, const Scalars *sc, double bytes) {
+            if (t.count)
+                launch<k_clip<CAP>>(t.first[t.count], true, 2.0 * bytes, s,
+                                    "clip kernel launch", t, sc);
+        };
+        if (count <= CAP) {  // one table for the norm and the scaling
+            for_tensor_tables<CAP>(grads, count, per, [&](const TensorTable<CAP> &t, double bytes) {
+                const uint32_t sums =
+                    given ? 0 : square_sums(t, bytes, ws + kScalarDoubles, s);
+                clip(t, scalars(sums, given, o, nullptr, norm, ws, s), bytes);
+            });
+            return;
+        }
+        const uint32_t sums = given ? 0 : square_sums(grads, count, per, ws, s);
+        const Scalars *sc = scalars(sums, given, o, nullptr, norm, ws, s);
+        for_tensor_tables<CAP>(grads, count, per, [&](const TensorTable<CAP> &t, double bytes) {
+            clip(t, sc, bytes);
+        });
+    });
 }
 
 void adam_step_device(const ArcqmlTensor *params, const ArcqmlTensor *grads,
@@ -1041,7 +1065,8 @@ void adam_step_device(const ArcqmlTensor *params, const ArcqmlTensor *grads,
     if (one) {
         bool launched = false;
         const auto run = [&](const AdamTable<kShortTensors> &t, double bytes) {
-            launch_cluster<k_short_adam>(bytes, s, "Adam kernel launch", t, o, step, given, norm);
+            launch_cluster<k_short_adam>(t.first[t.count], bytes, s, "Adam kernel launch", t, o, step,
+                                         given, norm);
             launched = true;
         };
         for_adam_tables<kShortTensors>(lists, kShortGroups, run);
@@ -1058,8 +1083,13 @@ void adam_step_device(const ArcqmlTensor *params, const ArcqmlTensor *grads,
     uint64_t groups = 0;
     for (size_t i = 0; i < count; ++i) groups += params[i].length / group_size(params[i]);
     const uint32_t per = chunk_size(groups, kMaxBlocks);
-    if (are_few(params, count)) adam_in<kFewTensors>(lists, per, o.decoupled != 0, sc, s);
-    else adam_in<kMaxAdamTensors>(lists, per, o.decoupled != 0, sc, s);
+    for_table_size(params, count, [&](auto capacity) {
+        constexpr uint32_t CAP = capacity < kSomeTensors ? uint32_t(capacity) : kSomeTensors;
+        for_adam_tables<CAP>(lists, per, [&](const AdamTable<CAP> &t, double bytes) {
+            launch<k_adam<CAP>>(t.first[t.count], true, bytes, s, "Adam kernel launch", t,
+                                o.decoupled != 0, sc);
+        });
+    });
 }
 
 }  // namespace arcqml

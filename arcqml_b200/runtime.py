@@ -661,6 +661,8 @@ class TensorList:
         if len(devices) > 1:
             raise TypeError("the tensors of a list must be on one device")
         self.device_index = devices.pop() if devices else None
+        self._blank = None if self.device_index is None else torch.empty(
+            0, dtype=torch.float64, device=self.device_index)
         self._table, self._layouts = table, layouts
         self._address = table.ctypes.data
         self._words = load().arcqml_rt_v2_gradient_workspace(self._address, len(self.tensors))
@@ -706,16 +708,17 @@ def _tensor_list(tensors) -> TensorList:
     return tensors if isinstance(tensors, TensorList) else TensorList(tensors)
 
 
-def _call_memory(torch, device: int, stream, words: int, norm: bool):
+def _call_memory(torch, device: int, blank, stream, words: int, norm: bool):
     """(stream, norm, scratch) of one call. All of it is allocated for the call alone, on its stream,
     so calls on other streams and captured graphs share nothing."""
     if stream is not None:
         with torch.cuda.stream(torch.cuda.ExternalStream(int(stream))):
-            return (int(stream),) + _call_memory(torch, device, None, words, norm)[1:]
+            return (int(stream),) + _call_memory(torch, device, blank, None, words, norm)[1:]
     # the raw handle: a Stream object costs as much as the launch
     raw = torch._C._cuda_getCurrentRawStream(device)
-    return (raw, torch.empty((), dtype=torch.float64, device=device) if norm else None,
-            torch.empty(words, dtype=torch.float64, device=device) if words else None)
+    if blank is None:  # a list without tensors
+        blank = torch.empty(0, dtype=torch.float64, device=device)
+    return raw, blank.new_empty(()) if norm else None, blank.new_empty(words) if words else None
 
 
 def _scalar_ptr(torch, device: int, t) -> int:
@@ -733,7 +736,7 @@ def gradient_norm_device(gradients, stream=None):
     g = _tensor_list(gradients)
     device = torch.cuda.current_device()
     table = g._current(torch, device)
-    on, out, ws = _call_memory(torch, device, stream, g._words, True)
+    on, out, ws = _call_memory(torch, device, g._blank, stream, g._words, True)
     _status(load().arcqml_rt_v2_gradient_norm(table, len(g), out.data_ptr(),
                                               None if ws is None else ws.data_ptr(), g._words, on))
     return out
@@ -749,7 +752,7 @@ def clip_gradients_device(gradients, max_norm: float, norm=None, stream=None):
     table = g._current(torch, device)
     g._check_apart("the gradients")
     given = None if norm is None else _scalar_ptr(torch, device, norm)
-    on, out, ws = _call_memory(torch, device, stream, g._words, True)
+    on, out, ws = _call_memory(torch, device, g._blank, stream, g._words, True)
     _status(load().arcqml_rt_v2_clip_gradients(table, len(g), float(max_norm), given,
                                                out.data_ptr(),
                                                None if ws is None else ws.data_ptr(), g._words, on))
@@ -832,7 +835,7 @@ def adam_step_device(parameters, gradients, state: DeviceAdamState, lr: float = 
                 x._check_apart("the " + name)
         state._checked = states
     options = AdamOptions(lr, betas[0], betas[1], eps, weight_decay, max_norm, bool(decoupled), 0)
-    on, out, ws = _call_memory(torch, device, stream, p._adam_words, max_norm >= 0.0)
+    on, out, ws = _call_memory(torch, device, p._blank, stream, p._adam_words, max_norm >= 0.0)
     _status(load().arcqml_rt_v2_adam_step(
         *tables, len(p), state.step.data_ptr(), C.byref(options), given,
         None if out is None else out.data_ptr(), None if ws is None else ws.data_ptr(),
