@@ -603,11 +603,17 @@ class AdamOptions(C.Structure):
                 ("decoupled", C.c_int32), ("reserved", C.c_int32)]
 
 
-def _dtype_code(dtype):
-    """(code of the components, components per element) of a torch dtype, or None."""
-    import torch
-    return {torch.float64: (0, 1), torch.float32: (1, 1), torch.bfloat16: (2, 1),
-            torch.float16: (3, 1), torch.complex128: (0, 2), torch.complex64: (1, 2)}.get(dtype)
+_tensor_types = {}
+
+
+def _tensor_kinds() -> dict:
+    """torch dtype -> (code of the components, components per element, bytes per element)."""
+    if not _tensor_types:
+        import torch
+        _tensor_types.update({
+            torch.float64: (0, 1, 8), torch.float32: (1, 1, 4), torch.bfloat16: (2, 1, 2),
+            torch.float16: (3, 1, 2), torch.complex128: (0, 2, 16), torch.complex64: (1, 2, 8)})
+    return _tensor_types
 
 
 def _layout(t):
@@ -641,38 +647,41 @@ class TensorList:
 
     def _write_down(self) -> None:
         import torch
-        table = np.zeros(max(1, len(self.tensors)), dtype=_TENSOR)
-        layouts, devices = [], set()
+        kinds = _tensor_kinds()
+        rows, self._layouts, spans, devices = [], [], [], set()
         for i, t in enumerate(self.tensors):
             if t is None:
-                table[i] = (0, 0, NO_TENSOR, 0)
-                layouts.append(None)
+                rows.append((0, 0, NO_TENSOR, 0))
+                self._layouts.append(None)
                 continue
-            kind = _dtype_code(t.dtype) if isinstance(t, torch.Tensor) else None
+            kind = kinds.get(t.dtype) if isinstance(t, torch.Tensor) else None
             if kind is None or not t.is_cuda or t.layout != torch.strided or t.is_conj() or \
                     t.is_neg():
                 raise TypeError("a tensor list takes dense float64, float32, bfloat16, float16 and "
                                 f"complex CUDA tensors or None: place {i} holds "
                                 + (f"{t.dtype} on {t.device}" if isinstance(t, torch.Tensor)
                                    else type(t).__name__))
-            layouts.append(_layout(t))
-            devices.add(t.device.index)
-            table[i] = (t.data_ptr(), t.numel() * kind[1], kind[0], 0)
+            self._layouts.append(None if t.is_contiguous() else _layout(t))
+            devices.add(t.get_device())
+            at, n = t.data_ptr(), t.numel()
+            rows.append((at, n * kind[1], kind[0], 0))
+            if n:
+                spans.append((at, at + n * kind[2]))
         if len(devices) > 1:
             raise TypeError("the tensors of a list must be on one device")
         self.device_index = devices.pop() if devices else None
         self._blank = None if self.device_index is None else torch.empty(
             0, dtype=torch.float64, device=self.device_index)
-        self._table, self._layouts = table, layouts
-        self._address = table.ctypes.data
-        self._words = load().arcqml_rt_v2_gradient_workspace(self._address, len(self.tensors))
-        self._adam_words = load().arcqml_rt_v2_adam_workspace(self._address, len(self.tensors))
+        self._table = np.array(rows or [(0, 0, NO_TENSOR, 0)], dtype=_TENSOR)
+        self._address = self._table.ctypes.data
+        self._words = load().arcqml_rt_v2_gradient_workspace(self._address, len(rows))
+        self._adam_words = load().arcqml_rt_v2_adam_workspace(self._address, len(rows))
         self._shapes = [None if t is None else t.shape for t in self.tensors]
-        self._pointers = [t.data_ptr() for t in self._present]
+        self._pointers = [r[0] for r in rows if r[2] != NO_TENSOR]
         # the tensors whose version counters stand for all: views share their base's
         roots = [t._base if t._is_view() else t for t in self._present]
         self._roots = list({id(t): t for t in roots}.values())
-        self._apart = None
+        self._apart = _spans_apart(spans)
         self._state = object()  # another one whenever the list is written down
 
     def _current(self, torch, device: int) -> int:
@@ -686,8 +695,6 @@ class TensorList:
 
     def _check_apart(self, name: str) -> None:
         """Refuses a list that is written to when two of its tensors share memory."""
-        if self._apart is None:
-            self._apart = _tables_apart([self._table])
         if not self._apart:
             raise RuntimeError(f"{name} share memory: each may be in the list once")
 
@@ -696,12 +703,10 @@ class TensorList:
         torch.autograd.graph.increment_version(self._roots)
 
 
-def _tables_apart(tables) -> bool:
-    t = np.concatenate(tables)
-    t = t[(t["dtype"] != NO_TENSOR) & (t["length"] > 0)]
-    t = t[np.argsort(t["data"], kind="stable")]
-    size = np.array([8, 4, 2, 2], dtype=np.uint64)[t["dtype"]]
-    return bool(np.all(t["data"][:-1] + t["length"][:-1] * size[:-1] <= t["data"][1:]))
+def _spans_apart(spans) -> bool:
+    """Whether no two of the (first, end) address ranges overlap."""
+    spans = sorted(spans)
+    return all(a[1] <= b[0] for a, b in zip(spans, spans[1:]))
 
 
 def _tensor_list(tensors) -> TensorList:

@@ -153,10 +153,7 @@ def test_layouts(runtime):
 
 
 def test_shared_memory_is_found(runtime):
-    apart = lambda *rows: runtime._tables_apart([table(runtime, *rows)])  # noqa: E731
-    assert apart() and apart((0, 0, 4, 0)) and apart((64, 4, 1, 0))
-    assert apart((80, 4, 1, 0), (64, 4, 1, 0), (0, 0, 4, 0), (96, 0, 0, 0))
-    assert not apart((76, 4, 1, 0), (64, 4, 1, 0))
-    assert not apart((64, 4, 1, 0), (64, 4, 1, 0))
-    assert apart((64, 4, 2, 0), (72, 4, 3, 0)) and not apart((64, 5, 2, 0), (72, 4, 3, 0))
-    assert apart((64, 4, 0, 0), (96, 1, 0, 0)) and not apart((64, 4, 0, 0), (88, 1, 3, 0))
+    apart = runtime._spans_apart
+    assert apart([]) and apart([(64, 80)]) and apart([(80, 96), (64, 80)])
+    assert not apart([(76, 92), (64, 80)]) and not apart([(64, 80), (64, 80)])
+    assert not apart([(64, 200), (70, 80), (200, 300)])
