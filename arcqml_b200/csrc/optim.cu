@@ -48,8 +48,14 @@ constexpr uint32_t kShortVectors = 256, kShortGroups = 64;
 struct AdamScalars64 {
     double lr, b1, b2, nb1, nb2, eps, wd, down, bc1, bc2, factor;
 };
+// The clip factor in f32, as a power of two and a rest: a factor below f32's normal range (a norm
+// near f32's largest values) keeps its precision.
+struct Factor32 {
+    float pre, rest;
+};
 struct AdamScalars32 {
-    float b1, b2, nb1, nb2, eps, wd, down, rate, root, factor;
+    float b1, b2, nb1, nb2, eps, wd, down, rate, root;
+    Factor32 factor;
 };
 
 // What k_scalars leaves for the launches behind it (the head of the scratch).
@@ -275,6 +281,10 @@ __device__ __forceinline__ double clip_factor(double norm, double max_norm) {
     return f > 1.0 ? 1.0 : f;
 }
 
+__device__ __forceinline__ Factor32 factor32(double f) {
+    return f < 0x1p-126 ? Factor32{0x1p-96f, float(f * 0x1p+96)} : Factor32{1.f, float(f)};
+}
+
 __device__ __forceinline__ double bias_correction(double beta, int64_t t) {
     return 1.0 - pow(beta, double(t));
 }
@@ -289,7 +299,7 @@ __device__ __forceinline__ AdamScalars64 scalars64(const ArcqmlAdamOptions &o, d
 __device__ __forceinline__ AdamScalars32 scalars32(const AdamScalars64 &h) {
     return AdamScalars32{float(h.b1), float(h.b2), float(h.nb1), float(h.nb2), float(h.eps),
                          float(h.wd), float(h.down), float(h.lr / h.bc1), float(1.0 / h.bc2),
-                         float(h.factor)};
+                         factor32(h.factor)};
 }
 
 // One block. given != null: n = *given; else the root of the count sums. step != null: one more
@@ -331,7 +341,14 @@ __device__ __forceinline__ void clip_chunk(void *data, uint64_t length, uint32_t
     using T = typename Elem<DTYPE>::type;
     using W = typename Elem<DTYPE>::wide;
     constexpr int N = 16 / sizeof(T), U = 4;
-    const W f = W(factor);
+    const auto times = [&](W x) {
+        if constexpr (DTYPE == ARCQML_F64) {
+            return x * factor;
+        } else {
+            const Factor32 f = factor32(factor);
+            return x * f.pre * f.rest;
+        }
+    };
     T *p = static_cast<T *>(data);
     const uint32_t head = head_of(p, length);
     const uint64_t vectors = (length - head) / N;
@@ -342,7 +359,7 @@ __device__ __forceinline__ void clip_chunk(void *data, uint64_t length, uint32_t
         W x[N];
         raw.unpack(x);
 #pragma unroll
-        for (int j = 0; j < N; ++j) x[j] *= f;
+        for (int j = 0; j < N; ++j) x[j] = times(x[j]);
         raw.pack(x);
     };
     uint32_t v = lane;
@@ -368,10 +385,10 @@ __device__ __forceinline__ void clip_chunk(void *data, uint64_t length, uint32_t
                 q[v0 + v + u * LANES] = x[u];
             }
     }
-    if (chunk == 0 && lane < head) narrow(widen(p[lane]) * f, p[lane]);
+    if (chunk == 0 && lane < head) narrow(times(widen(p[lane])), p[lane]);
     const uint64_t done = head + vectors * N;
     if (v0 + per >= vectors && lane < length - done)
-        narrow(widen(p[done + lane]) * f, p[done + lane]);
+        narrow(times(widen(p[done + lane])), p[done + lane]);
 }
 
 template <uint32_t LANES, class Table>
@@ -414,7 +431,7 @@ __device__ __forceinline__ void adam_update(double &p, double &m, double &v, dou
 
 __device__ __forceinline__ void adam_update(float &p, float &m, float &v, float g,
                                             const AdamScalars32 &h, bool decoupled) {
-    float a = g * h.factor;
+    float a = g * h.factor.pre * h.factor.rest;
     if (!decoupled) a = fmaf(h.wd, p, a);
     m = fmaf(h.b1, m, h.nb1 * a);
     v = fmaf(h.b2, v, h.nb2 * a * a);

@@ -632,13 +632,14 @@ def _layout(t):
 
 class TensorList:
     """The tensors of a model, or their gradients, as the calls below take them: floating or complex
-    CUDA tensors of one device; None where a parameter has no gradient. Checking a list and writing
+    CUDA tensors of one device (or one such tensor); None where a parameter has no gradient. Checking a list and writing
     it down costs about a microsecond per tensor: a training loop whose tensors stay keeps its lists.
     Every call reads the tensors' addresses anew, and one that has moved (a new ``.data``) is
     checked and written down again; a list whose tensors change shape in place is made anew."""
 
     def __init__(self, tensors):
-        self.tensors = list(tensors)
+        import torch
+        self.tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
         self._present = [t for t in self.tensors if t is not None]
         self._write_down()
 
@@ -681,7 +682,7 @@ class TensorList:
         # the tensors whose version counters stand for all: views share their base's
         roots = [t._base if t._is_view() else t for t in self._present]
         self._roots = list({id(t): t for t in roots}.values())
-        self._apart = _spans_apart(spans)
+        self._spans, self._apart = spans, None
         self._state = object()  # another one whenever the list is written down
 
     def _current(self, torch, device: int) -> int:
@@ -695,6 +696,8 @@ class TensorList:
 
     def _check_apart(self, name: str) -> None:
         """Refuses a list that is written to when two of its tensors share memory."""
+        if self._apart is None:
+            self._apart = _spans_apart(self._spans)
         if not self._apart:
             raise RuntimeError(f"{name} share memory: each may be in the list once")
 
@@ -736,7 +739,8 @@ def _scalar_ptr(torch, device: int, t) -> int:
 def gradient_norm_device(gradients, stream=None):
     """The 2-norm over every element of every tensor of `gradients` (a TensorList, or a sequence of
     CUDA tensors and None) as a float64 CUDA scalar (arcqml_rt_v2_gradient_norm). Nothing is read
-    back: the norm can go into the calls below, or its square into an all-reduce."""
+    back: the norm can go into the calls below, or its square into an all-reduce. With `stream` the
+    call runs on that stream and its result is ready there, here and below."""
     import torch
     g = _tensor_list(gradients)
     device = torch.cuda.current_device()
@@ -789,7 +793,7 @@ class DeviceAdamState:
                 raise ValueError("the step count must not be negative")
             self.step = torch.full((), int(step), dtype=torch.int64, device=device)
         self._m, self._v = TensorList(self.m), TensorList(self.v)
-        self._checked = None
+        self._checked = self._gradients = None
         for name, other in (("first", self._m), ("second", self._v)):
             if other._shapes != p._shapes or other._layouts != p._layouts:
                 raise ValueError(f"the {name} moments must have the parameters' shapes and strides")
@@ -830,15 +834,18 @@ def adam_step_device(parameters, gradients, state: DeviceAdamState, lr: float = 
     tables = [x._current(torch, device) for x in (p, g, m, v)]
     tables.append(None if c is None else c._current(torch, device))
     # the lists are held against one another once, and again when one is written down anew
-    states = (p._state, g._state, m._state, v._state, None if c is None else c._state)
+    states = (p._state, m._state, v._state, None if c is None else c._state)
     if states != state._checked:
-        for name, x in (("gradients", g), ("moments", m), ("moments", v), ("copies", c)):
+        for name, x in (("moments", m), ("moments", v), ("copies", c)):
             if x is not None:
                 _check_places(name, x, p)
-        for name, x in (("parameters", p), ("moments", m), ("moments", v), ("copies", c)):
-            if x is not None:
-                x._check_apart("the " + name)
-        state._checked = states
+        written = [x for x in (p, m, v, c) if x is not None]
+        if not _spans_apart([s for x in written for s in x._spans]):
+            raise RuntimeError("the parameters, moments and copies share memory")
+        state._checked, state._gradients = states, None
+    if state._gradients is not g._state:
+        _check_places("gradients", g, p)
+        state._gradients = g._state
     options = AdamOptions(lr, betas[0], betas[1], eps, weight_decay, max_norm, bool(decoupled), 0)
     on, out, ws = _call_memory(torch, device, p._blank, stream, p._adam_words, max_norm >= 0.0)
     _status(load().arcqml_rt_v2_adam_step(

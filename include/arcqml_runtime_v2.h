@@ -259,7 +259,8 @@ typedef struct ArcqmlAdamOptions {
  * types take gradients of any of those types and f32 moments, and are computed in f32. A place
  * whose gradient is ARCQML_NO_TENSOR is left as it is. copies (may be null; places may be
  * ARCQML_NO_TENSOR) receive the new values of f32 parameters rounded to bf16 or f16. given_norm,
- * norm: as above, used with max_norm >= 0 only. Parameters, moments and copies must not overlap. */
+ * norm: as above, used with max_norm >= 0 only. What the call writes must not overlap anything else
+ * that it takes. *step must not be negative. */
 int32_t arcqml_rt_v2_adam_step(const ArcqmlTensor *parameters, const ArcqmlTensor *gradients,
                                const ArcqmlTensor *first_moments,
                                const ArcqmlTensor *second_moments, const ArcqmlTensor *copies,

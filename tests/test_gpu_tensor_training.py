@@ -142,6 +142,28 @@ def test_infinities_and_nan(runtime, dtype, place):
             assert t.nan_to_num(0.0).eq(0).all()
 
 
+@pytest.mark.parametrize("n", [300, 3_000_000])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_factors_below_the_normal_range(runtime, dtype, n):
+    """Gradients near the type's largest values, and a small maximum: the factor is subnormal in
+    f32, the results are not."""
+    kind = TYPES[dtype]
+    t = (torch.rand(n, generator=gen(9), device="cuda") + 0.5).to(kind) * 1e38
+    was = t.clone()
+    want = ts.norm64([was])
+    runtime.clip_gradients_device([t], 1e-2)
+    y, bound = ts.clip64(was, ts.clip_factor(want, 1e-2), n)
+    assert ts.clip_factor(want, 1e-2) < 2.0 ** -126 and y.min() > 2.0 ** -120
+    ts.assert_within(ts.components(t), y, bound, dtype)
+    run_adam(runtime, [torch.zeros(n, dtype=kind, device="cuda")], [was], max_norm=1e-2)
+
+
+def test_one_tensor_in_place_of_a_list(runtime):
+    t = normal((60, 70), torch.float32, gen(6))
+    check_norm(runtime.gradient_norm_device(t), [t])
+    check_norm(runtime.clip_gradients_device(t[3], 1e9), [t[3]])
+
+
 def test_equal_inputs_give_equal_bits(runtime):
     _, grads = views([300_001, 17, 5_000_000], torch.bfloat16, gen(8), 1)
     first = runtime.gradient_norm_device(grads)
@@ -451,6 +473,10 @@ def test_refusals_on_the_device(runtime):
     with pytest.raises(runtime.RuntimeError, match="share memory"):
         runtime.adam_step_device([a, a], [before.clone(), before.clone()],
                                  runtime.DeviceAdamState([a, a]))
+    z = torch.zeros(100, device="cuda")
+    for m, v in (([z], [z]), ([a], [z]), ([z], [a])):
+        with pytest.raises(runtime.RuntimeError, match="share memory"):
+            runtime.adam_step_device([a], [before.clone()], runtime.DeviceAdamState([a], m=m, v=v))
     with pytest.raises(ValueError, match="moments"):
         runtime.DeviceAdamState([a], m=[torch.zeros(99, device="cuda")])
     with pytest.raises(runtime.RuntimeError, match="first moment"):

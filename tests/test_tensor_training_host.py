@@ -157,3 +157,20 @@ def test_shared_memory_is_found(runtime):
     assert apart([]) and apart([(64, 80)]) and apart([(80, 96), (64, 80)])
     assert not apart([(76, 92), (64, 80)]) and not apart([(64, 80), (64, 80)])
     assert not apart([(64, 200), (70, 80), (200, 300)])
+
+
+def test_hybrid_optimizer_refusals(runtime):
+    from arcqml_b200 import Circuit
+    from arcqml_b200.optim import Adam
+    c = Circuit(2)
+    c.append("ry", (0,), c.add_parameter(0.5, requires_grad=False))
+    for bad in (dict(), dict(circuits=[c]), dict(circuits=[Circuit(1)])):
+        with pytest.raises(ValueError, match="nothing to train"):
+            Adam(**bad)
+    c.append("ry", (1,), c.add_parameter(0.5))
+    with pytest.raises(ValueError, match="trained once"):
+        Adam([c, c])
+    with pytest.raises(TypeError, match="must not be None"):
+        Adam([c], [None])
+    with pytest.raises(TypeError, match="place 0"):
+        Adam([c], [torch.ones(3)])
