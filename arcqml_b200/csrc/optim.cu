@@ -302,34 +302,35 @@ __device__ __forceinline__ AdamScalars32 scalars32(const AdamScalars64 &h) {
                          factor32(h.factor)};
 }
 
-// One block. given != null: n = *given; else the root of the count sums. step != null: one more
-// step is counted.
-__global__ void __launch_bounds__(kOT)
+// One block of a thread per sum. given != null: n = *given; else the root of the count sums.
+// step != null: one more step is counted. The step count is no work of the launch before this one:
+// what follows from it alone is formed while that launch still runs.
+constexpr int kScalarThreads = 1024;
+__global__ void __launch_bounds__(kScalarThreads)
     k_scalars(const double *sums, uint32_t count, const double *given,
               const __grid_constant__ ArcqmlAdamOptions o, int64_t *step, double *norm,
               Scalars *out) {
-    __shared__ double bc[2];
     let_next_start();
-    // the step count is no work of the launch before this one: its powers need not wait
-    int64_t now = 0;
-    if (step) {
-        now = *step + 1;
-        if (threadIdx.x == 32) bc[0] = bias_correction(o.beta1, now);
-        if (threadIdx.x == 64) bc[1] = bias_correction(o.beta2, now);
+    if (step && threadIdx.x == kScalarThreads - 32) {
+        const int64_t now = *step + 1;
+        const AdamScalars64 h =
+            scalars64(o, bias_correction(o.beta1, now), bias_correction(o.beta2, now), 1.0);
+        out->h = h;
+        out->hf = scalars32(h);
     }
     wait_for_last();
     double acc = 0.0;
-    for (uint32_t i = threadIdx.x; i < count; i += kOT) acc += sums[i];
-    acc = o_block_sum<kOT>(acc);
+    for (uint32_t i = threadIdx.x; i < count; i += kScalarThreads) acc += sums[i];
+    acc = o_block_sum<kScalarThreads>(acc);  // and the scalars above are written
     if (threadIdx.x != 0) return;
     const double n = given ? *given : sqrt(acc);
     if (norm) *norm = n;
     const double factor = clip_factor(n, o.max_norm);
     out->factor = factor;
     if (step) {
-        *step = now;
-        out->h = scalars64(o, bc[0], bc[1], factor);
-        out->hf = scalars32(out->h);
+        out->h.factor = factor;
+        out->hf.factor = factor32(factor);
+        *step += 1;
     }
 }
 
@@ -895,7 +896,7 @@ void launch_cluster(uint32_t chunks, double bytes, cudaStream_t s, const char *w
 }
 
 // A launch of `blocks` blocks that, with `follows`, may start while the last one ends.
-template <auto KERNEL, class... Args>
+template <auto KERNEL, int THREADS = kOT, class... Args>
 void launch(uint32_t blocks, bool follows, double bytes, cudaStream_t s, const char *what,
             const Args &...args) {
     cudaLaunchConfig_t c{};
@@ -903,7 +904,7 @@ void launch(uint32_t blocks, bool follows, double bytes, cudaStream_t s, const c
     a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     a.val.programmaticStreamSerializationAllowed = 1;
     c.gridDim = dim3(blocks);
-    c.blockDim = dim3(kOT);
+    c.blockDim = dim3(THREADS);
     c.stream = s;
     c.attrs = &a;
     c.numAttrs = follows ? 1 : 0;
@@ -962,7 +963,7 @@ uint32_t vectors_per_chunk(const ArcqmlTensor *list, size_t count) {
 const Scalars *scalars(uint32_t sums, const double *given, const ArcqmlAdamOptions &o,
                        int64_t *step, double *norm, double *ws, cudaStream_t s) {
     auto *out = reinterpret_cast<Scalars *>(ws);
-    launch<k_scalars>(1, sums != 0, 8.0 * sums, s, "gradient norm kernel launch",
+    launch<k_scalars, kScalarThreads>(1, sums != 0, 8.0 * sums, s, "gradient norm kernel launch",
                       static_cast<const double *>(ws + kScalarDoubles), sums, given, o, step, norm,
                       out);
     return out;
