@@ -56,9 +56,9 @@ constexpr uint32_t kChunk = 2048;
 constexpr uint32_t kFewTensors = 64, kSomeTensors = 512, kMaxTensors = 1500;
 // Short lists: one cluster, a warp per chunk. Against the several launches: norm of 4 MB of f32 in 20
 // tensors 10 and 15 us, clip 16 and 20 us; norm of 17 MB 16 and 11 us; Adam on 0.4 MB of f32
-// parameters 16 and 21 us, on 4 MB 45 and 21 us.
+// parameters 16 and 21 us, on 1.2 MB 20 and 21 us, on 4 MB 45 and 21 us.
 constexpr uint32_t kShortTensors = kFewTensors;
-constexpr uint64_t kShortBytes = uint64_t(4) << 20, kShortAdamBytes = uint64_t(1) << 20;
+constexpr uint64_t kShortBytes = uint64_t(4) << 20, kShortMoments = uint64_t(1) << 20;
 constexpr uint32_t kCluster = 16, kShortThreads = 512;
 // Chunks of a warp: one batch of accesses per thread.
 constexpr uint32_t kShortVectors = 256, kShortGroups = 64;
@@ -797,13 +797,16 @@ void check_tensors(const ArcqmlTensor *list, size_t count, const char *name) {
     if (chunks >> 31) fail(std::string(name) + " list holds too many elements");
 }
 
-// Whether one cluster takes the list in one launch.
-bool is_short(const ArcqmlTensor *list, size_t count, uint64_t most) {
+// Whether one cluster takes a list of gradients in one launch, or (by its moments' bytes) a list of
+// parameters.
+bool is_short(const ArcqmlTensor *list, size_t count, bool adam = false) {
+    const uint64_t most = adam ? kShortMoments : kShortBytes;
     uint64_t bytes = 0;
     uint32_t tensors = 0;
     for (size_t i = 0; i < count; ++i) {
         if (!present(list[i])) continue;
-        bytes += list[i].length * element_size(list[i].dtype);
+        const uint32_t size = element_size(list[i].dtype);
+        bytes += list[i].length * (adam ? std::max(size, 4u) : size);
         if (++tensors > kShortTensors || bytes > most) return false;
     }
     return true;
@@ -1027,17 +1030,17 @@ static size_t workspace_of(size_t count) {
 }
 
 size_t gradient_workspace(const ArcqmlTensor *list, size_t count) {
-    return !list || is_short(list, count, kShortBytes) ? 0 : workspace_of(count);
+    return !list || is_short(list, count) ? 0 : workspace_of(count);
 }
 
 size_t adam_workspace(const ArcqmlTensor *list, size_t count) {
-    return !list || is_short(list, count, kShortAdamBytes) ? 0 : workspace_of(count);
+    return !list || is_short(list, count, true) ? 0 : workspace_of(count);
 }
 
 void gradient_norm_device(const ArcqmlTensor *grads, size_t count, double *norm, double *ws,
                           size_t ws_len, cudaStream_t s) {
     check_tensors(grads, count, "gradient");
-    if (is_short(grads, count, kShortBytes)) return short_clip(grads, count, nullptr, -1.0, norm, s);
+    if (is_short(grads, count)) return short_clip(grads, count, nullptr, -1.0, norm, s);
     check_workspace(ws, ws_len, workspace_of(count));
     const uint32_t sums = square_sums(grads, count, vectors_per_chunk(grads, count), ws, s);
     scalars(sums, nullptr, clip_options(-1.0), nullptr, norm, ws, s);
@@ -1049,7 +1052,7 @@ void clip_gradients_device(const ArcqmlTensor *grads, size_t count, double max_n
     check_tensors(grads, count, "gradient");
     if (!std::isfinite(max_norm) || max_norm < 0.0)
         fail("the maximum norm must be finite and not negative");
-    if (is_short(grads, count, kShortBytes)) return short_clip(grads, count, given, max_norm, norm, s);
+    if (is_short(grads, count)) return short_clip(grads, count, given, max_norm, norm, s);
     check_workspace(ws, ws_len, workspace_of(count));
     const uint32_t per = vectors_per_chunk(grads, count);
     const auto o = clip_options(max_norm);
@@ -1092,7 +1095,7 @@ void adam_step_device(const ArcqmlTensor *params, const ArcqmlTensor *grads,
         fail("invalid Adam hyperparameters (finite lr and weight decay, 0 <= beta < 1, eps >= 0)");
     if (!std::isfinite(o.max_norm)) fail("the maximum norm must be finite");
     if (o.reserved != 0 || (o.decoupled != 0 && o.decoupled != 1)) fail("invalid Adam options");
-    const bool one = is_short(params, count, kShortAdamBytes);
+    const bool one = is_short(params, count, true);
     if (!one) check_workspace(ws, ws_len, workspace_of(count));
     for (size_t i = 0; i < count; ++i) {
         const uint32_t pt = params[i].dtype, wide = pt == ARCQML_F64 ? ARCQML_F64 : ARCQML_F32;

@@ -84,7 +84,6 @@ class Adam:
         self._circuits = [_CircuitParameters(p, d) for p, d in parts]
         self._parameters = rt.TensorList([c.values for c in self._circuits] + self.tensors)
         self.state = rt.DeviceAdamState(self._parameters)
-        self._gradients = None
 
     def zero_grad(self) -> None:
         for c in self._circuits:
@@ -100,10 +99,8 @@ class Adam:
         has = [c.upload() for c in self._circuits]
         grads = [c.gradient if h else None for c, h in zip(self._circuits, has)]
         grads += [t.grad for t in self.tensors]
-        old = self._gradients
-        if old is None or any(a is not b for a, b in zip(old.tensors, grads)):
-            self._gradients = rt.TensorList(grads)
-        norm = rt.adam_step_device(self._parameters, self._gradients, self.state, lr=self.lr,
+        # a new list every step: one that is kept would keep the gradients' memory
+        norm = rt.adam_step_device(self._parameters, grads, self.state, lr=self.lr,
                                    betas=self.betas, eps=self.eps, weight_decay=self.weight_decay,
                                    decoupled=self.decoupled, max_norm=self.max_norm)
         moved = [c for c, h in zip(self._circuits, has) if h]

@@ -589,7 +589,6 @@ def small_adam_device(plan: CircuitPlan, observable: "Observable", num_qubits: i
     return energies, params
 
 
-
 # ------------------------------------------------------------------ training over many tensors
 
 NO_TENSOR = 4
@@ -632,28 +631,32 @@ def _layout(t):
 
 class TensorList:
     """The tensors of a model, or their gradients, as the calls below take them: floating or complex
-    CUDA tensors of one device (or one such tensor); None where a parameter has no gradient. Checking a list and writing
-    it down costs about a microsecond per tensor: a training loop whose tensors stay keeps its lists.
-    Every call reads the tensors' addresses anew, and one that has moved (a new ``.data``) is
-    checked and written down again; a list whose tensors change shape in place is made anew."""
+    CUDA tensors of one device (or one such tensor); None where a parameter has no gradient. Checking
+    a list and writing it down costs about two microseconds per tensor: a training loop whose tensors
+    stay keeps its lists. Every call reads the tensors' addresses anew, and one that has moved (a new
+    ``.data``) is checked and written down again; for tensors that change shape where they are (a
+    view of their own memory, ``resize_``) a new list is made. A list keeps its tensors' memory alive."""
 
     def __init__(self, tensors):
         import torch
-        self.tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+        self.tensors = (tensors,) if isinstance(tensors, torch.Tensor) else tuple(tensors)
         self._present = [t for t in self.tensors if t is not None]
         self._write_down()
 
     def __len__(self) -> int:
         return len(self.tensors)
 
+    def __reduce__(self):  # a copy is written down anew
+        return TensorList, (self.tensors,)
+
     def _write_down(self) -> None:
         import torch
         kinds = _tensor_kinds()
-        rows, self._layouts, spans, devices = [], [], [], set()
+        rows, layouts, spans, devices = [], [], [], set()
         for i, t in enumerate(self.tensors):
             if t is None:
                 rows.append((0, 0, NO_TENSOR, 0))
-                self._layouts.append(None)
+                layouts.append(None)
                 continue
             kind = kinds.get(t.dtype) if isinstance(t, torch.Tensor) else None
             if kind is None or not t.is_cuda or t.layout != torch.strided or t.is_conj() or \
@@ -662,7 +665,7 @@ class TensorList:
                                 f"complex CUDA tensors or None: place {i} holds "
                                 + (f"{t.dtype} on {t.device}" if isinstance(t, torch.Tensor)
                                    else type(t).__name__))
-            self._layouts.append(None if t.is_contiguous() else _layout(t))
+            layouts.append(None if t.is_contiguous() else _layout(t))
             devices.add(t.get_device())
             at, n = t.data_ptr(), t.numel()
             rows.append((at, n * kind[1], kind[0], 0))
@@ -670,6 +673,9 @@ class TensorList:
                 spans.append((at, at + n * kind[2]))
         if len(devices) > 1:
             raise TypeError("the tensors of a list must be on one device")
+        # With the memory held, a tensor at the address it had is in the memory it had: nothing else
+        # can have been put there since.
+        self._held = [t.detach() for t in self._present]
         self.device_index = devices.pop() if devices else None
         self._blank = None if self.device_index is None else torch.empty(
             0, dtype=torch.float64, device=self.device_index)
@@ -677,12 +683,12 @@ class TensorList:
         self._address = self._table.ctypes.data
         self._words = load().arcqml_rt_v2_gradient_workspace(self._address, len(rows))
         self._adam_words = load().arcqml_rt_v2_adam_workspace(self._address, len(rows))
+        self._layouts, self._spans, self._apart = layouts, spans, None
         self._shapes = [None if t is None else t.shape for t in self.tensors]
         self._pointers = [r[0] for r in rows if r[2] != NO_TENSOR]
         # the tensors whose version counters stand for all: views share their base's
         roots = [t._base if t._is_view() else t for t in self._present]
         self._roots = list({id(t): t for t in roots}.values())
-        self._spans, self._apart = spans, None
         self._state = object()  # another one whenever the list is written down
 
     def _current(self, torch, device: int) -> int:
@@ -780,23 +786,27 @@ class DeviceAdamState:
         p = _tensor_list(parameters)
         if len(p._present) != len(p):
             raise TypeError("a parameter list has no empty places")
-        self.m = self._zeros(p) if m is None else list(m)
-        self.v = self._zeros(p) if v is None else list(v)
+        self.m = list(self._zeros(p) if m is None else m)
+        self.v = list(self._zeros(p) if v is None else v)
         device = torch.device("cuda", torch.cuda.current_device() if p.device_index is None
                               else p.device_index)
         if isinstance(step, torch.Tensor):
             if step.dtype != torch.int64 or step.numel() != 1 or step.device != device:
                 raise TypeError(f"the step count must be one int64 on {device}")
-            self.step = step
+            self._step = step
         else:
             if int(step) < 0:
                 raise ValueError("the step count must not be negative")
-            self.step = torch.full((), int(step), dtype=torch.int64, device=device)
+            self._step = torch.full((), int(step), dtype=torch.int64, device=device)
         self._m, self._v = TensorList(self.m), TensorList(self.v)
         self._checked = self._gradients = None
         for name, other in (("first", self._m), ("second", self._v)):
             if other._shapes != p._shapes or other._layouts != p._layouts:
                 raise ValueError(f"the {name} moments must have the parameters' shapes and strides")
+
+    @property
+    def step(self):
+        return self._step
 
     @staticmethod
     def _zeros(p: TensorList):
@@ -831,6 +841,9 @@ def adam_step_device(parameters, gradients, state: DeviceAdamState, lr: float = 
         max_norm, given = float(max_norm), None if norm is None else _scalar_ptr(torch, device, norm)
         if not max_norm >= 0.0:
             raise ValueError("the maximum norm must be finite and not negative")
+    if state._step.get_device() != device:
+        raise RuntimeError(f"the step count is on {state._step.device} and the current device is "
+                           f"cuda:{device}")
     tables = [x._current(torch, device) for x in (p, g, m, v)]
     tables.append(None if c is None else c._current(torch, device))
     # the lists are held against one another once, and again when one is written down anew
@@ -849,7 +862,7 @@ def adam_step_device(parameters, gradients, state: DeviceAdamState, lr: float = 
     options = AdamOptions(lr, betas[0], betas[1], eps, weight_decay, max_norm, bool(decoupled), 0)
     on, out, ws = _call_memory(torch, device, p._blank, stream, p._adam_words, max_norm >= 0.0)
     _status(load().arcqml_rt_v2_adam_step(
-        *tables, len(p), state.step.data_ptr(), C.byref(options), given,
+        *tables, len(p), state._step.data_ptr(), C.byref(options), given,
         None if out is None else out.data_ptr(), None if ws is None else ws.data_ptr(),
         p._adam_words, on))
     p._written(torch)

@@ -525,3 +525,57 @@ def test_mixed_long_lists(runtime, narrow):
     run_adam(runtime, params, grads, max_norm=1.0, wd=0.01, steps=2)
     check_norm(runtime.gradient_norm_device(grads), grads)
     run_adam(runtime, params, [None, None] + grads[2:], max_norm=1.0)
+
+
+def test_a_list_keeps_its_memory(runtime):
+    """Memory that a list has written down is not given to another tensor while the list lives, so
+    an address that is met again is the same memory."""
+    p = torch.nn.Parameter(torch.ones(1 << 20, device="cuda"))
+    pl = runtime.TensorList([p])
+    at = p.data_ptr()
+    p.data = torch.empty(0, device="cuda")  # the parameter's memory would be free now
+    others = [torch.empty(1 << 20, device="cuda") for _ in range(4)]
+    assert at not in [t.data_ptr() for t in others]
+    del others
+    p.data = torch.full((1 << 10,), 2.0, device="cuda")
+    assert abs(float(runtime.gradient_norm_device(pl)) - 64.0) <= 1e-12  # sqrt(1024 * 4)
+
+
+def test_copies_of_lists_and_states_are_their_own(runtime):
+    import copy
+    g = gen(97)
+    p, q = [normal((300,), torch.float32, g)], [normal((300,), torch.float32, g)]
+    state = runtime.DeviceAdamState(p)
+    runtime.adam_step_device(p, q, state)
+    other, ql = copy.deepcopy(state), copy.deepcopy(runtime.TensorList(q))
+    assert ql.tensors[0].data_ptr() != q[0].data_ptr()
+    check_norm(runtime.gradient_norm_device(ql), q)
+    p2 = [p[0].clone()]
+    for _ in range(3):
+        runtime.adam_step_device(p, q, state)
+        runtime.adam_step_device(p2, ql, other)
+    assert torch.equal(p[0], p2[0]) and torch.equal(state.v[0], other.v[0])
+    assert state.v[0].data_ptr() != other.v[0].data_ptr() and int(other.step) == 4
+    with pytest.raises(AttributeError):
+        state.step = 5
+
+
+def test_no_momentum(runtime):
+    g = gen(98)
+    p, q = [normal((3000,), torch.float32, g)], [normal((3000,), torch.float32, g)]
+    run_adam(runtime, p, q, betas=(0.0, 0.0), lr=0.1, steps=2)
+    run_adam(runtime, p, q, betas=(0.0, 0.999), lr=0.1, eps=1e-3, wd=0.1, max_norm=1.0)
+
+
+@pytest.mark.parametrize("n", [262_144, 262_145])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_both_sides_of_the_short_list(runtime, dtype, n):
+    g = gen(99)
+    p, q = [normal((n,), TYPES[dtype], g)], [normal((n,), TYPES[dtype], g)]
+    run_adam(runtime, p, q, max_norm=1.0, wd=0.01)
+    big = [normal((4 * n,), torch.float32, g)]  # 4 MB, and a little more
+    check_norm(runtime.gradient_norm_device(big), big)
+    was, norm = big[0].clone(), ts.norm64(big)
+    runtime.clip_gradients_device(big, 3.0)
+    y, bound = ts.clip64(was, ts.clip_factor(norm, 3.0), 4 * n)
+    ts.assert_within(ts.components(big[0]), y, bound, "clip")
