@@ -54,11 +54,13 @@ constexpr uint32_t kChunk = 2048;
 // Tensors of one launch. A launch costs the host 2.3 us more with 28 KB of parameters than with 3 KB,
 // and blocks look their tensor up faster in a small table.
 constexpr uint32_t kFewTensors = 64, kSomeTensors = 512, kMaxTensors = 1500;
-// Short lists: one cluster, a warp per chunk. Against the several launches: norm of 4 MB of f32 in 20
-// tensors 10 and 15 us, clip 16 and 20 us; norm of 17 MB 16 and 11 us; Adam on 0.4 MB of f32
-// parameters 16 and 21 us, on 1.2 MB 20 and 21 us, on 4 MB 45 and 21 us.
+// Short lists: one cluster, a warp per chunk. Against the several launches (whose time is the host's),
+// f32 in 20 tensors: norm of 4 MB 10 and 12 us, of 6 MB 12 and 12, of 10 MB 16 and 12; clip of 2 MB 12
+// and 15, of 2.8 MB 14 and 15, of 4 MB 16 and 15; Adam with 0.8 MB in each array 17 and 21, with 1.2 MB
+// 20 and 21, with 1.6 MB 25 and 21.
 constexpr uint32_t kShortTensors = kFewTensors;
-constexpr uint64_t kShortBytes = uint64_t(4) << 20, kShortMoments = uint64_t(1) << 20;
+constexpr uint64_t kShortNorm = uint64_t(6) << 20, kShortClip = uint64_t(5) << 19,
+                   kShortMoments = uint64_t(1) << 20;
 constexpr uint32_t kCluster = 16, kShortThreads = 512;
 // Chunks of a warp: one batch of accesses per thread.
 constexpr uint32_t kShortVectors = 256, kShortGroups = 64;
@@ -797,10 +799,9 @@ void check_tensors(const ArcqmlTensor *list, size_t count, const char *name) {
     if (chunks >> 31) fail(std::string(name) + " list holds too many elements");
 }
 
-// Whether one cluster takes a list of gradients in one launch, or (by its moments' bytes) a list of
-// parameters.
-bool is_short(const ArcqmlTensor *list, size_t count, bool adam = false) {
-    const uint64_t most = adam ? kShortMoments : kShortBytes;
+// Whether one cluster takes the list in one launch: a list of gradients by its bytes, a list of
+// parameters (adam) by its moments'.
+bool is_short(const ArcqmlTensor *list, size_t count, uint64_t most, bool adam = false) {
     uint64_t bytes = 0;
     uint32_t tensors = 0;
     for (size_t i = 0; i < count; ++i) {
@@ -1030,17 +1031,17 @@ static size_t workspace_of(size_t count) {
 }
 
 size_t gradient_workspace(const ArcqmlTensor *list, size_t count) {
-    return !list || is_short(list, count) ? 0 : workspace_of(count);
+    return !list || is_short(list, count, kShortClip) ? 0 : workspace_of(count);
 }
 
 size_t adam_workspace(const ArcqmlTensor *list, size_t count) {
-    return !list || is_short(list, count, true) ? 0 : workspace_of(count);
+    return !list || is_short(list, count, kShortMoments, true) ? 0 : workspace_of(count);
 }
 
 void gradient_norm_device(const ArcqmlTensor *grads, size_t count, double *norm, double *ws,
                           size_t ws_len, cudaStream_t s) {
     check_tensors(grads, count, "gradient");
-    if (is_short(grads, count)) return short_clip(grads, count, nullptr, -1.0, norm, s);
+    if (is_short(grads, count, kShortNorm)) return short_clip(grads, count, nullptr, -1.0, norm, s);
     check_workspace(ws, ws_len, workspace_of(count));
     const uint32_t sums = square_sums(grads, count, vectors_per_chunk(grads, count), ws, s);
     scalars(sums, nullptr, clip_options(-1.0), nullptr, norm, ws, s);
@@ -1052,7 +1053,7 @@ void clip_gradients_device(const ArcqmlTensor *grads, size_t count, double max_n
     check_tensors(grads, count, "gradient");
     if (!std::isfinite(max_norm) || max_norm < 0.0)
         fail("the maximum norm must be finite and not negative");
-    if (is_short(grads, count)) return short_clip(grads, count, given, max_norm, norm, s);
+    if (is_short(grads, count, kShortClip)) return short_clip(grads, count, given, max_norm, norm, s);
     check_workspace(ws, ws_len, workspace_of(count));
     const uint32_t per = vectors_per_chunk(grads, count);
     const auto o = clip_options(max_norm);
@@ -1095,7 +1096,7 @@ void adam_step_device(const ArcqmlTensor *params, const ArcqmlTensor *grads,
         fail("invalid Adam hyperparameters (finite lr and weight decay, 0 <= beta < 1, eps >= 0)");
     if (!std::isfinite(o.max_norm)) fail("the maximum norm must be finite");
     if (o.reserved != 0 || (o.decoupled != 0 && o.decoupled != 1)) fail("invalid Adam options");
-    const bool one = is_short(params, count, true);
+    const bool one = is_short(params, count, kShortMoments, true);
     if (!one) check_workspace(ws, ws_len, workspace_of(count));
     for (size_t i = 0; i < count; ++i) {
         const uint32_t pt = params[i].dtype, wide = pt == ARCQML_F64 ? ARCQML_F64 : ARCQML_F32;

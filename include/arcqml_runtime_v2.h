@@ -217,7 +217,8 @@ typedef struct ArcqmlTensor {
 
 /* Doubles of device scratch that a call takes for its list: the norm and clipping for their
  * gradients, the Adam step for its parameters. 0 for a short list, whose calls take a null
- * workspace. It depends on the places, types and lengths alone. The scratch belongs to one call at a
+ * workspace (a norm also takes one that it does not need). It depends on the places, types and
+ * lengths alone. The scratch belongs to one call at a
  * time: calls that can overlap (other streams, replayed graphs) need their own. */
 size_t arcqml_rt_v2_gradient_workspace(const ArcqmlTensor *gradients, size_t num_tensors);
 size_t arcqml_rt_v2_adam_workspace(const ArcqmlTensor *parameters, size_t num_tensors);

@@ -573,9 +573,11 @@ def test_both_sides_of_the_short_list(runtime, dtype, n):
     g = gen(99)
     p, q = [normal((n,), TYPES[dtype], g)], [normal((n,), TYPES[dtype], g)]
     run_adam(runtime, p, q, max_norm=1.0, wd=0.01)
-    big = [normal((4 * n,), torch.float32, g)]  # 4 MB, and a little more
-    check_norm(runtime.gradient_norm_device(big), big)
-    was, norm = big[0].clone(), ts.norm64(big)
-    runtime.clip_gradients_device(big, 3.0)
-    y, bound = ts.clip64(was, ts.clip_factor(norm, 3.0), 4 * n)
-    ts.assert_within(ts.components(big[0]), y, bound, "clip")
+    # 2.5, 4 and 6 MB of gradients, and a little more
+    for big in (5 * n // 2, 4 * n, 6 * n):
+        t = normal((big,), torch.float32, g)
+        check_norm(runtime.gradient_norm_device([t]), [t])
+        was, norm = t.clone(), ts.norm64([t])
+        runtime.clip_gradients_device([t], 3.0)
+        y, bound = ts.clip64(was, ts.clip_factor(norm, 3.0), big)
+        ts.assert_within(ts.components(t), y, bound, "clip")
