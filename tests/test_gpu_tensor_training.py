@@ -581,3 +581,17 @@ def test_both_sides_of_the_short_list(runtime, dtype, n):
         runtime.clip_gradients_device([t], 3.0)
         y, bound = ts.clip64(was, ts.clip_factor(norm, 3.0), big)
         ts.assert_within(ts.components(t), y, bound, "clip")
+
+
+def test_launches_are_counted_and_timed(runtime):
+    g = gen(101)
+    short, long = [normal((100,), torch.float32, g)], [normal((3_000_000,), torch.float32, g)]
+    runtime.gradient_norm_device(long)
+    for grads, launches, nbytes in ((short, 1, 400.0), (long, 2, 12e6)):
+        before = runtime.launch_count()
+        runtime.profile_enable(True)
+        runtime.gradient_norm_device(grads)
+        other = runtime.profile_read()["other"]
+        runtime.profile_enable(False)
+        assert runtime.launch_count() - before == launches and other[0] == launches
+        assert nbytes <= other[2] <= nbytes + 1e4
