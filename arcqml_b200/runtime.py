@@ -775,19 +775,34 @@ def clip_gradients_device(gradients, max_norm: float, norm=None, stream=None):
     return out
 
 
+class _Moments(list):
+    """The tensors of a written-down list. Another tensor put in a place would not be seen by the steps,
+    so that is refused. Copies and pickles are plain lists."""
+
+    def _refuse(self, *args, **kwargs):
+        raise TypeError("moments are written in place (state.m[i].copy_(...)) or assigned as a whole "
+                        "(state.m = [...])")
+
+    __setitem__ = __delitem__ = __iadd__ = __imul__ = _refuse
+    append = clear = extend = insert = pop = remove = reverse = sort = _refuse
+
+    def __reduce__(self):
+        return list, (list(self),)
+
+
 class DeviceAdamState:
     """Moments and step count of Adam over device tensors (``adam_step_device``): ``m`` and ``v``
     hold one tensor per parameter, of its shape and strides, in float32 (float64 or complex128 for
     float64 and complex128 parameters, complex64 for complex64 ones); ``step`` is an int64 CUDA
-    scalar with the steps taken. They start at zero, or continue the ones given."""
+    scalar with the steps taken. They start at zero, or continue the ones given. Saved ones go on in an
+    existing state when they are copied into its tensors (``state.step.copy_``) or, for the moments,
+    when whole lists are assigned."""
 
     def __init__(self, parameters, m=None, v=None, step=0):
         import torch
         p = _tensor_list(parameters)
         if len(p._present) != len(p):
             raise TypeError("a parameter list has no empty places")
-        self.m = list(self._zeros(p) if m is None else m)
-        self.v = list(self._zeros(p) if v is None else v)
         device = torch.device("cuda", torch.cuda.current_device() if p.device_index is None
                               else p.device_index)
         if isinstance(step, torch.Tensor):
@@ -798,15 +813,36 @@ class DeviceAdamState:
             if int(step) < 0:
                 raise ValueError("the step count must not be negative")
             self._step = torch.full((), int(step), dtype=torch.int64, device=device)
-        self._m, self._v = TensorList(self.m), TensorList(self.v)
+        self._m = self._fitting("first", self._zeros(p) if m is None else m, p)
+        self._v = self._fitting("second", self._zeros(p) if v is None else v, p)
         self._checked = self._gradients = None
-        for name, other in (("first", self._m), ("second", self._v)):
-            if other._shapes != p._shapes or other._layouts != p._layouts:
-                raise ValueError(f"the {name} moments must have the parameters' shapes and strides")
+
+    @property
+    def m(self):
+        return _Moments(self._m.tensors)
+
+    @m.setter
+    def m(self, tensors):
+        self._m = self._fitting("first", tensors, self._m)
+
+    @property
+    def v(self):
+        return _Moments(self._v.tensors)
+
+    @v.setter
+    def v(self, tensors):
+        self._v = self._fitting("second", tensors, self._v)
 
     @property
     def step(self):
         return self._step
+
+    @staticmethod
+    def _fitting(name: str, tensors, like: TensorList) -> TensorList:
+        x = TensorList(tensors)
+        if x._shapes != like._shapes or x._layouts != like._layouts:
+            raise ValueError(f"the {name} moments must have the parameters' shapes and strides")
+        return x
 
     @staticmethod
     def _zeros(p: TensorList):

@@ -1,0 +1,80 @@
+"""What a training program does with the state and the lists of the tensor operators between its
+steps (needs a B200)."""
+import copy
+import pickle
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def normal(n, seed, dtype=torch.float32):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(n, generator=g, device="cuda", dtype=dtype)
+
+
+def test_assigned_moments_are_the_ones_that_the_step_takes(runtime):
+    """A run that goes on from saved moments and one that was never stopped are equal bit by bit."""
+    p, q = [normal(300, 1), normal(80, 2, torch.float64)], [normal(300, 3), normal(80, 4, torch.float64)]
+    state = runtime.DeviceAdamState(p)
+    for _ in range(3):
+        runtime.adam_step_device(p, q, state)
+    saved = [[t.clone() for t in x] for x in (p, state.m, state.v)]
+    runtime.adam_step_device(p, q, state)
+
+    by_list = runtime.DeviceAdamState(saved[0])
+    runtime.adam_step_device([t.clone() for t in saved[0]], q, by_list)  # used before, other moments
+    by_list.m, by_list.v = [t.clone() for t in saved[1]], tuple(t.clone() for t in saved[2])
+    by_list.step.fill_(3)
+    p2 = [t.clone() for t in saved[0]]
+    runtime.adam_step_device(p2, q, by_list)
+    in_place = runtime.DeviceAdamState(saved[0])
+    for mine, old in zip(in_place.m + in_place.v, saved[1] + saved[2]):
+        mine.copy_(old)
+    in_place.step.copy_(torch.tensor(3))
+    p3 = [t.clone() for t in saved[0]]
+    runtime.adam_step_device(p3, q, in_place)
+    for other, params in ((by_list, p2), (in_place, p3)):
+        assert int(other.step) == 4
+        for a, b in zip(p + state.m + state.v, params + other.m + other.v):
+            assert torch.equal(a, b)
+
+
+def test_moments_cannot_be_replaced_unseen(runtime):
+    p = [normal(30, 1), normal(40, 2)]
+    state = runtime.DeviceAdamState(p)
+    t = torch.zeros(30, device="cuda")
+    for change in (lambda m: m.__setitem__(0, t), lambda m: m.append(t), lambda m: m.pop(),
+                   lambda m: m.clear(), lambda m: m.__delitem__(0), lambda m: m.extend([t]),
+                   lambda m: m.insert(0, t), lambda m: m.reverse()):
+        for moments in (state.m, state.v):
+            with pytest.raises(TypeError, match="assigned as a whole"):
+                change(moments)
+    with pytest.raises(TypeError, match="assigned as a whole"):
+        state.m += [t]
+    for bad in ([t], [t, t], [t, None], [t[:29], torch.zeros(40, device="cuda")]):
+        with pytest.raises(ValueError, match="first moments"):
+            state.m = bad
+        with pytest.raises(ValueError, match="second moments"):
+            state.v = bad
+    # assigned moments are held against the parameters like any others
+    q = [normal(30, 3), normal(40, 4)]
+    state.m = [p[0], torch.zeros(40, device="cuda")]
+    with pytest.raises(runtime.RuntimeError, match="share memory"):
+        runtime.adam_step_device(p, q, state)
+    state.m = [torch.zeros(n, device="cuda", dtype=torch.float64) for n in (30, 40)]
+    with pytest.raises(runtime.RuntimeError, match="first moment"):
+        runtime.adam_step_device(p, q, state)
+    assert int(state.step) == 0
+    state.m = [torch.zeros_like(x) for x in p]
+    runtime.adam_step_device(p, q, state)
+    assert int(state.step) == 1 and all(bool((m != 0).all()) for m in state.m)
+
+
+def test_copies_of_moments_are_plain_lists(runtime):
+    state = runtime.DeviceAdamState([normal(30, 1)])
+    for other in (copy.copy(state.m), copy.deepcopy(state.m), pickle.loads(pickle.dumps(state.m))):
+        assert type(other) is list and torch.equal(other[0], state.m[0])
+        other[0] = None
+    assert state.m[0] is not None
