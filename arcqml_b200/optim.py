@@ -54,11 +54,12 @@ class _CircuitParameters:
 
 
 class Adam:
-    """Adam over ``circuits`` (their parameters with ``requires_grad``) and ``tensors`` (floating or
-    complex CUDA tensors). ``weight_decay`` is coupled (added to the gradient, as in the reference)
-    unless ``decoupled``; ``max_norm`` clips by the global norm of all gradients. A tensor without
-    gradient, and a circuit without any, stays as it is and out of the norm. The moments and the
-    step count are ``state`` (``runtime.DeviceAdamState``), the circuits' vectors first."""
+    """Adam over ``circuits`` (the parameters with ``requires_grad`` that they have now) and
+    ``tensors`` (floating or complex CUDA tensors). ``weight_decay`` is coupled (added to the gradient,
+    as in the reference) unless ``decoupled``; ``max_norm`` clips by the global norm of all gradients.
+    A tensor without gradient, and a circuit without any, stays as it is and out of the norm. The
+    moments and the step count are ``state`` (``runtime.DeviceAdamState``), the circuits' vectors
+    first."""
 
     def __init__(self, circuits=(), tensors=(), lr: float = 0.05, betas=(0.9, 0.999),
                  eps: float = 1e-8, weight_decay: float = 0.0, decoupled: bool = False,
@@ -66,8 +67,8 @@ class Adam:
         import torch
         self.lr, self.betas, self.eps = lr, betas, eps
         self.weight_decay, self.decoupled, self.max_norm = weight_decay, decoupled, max_norm
-        self.tensors = list(tensors)
-        if any(t is None for t in self.tensors):
+        self._tensors = tuple(tensors)
+        if any(t is None for t in self._tensors):
             raise TypeError("the tensors to train must not be None")
         parts = []
         for c in circuits:
@@ -78,18 +79,23 @@ class Adam:
         everything = [id(p) for trained, _ in parts for p in trained]
         if len(set(everything)) != len(everything):
             raise ValueError("a circuit parameter may be trained once")
-        if not parts and not self.tensors:
+        if not parts and not self._tensors:
             raise ValueError("there is nothing to train")
-        rt.TensorList(self.tensors)._check_apart("the tensors")
+        rt.TensorList(self._tensors)._check_apart("the tensors")
         self._circuits = [_CircuitParameters(p, d) for p, d in parts]
-        self._parameters = rt.TensorList([c.values for c in self._circuits] + self.tensors)
+        self._parameters = rt.TensorList([c.values for c in self._circuits] + list(self._tensors))
         self.state = rt.DeviceAdamState(self._parameters)
+
+    @property
+    def tensors(self) -> tuple:
+        """The trained tensors. Others need an optimizer, and moments, of their own."""
+        return self._tensors
 
     def zero_grad(self) -> None:
         for c in self._circuits:
             for p in c.parameters:
                 p.grad = None
-        for t in self.tensors:
+        for t in self._tensors:
             t.grad = None
 
     def step(self):
@@ -98,7 +104,7 @@ class Adam:
         import torch
         has = [c.upload() for c in self._circuits]
         grads = [c.gradient if h else None for c, h in zip(self._circuits, has)]
-        grads += [t.grad for t in self.tensors]
+        grads += [t.grad for t in self._tensors]
         # a new list every step: one that is kept would keep the gradients' memory
         norm = rt.adam_step_device(self._parameters, grads, self.state, lr=self.lr,
                                    betas=self.betas, eps=self.eps, weight_decay=self.weight_decay,

@@ -78,3 +78,23 @@ def test_copies_of_moments_are_plain_lists(runtime):
         assert type(other) is list and torch.equal(other[0], state.m[0])
         other[0] = None
     assert state.m[0] is not None
+
+
+def test_an_optimizers_tensors_cannot_be_replaced_unseen(runtime):
+    """A tensor put in another's place would have its gradient applied to the other one."""
+    from arcqml_b200.optim import Adam
+    a, b = (torch.zeros(3, device="cuda").requires_grad_(True) for _ in range(2))
+    opt = Adam(tensors=[a])
+    with pytest.raises(TypeError):
+        opt.tensors[0] = b
+    with pytest.raises(AttributeError):
+        opt.tensors = [b]
+    with pytest.raises(AttributeError):
+        opt.tensors.append(b)
+    assert len(opt.tensors) == 1 and opt.tensors[0] is a
+    b.grad = torch.ones(3, device="cuda")
+    opt.step()
+    assert bool((a == 0).all()) and bool((b == 0).all())
+    a.grad = torch.ones(3, device="cuda")
+    opt.step()
+    assert bool((a < 0).all()) and bool((b == 0).all())
