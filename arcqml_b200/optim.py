@@ -55,11 +55,11 @@ class _CircuitParameters:
 
 class Adam:
     """Adam over ``circuits`` (the parameters with ``requires_grad`` that they have now) and
-    ``tensors`` (floating or complex CUDA tensors). ``weight_decay`` is coupled (added to the gradient,
-    as in the reference) unless ``decoupled``; ``max_norm`` clips by the global norm of all gradients.
-    A tensor without gradient, and a circuit without any, stays as it is and out of the norm. The
-    moments and the step count are ``state`` (``runtime.DeviceAdamState``), the circuits' vectors
-    first."""
+    ``tensors`` (floating or complex CUDA tensors that autograd leaves gradients in, or one such
+    tensor). ``weight_decay`` is coupled (added to the gradient, as in the reference) unless
+    ``decoupled``; ``max_norm`` clips by the global norm of all gradients. A tensor without gradient,
+    and a circuit without any, stays as it is and out of the norm. The moments and the step count are
+    ``state`` (``runtime.DeviceAdamState``), the circuits' vectors first."""
 
     def __init__(self, circuits=(), tensors=(), lr: float = 0.05, betas=(0.9, 0.999),
                  eps: float = 1e-8, weight_decay: float = 0.0, decoupled: bool = False,
@@ -67,9 +67,13 @@ class Adam:
         import torch
         self.lr, self.betas, self.eps = lr, betas, eps
         self.weight_decay, self.decoupled, self.max_norm = weight_decay, decoupled, max_norm
-        self._tensors = tuple(tensors)
-        if any(t is None for t in self._tensors):
-            raise TypeError("the tensors to train must not be None")
+        self._tensors = (tensors,) if isinstance(tensors, torch.Tensor) else tuple(tensors)
+        for i, t in enumerate(self._tensors):
+            if t is None:
+                raise TypeError("the tensors to train must not be None")
+            if isinstance(t, torch.Tensor) and not (t.is_leaf or t.retains_grad):
+                raise ValueError(f"the tensor to train at place {i} was computed from others: its "
+                                 "gradient would go to them")
         parts = []
         for c in circuits:
             for name, dtype in (("f64", torch.float64), ("f32", torch.float32)):

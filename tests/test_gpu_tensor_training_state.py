@@ -98,3 +98,14 @@ def test_an_optimizers_tensors_cannot_be_replaced_unseen(runtime):
     a.grad = torch.ones(3, device="cuda")
     opt.step()
     assert bool((a < 0).all()) and bool((b == 0).all())
+
+
+def test_an_optimizer_of_one_tensor(runtime):
+    from arcqml_b200.optim import Adam
+    w = torch.ones(4, 3, device="cuda", requires_grad=True)
+    opt = Adam(tensors=w, lr=0.5)
+    (w * w).sum().backward()
+    opt.step()
+    # the first step moves each value by lr against its gradient's sign, to a rounding of 1 / (1 + eps)
+    assert len(opt.tensors) == 1 and bool(((w - 0.5).abs() <= 1e-6).all())
+    assert opt.state.m[0].shape == (4, 3)

@@ -174,3 +174,18 @@ def test_hybrid_optimizer_refusals(runtime):
         Adam([c], [None])
     with pytest.raises(TypeError, match="place 0"):
         Adam([c], [torch.ones(3)])
+
+
+def test_hybrid_optimizer_takes_no_computed_tensors(runtime):
+    """Their gradients go to the tensors that they were computed from: they would never move."""
+    from arcqml_b200.optim import Adam
+    w = torch.ones(4, 3, requires_grad=True)
+    for bad in ([2 * w], w.unbind(), [w[0]], [torch.ones(2), w.t()]):
+        with pytest.raises(ValueError, match="computed from others"):
+            Adam(tensors=bad)
+    # what keeps its gradient, and one tensor by itself, get as far as the check of the device
+    kept = 2 * w
+    kept.retain_grad()
+    for tensors in ([kept], w):
+        with pytest.raises(TypeError, match="place 0"):
+            Adam(tensors=tensors)
