@@ -11,6 +11,7 @@ loudly if it is missing.
 """
 from __future__ import annotations
 
+import bisect
 import ctypes as C
 import os
 from typing import Optional, Sequence
@@ -703,6 +704,7 @@ class TensorList:
     def _check_apart(self, name: str) -> None:
         """Refuses a list that is written to when two of its tensors share memory."""
         if self._apart is None:
+            self._spans.sort()
             self._apart = _spans_apart(self._spans)
         if not self._apart:
             raise RuntimeError(f"{name} share memory: each may be in the list once")
@@ -716,6 +718,14 @@ def _spans_apart(spans) -> bool:
     """Whether no two of the (first, end) address ranges overlap."""
     spans = sorted(spans)
     return all(a[1] <= b[0] for a, b in zip(spans, spans[1:]))
+
+
+def _check_outside(name: str, spans, taken, of: str) -> None:
+    """Refuses (first, end) ranges that overlap one of `taken`, which are sorted and apart."""
+    for first, end in spans:
+        i = bisect.bisect_left(taken, (end,))  # those before i start before the range's end
+        if i and taken[i - 1][1] > first:
+            raise RuntimeError(f"{name} shares memory with {of}")
 
 
 def _tensor_list(tensors) -> TensorList:
@@ -760,13 +770,15 @@ def gradient_norm_device(gradients, stream=None):
 def clip_gradients_device(gradients, max_norm: float, norm=None, stream=None):
     """Scales `gradients` in place by min(1, max_norm / (n + 1e-6)) with n their global norm, or
     `norm` (a float64 CUDA scalar: over several lists, or over ranks), and returns n
-    (arcqml_rt_v2_clip_gradients)."""
+    (arcqml_rt_v2_clip_gradients). No two gradients, nor the given norm and one, may share memory."""
     import torch
     g = _tensor_list(gradients)
     device = torch.cuda.current_device()
     table = g._current(torch, device)
     g._check_apart("the gradients")
     given = None if norm is None else _scalar_ptr(torch, device, norm)
+    if given is not None:
+        _check_outside("the given norm", [(given, given + 8)], g._spans, "the gradients")
     on, out, ws = _call_memory(torch, device, g._blank, stream, g._words, True)
     _status(load().arcqml_rt_v2_clip_gradients(table, len(g), float(max_norm), given,
                                                out.data_ptr(),
@@ -861,8 +873,9 @@ def adam_step_device(parameters, gradients, state: DeviceAdamState, lr: float = 
     ``clip_gradients_device`` scales them (they stay as they are) and their global norm is returned;
     `norm` gives that norm instead. A parameter whose gradient is None is left as it is. `copies`
     (bfloat16 or float16 tensors, or None, one per parameter) receive the new values of float32
-    parameters. The step count is on the device: a captured step counts on when it is replayed
-    (`lr` and the other numbers stay those of the capture)."""
+    parameters. What is written (parameters, moments, copies, the step count) may share no memory with
+    anything else here; gradients may share theirs. The step count is on the device: a captured step
+    counts on when it is replayed (`lr` and the other numbers stay those of the capture)."""
     import torch
     p, g, m, v = _tensor_list(parameters), _tensor_list(gradients), state._m, state._v
     c = None if copies is None else _tensor_list(copies)
@@ -888,13 +901,20 @@ def adam_step_device(parameters, gradients, state: DeviceAdamState, lr: float = 
         for name, x in (("moments", m), ("moments", v), ("copies", c)):
             if x is not None:
                 _check_places(name, x, p)
-        written = [x for x in (p, m, v, c) if x is not None]
-        if not _spans_apart([s for x in written for s in x._spans]):
-            raise RuntimeError("the parameters, moments and copies share memory")
-        state._checked, state._gradients = states, None
+        at = state._step.data_ptr()
+        written = sorted([s for x in (p, m, v, c) if x is not None for s in x._spans]
+                         + [(at, at + 8)])
+        if not _spans_apart(written):
+            raise RuntimeError("the parameters, moments, copies and step count share memory")
+        state._checked, state._gradients, state._written = states, None, written
+    # what other places read while one place is written
+    written = "the parameters, moments, copies or step count"
     if state._gradients is not g._state:
         _check_places("gradients", g, p)
+        _check_outside("a gradient", g._spans, state._written, written)
         state._gradients = g._state
+    if given is not None:
+        _check_outside("the given norm", [(given, given + 8)], state._written, written)
     options = AdamOptions(lr, betas[0], betas[1], eps, weight_decay, max_norm, bool(decoupled), 0)
     on, out, ws = _call_memory(torch, device, p._blank, stream, p._adam_words, max_norm >= 0.0)
     _status(load().arcqml_rt_v2_adam_step(

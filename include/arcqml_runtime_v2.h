@@ -236,7 +236,8 @@ int32_t arcqml_rt_v2_gradient_norm(const ArcqmlTensor *gradients, size_t num_ten
  * ranks of a sharded model. *norm (device, may be null) <- n. A factor of 1 leaves the gradients
  * unwritten; a NaN norm makes every gradient NaN and an infinite one makes the finite gradients 0,
  * the others NaN. Products are f64 for f64 tensors and f32 otherwise, rounded once to the type.
- * The tensors must not overlap. max_norm must be finite and not negative. */
+ * Neither the tensors nor a tensor and *given_norm may overlap. max_norm must be finite and not
+ * negative. */
 int32_t arcqml_rt_v2_clip_gradients(const ArcqmlTensor *gradients, size_t num_tensors,
                                     double max_norm, const double *given_norm, double *norm,
                                     double *workspace, size_t workspace_len, void *stream);

@@ -109,3 +109,54 @@ def test_an_optimizer_of_one_tensor(runtime):
     # the first step moves each value by lr against its gradient's sign, to a rounding of 1 / (1 + eps)
     assert len(opt.tensors) == 1 and bool(((w - 0.5).abs() <= 1e-6).all())
     assert opt.state.m[0].shape == (4, 3)
+
+
+def test_gradients_share_no_memory_with_what_the_step_writes(runtime):
+    """One block would read what another writes. Gradients may share memory with one another."""
+    n = 3000
+    flat = normal(8 * n, 11)
+    p, g, m, v = [flat[:n]], [flat[n:2 * n]], [flat[2 * n:3 * n]], [flat[3 * n:4 * n].abs_()]
+    c = [torch.zeros(n, device="cuda", dtype=torch.bfloat16)]
+    count = torch.zeros(2, dtype=torch.int64, device="cuda")
+    state = runtime.DeviceAdamState(p, m=m, v=v, step=count[1])
+    was = flat.clone()
+
+    def refused(match, **kw):
+        kw = {"grads": g, "norm": None, "copies": c, **kw}
+        with pytest.raises(runtime.RuntimeError, match=match):
+            runtime.adam_step_device(p, kw["grads"], state, copies=kw["copies"], norm=kw["norm"],
+                                     max_norm=None if kw["norm"] is None else 1.0)
+        assert torch.equal(flat, was) and count.tolist() == [0, 0]
+
+    for at in (0, 1, n - 1, n + 1, 2 * n - 1, 3 * n - 1, 4 * n - 1):
+        refused("a gradient shares memory", grads=[flat[at:at + n]])
+    refused("a gradient shares memory", grads=c)  # one bucket for gradients and copies
+    norm = flat[:2 * n].view(torch.float64)
+    refused("the given norm shares memory", norm=norm[0])
+    refused("the given norm shares memory", norm=flat[2 * n:4 * n].view(torch.float64)[-1])
+    refused("copies and step count share memory", copies=[flat[n // 2:n].view(torch.bfloat16)])
+    refused("a gradient shares memory", copies=[flat[3 * n // 2:2 * n].view(torch.bfloat16)])
+    # right beside what is written, and twice the same gradient
+    runtime.adam_step_device(p, g, state, copies=c, max_norm=1.0, norm=norm[n // 2])
+    assert count.tolist() == [0, 1]
+    two = runtime.DeviceAdamState([flat[:n], flat[4 * n:5 * n]])
+    runtime.adam_step_device([flat[:n], flat[4 * n:5 * n]], [g[0], g[0]], two)
+    assert torch.equal(two.m[0], two.m[1])
+    # a list that was taken once is looked at again when the state is another one
+    kept = runtime.TensorList(g)
+    runtime.adam_step_device(p, kept, state)
+    state.m = [flat[n + 1:2 * n + 1]]
+    was = flat.clone()
+    with pytest.raises(runtime.RuntimeError, match="a gradient shares memory"):
+        runtime.adam_step_device(p, kept, state)
+    assert torch.equal(flat, was)
+    one = count.view(torch.float64)
+    with pytest.raises(runtime.RuntimeError, match="share memory"):
+        runtime.adam_step_device([one], [torch.zeros_like(one)],
+                                 runtime.DeviceAdamState([one], step=count[0]))
+    # clipping: the given norm
+    grads = [torch.ones(10, dtype=torch.float64, device="cuda") for _ in range(3)]
+    for bad in (grads[0][0], grads[1][9], grads[2][4]):
+        with pytest.raises(runtime.RuntimeError, match="the given norm shares memory"):
+            runtime.clip_gradients_device(grads, 1.0, norm=bad)
+    assert all(bool((t == 1).all()) for t in grads)

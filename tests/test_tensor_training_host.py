@@ -189,3 +189,15 @@ def test_hybrid_optimizer_takes_no_computed_tensors(runtime):
     for tensors in ([kept], w):
         with pytest.raises(TypeError, match="place 0"):
             Adam(tensors=tensors)
+
+
+def test_what_is_read_lies_outside_what_is_written(runtime):
+    outside = runtime._check_outside
+    taken = [(64, 80), (80, 96), (128, 200), (1000, 1001)]
+    for free in ([], [(0, 64)], [(96, 128)], [(200, 300), (96, 100), (96, 100)], [(1001, 1 << 62)]):
+        outside("a", free, taken, "b")
+        outside("a", free, [], "b")
+    for bad in ((0, 65), (64, 80), (79, 81), (95, 96), (95, 300), (127, 129), (130, 140), (199, 1000),
+                (0, 2000), (1000, 1001)):
+        with pytest.raises(runtime.RuntimeError, match="a shares memory with b"):
+            outside("a", [(96, 128), bad], taken, "b")
