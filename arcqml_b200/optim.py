@@ -53,6 +53,14 @@ class _CircuitParameters:
             p.value = x
 
 
+def _resolved(gradient):
+    """A gradient with its values in memory: autograd leaves a complex one conjugated by a bit alone
+    when the loss took its tensor's conjugate."""
+    if gradient is None or not (gradient.is_conj() or gradient.is_neg()):
+        return gradient
+    return gradient.resolve_conj().resolve_neg()
+
+
 class Adam:
     """Adam over ``circuits`` (the parameters with ``requires_grad`` that they have now) and
     ``tensors`` (floating or complex CUDA tensors that autograd leaves gradients in, or one such
@@ -108,7 +116,7 @@ class Adam:
         import torch
         has = [c.upload() for c in self._circuits]
         grads = [c.gradient if h else None for c, h in zip(self._circuits, has)]
-        grads += [t.grad for t in self._tensors]
+        grads += [_resolved(t.grad) for t in self._tensors]
         # a new list every step: one that is kept would keep the gradients' memory
         norm = rt.adam_step_device(self._parameters, grads, self.state, lr=self.lr,
                                    betas=self.betas, eps=self.eps, weight_decay=self.weight_decay,

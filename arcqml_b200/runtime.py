@@ -616,6 +616,15 @@ def _tensor_kinds() -> dict:
     return _tensor_types
 
 
+def _kind_of(torch, t) -> str:
+    """What a tensor list is told that it cannot take."""
+    if not isinstance(t, torch.Tensor):
+        return type(t).__name__
+    lazy = [bit for bit, on in (("conj", t.is_conj()), ("neg", t.is_neg())) if on]
+    return (f"{t.dtype} on {t.device}" + (f" laid out as {t.layout}" if t.layout != torch.strided else "")
+            + (f" with its lazy {' and '.join(lazy)} bit set (resolve_conj, resolve_neg)" if lazy else ""))
+
+
 def _layout(t):
     """None for a contiguous tensor, (shape, strides) for another one that fills its memory without
     gaps or overlap; anything else is refused."""
@@ -663,9 +672,7 @@ class TensorList:
             if kind is None or not t.is_cuda or t.layout != torch.strided or t.is_conj() or \
                     t.is_neg():
                 raise TypeError("a tensor list takes dense float64, float32, bfloat16, float16 and "
-                                f"complex CUDA tensors or None: place {i} holds "
-                                + (f"{t.dtype} on {t.device}" if isinstance(t, torch.Tensor)
-                                   else type(t).__name__))
+                                f"complex CUDA tensors or None: place {i} holds {_kind_of(torch, t)}")
             layouts.append(None if t.is_contiguous() else _layout(t))
             devices.add(t.get_device())
             at, n = t.data_ptr(), t.numel()

@@ -161,3 +161,40 @@ def test_parts_without_gradients_stay(runtime):
         # as test_adam_matches_the_hosts_update: |step| below 4 lr, |x| below 5
         assert np.max(np.abs(np.array([p.value for p in trained]) - x)) <= t * (
             0.1 * 4 * (2 * 4 * ts.U64 / 1e-3 + 8 * ts.U64) + 8 * ts.U64 * 5)
+
+
+def test_complex_leaves_whose_gradients_are_conjugated(runtime):
+    """The amplitudes that normalised states are made from, and leaves that enter by their conjugate:
+    autograd conjugates the gradient by a bit alone where the strides allow it. Steps against 64 bits."""
+    from arcqml_b200.optim import Adam
+    g = torch.Generator(device="cuda").manual_seed(4)
+
+    def normal(*shape):
+        return torch.randn(*shape, dtype=torch.complex128, device="cuda", generator=g)
+
+    x, z = normal(ROWS, 1 << N).requires_grad_(True), normal(4, 6).t().requires_grad_(True)
+    target, other = normal(ROWS, 1 << N), normal(6, 4)
+    c64 = normal(7).to(torch.complex64).requires_grad_(True)
+    w, third = normal(4, 6).t().requires_grad_(True), normal(4, 6).t()
+    opt = Adam(tensors=[x, z, c64, w], lr=0.02, weight_decay=0.01, max_norm=0.5)
+    for t in range(1, 4):
+        opt.zero_grad()
+        states = x / x.abs().square().sum(dim=1, keepdim=True).sqrt()
+        overlap = (target.conj() * states).sum(dim=1).abs().square().sum()
+        (overlap + (z.conj() * other).real.sum() + c64.conj().real.sum()
+         + (third.mH @ w.conj()).sum().abs()).backward()
+        assert w.grad.is_conj() and w.grad.stride() == w.stride()
+        old = [[ts.components(u.resolve_conj()) for u in (a, a.grad, m, v)]
+               for a, m, v in zip(opt.tensors, opt.state.m, opt.state.v)]
+        norm = opt.step()
+        count = sum(o[0].size for o in old)
+        want = float(np.sqrt(sum(float(np.sum(o[1] * o[1])) for o in old)))
+        assert abs(float(norm) - want) <= 2 * ts.norm_bound(count) * want
+        for a, m, v, o in zip(opt.tensors, opt.state.m, opt.state.v, old):
+            u = ts.U64 if a.dtype == torch.complex128 else ts.U32
+            p2, m2, v2, pe, me, ve = ts.adam64(*o, t, 0.02, 0.9, 0.999, 1e-8, 0.01, False,
+                                               ts.clip_factor(want, 0.5), u,
+                                               2 * ts.norm_bound(count) + 3 * ts.U64)
+            tiny = ts.TINY[ts.real_type(a)]
+            for got, value, bound in ((a, p2, pe), (m, m2, me), (v, v2, ve)):
+                ts.assert_within(ts.components(got), value, bound + 4 * tiny, (t, a.dtype))

@@ -201,3 +201,33 @@ def test_what_is_read_lies_outside_what_is_written(runtime):
                 (0, 2000), (1000, 1001)):
         with pytest.raises(runtime.RuntimeError, match="a shares memory with b"):
             outside("a", [(96, 128), bad], taken, "b")
+
+
+def test_conjugated_gradients(runtime):
+    """Autograd leaves the gradient of a conjugated leaf with its conj bit set, unless it has to copy it
+    into the leaf's strides. Lists name the bit; the optimizer resolves it, in the gradient's strides."""
+    from arcqml_b200.optim import _resolved
+    for shape, order, lazy in (((5,), (0,), True), ((3, 4), (0, 1), True), ((3, 4), (1, 0), False)):
+        g = torch.Generator().manual_seed(3)
+        x = torch.randn(shape, dtype=torch.complex128, generator=g).permute(order)
+        y = torch.randn(x.shape, dtype=torch.complex128, generator=g)
+        x.requires_grad_(True)
+        (x.conj() * y).real.sum().backward()
+        assert x.grad.is_conj() == lazy and x.grad.stride() == x.stride()
+        if lazy:
+            with pytest.raises(TypeError, match="torch.complex128 on cpu with its lazy conj bit"):
+                runtime.TensorList([x.grad])
+        z = _resolved(x.grad)
+        assert not z.is_conj() and z.stride() == x.grad.stride()
+        # d Re(conj(x) y) / d conj(x), doubled: y
+        assert torch.equal(z, y)
+        assert _resolved(z) is z
+    z = _resolved(y.mH)
+    assert not z.is_conj() and z.stride() == y.mH.stride() and torch.equal(z, y.mH)
+    neg = torch.ones(3, dtype=torch.complex64).conj().imag
+    assert neg.is_neg() and not _resolved(neg).is_neg()
+    with pytest.raises(TypeError, match="lazy neg bit"):
+        runtime.TensorList([neg])
+    assert _resolved(None) is None
+    with pytest.raises(TypeError, match="laid out as torch.sparse_coo"):
+        runtime.TensorList([torch.eye(3).to_sparse()])
