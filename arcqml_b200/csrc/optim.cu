@@ -321,10 +321,10 @@ __device__ __forceinline__ AdamScalars64 scalars64(const ArcqmlAdamOptions &o, d
                          o.epsilon, o.weight_decay, 1.0 - o.learning_rate * o.weight_decay, bc1,
                          bc2, factor};
 }
-// f32: rate = lr / (1 - beta1^t) and root = 1 / (1 - beta2^t) are formed in f64 and rounded once.
+// f32: rate = lr / (1 - beta1^t) and root = 1 / sqrt(1 - beta2^t) are formed in f64 and rounded once.
 __device__ __forceinline__ AdamScalars32 scalars32(const AdamScalars64 &h) {
     return AdamScalars32{float(h.b1), float(h.b2), float(h.nb1), float(h.nb2), float(h.eps),
-                         float(h.wd), float(h.down), float(h.lr / h.bc1), float(1.0 / h.bc2),
+                         float(h.wd), float(h.down), float(h.lr / h.bc1), float(1.0 / sqrt(h.bc2)),
                          factor32(h.factor)};
 }
 
@@ -457,14 +457,16 @@ __device__ __forceinline__ void adam_update(double &p, double &m, double &v, dou
 }
 
 // f32 for every other type. A 16-bit parameter is rounded to nearest once per step: updates below
-// half its step are lost, which is what f32 parameters with 16-bit copies are for.
+// half its step are lost, which is what f32 parameters with 16-bit copies are for. The root is taken
+// before the bias correction: in the first steps v / (1 - beta2^t) leaves f32's range from gradients of
+// 2e19 on, which v itself holds up to 6e20.
 __device__ __forceinline__ void adam_update(float &p, float &m, float &v, float g,
                                             const AdamScalars32 &h, bool decoupled) {
     float a = g * h.factor.pre * h.factor.rest;
     if (!decoupled) a = fmaf(h.wd, p, a);
     m = fmaf(h.b1, m, h.nb1 * a);
     v = fmaf(h.b2, v, h.nb2 * a * a);
-    const float u = m / (sqrtf(v * h.root) + h.eps);
+    const float u = m / fmaf(sqrtf(v), h.root, h.eps);
     if (decoupled) p *= h.down;
     p = fmaf(-h.rate, u, p);
 }
