@@ -322,8 +322,11 @@ __device__ __forceinline__ AdamScalars64 scalars64(const ArcqmlAdamOptions &o, d
                          bc2, factor};
 }
 // f32: rate = lr / (1 - beta1^t) and root = 1 / sqrt(1 - beta2^t) are formed in f64 and rounded once.
+// An epsilon below f32's range stays its smallest value: with 0 in its place a zero gradient's step
+// would be 0 / 0.
 __device__ __forceinline__ AdamScalars32 scalars32(const AdamScalars64 &h) {
-    return AdamScalars32{float(h.b1), float(h.b2), float(h.nb1), float(h.nb2), float(h.eps),
+    const float eps = h.eps > 0.0 ? fmaxf(float(h.eps), 0x1p-149f) : 0.f;
+    return AdamScalars32{float(h.b1), float(h.b2), float(h.nb1), float(h.nb2), eps,
                          float(h.wd), float(h.down), float(h.lr / h.bc1), float(1.0 / sqrt(h.bc2)),
                          factor32(h.factor)};
 }
