@@ -6,7 +6,8 @@
 // pointers and lengths travel as a kernel parameter, every tensor is cut into chunks, and blocks (in
 // short lists warps) take chunks. No call reads anything back: the norm, the clip factor and the bias
 // corrections pass between the launches in device scratch that the caller gives, so nothing is
-// shared between calls, and sums are formed in an order that the lengths fix, without atomics.
+// shared between calls. Sums are formed without atomics, in an order that the lengths, the types and the
+// tensors' starts within 16 bytes fix (vectors begin at the first boundary).
 //
 //   k_square_sums      per block the f64 sum of squares of its chunks
 //   k_scalars          one block: the sums in order -> norm, clip factor, step, bias corrections

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import tensor_training_support as ts
-from test_gpu_tensor_training import TYPES, gen, normal, run_adam
+from test_gpu_tensor_training import TYPES, check_norm, gen, normal, run_adam
 
 pytestmark = pytest.mark.gpu
 
@@ -39,3 +39,42 @@ def test_epsilon_below_the_types_range(runtime, n):
         runtime.adam_step_device(params, [torch.zeros_like(was)], runtime.DeviceAdamState(params),
                                  eps=1e-300)
         assert torch.equal(params[0], was)
+
+
+def placed(tensors, starts):
+    """Copies of the tensors in new memory, tensor i starting starts[i] elements behind 512 bytes."""
+    out = []
+    for t, start in zip(tensors, starts):
+        flat = torch.empty(start + t.numel(), dtype=t.dtype, device="cuda")
+        out.append(flat[start:].copy_(t))
+    return out
+
+
+@pytest.mark.parametrize("lengths", [[5, 3001, 64], [1_000_003, 5, 262_144]], ids=["short", "long"])
+@pytest.mark.parametrize("dtype", ["f64", "f32", "bf16"])
+def test_equal_values_that_start_alike_give_equal_bits(runtime, dtype, lengths):
+    """In other memory too. Other starts within 16 bytes add in another order: the same to the bound."""
+    kind = TYPES[dtype]
+    step = 16 // torch.empty((), dtype=kind).element_size()
+    g = gen(6)
+    params, grads = ([normal((n,), kind, g) for n in lengths] for _ in range(2))
+    long = runtime.TensorList(params)._adam_words > 0
+    assert long == (sum(lengths) > 100_000)
+
+    def results(starts):
+        q = placed(grads, starts)
+        norm = runtime.gradient_norm_device(q)
+        check_norm(norm, grads)
+        p = placed(params, starts)
+        state = runtime.DeviceAdamState(p)
+        inside = runtime.adam_step_device(p, q, state, max_norm=0.5)
+        check_norm(inside, grads)
+        clipped = runtime.clip_gradients_device(q, 0.5)
+        check_norm(clipped, grads)
+        return [norm, inside, clipped] + p + q + state.m + state.v
+
+    for starts in ([0, 0, 0], [1, step - 1, 0]):
+        first = results(starts)
+        again = results([s + k * step for s, k in zip(starts, (1, 0, 5))])
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
+    results([1, 0, 1])
