@@ -754,8 +754,9 @@ def _call_memory(torch, device: int, blank, stream, words: int, norm: bool):
 
 def _scalar_ptr(torch, device: int, t) -> int:
     if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == torch.float64
-            and t.numel() == 1 and t.get_device() == device):
-        raise TypeError("a given norm must be one float64 on the current CUDA device")
+            and t.numel() == 1 and t.get_device() == device and not t.is_neg()):
+        raise TypeError("a given norm must be one float64 on the current CUDA device, its lazy neg bit "
+                        "not set")
     return t.data_ptr()
 
 

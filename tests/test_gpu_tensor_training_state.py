@@ -160,3 +160,16 @@ def test_gradients_share_no_memory_with_what_the_step_writes(runtime):
         with pytest.raises(runtime.RuntimeError, match="the given norm shares memory"):
             runtime.clip_gradients_device(grads, 1.0, norm=bad)
     assert all(bool((t == 1).all()) for t in grads)
+
+
+def test_a_given_norm_that_is_negated_by_a_bit_alone(runtime):
+    """Its memory holds the negative of its value."""
+    t = torch.ones(10, dtype=torch.float64, device="cuda")
+    norm = torch.tensor([1 - 4j], dtype=torch.complex128, device="cuda").conj().imag[0]
+    assert norm.is_neg() and float(norm) == 4.0
+    with pytest.raises(TypeError, match="neg bit"):
+        runtime.clip_gradients_device([t], 2.0, norm=norm)
+    with pytest.raises(TypeError, match="neg bit"):
+        runtime.adam_step_device([t], [t.clone()], runtime.DeviceAdamState([t]), max_norm=2.0, norm=norm)
+    assert bool((t == 1).all())
+    assert float(runtime.clip_gradients_device([t], 2.0, norm=norm.resolve_neg())) == 4.0
