@@ -334,7 +334,9 @@ __device__ __forceinline__ AdamScalars32 scalars32(const AdamScalars64 &h) {
 
 // One block of a thread per sum. given != null: n = *given; else the root of the count sums.
 // step != null: one more step is counted. The step count is no work of the launch before this one:
-// what follows from it alone is formed while that launch still runs.
+// what follows from it alone is formed without waiting for that launch. This block fits on an SM once four
+// of the six blocks of k_square_sums there have ended (40 registers for each of its 1024 threads): behind a
+// full grid that is in its tail, where no gain was measured; behind a smaller one it runs beside it.
 constexpr int kScalarThreads = 1024;
 __global__ void __launch_bounds__(kScalarThreads)
     k_scalars(const double *sums, uint32_t count, const double *given,

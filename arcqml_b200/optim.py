@@ -8,7 +8,9 @@ updates them in one ``runtime.adam_step_device``; the update is that of ``runtim
 them: ``Parameter.grad`` (``RunResult.backward``, ``StateVectorSimulator.gradient``,
 ``UnitaryLoss.backward``) and ``Tensor.grad``. ``RunResult.backward``'s initial-state gradient is in
 torch's convention for complex tensors, so a network that made the states gets its gradients by
-``states.backward(initial_state_grad)``.
+``states.backward(initial_state_grad)``. Amplitudes are trained the same way, through the normalisation that
+makes states of them: a step on normalised states themselves would leave them unnormalised, which
+``BatchStateVectorSimulator.from_device_state`` does not check.
 """
 from __future__ import annotations
 
