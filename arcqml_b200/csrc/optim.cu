@@ -21,7 +21,7 @@
 // 594 us, 7.2 TB/s; norm of 251M bf16 elements in 300 tensors 91 us, 5.5 TB/s (the conversion to f64
 // keeps its unit 75 % busy); clip of a 26-qubit state's gradient 485 us, 6.6 TB/s of its three passes;
 // Adam on 400M f32 parameters with clipping 1914 us, 6.7 TB/s with the second read of the gradients;
-// f32 parameters with bf16 gradients and copies (150M) 702 us, 6.4 TB/s; 8 f64 parameters' norm 7 us
+// f32 parameters with bf16 gradients and copies (150M) 700 us, 6.4 TB/s; 8 f64 parameters' norm 7 us
 // (the host's time for one launch).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -75,7 +75,7 @@ struct Factor32 {
     float pre, rest;
 };
 struct AdamScalars32 {
-    float b1, b2, nb1, nb2, eps, wd, down, rate, root;
+    float b1, b2, nb1, nb2, eps, wd, down, rate;
     Factor32 factor;
 };
 
@@ -322,13 +322,14 @@ __device__ __forceinline__ AdamScalars64 scalars64(const ArcqmlAdamOptions &o, d
                          o.epsilon, o.weight_decay, 1.0 - o.learning_rate * o.weight_decay, bc1,
                          bc2, factor};
 }
-// f32: rate = lr / (1 - beta1^t) and root = 1 / sqrt(1 - beta2^t) are formed in f64 and rounded once.
-// An epsilon below f32's range stays its smallest value: with 0 in its place a zero gradient's step
-// would be 0 / 0.
+// f32: with r = sqrt(1 - beta2^t) the step is lr r / (1 - beta1^t) times m / (sqrt(v) + r epsilon). The
+// two factors are formed in f64 and rounded once. An epsilon below f32's range stays its smallest value:
+// with 0 in its place a zero gradient's step would be 0 / 0.
 __device__ __forceinline__ AdamScalars32 scalars32(const AdamScalars64 &h) {
-    const float eps = h.eps > 0.0 ? fmaxf(float(h.eps), 0x1p-149f) : 0.f;
+    const double r = sqrt(h.bc2);
+    const float eps = h.eps > 0.0 ? fmaxf(float(r * h.eps), 0x1p-149f) : 0.f;
     return AdamScalars32{float(h.b1), float(h.b2), float(h.nb1), float(h.nb2), eps,
-                         float(h.wd), float(h.down), float(h.lr / h.bc1), float(1.0 / sqrt(h.bc2)),
+                         float(h.wd), float(h.down), float(h.lr * r / h.bc1),
                          factor32(h.factor)};
 }
 
@@ -463,16 +464,16 @@ __device__ __forceinline__ void adam_update(double &p, double &m, double &v, dou
 }
 
 // f32 for every other type. A 16-bit parameter is rounded to nearest once per step: updates below
-// half its step are lost, which is what f32 parameters with 16-bit copies are for. The root is taken
-// before the bias correction: in the first steps v / (1 - beta2^t) leaves f32's range from gradients of
-// 2e19 on, which v itself holds up to 6e20.
+// half its step are lost, which is what f32 parameters with 16-bit copies are for. v's own root is taken,
+// its bias correction is in the scalars: in the first steps v / (1 - beta2^t) leaves f32's range from
+// gradients of 2e19 on, which v itself holds up to 6e20.
 __device__ __forceinline__ void adam_update(float &p, float &m, float &v, float g,
                                             const AdamScalars32 &h, bool decoupled) {
     float a = g * h.factor.pre * h.factor.rest;
     if (!decoupled) a = fmaf(h.wd, p, a);
     m = fmaf(h.b1, m, h.nb1 * a);
     v = fmaf(h.b2, v, h.nb2 * a * a);
-    const float u = m / fmaf(sqrtf(v), h.root, h.eps);
+    const float u = m / (sqrtf(v) + h.eps);
     if (decoupled) p *= h.down;
     p = fmaf(-h.rate, u, p);
 }
