@@ -644,8 +644,9 @@ class TensorList:
     CUDA tensors of one device (or one such tensor); None where a parameter has no gradient. Checking
     a list and writing it down costs about two microseconds per tensor: a training loop whose tensors
     stay keeps its lists. Every call reads the tensors' addresses anew, and one that has moved (a new
-    ``.data``) is checked and written down again; for tensors that change shape where they are (a
-    view of their own memory, ``resize_``) a new list is made. A list keeps its tensors' memory alive."""
+    ``.data``) is checked and written down again. For tensors that change shape or type where they are (a
+    view of their own memory), or that are resized, they or their storage (``resize_``), a new list is
+    made: reading shapes as well would double a call's time. A list keeps its tensors' memory alive."""
 
     def __init__(self, tensors):
         import torch
