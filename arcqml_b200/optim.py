@@ -118,8 +118,12 @@ class Adam:
         import torch
         has = [c.upload() for c in self._circuits]
         grads = [c.gradient if h else None for c, h in zip(self._circuits, has)]
-        grads += [_resolved(t.grad) for t in self._tensors]
+        grads += [t.grad for t in self._tensors]
         # a new list every step: one that is kept would keep the gradients' memory
+        try:
+            grads = rt.TensorList(grads)
+        except TypeError:  # what it refuses may only have to be resolved; looking first costs more
+            grads = rt.TensorList([_resolved(g) for g in grads])
         norm = rt.adam_step_device(self._parameters, grads, self.state, lr=self.lr,
                                    betas=self.betas, eps=self.eps, weight_decay=self.weight_decay,
                                    decoupled=self.decoupled, max_norm=self.max_norm)

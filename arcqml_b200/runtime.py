@@ -11,9 +11,9 @@ loudly if it is missing.
 """
 from __future__ import annotations
 
-import bisect
 import ctypes as C
 import os
+from bisect import bisect_left
 from typing import Optional, Sequence
 
 import numpy as np
@@ -695,9 +695,7 @@ class TensorList:
         self._layouts, self._spans, self._apart = layouts, spans, None
         self._shapes = [None if t is None else t.shape for t in self.tensors]
         self._pointers = [r[0] for r in rows if r[2] != NO_TENSOR]
-        # the tensors whose version counters stand for all: views share their base's
-        roots = [t._base if t._is_view() else t for t in self._present]
-        self._roots = list({id(t): t for t in roots}.values())
+        self._roots = None
         self._state = object()  # another one whenever the list is written down
 
     def _current(self, torch, device: int) -> int:
@@ -712,13 +710,16 @@ class TensorList:
     def _check_apart(self, name: str) -> None:
         """Refuses a list that is written to when two of its tensors share memory."""
         if self._apart is None:
-            self._spans.sort()
             self._apart = _spans_apart(self._spans)
         if not self._apart:
             raise RuntimeError(f"{name} share memory: each may be in the list once")
 
     def _written(self, torch) -> None:
         """Tells autograd that the tensors changed."""
+        if self._roots is None:
+            # the tensors whose version counters stand for all: views share their base's
+            roots = [t._base if t._is_view() else t for t in self._present]
+            self._roots = list({id(t): t for t in roots}.values())
         torch.autograd.graph.increment_version(self._roots)
 
 
@@ -728,11 +729,17 @@ def _spans_apart(spans) -> bool:
     return all(a[1] <= b[0] for a, b in zip(spans, spans[1:]))
 
 
-def _check_outside(name: str, spans, taken, of: str) -> None:
-    """Refuses (first, end) ranges that overlap one of `taken`, which are sorted and apart."""
+def _edges(spans):
+    """The starts, and behind a 0 the ends, of (first, end) ranges that are sorted and apart."""
+    return [s[0] for s in spans], [0] + [s[1] for s in spans]
+
+
+def _check_outside(name: str, spans, edges, of: str) -> None:
+    """Refuses (first, end) ranges that overlap one of those whose ``_edges`` are given."""
+    starts, ends = edges
     for first, end in spans:
-        i = bisect.bisect_left(taken, (end,))  # those before i start before the range's end
-        if i and taken[i - 1][1] > first:
+        # of the ranges that start before this one's end, the last one ends last
+        if ends[bisect_left(starts, end)] > first:
             raise RuntimeError(f"{name} shares memory with {of}")
 
 
@@ -786,8 +793,8 @@ def clip_gradients_device(gradients, max_norm: float, norm=None, stream=None):
     table = g._current(torch, device)
     g._check_apart("the gradients")
     given = None if norm is None else _scalar_ptr(torch, device, norm)
-    if given is not None:
-        _check_outside("the given norm", [(given, given + 8)], g._spans, "the gradients")
+    if given is not None and any(first < given + 8 and given < end for first, end in g._spans):
+        raise RuntimeError("the given norm shares memory with the gradients")
     on, out, ws = _call_memory(torch, device, g._blank, stream, g._words, True)
     _status(load().arcqml_rt_v2_clip_gradients(table, len(g), float(max_norm), given,
                                                out.data_ptr(),
@@ -915,7 +922,7 @@ def adam_step_device(parameters, gradients, state: DeviceAdamState, lr: float = 
                          + [(at, at + 8)])
         if not _spans_apart(written):
             raise RuntimeError("the parameters, moments, copies and step count share memory")
-        state._checked, state._gradients, state._written = states, None, written
+        state._checked, state._gradients, state._written = states, None, _edges(written)
     # what other places read while one place is written
     written = "the parameters, moments, copies or step count"
     if state._gradients is not g._state:

@@ -227,8 +227,9 @@ size_t arcqml_rt_v2_adam_workspace(const ArcqmlTensor *parameters, size_t num_te
  * kept in f64. Its order is fixed by the lengths, the types and how far from a 16-byte boundary each
  * tensor starts: equal values in tensors that start alike give equal bits from the same call. Tensors
  * that start elsewhere, and the norms inside the calls below (an Adam step of a short list adds in the
- * order of its parameters), can differ in the last bits. A NaN or an infinity in a gradient gives a NaN or infinite norm; squares leave the f64
- * range for elements above 1e154. No tensors, or empty ones: 0. */
+ * order of its parameters), can differ in the last bits. A NaN or an infinity in a gradient gives a
+ * NaN or infinite norm; squares leave the f64 range for elements above 1e154. No tensors, or empty
+ * ones: 0. */
 int32_t arcqml_rt_v2_gradient_norm(const ArcqmlTensor *gradients, size_t num_tensors,
                                    double *norm, double *workspace, size_t workspace_len,
                                    void *stream);

@@ -192,7 +192,9 @@ def test_hybrid_optimizer_takes_no_computed_tensors(runtime):
 
 
 def test_what_is_read_lies_outside_what_is_written(runtime):
-    outside = runtime._check_outside
+    def outside(name, spans, taken, of):
+        runtime._check_outside(name, spans, runtime._edges(taken), of)
+
     taken = [(64, 80), (80, 96), (128, 200), (1000, 1001)]
     for free in ([], [(0, 64)], [(96, 128)], [(200, 300), (96, 100), (96, 100)], [(1001, 1 << 62)]):
         outside("a", free, taken, "b")
