@@ -12,8 +12,10 @@
 #include "../../include/arcqml_runtime.h"
 #include "../../include/arcqml_runtime_v2.h"
 #include "analysis.h"
+#include "embedding.h"
 #include "jit.h"
 #include "launch.h"
+#include "muon.h"
 #include "optim.h"
 #include "planner.h"
 #include "profile.h"
@@ -986,6 +988,63 @@ int32_t arcqml_rt_v2_adam_step(const ArcqmlTensor *parameters, const ArcqmlTenso
         if (!options) fail("Adam options are null");
         adam_step_device(parameters, gradients, first_moments, second_moments, copies,
                          num_tensors, step, *options, given_norm, norm, workspace, workspace_len,
+                         static_cast<cudaStream_t>(stream));
+    });
+}
+
+size_t arcqml_rt_v2_embedding_lookup_workspace(const ArcqmlRows *table, size_t count,
+                                               const ArcqmlEmbeddingOptions *options) {
+    return table && options ? embedding_lookup_workspace(*table, count, *options) : 0;
+}
+
+size_t arcqml_rt_v2_embedding_gradient_workspace(const ArcqmlRows *gradient, uint64_t rows,
+                                                 const ArcqmlEmbeddingOptions *options) {
+    return gradient && options ? embedding_gradient_workspace(*gradient, rows, *options) : 0;
+}
+
+int32_t arcqml_rt_v2_embedding_lookup(const ArcqmlRows *table, const void *indices, size_t count,
+                                      const ArcqmlEmbeddingOptions *options, const ArcqmlRows *output,
+                                      double *workspace, size_t workspace_len, void *stream) {
+    return guarded([&] {
+        if (!table || !output) fail("the embedding's table or output is null");
+        if (!options) fail("embedding options are null");
+        embedding_lookup_device(*table, indices, count, *options, *output, workspace, workspace_len,
+                                static_cast<cudaStream_t>(stream));
+    });
+}
+
+int32_t arcqml_rt_v2_embedding_gradient(const ArcqmlRows *gradient, const void *indices,
+                                        const ArcqmlEmbeddingOptions *options, const ArcqmlRows *table,
+                                        const ArcqmlRows *output, double *workspace,
+                                        size_t workspace_len, void *stream) {
+    return guarded([&] {
+        if (!gradient || !output) fail("the embedding's gradient or output is null");
+        if (!options) fail("embedding options are null");
+        embedding_gradient_device(*gradient, indices, *options, table, *output, workspace, workspace_len,
+                                  static_cast<cudaStream_t>(stream));
+    });
+}
+
+size_t arcqml_rt_v2_orthogonalize_workspace(const ArcqmlMatrix *matrices, size_t num_matrices) {
+    return orthogonalize_workspace(matrices, num_matrices);
+}
+
+int32_t arcqml_rt_v2_orthogonalize(const ArcqmlMatrix *matrices, const ArcqmlMatrix *outputs,
+                                   size_t num_matrices, int32_t steps, double epsilon,
+                                   double *workspace, size_t workspace_len, void *stream) {
+    return guarded([&] {
+        orthogonalize_device(matrices, outputs, num_matrices, steps, epsilon, workspace, workspace_len,
+                             static_cast<cudaStream_t>(stream));
+    });
+}
+
+int32_t arcqml_rt_v2_muon_step(const ArcqmlMatrix *parameters, const ArcqmlMatrix *gradients,
+                               const ArcqmlMatrix *momenta, size_t num_matrices,
+                               const ArcqmlMuonOptions *options, double *workspace,
+                               size_t workspace_len, void *stream) {
+    return guarded([&] {
+        if (!options) fail("Muon options are null");
+        muon_step_device(parameters, gradients, momenta, num_matrices, *options, workspace, workspace_len,
                          static_cast<cudaStream_t>(stream));
     });
 }

@@ -1,0 +1,76 @@
+// elements.cuh — element types of device tensors: conversion, and vectors of them as one access moves
+// them (embedding.cu, muon.cu).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "../../include/arcqml_runtime_v2.h"
+
+namespace arcqml {
+
+// The type in memory, and the type of the arithmetic on it.
+template <uint32_t DTYPE> struct ElementOf;
+template <> struct ElementOf<ARCQML_F64> {
+    using type = double;
+    using wide = double;
+};
+template <> struct ElementOf<ARCQML_F32> {
+    using type = float;
+    using wide = float;
+};
+template <> struct ElementOf<ARCQML_BF16> {
+    using type = __nv_bfloat16;
+    using wide = float;
+};
+template <> struct ElementOf<ARCQML_F16> {
+    using type = __half;
+    using wide = float;
+};
+template <uint32_t DTYPE> using Element = typename ElementOf<DTYPE>::type;
+template <uint32_t DTYPE> using WideElement = typename ElementOf<DTYPE>::wide;
+
+inline uint32_t bytes_of_element(uint32_t dtype) {
+    return dtype == ARCQML_F64 ? 8 : dtype == ARCQML_F32 ? 4 : 2;
+}
+
+__device__ __forceinline__ double to_wide(double x) { return x; }
+__device__ __forceinline__ float to_wide(float x) { return x; }
+__device__ __forceinline__ float to_wide(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_wide(__half x) { return __half2float(x); }
+template <class T> __device__ __forceinline__ T to_element(double x);
+template <> __device__ __forceinline__ double to_element<double>(double x) { return x; }
+template <> __device__ __forceinline__ float to_element<float>(double x) { return float(x); }
+template <class T> __device__ __forceinline__ T to_element(float x);
+template <> __device__ __forceinline__ float to_element<float>(float x) { return x; }
+template <> __device__ __forceinline__ double to_element<double>(float x) { return x; }
+template <> __device__ __forceinline__ __nv_bfloat16 to_element<__nv_bfloat16>(float x) {
+    return __float2bfloat16_rn(x);
+}
+template <> __device__ __forceinline__ __half to_element<__half>(float x) { return __float2half_rn(x); }
+
+// N elements that are loaded and stored as one access of N * sizeof(T) bytes (2, 4, 8 or 16).
+template <class T, int N> struct alignas(sizeof(T) * N) VectorOf {
+    T x[N];
+};
+
+template <class T, int N> __device__ __forceinline__ VectorOf<T, N> load_vector(const void *p) {
+    constexpr int BYTES = sizeof(T) * N;
+    VectorOf<T, N> v;
+    if constexpr (BYTES == 16) *reinterpret_cast<uint4 *>(&v) = *static_cast<const uint4 *>(p);
+    else if constexpr (BYTES == 8) *reinterpret_cast<uint2 *>(&v) = *static_cast<const uint2 *>(p);
+    else if constexpr (BYTES == 4) *reinterpret_cast<uint32_t *>(&v) = *static_cast<const uint32_t *>(p);
+    else *reinterpret_cast<uint16_t *>(&v) = *static_cast<const uint16_t *>(p);
+    return v;
+}
+
+template <class T, int N> __device__ __forceinline__ void store_vector(void *p, const VectorOf<T, N> &v) {
+    constexpr int BYTES = sizeof(T) * N;
+    if constexpr (BYTES == 16) *static_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(&v);
+    else if constexpr (BYTES == 8) *static_cast<uint2 *>(p) = *reinterpret_cast<const uint2 *>(&v);
+    else if constexpr (BYTES == 4) *static_cast<uint32_t *>(p) = *reinterpret_cast<const uint32_t *>(&v);
+    else *static_cast<uint16_t *>(p) = *reinterpret_cast<const uint16_t *>(&v);
+}
+
+}  // namespace arcqml

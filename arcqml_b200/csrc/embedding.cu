@@ -1,0 +1,819 @@
+// embedding.cu — rows of a table looked up by index (token embeddings, or states normalised from trained
+// amplitudes), and that lookup's gradient by sorted indices.
+//
+//   lookup    out[i] = s t[x_i], or s t[x_i] / |t[x_i]|
+//   gradient  G_v = s sum of g_i over the places i with x_i = v, in the places' order; for normalised rows
+//             (G_v - u <u, G_v>) / |t_v| with u = t_v / |t_v|: every place of a row has the same u, so the
+//             sum is formed first and taken through the norm once
+//
+// Both move each number once and do next to nothing with it: HBM bounds them at real sizes, launches at
+// small ones. The gradient's places are sorted by their row first (a stable radix sort, so that a row's
+// places stay in order and equal inputs give equal bits without atomics on values); chunks of the sorted
+// places are then summed side by side, whatever rows they belong to, so a row that most places point to
+// costs no more than others; rows that cross chunks are put together from the chunks' partial sums.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <sstream>
+#include <string>
+#include <tuple>
+#include <type_traits>
+
+#include "elements.cuh"
+#include "embedding.h"
+#include "launch.h"
+#include "profile.h"
+
+namespace arcqml {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr uint32_t kAbsent = 0xffffffffu; // the key of a place that counts nowhere
+
+// Indices as they lie in memory.
+struct Indices {
+    const void *at;
+    uint64_t rows;
+    int64_t padding;
+    uint32_t wide; // 8 bytes each
+    __device__ __forceinline__ int64_t operator[](uint64_t i) const {
+        return wide ? __ldg(static_cast<const long long *>(at) + i)
+                    : int64_t(__ldg(static_cast<const int *>(at) + i));
+    }
+    __device__ __forceinline__ bool inside(int64_t x) const { return uint64_t(x) < rows; }
+    __device__ __forceinline__ bool is_padding(int64_t x) const { return padding >= 0 && x == padding; }
+};
+
+struct Lookup {
+    const char *table;
+    char *out;
+    Indices index;
+    uint64_t places, stride, row_bytes; // stride: bytes between the table's rows
+    double scale;
+    const double *squares; // of normalised rows in pieces: sums of squares, `pieces` for each place
+    uint32_t vectors;      // of a row
+    uint32_t lanes;        // a power of two: threads that share a tile
+    uint32_t tiles, pieces;
+};
+
+constexpr uint32_t kTileVectors = 4;   // vectors of a tile for each of its threads
+constexpr uint32_t kRowVectors = 8;    // of a normalised row that its threads hold in registers
+constexpr uint32_t kPieceVectors = 2048;
+
+// ------------------------------------------------------------------ lookup
+
+template <class T> __device__ __forceinline__ T not_a_number() {
+    return to_element<T>(WideElement<ARCQML_F32>(__int_as_float(0x7fffffff)));
+}
+
+// Rows in tiles of 4 vectors a thread, a tile taken by `lanes` threads.
+template <uint32_t DT, int N>
+__global__ void __launch_bounds__(kThreads) k_lookup(const __grid_constant__ Lookup a) {
+    using T = Element<DT>;
+    using W = WideElement<DT>;
+    const uint64_t unit = (uint64_t(blockIdx.x) * kThreads + threadIdx.x) / a.lanes;
+    const uint32_t lane = threadIdx.x & (a.lanes - 1);
+    const uint64_t place = unit / a.tiles;
+    if (place >= a.places) return;
+    const uint32_t first = uint32_t(unit % a.tiles) * a.lanes * kTileVectors + lane;
+    const int64_t row = a.index[place];
+    const bool inside = a.index.inside(row), padding = a.index.is_padding(row);
+    const char *from = a.table + (inside ? uint64_t(row) : 0) * a.stride;
+    char *to = a.out + place * a.row_bytes;
+    VectorOf<T, N> v[kTileVectors];
+#pragma unroll
+    for (uint32_t j = 0; j < kTileVectors; ++j) {
+        const uint32_t k = first + j * a.lanes;
+        if (inside && k < a.vectors) v[j] = load_vector<T, N>(from + uint64_t(k) * sizeof(v[j]));
+    }
+    double factor = a.scale;
+    if (a.squares) {
+        double sum = 0.0;
+        if (inside && !padding)
+            for (uint32_t p = 0; p < a.pieces; ++p) sum += a.squares[place * a.pieces + p];
+        factor = sum == 0.0 ? 0.0 : a.scale / sqrt(sum);
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < kTileVectors; ++j) {
+        const uint32_t k = first + j * a.lanes;
+        if (k >= a.vectors) continue;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            if (padding) v[j].x[e] = to_element<T>(W(0));
+            else if (!inside) v[j].x[e] = not_a_number<T>();
+            else if (a.squares) v[j].x[e] = to_element<T>(W(double(to_wide(v[j].x[e])) * factor));
+            else v[j].x[e] = to_element<T>(to_wide(v[j].x[e]) * W(factor));
+        }
+        store_vector<T, N>(to + uint64_t(k) * sizeof(v[j]), v[j]);
+    }
+}
+
+// The sum over `lanes` threads (up to a block's), the same in each of them.
+template <bool BLOCK> __device__ __forceinline__ double sum_over(double v, uint32_t lanes) {
+    const uint32_t within = BLOCK ? 32 : lanes;
+    for (uint32_t o = within / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, int(o));
+    if constexpr (BLOCK) {
+        __shared__ double part[kThreads / 32];
+        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = 0.0;
+        for (int w = 0; w < kThreads / 32; ++w) v += part[w];
+    }
+    return v;
+}
+
+// Normalised rows that their threads hold: `lanes` threads of a warp, or a block, for each place.
+template <uint32_t DT, int N, bool BLOCK>
+__global__ void __launch_bounds__(kThreads) k_lookup_row(const __grid_constant__ Lookup a) {
+    using T = Element<DT>;
+    using W = WideElement<DT>;
+    const uint32_t lanes = BLOCK ? kThreads : a.lanes;
+    const uint64_t place = BLOCK ? blockIdx.x : (uint64_t(blockIdx.x) * kThreads + threadIdx.x) / lanes;
+    const uint32_t lane = threadIdx.x & (lanes - 1);
+    const bool on = place < a.places;
+    const int64_t row = on ? a.index[place] : -1;
+    const bool inside = a.index.inside(row), padding = a.index.is_padding(row);
+    const char *from = a.table + (inside ? uint64_t(row) : 0) * a.stride;
+    VectorOf<T, N> v[kRowVectors];
+#pragma unroll
+    for (uint32_t j = 0; j < kRowVectors; ++j) {
+        const uint32_t k = lane + j * lanes;
+        if (inside && !padding && k < a.vectors) v[j] = load_vector<T, N>(from + uint64_t(k) * sizeof(v[j]));
+        else
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[j].x[e] = to_element<T>(W(0));
+    }
+    double sum = 0.0;
+#pragma unroll
+    for (uint32_t j = 0; j < kRowVectors; ++j)
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const double x = to_wide(v[j].x[e]);
+            sum = fma(x, x, sum);
+        }
+    sum = sum_over<BLOCK>(sum, lanes);
+    const double factor = sum == 0.0 ? 0.0 : a.scale / sqrt(sum);
+    char *to = a.out + place * a.row_bytes;
+#pragma unroll
+    for (uint32_t j = 0; j < kRowVectors; ++j) {
+        const uint32_t k = lane + j * lanes;
+        if (!on || k >= a.vectors) continue;
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            v[j].x[e] = padding || inside ? to_element<T>(W(double(to_wide(v[j].x[e])) * factor))
+                                          : not_a_number<T>();
+        store_vector<T, N>(to + uint64_t(k) * sizeof(v[j]), v[j]);
+    }
+}
+
+// Squares of one piece of the row of one place: a block each.
+template <uint32_t DT, int N>
+__global__ void __launch_bounds__(kThreads) k_row_squares(const __grid_constant__ Lookup a, double *squares) {
+    using T = Element<DT>;
+    const uint64_t place = blockIdx.x / a.pieces;
+    const uint32_t piece = blockIdx.x % a.pieces;
+    const int64_t row = a.index[place];
+    double sum = 0.0;
+    if (a.index.inside(row) && !a.index.is_padding(row)) {
+        const char *from = a.table + uint64_t(row) * a.stride;
+        const uint32_t end = min(a.vectors, (piece + 1) * kPieceVectors);
+#pragma unroll 8
+        for (uint32_t k = piece * kPieceVectors + threadIdx.x; k < end; k += kThreads) {
+            const auto v = load_vector<T, N>(from + uint64_t(k) * sizeof(VectorOf<T, N>));
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const double x = to_wide(v.x[e]);
+                sum = fma(x, x, sum);
+            }
+        }
+    }
+    sum = sum_over<true>(sum, kThreads);
+    if (threadIdx.x == 0) squares[uint64_t(place) * a.pieces + piece] = sum;
+}
+
+// ------------------------------------------------------------------ sorting the places by their rows
+
+// Keys are rows; places that count nowhere have the key kAbsent and end up last. A pass takes up to 9
+// bits; blocks of 2048 keys are ranked by their warps in the order of the places.
+constexpr uint32_t kBins = 512, kSortKeys = 2048, kKeysPerThread = kSortKeys / kThreads;
+constexpr uint32_t kWarps = kThreads / 32;
+
+struct Sort {
+    Indices index;
+    const uint32_t *keys, *from; // null in the first pass, which reads the indices
+    uint32_t *out_keys, *out_places;
+    uint32_t *counts; // [blocks][kBins] of this pass, as prefixes over the blocks if `totals` is not null
+    uint32_t *totals; // [kBins]
+    uint32_t *next;   // counts of the next pass, zero so far; null in the last one
+    uint32_t places, blocks, shift, next_shift, bits;
+};
+
+__device__ __forceinline__ uint32_t key_at(const Indices &x, uint64_t i) {
+    const int64_t v = x[i];
+    return x.inside(v) && !x.is_padding(v) ? uint32_t(v) : kAbsent;
+}
+__device__ __forceinline__ uint32_t digit_of(uint32_t key, uint32_t shift, uint32_t bits) {
+    return key >> shift & ((1u << bits) - 1);
+}
+
+// The first pass's counts; clears those of the passes behind it (`clear` words at s.next).
+__global__ void __launch_bounds__(kThreads) k_count_digits(const __grid_constant__ Sort s, uint64_t clear) {
+    __shared__ uint32_t bins[kBins];
+    for (uint32_t b = threadIdx.x; b < kBins; b += kThreads) bins[b] = 0;
+    for (uint64_t i = uint64_t(blockIdx.x) * kThreads + threadIdx.x; i < clear; i += uint64_t(gridDim.x) * kThreads)
+        s.next[i] = 0;
+    __syncthreads();
+    const uint32_t end = uint32_t(min(uint64_t(s.places), (uint64_t(blockIdx.x) + 1) * kSortKeys));
+    for (uint32_t i = blockIdx.x * kSortKeys + threadIdx.x; i < end; i += kThreads)
+        atomicAdd(&bins[digit_of(key_at(s.index, i), s.shift, s.bits)], 1u);
+    __syncthreads();
+    for (uint32_t b = threadIdx.x; b < kBins; b += kThreads) s.counts[uint64_t(blockIdx.x) * kBins + b] = bins[b];
+}
+
+// For many blocks: counts -> the number of the digit's keys in earlier blocks, and the digits' totals.
+// A block takes 32 digits, 32 threads each.
+__global__ void __launch_bounds__(1024) k_prefix_counts(uint32_t *counts, uint32_t *totals, uint32_t blocks) {
+    __shared__ uint32_t part[32][33];
+    const uint32_t digit = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
+    const uint32_t each = (blocks + 31) / 32, lo = slice * each, hi = min(blocks, lo + each);
+    uint32_t sum = 0;
+    for (uint32_t b = lo; b < hi; ++b) sum += counts[uint64_t(b) * kBins + digit];
+    part[slice][threadIdx.x & 31] = sum;
+    __syncthreads();
+    uint32_t before = 0, all = 0;
+    for (uint32_t i = 0; i < 32; ++i) {
+        if (i == slice) before = all;
+        all += part[i][threadIdx.x & 31];
+    }
+    for (uint32_t b = lo; b < hi; ++b) {
+        const uint32_t c = counts[uint64_t(b) * kBins + digit];
+        counts[uint64_t(b) * kBins + digit] = before;
+        before += c;
+    }
+    if (slice == 0) totals[digit] = all;
+}
+
+__global__ void __launch_bounds__(kThreads) k_sort_pass(const __grid_constant__ Sort s) {
+    __shared__ uint32_t hist[kWarps][kBins];
+    __shared__ uint32_t base[kBins];
+    __shared__ uint32_t warp_sum[kWarps];
+    const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    for (uint32_t b = t; b < kWarps * kBins; b += kThreads) (&hist[0][0])[b] = 0;
+    __syncthreads();
+    uint32_t key[kKeysPerThread], rank[kKeysPerThread];
+    const uint32_t first = blockIdx.x * kSortKeys + warp * (kSortKeys / kWarps) + lane;
+#pragma unroll
+    for (uint32_t j = 0; j < kKeysPerThread; ++j) {
+        const uint32_t i = first + j * 32;
+        key[j] = i >= s.places ? kAbsent : s.keys ? s.keys[i] : key_at(s.index, i);
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < kKeysPerThread; ++j) {
+        const bool on = first + j * 32 < s.places; // the warp's first lanes, all of it but at the end
+        const uint32_t d = on ? digit_of(key[j], s.shift, s.bits) : kBins; // kBins: matches no digit
+        const uint32_t same = __match_any_sync(0xffffffffu, d);
+        const uint32_t before = __popc(same & ((1u << lane) - 1));
+        if (on) rank[j] = hist[warp][d] + before;
+        __syncwarp();
+        if (on && before == 0) hist[warp][d] += __popc(same);
+        __syncwarp();
+    }
+    __syncthreads();
+    // each thread: two neighbouring digits
+    uint32_t all[2], mine[2];
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) {
+        const uint32_t d = 2 * t + h;
+        uint32_t sum = 0;
+        for (uint32_t w = 0; w < kWarps; ++w) {
+            const uint32_t c = hist[w][d];
+            hist[w][d] = sum;
+            sum += c;
+        }
+        all[h] = mine[h] = 0;
+        if (s.totals) {
+            all[h] = s.totals[d];
+            mine[h] = s.counts[uint64_t(blockIdx.x) * kBins + d];
+        }
+    }
+    if (!s.totals) {
+#pragma unroll 8
+        for (uint32_t b = 0; b < s.blocks; ++b) {
+            const uint2 c = *reinterpret_cast<const uint2 *>(s.counts + uint64_t(b) * kBins + 2 * t);
+            if (b < blockIdx.x) {
+                mine[0] += c.x;
+                mine[1] += c.y;
+            }
+            all[0] += c.x;
+            all[1] += c.y;
+        }
+    }
+    uint32_t sum = all[0] + all[1], scan = sum;
+    for (uint32_t o = 1; o < 32; o *= 2) {
+        const uint32_t up = __shfl_up_sync(0xffffffffu, scan, o);
+        if (lane >= o) scan += up;
+    }
+    if (lane == 31) warp_sum[warp] = scan;
+    __syncthreads();
+    uint32_t before = scan - sum;
+    for (uint32_t w = 0; w < warp; ++w) before += warp_sum[w];
+    base[2 * t] = before + mine[0];
+    base[2 * t + 1] = before + all[0] + mine[1];
+    __syncthreads();
+#pragma unroll
+    for (uint32_t j = 0; j < kKeysPerThread; ++j) {
+        const uint32_t i = first + j * 32;
+        if (i >= s.places) continue;
+        const uint32_t d = digit_of(key[j], s.shift, s.bits);
+        const uint32_t to = base[d] + hist[warp][d] + rank[j];
+        s.out_keys[to] = key[j];
+        s.out_places[to] = s.from ? s.from[i] : i;
+        if (s.next) atomicAdd(&s.next[uint64_t(to / kSortKeys) * kBins + digit_of(key[j], s.next_shift, s.bits)], 1u);
+    }
+}
+
+// ------------------------------------------------------------------ sums of the rows' places
+
+struct Sums {
+    const char *gradient;
+    char *out;
+    const uint32_t *keys, *at; // sorted: the row, and the place
+    void *partial;             // [2 chunks][width] of the wide type: rows that cross chunks
+    uint64_t stride;           // bytes between the gradient's rows
+    uint64_t width, rows;
+    double scale;
+    uint32_t places, chunk, chunks;
+    uint32_t vectors, lanes, tiles;
+};
+
+// Places at a time in flight for each thread.
+constexpr uint32_t kAhead = 8;
+
+template <class T, class O, class W, int N>
+__device__ __forceinline__ void write_sum(const Sums &a, uint32_t row, uint32_t vector, const W (&sum)[N]) {
+    constexpr int PART = sizeof(O) * N > 16 ? 16 / int(sizeof(O)) : N; // sums of 16-bit rows in 32 bits: two stores
+    char *to = a.out + (uint64_t(row) * a.width + uint64_t(vector) * N) * sizeof(O);
+#pragma unroll
+    for (int p = 0; p < N; p += PART) {
+        VectorOf<O, PART> v;
+#pragma unroll
+        for (int e = 0; e < PART; ++e) v.x[e] = to_element<O>(sum[p + e] * W(a.scale));
+        store_vector<O, PART>(to + p * sizeof(O), v);
+    }
+}
+
+// One vector of a row for each thread, over the places of one chunk. A row that lies inside the chunk is
+// done; the part of one that began earlier goes to partial 2c, of one that goes on to 2c + 1.
+template <uint32_t DT, uint32_t OT, int N>
+__global__ void __launch_bounds__(kThreads) k_sum_chunks(const __grid_constant__ Sums a) {
+    using T = Element<DT>;
+    using O = Element<OT>;
+    using W = WideElement<DT>;
+    const uint64_t unit = (uint64_t(blockIdx.x) * kThreads + threadIdx.x) / a.lanes;
+    const uint32_t c = uint32_t(unit / a.tiles);
+    const uint32_t vector = uint32_t(unit % a.tiles) * a.lanes + (threadIdx.x & (a.lanes - 1));
+    if (c >= a.chunks || vector >= a.vectors) return;
+    const uint32_t i0 = c * a.chunk, i1 = min(a.places, i0 + a.chunk);
+    uint32_t row = a.keys[i0], begin = i0;
+    if (row == kAbsent) return;
+    W sum[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) sum[e] = W(0);
+    const auto flush = [&](uint32_t end) {
+        const bool starts = begin > i0 || i0 == 0 || a.keys[i0 - 1] != row;
+        const bool ends = end < i1 || i1 == a.places || a.keys[i1] != row;
+        if (starts && ends) {
+            write_sum<T, O, W, N>(a, row, vector, sum);
+        } else {
+            W *p = static_cast<W *>(a.partial) + (uint64_t(2) * c + (starts ? 1 : 0)) * a.width + uint64_t(vector) * N;
+#pragma unroll
+            for (int e = 0; e < N; ++e) p[e] = sum[e];
+        }
+    };
+    for (uint32_t i = i0; i < i1; i += kAhead) {
+        uint32_t key[kAhead];
+        VectorOf<T, N> v[kAhead];
+#pragma unroll
+        for (uint32_t j = 0; j < kAhead; ++j) {
+            key[j] = i + j < i1 ? a.keys[i + j] : kAbsent;
+            if (key[j] != kAbsent)
+                v[j] = load_vector<T, N>(a.gradient + uint64_t(a.at[i + j]) * a.stride + uint64_t(vector) * sizeof(v[j]));
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < kAhead; ++j) {
+            if (key[j] != row) {
+                if (row != kAbsent) flush(i + j);
+                row = key[j];
+                begin = i + j;
+#pragma unroll
+                for (int e = 0; e < N; ++e) sum[e] = W(0);
+            }
+            if (key[j] == kAbsent) break;
+#pragma unroll
+            for (int e = 0; e < N; ++e) sum[e] += to_wide(v[j].x[e]);
+        }
+        if (row == kAbsent) return;
+    }
+    flush(i1);
+}
+
+// The first place in the sorted keys that is not below `key`.
+__device__ __forceinline__ uint32_t first_not_below(const uint32_t *keys, uint32_t n, uint32_t key) {
+    uint32_t lo = 0, hi = n;
+    while (lo < hi) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        if (keys[mid] < key) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// Rows that began in a chunk and went on: its partial sums in order.
+template <uint32_t DT, uint32_t OT, int N>
+__global__ void __launch_bounds__(kThreads) k_join_chunks(const __grid_constant__ Sums a) {
+    using T = Element<DT>;
+    using O = Element<OT>;
+    using W = WideElement<DT>;
+    const uint64_t unit = (uint64_t(blockIdx.x) * kThreads + threadIdx.x) / a.lanes;
+    const uint32_t c = uint32_t(unit / a.tiles);
+    const uint32_t vector = uint32_t(unit % a.tiles) * a.lanes + (threadIdx.x & (a.lanes - 1));
+    if (c + 1 >= a.chunks || vector >= a.vectors) return;
+    const uint32_t i0 = c * a.chunk, i1 = i0 + a.chunk, row = a.keys[i1 - 1];
+    if (row == kAbsent || a.keys[i1] != row) return;
+    if (a.keys[i0] == row && i0 != 0 && a.keys[i0 - 1] == row) return; // it began earlier
+    const uint32_t last = (first_not_below(a.keys, a.places, row + 1) - 1) / a.chunk;
+    W sum[N];
+    const W *p = static_cast<const W *>(a.partial) + uint64_t(vector) * N;
+#pragma unroll
+    for (int e = 0; e < N; ++e) sum[e] = p[(uint64_t(2) * c + 1) * a.width + e];
+#pragma unroll 8
+    for (uint32_t d = c + 1; d <= last; ++d)
+#pragma unroll
+        for (int e = 0; e < N; ++e) sum[e] += p[uint64_t(2) * d * a.width + e];
+    write_sum<T, O, W, N>(a, row, vector, sum);
+}
+
+// Rows that no index points to: a warp looks at 32 rows.
+template <uint32_t OT> __global__ void __launch_bounds__(kThreads) k_zero_rows(const __grid_constant__ Sums a) {
+    using O = Element<OT>;
+    const uint32_t lane = threadIdx.x & 31;
+    const uint64_t first = (uint64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5)) * 32;
+    if (first >= a.rows) return;
+    bool absent = false;
+    if (first + lane < a.rows) {
+        const uint32_t key = uint32_t(first) + lane, at = first_not_below(a.keys, a.places, key);
+        absent = at == a.places || a.keys[at] != key;
+    }
+    O *out = reinterpret_cast<O *>(a.out);
+    for (uint32_t m = __ballot_sync(0xffffffffu, absent); m; m &= m - 1) {
+        O *row = out + (first + __ffs(int(m)) - 1) * a.width;
+        for (uint64_t k = lane; k < a.width; k += 32) row[k] = to_element<O>(WideElement<OT>(0));
+    }
+}
+
+// Sums through the norm of their rows, a block for each row; `sums` may be the output itself.
+struct Project {
+    const char *table, *sums;
+    char *out;
+    const uint32_t *keys;
+    uint64_t table_stride, width, rows;
+    uint32_t places;
+};
+template <uint32_t DT>
+__global__ void __launch_bounds__(kThreads) k_project(const __grid_constant__ Project a) {
+    using T = Element<DT>;
+    using W = WideElement<DT>;
+    __shared__ double part[2][kWarps];
+    const uint32_t row = blockIdx.x;
+    const uint32_t at = first_not_below(a.keys, a.places, row);
+    T *out = reinterpret_cast<T *>(a.out) + uint64_t(row) * a.width;
+    if (at == a.places || a.keys[at] != row) {
+        for (uint64_t k = threadIdx.x; k < a.width; k += kThreads) out[k] = to_element<T>(W(0));
+        return;
+    }
+    const T *t = reinterpret_cast<const T *>(a.table + uint64_t(row) * a.table_stride);
+    const W *g = reinterpret_cast<const W *>(a.sums) + uint64_t(row) * a.width;
+    double tt = 0.0, tg = 0.0;
+#pragma unroll 4
+    for (uint64_t k = threadIdx.x; k < a.width; k += kThreads) {
+        const double x = to_wide(t[k]);
+        tt = fma(x, x, tt);
+        tg = fma(x, double(g[k]), tg);
+    }
+    for (int o = 16; o > 0; o >>= 1) {
+        tt += __shfl_xor_sync(0xffffffffu, tt, o);
+        tg += __shfl_xor_sync(0xffffffffu, tg, o);
+    }
+    if ((threadIdx.x & 31) == 0) {
+        part[0][threadIdx.x >> 5] = tt;
+        part[1][threadIdx.x >> 5] = tg;
+    }
+    __syncthreads();
+    tt = tg = 0.0;
+    for (uint32_t w = 0; w < kWarps; ++w) {
+        tt += part[0][w];
+        tg += part[1][w];
+    }
+    const double inverse = tt == 0.0 ? 0.0 : 1.0 / sqrt(tt), along = tt == 0.0 ? 0.0 : tg / tt;
+#pragma unroll 4
+    for (uint64_t k = threadIdx.x; k < a.width; k += kThreads)
+        out[k] = to_element<T>(W((double(g[k]) - double(to_wide(t[k])) * along) * inverse));
+}
+
+// ------------------------------------------------------------------ host
+
+[[noreturn]] void refuse(const char *what, const char *why) {
+    fail(std::string("the embedding's ") + what + " " + why);
+}
+
+void check_rows(const ArcqmlRows &r, const char *what) {
+    if (r.dtype > ARCQML_F16) refuse(what, "has an unknown type");
+    if (r.reserved != 0) refuse(what, "has a nonzero reserved field");
+    if (r.rows >> 31) refuse(what, "has too many rows (2^31 at most)");
+    if (r.width == 0) refuse(what, "has rows without elements");
+    if (r.width >> 30) refuse(what, "has rows that are too long (below 2^30 elements)");
+    if (r.stride >> 40) refuse(what, "has rows too far apart");
+    if (!r.rows) return;
+    if (!r.data) refuse(what, "is null");
+    if (reinterpret_cast<uintptr_t>(r.data) % bytes_of_element(r.dtype))
+        refuse(what, "is not aligned to its elements");
+}
+
+void check_options(const ArcqmlEmbeddingOptions &o) {
+    if (!std::isfinite(o.scale)) refuse("scale", "must be finite");
+    if (o.normalize != 0 && o.normalize != 1) refuse("options", "are invalid (normalize is 0 or 1)");
+    if (o.index_bytes != 4 && o.index_bytes != 8) refuse("indices", "must have 4 or 8 bytes");
+}
+
+void check_indices(const void *indices, size_t count, const ArcqmlEmbeddingOptions &o) {
+    if (count >> 31) refuse("indices", "are too many (below 2^31)");
+    if (!count) return;
+    if (!indices) refuse("indices", "are null");
+    if (reinterpret_cast<uintptr_t>(indices) % size_t(o.index_bytes)) refuse("indices", "are not aligned");
+}
+
+void check_scratch(const double *ws, size_t len, size_t need) {
+    if (!need) return;
+    if (!ws) fail("workspace is null");
+    if (reinterpret_cast<uintptr_t>(ws) % 16) fail("workspace is not aligned to 16 bytes");
+    if (len < need) {
+        std::ostringstream m;
+        m << "workspace of " << len << " doubles is too small: the call needs " << need;
+        fail(m.str());
+    }
+}
+
+uint32_t power_of_two_from(uint64_t n) {
+    uint32_t p = 1;
+    while (p < n && p < 32) p *= 2;
+    return p;
+}
+
+// The largest access, up to 16 bytes, on which every row starts and ends.
+uint32_t access_bytes(uint64_t bits) {
+    uint32_t v = 16;
+    while (v > 1 && bits % v) v /= 2;
+    return v;
+}
+
+// f(type code, elements of an access), for what an access of `bytes` can hold.
+template <class F> void for_access(uint32_t dtype, uint32_t bytes, F &&f) {
+    const auto pick = [&](auto type) {
+        constexpr uint32_t DT = type, SIZE = sizeof(Element<DT>);
+        if constexpr (SIZE <= 2)
+            if (bytes == 2) return f(type, std::integral_constant<int, 2 / SIZE>{});
+        if constexpr (SIZE <= 4)
+            if (bytes == 4) return f(type, std::integral_constant<int, 4 / SIZE>{});
+        if (bytes == 8) return f(type, std::integral_constant<int, 8 / SIZE>{});
+        return f(type, std::integral_constant<int, 16 / SIZE>{});
+    };
+    switch (dtype) {
+    case ARCQML_F64: return pick(std::integral_constant<uint32_t, ARCQML_F64>{});
+    case ARCQML_F32: return pick(std::integral_constant<uint32_t, ARCQML_F32>{});
+    case ARCQML_BF16: return pick(std::integral_constant<uint32_t, ARCQML_BF16>{});
+    default: return pick(std::integral_constant<uint32_t, ARCQML_F16>{});
+    }
+}
+
+template <class... P, class... A>
+void start(void (*kernel)(P...), uint64_t blocks, uint32_t threads, double bytes, cudaStream_t s, const A &...args) {
+    if (blocks >> 31) fail("the embedding call is too large for one launch");
+    cudaLaunchConfig_t c{};
+    c.gridDim = dim3(uint32_t(blocks));
+    c.blockDim = dim3(threads);
+    c.stream = s;
+    std::tuple<P...> held{P(args)...};
+    const ProfToken tok = prof_begin(PROF_OTHER, s);
+    const cudaError_t e = std::apply([&](auto &...x) { return cudaLaunchKernelEx(&c, kernel, x...); }, held);
+    check_cuda(e, "embedding kernel launch");
+    prof_end(tok, s, bytes);
+}
+
+uint64_t blocks_for(uint64_t threads) { return (threads + kThreads - 1) / kThreads; }
+
+uint64_t address(const void *p) { return reinterpret_cast<uintptr_t>(p); }
+
+// The most pieces that a normalised row may be cut into (0: its threads hold it): accesses are as small as
+// an element where rows start anywhere.
+uint32_t most_pieces(const ArcqmlRows &t, const ArcqmlEmbeddingOptions &o) {
+    return o.normalize && t.width > kThreads * kRowVectors ? uint32_t((t.width + kPieceVectors - 1) / kPieceVectors) : 0;
+}
+
+// Scratch of the gradient, in 4-byte words from its start.
+struct GradientScratch {
+    uint64_t keys[2], places[2], counts, totals, partial, sums, words;
+    uint32_t blocks, passes, bits, chunk, chunks;
+};
+
+GradientScratch gradient_scratch(const ArcqmlRows &g, uint64_t rows, const ArcqmlEmbeddingOptions &o) {
+    GradientScratch s{};
+    const uint64_t n = g.rows;
+    const auto take = [&](uint64_t words) {
+        const uint64_t at = s.words;
+        s.words += (words + 3) / 4 * 4;
+        return at;
+    };
+    uint32_t bits = 1;
+    while (bits < 32 && (rows >> bits)) ++bits; // kAbsent's digits are all ones: above any row's
+    s.passes = (bits + 8) / 9;
+    s.bits = (bits + s.passes - 1) / s.passes;
+    s.blocks = uint32_t((n + kSortKeys - 1) / kSortKeys);
+    for (int i = 0; i < 2; ++i) {
+        s.keys[i] = take(n);
+        s.places[i] = take(n);
+    }
+    s.counts = take(uint64_t(s.passes) * s.blocks * kBins);
+    s.totals = take(kBins);
+    // chunks: enough of them to fill the GPU, 128 places at most
+    const uint64_t tiles = std::max<uint64_t>(1, g.width * bytes_of_element(g.dtype) / 512);
+    s.chunk = 8;
+    while (s.chunk < 128 && n * tiles / (s.chunk * 2) >= 148 * 32) s.chunk *= 2;
+    s.chunks = uint32_t((n + s.chunk - 1) / s.chunk);
+    const uint64_t wide = g.dtype == ARCQML_F64 ? 2 : 1;
+    s.partial = take(2 * uint64_t(s.chunks) * g.width * wide);
+    s.sums = s.words;
+    if (o.normalize && (g.dtype == ARCQML_BF16 || g.dtype == ARCQML_F16)) take(rows * g.width);
+    return s;
+}
+
+}  // namespace
+
+size_t embedding_lookup_workspace(const ArcqmlRows &table, size_t count, const ArcqmlEmbeddingOptions &o) {
+    return size_t(most_pieces(table, o)) * count;
+}
+
+size_t embedding_gradient_workspace(const ArcqmlRows &gradient, uint64_t rows, const ArcqmlEmbeddingOptions &o) {
+    return size_t((gradient_scratch(gradient, rows, o).words + 1) / 2);
+}
+
+void embedding_lookup_device(const ArcqmlRows &table, const void *indices, size_t count,
+                             const ArcqmlEmbeddingOptions &o, const ArcqmlRows &out, double *ws,
+                             size_t ws_len, cudaStream_t s) {
+    check_options(o);
+    check_rows(table, "table");
+    check_rows(out, "output");
+    check_indices(indices, count, o);
+    if (out.dtype != table.dtype || out.width != table.width || out.rows != count || out.stride != out.width)
+        refuse("output", "does not have the table's type and width, a row for each index and no gaps");
+    check_scratch(ws, ws_len, embedding_lookup_workspace(table, count, o));
+    if (!count) return;
+    const uint64_t size = bytes_of_element(table.dtype);
+    Lookup a{};
+    a.table = static_cast<const char *>(table.data);
+    a.out = static_cast<char *>(out.data);
+    a.index = {indices, table.rows, o.padding, o.index_bytes == 8};
+    a.places = count;
+    a.stride = table.stride * size;
+    a.row_bytes = table.width * size;
+    a.scale = o.scale;
+    const uint32_t bytes = access_bytes(address(table.data) | address(out.data) | a.stride | a.row_bytes | 16);
+    const uint64_t vectors = a.row_bytes / bytes;
+    a.vectors = uint32_t(vectors);
+    const double moved = 2.0 * double(count) * double(a.row_bytes);
+    const bool held = o.normalize && vectors <= kThreads * kRowVectors;
+    for_access(table.dtype, bytes, [&](auto type, auto n) {
+        constexpr uint32_t DT = type;
+        constexpr int N = n;
+        if (held && vectors > 32 * kRowVectors) return start(k_lookup_row<DT, N, true>, count, kThreads, moved, s, a);
+        if (held) {
+            a.lanes = power_of_two_from((vectors + 1) / 2);
+            while (a.lanes * kRowVectors < vectors) a.lanes *= 2;
+            return start(k_lookup_row<DT, N, false>, blocks_for(count * a.lanes), kThreads, moved, s, a);
+        }
+        if (o.normalize) {
+            a.pieces = uint32_t((vectors + kPieceVectors - 1) / kPieceVectors);
+            start(k_row_squares<DT, N>, count * a.pieces, kThreads, moved / 2, s, a, ws);
+            a.squares = ws;
+        }
+        a.lanes = power_of_two_from((vectors + kTileVectors - 1) / kTileVectors);
+        a.tiles = uint32_t((vectors + a.lanes * kTileVectors - 1) / (a.lanes * kTileVectors));
+        start(k_lookup<DT, N>, blocks_for(count * a.tiles * a.lanes), kThreads, moved, s, a);
+    });
+}
+
+void embedding_gradient_device(const ArcqmlRows &gradient, const void *indices, const ArcqmlEmbeddingOptions &o,
+                               const ArcqmlRows *table, const ArcqmlRows &out, double *ws, size_t ws_len,
+                               cudaStream_t s) {
+    check_options(o);
+    check_rows(gradient, "gradient");
+    check_rows(out, "output");
+    check_indices(indices, gradient.rows, o);
+    if (out.dtype != gradient.dtype || out.width != gradient.width || out.stride != out.width)
+        refuse("output", "does not have the gradient's type and width, without gaps");
+    if (o.normalize && !table) refuse("table", "is null and its rows are normalised");
+    if (!o.normalize && table) refuse("table", "is given and its rows are not normalised");
+    if (table) {
+        check_rows(*table, "table");
+        if (table->dtype != out.dtype || table->width != out.width || table->rows != out.rows)
+            refuse("table", "does not have the output's type and shape");
+    }
+    const GradientScratch w = gradient_scratch(gradient, out.rows, o);
+    check_scratch(ws, ws_len, size_t((w.words + 1) / 2));
+    if (!out.rows) return;
+    const uint64_t size = bytes_of_element(gradient.dtype), n = gradient.rows;
+    uint32_t *base = reinterpret_cast<uint32_t *>(ws);
+    const uint32_t *keys = base + w.keys[w.passes & 1], *places = base + w.places[w.passes & 1];
+    if (n) {
+        Sort a{};
+        a.index = {indices, out.rows, o.padding, o.index_bytes == 8};
+        a.places = uint32_t(n);
+        a.blocks = w.blocks;
+        a.bits = w.bits;
+        const uint64_t each = uint64_t(w.blocks) * kBins;
+        a.counts = base + w.counts;
+        a.next = a.counts + each;
+        start(k_count_digits, w.blocks, kThreads, 8.0 * double(n), s, a, each * (w.passes - 1));
+        for (uint32_t p = 0; p < w.passes; ++p) {
+            a.shift = p * w.bits;
+            a.next_shift = a.shift + w.bits;
+            a.counts = base + w.counts + p * each;
+            a.next = p + 1 < w.passes ? a.counts + each : nullptr;
+            a.keys = p ? base + w.keys[p & 1] : nullptr;
+            a.from = p ? base + w.places[p & 1] : nullptr;
+            a.out_keys = base + w.keys[(p + 1) & 1];
+            a.out_places = base + w.places[(p + 1) & 1];
+            a.totals = nullptr;
+            if (w.blocks > 128) {
+                a.totals = base + w.totals;
+                start(k_prefix_counts, kBins / 32, 1024, 8.0 * double(each), s, a.counts, a.totals, w.blocks);
+            }
+            start(k_sort_pass, w.blocks, kThreads, 16.0 * double(n), s, a);
+        }
+    }
+    Sums a{};
+    a.gradient = static_cast<const char *>(gradient.data);
+    a.keys = keys;
+    a.at = places;
+    a.partial = base + w.partial;
+    a.stride = gradient.stride * size;
+    a.width = out.width;
+    a.rows = out.rows;
+    a.scale = o.scale;
+    a.places = uint32_t(n);
+    a.chunk = w.chunk;
+    a.chunks = w.chunks;
+    const bool apart = o.normalize && size == 2; // the sums keep 32 bits until the norm is through
+    a.out = apart ? reinterpret_cast<char *>(base + w.sums) : static_cast<char *>(out.data);
+    const uint64_t row = a.width * size;
+    const uint32_t bytes = access_bytes(address(gradient.data) | (apart ? 0 : address(out.data)) | a.stride | row | 16);
+    a.vectors = uint32_t(row / bytes);
+    a.lanes = power_of_two_from(a.vectors);
+    a.tiles = (a.vectors + a.lanes - 1) / a.lanes;
+    const double moved = double(n) * double(row);
+    for_access(gradient.dtype, bytes, [&](auto type, auto nn) {
+        constexpr uint32_t DT = type;
+        constexpr int N = nn;
+        constexpr uint32_t WIDE = DT == ARCQML_F64 ? ARCQML_F64 : ARCQML_F32;
+        const uint64_t blocks = blocks_for(uint64_t(a.chunks) * a.tiles * a.lanes);
+        const auto sums = [&](auto kind) {
+            constexpr uint32_t OT = kind;
+            if (!n) return;
+            start(k_sum_chunks<DT, OT, N>, blocks, kThreads, moved, s, a);
+            if (a.chunks > 1) start(k_join_chunks<DT, OT, N>, blocks, kThreads, 0.0, s, a);
+        };
+        if constexpr (WIDE != DT) {
+            if (apart) sums(std::integral_constant<uint32_t, WIDE>{});
+            else sums(type);
+        } else {
+            sums(type);
+        }
+    });
+    for_access(out.dtype, 16, [&](auto type, auto) {
+        constexpr uint32_t DT = type;
+        if (!o.normalize)
+            return start(k_zero_rows<DT>, (out.rows + kWarps * 32 - 1) / (kWarps * 32), kThreads, 0.0, s, a);
+        Project p{};
+        p.table = static_cast<const char *>(table->data);
+        p.sums = a.out;
+        p.out = static_cast<char *>(out.data);
+        p.keys = keys;
+        p.table_stride = table->stride * size;
+        p.width = out.width;
+        p.rows = out.rows;
+        p.places = uint32_t(n);
+        start(k_project<DT>, out.rows, kThreads, 3.0 * double(row) * double(out.rows), s, p);
+    });
+}
+
+}  // namespace arcqml

@@ -1,4 +1,5 @@
-"""Adam for hybrid models: circuits' parameters and device tensors trained together.
+"""Optimizers for hybrid models: ``Adam`` over circuits' parameters and device tensors together, ``Muon`` over
+the matrices of the network beside them.
 
 A model whose circuit is fed by a classical network, or starts from trained states, has its
 parameters in two places: the circuit's on the host (``Circuit.parameters``, bound into plans) and
@@ -10,7 +11,8 @@ them: ``Parameter.grad`` (``RunResult.backward``, ``StateVectorSimulator.gradien
 torch's convention for complex tensors, so a network that made the states gets its gradients by
 ``states.backward(initial_state_grad)``. Amplitudes are trained the same way, through the normalisation that
 makes states of them: a step on normalised states themselves would leave them unnormalised, which
-``BatchStateVectorSimulator.from_device_state`` does not check.
+``BatchStateVectorSimulator.from_device_state`` does not check (``embedding.lookup`` with ``normalize`` does
+both for a table of amplitudes).
 """
 from __future__ import annotations
 
@@ -135,3 +137,45 @@ class Adam:
         for c in moved:
             c.take()
         return norm
+
+
+class Muon:
+    """Momentum steps whose update is orthogonalised (``runtime.muon_step_device``), over the matrices of a
+    network (row-major float32, bfloat16 or float16 CUDA leaves, or one of them). Vectors, tables, circuits'
+    parameters and amplitudes go into an ``Adam`` of their own. A matrix without gradient stays as it is. The
+    momentum is ``state`` (``runtime.DeviceMuonState``)."""
+
+    def __init__(self, matrices, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True,
+                 weight_decay: float = 0.0, steps: int = 5, eps: float = 1e-7):
+        import torch
+        self.lr, self.momentum, self.nesterov = lr, momentum, nesterov
+        self.weight_decay, self.steps, self.eps = weight_decay, steps, eps
+        self._matrices = (matrices,) if isinstance(matrices, torch.Tensor) else tuple(matrices)
+        if not self._matrices:
+            raise ValueError("there is nothing to train")
+        for i, t in enumerate(self._matrices):
+            if t is None:
+                raise TypeError("the matrices to train must not be None")
+            if isinstance(t, torch.Tensor) and not (t.is_leaf or t.retains_grad):
+                raise ValueError(f"the matrix to train at place {i} was computed from others: its "
+                                 "gradient would go to them")
+        self._parameters = rt.TensorList(self._matrices)
+        self._parameters._check_apart("the matrices")
+        self.state = rt.DeviceMuonState(self._parameters)
+
+    @property
+    def matrices(self) -> tuple:
+        """The trained matrices. Others need an optimizer, and momentum, of their own."""
+        return self._matrices
+
+    def zero_grad(self) -> None:
+        for t in self._matrices:
+            t.grad = None
+
+    def step(self) -> None:
+        """One step. Nothing is waited for."""
+        # a new list every step: one that is kept would keep the gradients' memory
+        grads = rt.TensorList([t.grad for t in self._matrices])
+        rt.muon_step_device(self._parameters, grads, self.state, lr=self.lr, momentum=self.momentum,
+                            nesterov=self.nesterov, weight_decay=self.weight_decay, steps=self.steps,
+                            eps=self.eps)

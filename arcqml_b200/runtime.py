@@ -137,6 +137,13 @@ SIGNATURES = {
     "arcqml_rt_v2_gradient_norm": (_I32, [_P, _S, _P, _P, _S, _P]),
     "arcqml_rt_v2_clip_gradients": (_I32, [_P, _S, _D, _P, _P, _P, _S, _P]),
     "arcqml_rt_v2_adam_step": (_I32, [_P, _P, _P, _P, _P, _S, _P, _P, _P, _P, _P, _S, _P]),
+    "arcqml_rt_v2_embedding_lookup_workspace": (_S, [_P, _S, _P]),
+    "arcqml_rt_v2_embedding_gradient_workspace": (_S, [_P, C.c_uint64, _P]),
+    "arcqml_rt_v2_embedding_lookup": (_I32, [_P, _P, _S, _P, _P, _P, _S, _P]),
+    "arcqml_rt_v2_embedding_gradient": (_I32, [_P, _P, _P, _P, _P, _P, _S, _P]),
+    "arcqml_rt_v2_orthogonalize_workspace": (_S, [_P, _S]),
+    "arcqml_rt_v2_orthogonalize": (_I32, [_P, _P, _S, _I32, _D, _P, _S, _P]),
+    "arcqml_rt_v2_muon_step": (_I32, [_P, _P, _P, _S, _P, _P, _S, _P]),
     "arcqml_rt_v2_norms": (_I32, [_P, _S, _S, _P, _P]),
     "arcqml_rt_v2_norms_noalloc": (_I32, [_P, _S, _S, _P, _P]),
     "arcqml_rt_v2_set_basis_state": (_I32, [_P, _S, _S, C.c_uint64, _P]),
@@ -595,6 +602,8 @@ def small_adam_device(plan: CircuitPlan, observable: "Observable", num_qubits: i
 NO_TENSOR = 4
 _TENSOR = np.dtype([("data", np.uint64), ("length", np.uint64), ("dtype", np.uint32),
                     ("reserved", np.uint32)])  # ArcqmlTensor
+_MATRIX = np.dtype([("data", np.uint64), ("rows", np.uint64), ("columns", np.uint64),
+                    ("dtype", np.uint32), ("reserved", np.uint32)])  # ArcqmlMatrix
 
 
 class AdamOptions(C.Structure):
@@ -618,10 +627,10 @@ def _tensor_kinds() -> dict:
 
 def _kind_of(torch, t) -> str:
     """What a tensor list is told that it cannot take."""
-    if not isinstance(t, torch.Tensor):
+    if torch is not None and not isinstance(t, torch.Tensor):
         return type(t).__name__
     lazy = [bit for bit, on in (("conj", t.is_conj()), ("neg", t.is_neg())) if on]
-    return (f"{t.dtype} on {t.device}" + (f" laid out as {t.layout}" if t.layout != torch.strided else "")
+    return (f"{t.dtype} on {t.device}" + (f" laid out as {t.layout}" if str(t.layout) != "torch.strided" else "")
             + (f" with its lazy {' and '.join(lazy)} bit set (resolve_conj, resolve_neg)" if lazy else ""))
 
 
@@ -695,7 +704,7 @@ class TensorList:
         self._layouts, self._spans, self._apart = layouts, spans, None
         self._shapes = [None if t is None else t.shape for t in self.tensors]
         self._pointers = [r[0] for r in rows if r[2] != NO_TENSOR]
-        self._roots = None
+        self._roots = self._matrices = None
         self._state = object()  # another one whenever the list is written down
 
     def _current(self, torch, device: int) -> int:
@@ -713,6 +722,25 @@ class TensorList:
             self._apart = _spans_apart(self._spans)
         if not self._apart:
             raise RuntimeError(f"{name} share memory: each may be in the list once")
+
+    def _as_matrices(self, name: str) -> int:
+        """Address of the list as a table of matrices (ArcqmlMatrix); refuses what is none."""
+        if self._matrices is None:
+            rows = []
+            for i, t in enumerate(self.tensors):
+                if t is None:
+                    rows.append((0, 0, 0, NO_TENSOR, 0))
+                    continue
+                code, parts, _ = _tensor_kinds()[t.dtype]
+                if t.dim() != 2 or parts != 1 or code == 0 or self._layouts[i] is not None:
+                    raise TypeError(f"{name} are float32, bfloat16 or float16 matrices, row-major: place {i} "
+                                    f"holds {_kind_of(None, t)} of shape {list(t.shape)} with strides "
+                                    f"{list(t.stride())}")
+                rows.append((t.data_ptr(), t.shape[0], t.shape[1], code, 0))
+            self._matrices = np.array(rows or [(0, 0, 0, NO_TENSOR, 0)], dtype=_MATRIX)
+            self._matrix_words = load().arcqml_rt_v2_orthogonalize_workspace(
+                self._matrices.ctypes.data, len(rows))
+        return self._matrices.ctypes.data
 
     def _written(self, torch) -> None:
         """Tells autograd that the tensors changed."""
@@ -950,6 +978,259 @@ def _check_places(name: str, x: TensorList, p: TensorList) -> None:
     for i, t in enumerate(x.tensors):
         if t is not None and (x._layouts[i], x._shapes[i]) != (p._layouts[i], p._shapes[i]):
             raise ValueError(f"{name} and parameters differ in shape or strides at place {i}")
+
+
+# ------------------------------------------------------------------ matrices, orthogonalised updates
+
+
+class MuonOptions(C.Structure):
+    _fields_ = [("learning_rate", C.c_double), ("momentum", C.c_double), ("weight_decay", C.c_double),
+                ("epsilon", C.c_double), ("nesterov", C.c_int32), ("steps", C.c_int32)]
+
+
+def orthogonalize_device(matrices, steps: int = 5, eps: float = 1e-7, out=None, stream=None):
+    """`matrices` (a TensorList or a sequence of row-major float32, bfloat16 or float16 CUDA matrices, or
+    None) with their singular values pushed towards 1 (arcqml_rt_v2_orthogonalize): X = u / (|u| + eps),
+    then `steps` times X <- a X + (b A + c A^2) X with A = X X^T. The results are new matrices of the same
+    types, or `out` (`matrices` themselves, or others that share no memory with them). Products carry 22 bits of float32 and float16 matrices and 11
+    of bfloat16 ones, summed in float32. A matrix of zeros stays zero."""
+    import torch
+    x = _tensor_list(matrices)
+    device = torch.cuda.current_device()
+    x._current(torch, device)
+    table = x._as_matrices("the matrices")
+    given = out is not None
+    if given:
+        y = _tensor_list(out)
+        y._current(torch, device)
+        _check_places("outputs", y, x)
+        y._check_apart("the outputs")
+        if y._pointers == x._pointers:
+            x._check_apart("the matrices")
+        else:
+            _check_outside("an output", y._spans, _edges(_merged(x._spans)), "a matrix")
+        if [a is None for a in x.tensors] != [b is None for b in y.tensors]:
+            raise ValueError("outputs and matrices must have the same empty places")
+    on, ws = _scratch(torch, device, x._matrix_words, stream)
+    if not given:
+        y = TensorList(_on_stream(torch, stream, lambda: [
+            None if t is None else torch.empty_like(t) for t in x.tensors]))
+    _status(load().arcqml_rt_v2_orthogonalize(
+        table, y._as_matrices("the outputs"), len(x), int(steps), float(eps),
+        None if ws is None else ws.data_ptr(), x._matrix_words, on))
+    if given:
+        y._written(torch)
+    return list(y.tensors)
+
+
+class DeviceMuonState:
+    """Momentum of ``muon_step_device``: one float32 tensor per parameter, of its shape. It starts at zero,
+    or continues the one given. A saved one goes on in an existing state when it is copied into its tensors
+    or assigned as a whole."""
+
+    def __init__(self, parameters, momentum=None):
+        import torch
+        p = _tensor_list(parameters)
+        if len(p._present) != len(p):
+            raise TypeError("a parameter list has no empty places")
+        p._as_matrices("the parameters")
+        zeros = [torch.zeros_like(t, dtype=torch.float32) for t in p.tensors] if momentum is None else momentum
+        self._momentum = self._fitting(zeros, p)
+        self._checked = self._gradients = None
+
+    @property
+    def momentum(self):
+        return _Moments(self._momentum.tensors)
+
+    @momentum.setter
+    def momentum(self, tensors):
+        self._momentum = self._fitting(tensors, self._momentum)
+
+    @staticmethod
+    def _fitting(tensors, like: TensorList) -> TensorList:
+        x = TensorList(tensors)
+        if x._shapes != like._shapes or len(x._present) != len(x):
+            raise ValueError("the momentum must have the parameters' shapes")
+        x._as_matrices("the momentum")
+        if any(t.dtype != like.tensors[0].new_empty(0).float().dtype for t in x.tensors):
+            raise TypeError("the momentum must be float32")
+        return x
+
+
+def muon_step_device(parameters, gradients, state: DeviceMuonState, lr: float = 0.02, momentum: float = 0.95,
+                     nesterov: bool = True, weight_decay: float = 0.0, steps: int = 5, eps: float = 1e-7,
+                     stream=None) -> None:
+    """One step over `parameters` (row-major float32, bfloat16 or float16 CUDA matrices) in place, whose
+    update is orthogonalised (arcqml_rt_v2_muon_step): m <- momentum m + (1 - momentum) g; u = m, or
+    momentum m + (1 - momentum) g with `nesterov`; p <- (1 - lr weight_decay) p - lr sqrt(max(1, rows /
+    columns)) X(u), X as ``orthogonalize_device`` forms it with the precision of the parameter's type. A
+    parameter whose gradient is None is left as it is. Parameters and momentum may share no memory with
+    anything else here; gradients may share theirs."""
+    import torch
+    p, g, m = _tensor_list(parameters), _tensor_list(gradients), state._momentum
+    if len(p._present) != len(p):
+        raise TypeError("a parameter list has no empty places")
+    device = torch.cuda.current_device()
+    for x in (p, g, m):
+        x._current(torch, device)
+    tables = [x._as_matrices(name) for x, name in ((p, "the parameters"), (g, "the gradients"),
+                                                   (m, "the momentum"))]
+    # held against one another once, and again when a list is written down anew
+    if state._checked != (p._state, m._state):
+        _check_places("momenta", m, p)
+        written = sorted(p._spans + m._spans)
+        if not _spans_apart(written):
+            raise RuntimeError("the parameters and momentum share memory")
+        state._checked, state._gradients, state._written = (p._state, m._state), None, _edges(written)
+    if state._gradients is not g._state:
+        _check_places("gradients", g, p)
+        _check_outside("a gradient", g._spans, state._written, "the parameters or momentum")
+        state._gradients = g._state
+    options = MuonOptions(lr, momentum, weight_decay, eps, bool(nesterov), int(steps))
+    on, ws = _scratch(torch, device, p._matrix_words, stream)
+    _status(load().arcqml_rt_v2_muon_step(*tables, len(p), C.byref(options),
+                                          None if ws is None else ws.data_ptr(), p._matrix_words, on))
+    p._written(torch)
+
+
+def _merged(spans):
+    """(first, end) ranges sorted, those that overlap put together."""
+    out = []
+    for first, end in sorted(spans):
+        if out and first < out[-1][1]:
+            out[-1] = (out[-1][0], max(end, out[-1][1]))
+        else:
+            out.append((first, end))
+    return out
+
+
+def _on_stream(torch, stream, make):
+    if stream is None:
+        return make()
+    with torch.cuda.stream(torch.cuda.ExternalStream(int(stream))):
+        return make()
+
+
+def _scratch(torch, device: int, words: int, stream):
+    """(stream, scratch) of one call, allocated for it alone on its stream."""
+    on = torch._C._cuda_getCurrentRawStream(device) if stream is None else int(stream)
+    if not words:
+        return on, None
+    return on, _on_stream(torch, stream, lambda: torch.empty(words, dtype=torch.float64, device=device))
+
+
+# ------------------------------------------------------------------ tables looked up by index
+
+
+class EmbeddingRows(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("rows", C.c_uint64), ("width", C.c_uint64), ("stride", C.c_uint64),
+                ("dtype", C.c_uint32), ("reserved", C.c_uint32)]
+
+
+class EmbeddingOptions(C.Structure):
+    _fields_ = [("scale", C.c_double), ("padding", C.c_int64), ("normalize", C.c_int32),
+                ("index_bytes", C.c_int32)]
+
+
+def _embedding_rows(torch, t, outer: int, name: str, device: int):
+    """A tensor as rows: its first `outer` dimensions count them, the others are a row."""
+    kind = _tensor_kinds().get(t.dtype) if isinstance(t, torch.Tensor) else None
+    if kind is None or not t.is_cuda or t.layout != torch.strided or t.is_conj() or t.is_neg():
+        raise TypeError(f"{name} must be a dense float64, float32, bfloat16, float16 or complex CUDA tensor: "
+                        f"got {_kind_of(torch, t)}")
+    if t.get_device() != device:
+        raise RuntimeError(f"{name} is on cuda:{t.get_device()} and the current device is cuda:{device}")
+    if t.dim() <= outer:
+        raise TypeError(f"{name} has no dimension for its rows' elements: its shape is {list(t.shape)}")
+    shape, strides = t.shape, t.stride()
+    width, rows = 1, 1
+    fits = True
+    for n, st in zip(reversed(shape[outer:]), reversed(strides[outer:])):
+        fits = fits and (n == 1 or st == width)
+        width *= n
+    step = None  # between one row and the next
+    for n, st in zip(reversed(shape[:outer]), reversed(strides[:outer])):
+        if n != 1:
+            fits = fits and (step is None or st == step * rows)
+            step = st if step is None else step
+        rows *= n
+    if not fits and rows and width:
+        raise TypeError(f"{name} must have rows without gaps at equal distances: got shape {list(shape)} with "
+                        f"strides {list(strides)}")
+    return EmbeddingRows(t.data_ptr(), rows, width * kind[1], (width if step is None else step) * kind[1],
+                         kind[0], 0)
+
+
+def _embedding_call(torch, indices, scale, normalize, padding, device: int):
+    if not (isinstance(indices, torch.Tensor) and indices.is_cuda
+            and indices.dtype in (torch.int64, torch.int32)):
+        raise TypeError("indices must be an int64 or int32 CUDA tensor")
+    if indices.get_device() != device:
+        raise RuntimeError(f"the indices are on cuda:{indices.get_device()} and the current device is "
+                           f"cuda:{device}")
+    if padding is not None and int(padding) < 0:
+        raise ValueError("the padding index must not be negative")
+    return EmbeddingOptions(float(scale), -1 if padding is None else int(padding), bool(normalize),
+                            8 if indices.dtype == torch.int64 else 4)
+
+
+def embedding_lookup_device(table, indices, scale: float = 1.0, normalize: bool = False, padding=None,
+                            stream=None):
+    """Rows of `table` ([rows, ...], rows without gaps) picked by `indices` (int64 or int32 CUDA tensor):
+    ``scale * table[indices]`` of shape [*indices.shape, ...], with `normalize` each row over its 2-norm
+    (states from trained amplitudes; a row of zeros stays zero) (arcqml_rt_v2_embedding_lookup). Places
+    whose index is `padding` are zero. An index outside the table gives NaN: refusing it would wait for the
+    device."""
+    import torch
+    device = torch.cuda.current_device()
+    rows = _embedding_rows(torch, table, 1, "the table", device)
+    options = _embedding_call(torch, indices, scale, normalize, padding, device)
+    make = lambda: (indices.contiguous(), table.new_empty(indices.shape + table.shape[1:]))  # noqa: E731
+    x, out = _on_stream(torch, stream, make)
+    n = x.numel()
+    if out.numel():
+        to = EmbeddingRows(out.data_ptr(), n, rows.width, rows.width, rows.dtype, 0)
+        lib = load()
+        words = lib.arcqml_rt_v2_embedding_lookup_workspace(C.byref(rows), n, C.byref(options)) if normalize else 0
+        on, ws = _scratch(torch, device, words, stream)
+        _status(lib.arcqml_rt_v2_embedding_lookup(
+            C.byref(rows), x.data_ptr(), n, C.byref(options), C.byref(to),
+            None if ws is None else ws.data_ptr(), words, on))
+    return out
+
+
+def embedding_gradient_device(gradient, indices, rows: int, scale: float = 1.0, table=None, padding=None,
+                              stream=None):
+    """The gradient of a table of `rows` rows from `gradient` ([*indices.shape, ...]), the gradient of its
+    lookup by `indices` (arcqml_rt_v2_embedding_gradient): for each row `scale` times the sum over its places,
+    zeros where there is none. With `table` the lookup was a normalised one of that table, and the sum is
+    taken through the rows' norms. A row's places are added in their order: equal inputs give equal bits."""
+    import torch
+    device = torch.cuda.current_device()
+    options = _embedding_call(torch, indices, scale, table is not None, padding, device)
+    if not isinstance(gradient, torch.Tensor) or gradient.shape[:indices.dim()] != indices.shape:
+        raise ValueError("the gradient must have a row for each index")
+    g = _embedding_rows(torch, gradient, indices.dim(), "the gradient", device)
+    rows = int(rows)
+    if rows < 0:
+        raise ValueError("a table has no negative number of rows")
+    inner = gradient.shape[indices.dim():]
+    t = None
+    if table is not None:
+        t = _embedding_rows(torch, table, 1, "the table", device)
+        if table.dtype != gradient.dtype or table.shape != (rows,) + tuple(inner):
+            raise ValueError(f"the table must be {gradient.dtype} of shape {[rows, *inner]}")
+    make = lambda: (indices.contiguous(), gradient.new_empty((rows,) + tuple(inner)))  # noqa: E731
+    x, out = _on_stream(torch, stream, make)
+    if out.numel():
+        to = EmbeddingRows(out.data_ptr(), rows, g.width, g.width, g.dtype, 0)
+        lib = load()
+        words = lib.arcqml_rt_v2_embedding_gradient_workspace(C.byref(g), rows, C.byref(options))
+        on, ws = _scratch(torch, device, words, stream)
+        _status(lib.arcqml_rt_v2_embedding_gradient(
+            C.byref(g), x.data_ptr(), C.byref(options), None if t is None else C.byref(t), C.byref(to),
+            None if ws is None else ws.data_ptr(), words, on))
+    return out
 
 
 def norms_device(state, num_qubits: int, stream=None) -> np.ndarray:

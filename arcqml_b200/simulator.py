@@ -373,6 +373,25 @@ class BatchStateVectorSimulator:
         sim.initial_requires_grad = requires_grad
         return sim
 
+    @classmethod
+    def from_table(cls, num_qubits: int, table, indices):
+        """Rows of a complex128 CUDA table of amplitudes ([rows, 2^n]) picked by `indices` (one-dimensional
+        int64 or int32 CUDA tensor) and normalised. ``states`` of the simulator is the batch as autograd knows
+        it: ``sim.states.backward(initial_state_grad)`` gives the table its gradient after
+        ``RunResult.backward``. A row of zeros is no state and an index outside the table gives NaN; neither
+        is looked for."""
+        from .embedding import lookup
+        torch = _torch()
+        if not isinstance(table, torch.Tensor) or table.dtype != torch.complex128 or table.dim() != 2 \
+                or table.shape[1] != (1 << num_qubits):
+            raise SimError(f"a table of states must be complex128 of shape [rows, {1 << num_qubits}]")
+        if not isinstance(indices, torch.Tensor) or indices.dim() != 1 or indices.shape[0] == 0:
+            raise SimError("a batch of states is picked by a one-dimensional tensor of at least one index")
+        states = lookup(table, indices, normalize=True)
+        sim = cls.from_device_state(num_qubits, states.detach(), requires_grad=states.requires_grad)
+        sim.states = states
+        return sim
+
     def amplitudes(self) -> np.ndarray:
         return self.state.cpu().numpy()
 

@@ -274,6 +274,92 @@ int32_t arcqml_rt_v2_adam_step(const ArcqmlTensor *parameters, const ArcqmlTenso
                                double *norm, double *workspace, size_t workspace_len,
                                void *stream);
 
+/* Rows of a table, looked up by index: token embeddings, or states made of trained amplitudes. A
+ * complex table's row is its components. indices: device, `count` integers of index_bytes (4 or 8) each.
+ * With `normalize` a row is divided by its 2-norm, which makes states of amplitudes; a row of zeros stays
+ * zero. An index equal to `padding` (when it is not negative) gives a row of zeros. An index outside
+ * [0, rows) gives a row of NaN, since refusing it would take a wait for the device. */
+typedef struct ArcqmlRows {
+    void *data;       /* device pointer, aligned to the element's size */
+    uint64_t rows;
+    uint64_t width;   /* elements of a row, next to each other */
+    uint64_t stride;  /* elements from one row's start to the next one's */
+    uint32_t dtype;
+    uint32_t reserved; /* 0 */
+} ArcqmlRows;
+typedef struct ArcqmlEmbeddingOptions {
+    double scale;       /* every row is multiplied by it */
+    int64_t padding;    /* negative: none */
+    int32_t normalize;  /* 0 or 1 */
+    int32_t index_bytes;
+} ArcqmlEmbeddingOptions;
+
+/* Doubles of device scratch of the two calls below (0: none; it may then be null). The scratch belongs
+ * to one call at a time. */
+size_t arcqml_rt_v2_embedding_lookup_workspace(const ArcqmlRows *table, size_t count,
+                                               const ArcqmlEmbeddingOptions *options);
+size_t arcqml_rt_v2_embedding_gradient_workspace(const ArcqmlRows *gradient, uint64_t rows,
+                                                 const ArcqmlEmbeddingOptions *options);
+
+/* output[i] <- scale table[indices[i]], over the row's norm with `normalize` (the norm in f64). output: of
+ * the table's dtype and width, `count` rows; its memory may not overlap the table's. Products are f64 for
+ * f64 tables and for normalised rows, f32 otherwise, rounded once to the type. */
+int32_t arcqml_rt_v2_embedding_lookup(const ArcqmlRows *table, const void *indices, size_t count,
+                                      const ArcqmlEmbeddingOptions *options, const ArcqmlRows *output,
+                                      double *workspace, size_t workspace_len, void *stream);
+
+/* The gradient of that lookup: output[v] <- scale times the sum of gradient[i] over the i with
+ * indices[i] = v, and with `normalize` that sum s through the norm of t = table[v]:
+ * (s - u <u, s>) / |t|, u = t / |t| (0 for a row of zeros). Every row of the output is written, with zeros
+ * where no index points; indices equal to `padding` or outside [0, rows) count nowhere. The places of a row
+ * are added in their order, in groups that the count of indices fixes, in f64 for f64 and in f32 otherwise
+ * and rounded once: equal inputs give equal bits. table: null unless `normalize` is set, then of the
+ * output's rows, width and dtype. output: of the gradient's dtype. No two of them may overlap in memory but
+ * that gradient rows may coincide (stride 0). */
+int32_t arcqml_rt_v2_embedding_gradient(const ArcqmlRows *gradient, const void *indices,
+                                        const ArcqmlEmbeddingOptions *options, const ArcqmlRows *table,
+                                        const ArcqmlRows *output, double *workspace,
+                                        size_t workspace_len, void *stream);
+
+/* A matrix of a network, row-major without gaps. */
+typedef struct ArcqmlMatrix {
+    void *data;        /* device pointer, aligned to the element's size; ignored when it has no elements */
+    uint64_t rows, columns;
+    uint32_t dtype;    /* f32, bf16 or f16; ARCQML_NO_TENSOR: no matrix at this place of the list */
+    uint32_t reserved; /* 0 */
+} ArcqmlMatrix;
+
+/* Doubles of device scratch of the two calls below for such a list. The scratch belongs to one call at a
+ * time. */
+size_t arcqml_rt_v2_orthogonalize_workspace(const ArcqmlMatrix *matrices, size_t num_matrices);
+
+/* outputs[i] <- matrices[i] with its singular values pushed towards 1 by `steps` (1 to 20) steps of the
+ * polynomial X <- a X + (b A + c A^2) X, A = X X^T (X^T X for more rows than columns),
+ * (a, b, c) = (3.4445, -4.7750, 2.0315), from X = matrix / (its Frobenius norm + epsilon). Products of
+ * f32 and f16 matrices are formed from operands of 22 bits, those of bf16 matrices from operands of 11,
+ * sums in f32. outputs have the matrices' shapes and types; they are the matrices
+ * themselves, place by place, or overlap none of them, nor one another. A NaN or infinity in a matrix makes that output NaN. */
+int32_t arcqml_rt_v2_orthogonalize(const ArcqmlMatrix *matrices, const ArcqmlMatrix *outputs,
+                                   size_t num_matrices, int32_t steps, double epsilon,
+                                   double *workspace, size_t workspace_len, void *stream);
+
+typedef struct ArcqmlMuonOptions {
+    double learning_rate, momentum, weight_decay, epsilon;
+    int32_t nesterov; /* 0 or 1 */
+    int32_t steps;
+} ArcqmlMuonOptions;
+
+/* One step over a list of matrices whose update is orthogonalised:
+ *   m <- momentum m + (1 - momentum) g;   u = m, or momentum m + (1 - momentum) g with nesterov
+ *   p <- (1 - learning_rate weight_decay) p - learning_rate sqrt(max(1, rows / columns)) X(u)
+ * with X as arcqml_rt_v2_orthogonalize forms it, the precision of its products by the parameter's type.
+ * momenta: f32. Parameters and gradients: f32, bf16 or f16, in any mix. A place whose gradient is
+ * ARCQML_NO_TENSOR is left as it is. What the call writes must not overlap anything else that it takes. */
+int32_t arcqml_rt_v2_muon_step(const ArcqmlMatrix *parameters, const ArcqmlMatrix *gradients,
+                               const ArcqmlMatrix *momenta, size_t num_matrices,
+                               const ArcqmlMuonOptions *options, double *workspace,
+                               size_t workspace_len, void *stream);
+
 /* State analysis (crates/arcqml-analysis/src/statevector), on every row of a device state.
  * probabilities: probabilities[row][i] = |psi_row[i]|^2 (device, [batch, 2^n];
  *   probabilities.rs:22-25).
