@@ -4,118 +4,595 @@
 //
 // with X (m x n, m <= n) the matrix or its transpose: every singular value s goes through
 // a s + b s^3 + c s^5, which pushes it towards 1 (and never above 1.203, from 1 or less).
+//
+// The products run on the tensor cores (tcgen05, f16 operands, f32 sums in tensor memory). X, A and P are
+// bounded in that iteration (entries of at most 1.203, 1.447 and 2.807), so f16 at a fixed scale holds
+// 11 bits of every entry down to 2^-29 of the largest: more than bf16 at the same rate. Types of 11 bits
+// and more take operands of 22 bits, as the sum of two f16 numbers, and three products (the fourth is below
+// the sums' own rounding). An update far below epsilon makes a small X, which grows by at most 3.4445 a step:
+// it is stored 2^k times as large, k from its norm, and k falls by 2 a step until it is 0.
+//
+// Layout in the scratch: X, A and P in blocks of 128 rows x 64 columns, 16 KB each, row by row with their
+// 16-byte pieces permuted as the tensor cores want them in shared memory. So every copy is one run of 8 or
+// 16 KB that needs no tensor map, matrices of any size and address share a launch, and one block of X
+// serves both as a piece of X's rows (A = X X^T) and of its columns (P X).
+//
+// A and P are symmetric: only tiles on and above the diagonal are computed, and their mirror images stored.
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <sstream>
 #include <string>
 #include <tuple>
+#include <vector>
 
 #include "elements.cuh"
 #include "launch.h"
 #include "muon.h"
 #include "profile.h"
+#include "tensor_core.cuh"
 
 namespace arcqml {
 namespace {
 
 constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
+// Scales of the stored values: the largest powers of two that keep them in f16.
+constexpr float kScaleX = 32768.0f; // of X and A; P has half of it
 constexpr int kThreads = 256;
-constexpr uint32_t kSumBlocks = 256; // partial sums of a matrix
+constexpr uint32_t kMatrices = 64;      // of a launch
+constexpr uint32_t kSumBlocks = 148 * 8; // partial sums of a matrix, at most
+constexpr uint32_t kRows = 128, kDepth = 64;         // of a block
+constexpr uint32_t kBlock = kRows * kDepth * 2;      // bytes
+constexpr uint32_t kSMs = 148;
 
-// One matrix of a call. The update u is the matrix `in`, or follows from the momentum and the gradient.
-struct Job {
+// One matrix of a launch. The update u is the matrix `in`, or follows from the momentum and the gradient.
+struct Matrix {
     void *out;       // the orthogonalised matrix, or the parameter
     const void *in;  // the matrix, or the gradient
     float *momentum; // null without a step
-    uint64_t rows, columns;
-    uint32_t out_type, in_type;
+    uint64_t x[2], a, p; // offsets in the scratch; low parts lie behind their high parts
+    uint32_t m, n;       // of X
+    uint32_t down_blocks, x_blocks, a_blocks; // blocks of X down, and across X and A
+    uint8_t flip, out_type, in_type, nesterov;
     float beta, keep; // of the step: momentum, and 1 - momentum
     float down, rate; // the parameter's factor, and the update's
-    uint32_t nesterov;
 };
 
-__device__ __forceinline__ float load_as(const void *p, uint32_t type, uint64_t i) {
+struct Group {
+    Matrix matrix[kMatrices];
+    uint32_t first[kMatrices + 1]; // of the launch's blocks or tiles
+    uint32_t count;
+    char *scratch;
+    uint32_t *fault; // set by a wait that ran out
+    int *shift;      // of each matrix: X is stored 2^shift times as large at first
+    double *sums;
+    double eps;
+};
+
+__device__ __forceinline__ uint32_t matrix_of(const Group &g, uint32_t c) {
+    uint32_t lo = 0, hi = g.count;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (g.first[mid] <= c) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// ------------------------------------------------------------------ elements of any type
+
+template <class T> __device__ __forceinline__ void load8_as(float (&v)[8], const T *p, uint32_t count) {
+    constexpr int N = 16 / sizeof(T);
+    if (count >= 8 && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
+#pragma unroll
+        for (int i = 0; i < 8; i += N) {
+            const auto w = load_vector<T, N>(p + i);
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[i + e] = to_wide(w.x[e]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = uint32_t(i) < count ? to_wide(p[i]) : 0.0f;
+    }
+}
+// Up to 8 elements from place i on; zeros behind them.
+__device__ __forceinline__ void load8(float (&v)[8], const void *p, uint32_t type, uint64_t i, uint32_t count) {
+    if (type == ARCQML_F32) load8_as(v, static_cast<const float *>(p) + i, count);
+    else if (type == ARCQML_BF16) load8_as(v, static_cast<const __nv_bfloat16 *>(p) + i, count);
+    else load8_as(v, static_cast<const __half *>(p) + i, count);
+}
+template <class T> __device__ __forceinline__ void store8_as(const float (&v)[8], T *p, uint32_t count) {
+    constexpr int N = 16 / sizeof(T);
+    if (count >= 8 && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
+#pragma unroll
+        for (int i = 0; i < 8; i += N) {
+            VectorOf<T, N> w;
+#pragma unroll
+            for (int e = 0; e < N; ++e) w.x[e] = to_element<T>(v[i + e]);
+            store_vector<T, N>(p + i, w);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (uint32_t(i) < count) p[i] = to_element<T>(v[i]);
+    }
+}
+__device__ __forceinline__ void store8(const float (&v)[8], void *p, uint32_t type, uint64_t i, uint32_t count) {
+    if (type == ARCQML_F32) store8_as(v, static_cast<float *>(p) + i, count);
+    else if (type == ARCQML_BF16) store8_as(v, static_cast<__nv_bfloat16 *>(p) + i, count);
+    else store8_as(v, static_cast<__half *>(p) + i, count);
+}
+__device__ __forceinline__ float load1(const void *p, uint32_t type, uint64_t i) {
     if (type == ARCQML_F32) return static_cast<const float *>(p)[i];
     if (type == ARCQML_BF16) return to_wide(static_cast<const __nv_bfloat16 *>(p)[i]);
     return to_wide(static_cast<const __half *>(p)[i]);
 }
-__device__ __forceinline__ void store_as(void *p, uint32_t type, uint64_t i, float x) {
+__device__ __forceinline__ void store1(void *p, uint32_t type, uint64_t i, float x) {
     if (type == ARCQML_F32) static_cast<float *>(p)[i] = x;
     else if (type == ARCQML_BF16) static_cast<__nv_bfloat16 *>(p)[i] = to_element<__nv_bfloat16>(x);
     else static_cast<__half *>(p)[i] = to_element<__half>(x);
 }
 
-__device__ __forceinline__ float update_of(const Job &j, uint64_t i) {
-    const float g = load_as(j.in, j.in_type, i);
-    if (!j.momentum) return g;
-    const float m = j.momentum[i];
-    return j.nesterov ? j.beta * m + j.keep * g : m;
-}
-
-// The momentum's update, and the squares of u: one f64 sum for each block.
-__global__ void __launch_bounds__(kThreads) k_update_squares(const __grid_constant__ Job j, double *sums) {
-    __shared__ double part[kThreads / 32];
-    const uint64_t n = j.rows * j.columns;
-    double sum = 0.0;
-    for (uint64_t i = uint64_t(blockIdx.x) * kThreads + threadIdx.x; i < n; i += uint64_t(gridDim.x) * kThreads) {
-        if (j.momentum) j.momentum[i] = j.beta * j.momentum[i] + j.keep * load_as(j.in, j.in_type, i);
-        const double u = update_of(j, i);
-        sum = fma(u, u, sum);
-    }
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        sum = 0.0;
-        for (int w = 0; w < kThreads / 32; ++w) sum += part[w];
-        sums[blockIdx.x] = sum;
-    }
-}
-
-// X = u / (|u| + eps), transposed where the matrix has more rows than columns.
-__global__ void __launch_bounds__(kThreads) k_scale_update(const __grid_constant__ Job j, const double *sums,
-                                                           uint32_t blocks, double eps, float *x) {
-    double sum = 0.0;
-    for (uint32_t b = 0; b < blocks; ++b) sum += sums[b];
-    const double factor = 1.0 / (sqrt(sum) + eps);
-    const bool flip = j.rows > j.columns;
-    const uint64_t n = j.rows * j.columns;
-    for (uint64_t i = uint64_t(blockIdx.x) * kThreads + threadIdx.x; i < n; i += uint64_t(gridDim.x) * kThreads) {
-        const uint64_t r = i / j.columns, c = i % j.columns;
-        x[flip ? c * j.rows + r : i] = float(double(update_of(j, i)) * factor);
-    }
-}
-
-// out (m x n) = f add + h left right, right transposed with `turned`; 16 x 16 tiles.
-__global__ void __launch_bounds__(256) k_product(const float *left, const float *right, const float *add, float *out,
-                                                 uint64_t m, uint64_t n, uint64_t k, bool turned, float f, float h) {
-    __shared__ float l[16][17], r[16][17];
-    const uint32_t tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const uint64_t row = uint64_t(blockIdx.y) * 16 + ty, col = uint64_t(blockIdx.x) * 16 + tx;
-    float sum = 0.0f;
-    for (uint64_t k0 = 0; k0 < k; k0 += 16) {
-        l[ty][tx] = row < m && k0 + tx < k ? left[row * k + k0 + tx] : 0.0f;
-        const uint64_t c = uint64_t(blockIdx.x) * 16 + (turned ? ty : tx), kk = k0 + (turned ? tx : ty);
-        const float v = c < n && kk < k ? right[turned ? c * k + kk : kk * n + c] : 0.0f;
-        if (turned) r[tx][ty] = v;
-        else r[ty][tx] = v;
-        __syncthreads();
+// u of 8 elements, from the momentum as it is in memory.
+__device__ __forceinline__ void update8(float (&u)[8], const Matrix &a, uint64_t i, uint32_t count) {
+    if (!a.momentum) return load8(u, a.in, a.in_type, i, count);
+    float m[8];
+    load8_as(m, a.momentum + i, count);
+    if (!a.nesterov) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sum = fmaf(l[ty][i], r[i][tx], sum);
-        __syncthreads();
+        for (int e = 0; e < 8; ++e) u[e] = m[e];
+        return;
     }
-    if (row < m && col < n) out[row * n + col] = h * sum + (add ? f * add[row * n + col] : 0.0f);
+    load8(u, a.in, a.in_type, i, count);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) u[e] = a.beta * m[e] + a.keep * u[e];
 }
 
-// The result as it is, or the step with it.
-__global__ void __launch_bounds__(kThreads) k_finish(const __grid_constant__ Job j, const float *x) {
-    const bool flip = j.rows > j.columns;
-    const uint64_t n = j.rows * j.columns;
-    for (uint64_t i = uint64_t(blockIdx.x) * kThreads + threadIdx.x; i < n; i += uint64_t(gridDim.x) * kThreads) {
-        const float v = x[flip ? i % j.columns * j.rows + i / j.columns : i];
-        store_as(j.out, j.out_type, i, j.momentum ? j.down * load_as(j.out, j.out_type, i) - j.rate * v : v);
+// ------------------------------------------------------------------ the update and its norm
+
+// The sum over a block of kThreads, the same in every thread.
+__device__ __forceinline__ double block_sum(double v) {
+    __shared__ double part[kThreads / 32];
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0.0;
+    for (int w = 0; w < kThreads / 32; ++w) v += part[w];
+    return v;
+}
+
+// The momentum's update, and the squares of u: an f64 sum for each block.
+__global__ void __launch_bounds__(kThreads) k_update_squares(const __grid_constant__ Group g) {
+    cudaTriggerProgrammaticLaunchCompletion();
+    if (blockIdx.x == 0 && threadIdx.x == 0) *g.fault = 0;
+    const uint32_t k = matrix_of(g, blockIdx.x), blocks = g.first[k + 1] - g.first[k];
+    const Matrix &a = g.matrix[k];
+    const uint64_t n = uint64_t(a.m) * a.n;
+    double sum = 0.0;
+    for (uint64_t i = (uint64_t(blockIdx.x - g.first[k]) * kThreads + threadIdx.x) * 8; i < n;
+         i += uint64_t(blocks) * kThreads * 8) {
+        const uint32_t count = uint32_t(min(uint64_t(8), n - i));
+        float u[8], m[8];
+        load8(u, a.in, a.in_type, i, count);
+        if (a.momentum) {
+            load8_as(m, a.momentum + i, count);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) m[e] = a.beta * m[e] + a.keep * u[e];
+            store8_as(m, a.momentum + i, count);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) u[e] = a.nesterov ? a.beta * m[e] + a.keep * u[e] : m[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = fma(double(u[e]), double(u[e]), sum);
+    }
+    sum = block_sum(sum);
+    if (threadIdx.x == 0) g.sums[blockIdx.x] = sum;
+}
+
+// Where 8 neighbouring values of a row start in an array of blocks.
+__device__ __forceinline__ uint64_t place_of(uint32_t row, uint32_t column, uint32_t blocks) {
+    return (uint64_t(row / kRows) * blocks + column / kDepth) * kBlock + (row % kRows) * 128 +
+           ((column % kDepth / 8) ^ (row % 8)) * 16;
+}
+__host__ __device__ inline uint64_t bytes_of(uint32_t down, uint32_t across) { return uint64_t(down) * across * kBlock; }
+
+// 8 values as f16, and with SPLIT what that leaves behind them.
+template <bool SPLIT> __device__ __forceinline__ void store_operand(char *at, uint64_t low, const float (&v)[8]) {
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __half2 x = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+        h[i] = *reinterpret_cast<const uint32_t *>(&x);
+        if constexpr (SPLIT) {
+            const float2 y = __half22float2(x);
+            const __half2 z = __floats2half2_rn(v[2 * i] - y.x, v[2 * i + 1] - y.y);
+            l[i] = *reinterpret_cast<const uint32_t *>(&z);
+        }
+    }
+    *reinterpret_cast<uint4 *>(at) = make_uint4(h[0], h[1], h[2], h[3]);
+    if constexpr (SPLIT) *reinterpret_cast<uint4 *>(at + low) = make_uint4(l[0], l[1], l[2], l[3]);
+}
+template <bool SPLIT> __device__ __forceinline__ void load_operand(float (&v)[8], const char *at, uint64_t low) {
+    const uint4 h = *reinterpret_cast<const uint4 *>(at);
+    const uint32_t w[4] = {h.x, h.y, h.z, h.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+        v[2 * i] = y.x;
+        v[2 * i + 1] = y.y;
+    }
+    if constexpr (SPLIT) {
+        const uint4 l = *reinterpret_cast<const uint4 *>(at + low);
+        const uint32_t z[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&z[i]));
+            v[2 * i] += y.x;
+            v[2 * i + 1] += y.y;
+        }
+    }
+}
+
+// X = u / (|u| + eps) in blocks, one for each thread block; zeros behind the matrix's edges.
+template <bool SPLIT> __global__ void __launch_bounds__(kThreads) k_spread(const __grid_constant__ Group g,
+                                                                           const __grid_constant__ Group sums) {
+    __shared__ float turned[kDepth][kRows + 1];
+    cudaTriggerProgrammaticLaunchCompletion();
+    const uint32_t k = matrix_of(g, blockIdx.x), block = blockIdx.x - g.first[k];
+    const Matrix &a = g.matrix[k];
+    cudaGridDependencySynchronize();
+    double sum = 0.0;
+    for (uint32_t b = sums.first[k] + threadIdx.x; b < sums.first[k + 1]; b += kThreads) sum += g.sums[b];
+    const double norm = sqrt(block_sum(sum)), whole = norm + g.eps;
+    // |X| 2^shift lies in [1/2, 1]; a norm of zero, infinity or NaN has no shift
+    const int shift = norm > 0.0 && norm < whole && whole < INFINITY ? max(0, ilogb(whole) - ilogb(norm) - 1) : 0;
+    if (block == 0 && threadIdx.x == 0) g.shift[k] = shift;
+    const double factor = ldexp(double(kScaleX) / whole, shift);
+    const uint32_t row0 = block / a.x_blocks * kRows, column0 = block % a.x_blocks * kDepth;
+    const uint64_t low = bytes_of(a.down_blocks, a.x_blocks);
+    char *to = g.scratch + a.x[0];
+    if (a.flip) { // X's rows are the matrix's columns
+        for (uint32_t t = threadIdx.x; t < kDepth * (kRows / 8); t += kThreads) {
+            const uint32_t c = t / (kRows / 8), r = t % (kRows / 8) * 8;
+            float u[8];
+            if (column0 + c < a.n && row0 + r < a.m)
+                update8(u, a, uint64_t(column0 + c) * a.m + row0 + r, min(8u, a.m - row0 - r));
+            else
+#pragma unroll
+                for (int e = 0; e < 8; ++e) u[e] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) turned[c][r + e] = u[e];
+        }
+        __syncthreads();
+    }
+    for (uint32_t t = threadIdx.x; t < kRows * (kDepth / 8); t += kThreads) {
+        const uint32_t r = t / (kDepth / 8), c = t % (kDepth / 8) * 8;
+        float u[8];
+        if (a.flip) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) u[e] = turned[c + e][r];
+        } else if (row0 + r < a.m && column0 + c < a.n) {
+            update8(u, a, uint64_t(row0 + r) * a.n + column0 + c, min(8u, a.n - column0 - c));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) u[e] = 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) // 0 behind the edges also where the factor is not finite
+            u[e] = row0 + r < a.m && column0 + c + e < a.n ? float(double(u[e]) * factor) : 0.0f;
+        store_operand<SPLIT>(to + place_of(row0 + r, column0 + c, a.x_blocks), low, u);
+    }
+}
+
+// ------------------------------------------------------------------ products
+
+enum Phase { GRAM, POLYNOMIAL, APPLY };
+constexpr uint32_t kStageBytes = 32768; // one depth of 64: 128 rows of the left operand, 128 of the right
+constexpr uint32_t kProductThreads = 256;
+
+// Stages of a block: 192 KB of operands.
+template <bool SPLIT> constexpr uint32_t kStages = SPLIT ? 3 : 6;
+template <bool SPLIT> constexpr uint32_t kProductShared = 1024 + kStages<SPLIT> * (SPLIT ? 2 : 1) * kStageBytes + 256;
+
+struct ProductState {
+    uint64_t full[6], empty[6], peer[6], done[2], taken[2];
+    uint32_t tmem, stop;
+};
+static_assert(sizeof(ProductState) <= 256, "the end of the shared memory");
+
+// Waits for a barrier's phase; false once a wait of this block has run out.
+__device__ __forceinline__ bool wait_for(uint64_t *b, uint32_t parity, uint32_t *stop) {
+    if (tc::barrier_try(b, parity)) return true;
+    const long long begin = clock64();
+    for (uint32_t i = 0; i < (1u << 26); ++i) {
+        if (tc::barrier_try(b, parity)) return true;
+        if (*reinterpret_cast<volatile uint32_t *>(stop)) return false;
+        if (clock64() - begin > 4000000000ll) break;
+    }
+    *reinterpret_cast<volatile uint32_t *>(stop) = 1;
+    return false;
+}
+
+// The tile t of a phase.
+struct Tile {
+    const Matrix *a;
+    uint32_t index, i, j, depth; // rows and columns in tiles; steps of 64 of the depth
+};
+template <int PHASE, uint32_t SIZE> __device__ __forceinline__ Tile tile_of(const Group &g, uint32_t t) {
+    Tile r;
+    r.index = matrix_of(g, t);
+    r.a = &g.matrix[r.index];
+    t -= g.first[r.index];
+    if constexpr (PHASE == APPLY) {
+        const uint32_t across = (r.a->n + SIZE - 1) / SIZE;
+        r.i = t / across;
+        r.j = t % across;
+    } else { // on and above the diagonal, row by row
+        uint32_t side = (r.a->m + SIZE - 1) / SIZE;
+        r.i = 0;
+        while (t >= side) {
+            t -= side;
+            --side;
+            ++r.i;
+        }
+        r.j = r.i + t;
+    }
+    r.depth = ((PHASE == GRAM ? r.a->n : r.a->m) + kDepth - 1) / kDepth;
+    return r;
+}
+
+// One phase for all matrices of a group: D = L R^T in tiles of 128 CG x 128 CG, a pair of blocks a tile with
+// CG = 2 (each has half of the tile's rows, and brings half of the right operand's).
+template <int PHASE, bool SPLIT, int CG>
+__global__ void __launch_bounds__(kProductThreads, 1)
+    k_product(const __grid_constant__ Group g, uint32_t step, uint32_t last) {
+    constexpr uint32_t SIZE = kRows * CG, S = kStages<SPLIT>, STAGE = kStageBytes * (SPLIT ? 2 : 1);
+    extern __shared__ char raw[];
+    char *shared = raw + (1024 - (tc::shared_address(raw) & 1023)) % 1024;
+    ProductState &st = *reinterpret_cast<ProductState *>(shared + S * STAGE);
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, current = step & 1;
+    const uint32_t rank = CG == 2 ? tc::block_rank() : 0;
+    if (warp == 0 && lane == 0) {
+        for (uint32_t s = 0; s < S; ++s) {
+            tc::barrier_init(&st.full[s], 1);
+            tc::barrier_init(&st.empty[s], 1);
+            tc::barrier_init(&st.peer[s], 1);
+        }
+        for (uint32_t s = 0; s < 2; ++s) {
+            tc::barrier_init(&st.done[s], 1);
+            tc::barrier_init(&st.taken[s], 4 * CG);
+        }
+        st.stop = 0;
+        tc::barrier_init_fence();
+    }
+    if (warp == 1) tc::tmem_alloc<CG>(&st.tmem, 2 * SIZE);
+    tc::fence_before();
+    __syncthreads();
+    if constexpr (CG == 2) tc::cluster_sync();
+    tc::fence_after();
+    cudaTriggerProgrammaticLaunchCompletion();
+    cudaGridDependencySynchronize();
+    const uint32_t tmem = st.tmem;
+    const uint32_t units = gridDim.x / CG, unit = blockIdx.x / CG, tiles = g.first[g.count];
+    const bool broken = *reinterpret_cast<volatile uint32_t *>(g.fault) != 0;
+
+    if (warp == 0 && lane == 0 && !broken) { // copies operands in
+        uint32_t at = 0, phase = 0;
+        bool on = true;
+        for (uint32_t t = unit; t < tiles && on; t += units) {
+            const Tile tile = tile_of<PHASE, SIZE>(g, t);
+            const Matrix &a = *tile.a;
+            const uint32_t left = tile.i * CG + rank, right = tile.j * CG + rank;
+            const uint32_t left_across = PHASE == GRAM ? a.x_blocks : a.a_blocks;
+            const char *from = g.scratch + (PHASE == GRAM ? a.x[current] : PHASE == POLYNOMIAL ? a.a : a.p);
+            const char *from_right = PHASE == APPLY ? g.scratch + a.x[current] : from;
+            const uint64_t low = bytes_of(a.down_blocks, left_across);
+            const uint64_t low_right = PHASE == APPLY ? bytes_of(a.down_blocks, a.x_blocks) : low;
+            const uint32_t parts = SPLIT ? 2 : 1;
+            // blocks behind the edges are not read: the sums that they would enter are not stored
+            const bool has_left = left < a.down_blocks;
+            const uint32_t wide = PHASE == APPLY ? min(2u, a.x_blocks - min(a.x_blocks, right * 2)) : 0;
+            const bool has_right = right < a.down_blocks;
+            const uint32_t bytes = parts * ((has_left ? kBlock : 0) + (PHASE == APPLY ? wide * (kBlock / 2) : has_right ? kBlock : 0));
+            for (uint32_t d = 0; d < tile.depth; ++d) {
+                if (!(on = wait_for(&st.empty[at], phase ^ 1, &st.stop))) break;
+                char *to = shared + at * STAGE;
+                tc::barrier_expect(&st.full[at], bytes);
+                for (uint32_t part = 0; part < parts; ++part, to += kStageBytes) {
+                    if (has_left)
+                        tc::copy_in(to, from + part * low + (uint64_t(left) * left_across + d) * kBlock, kBlock, &st.full[at]);
+                    if constexpr (PHASE == APPLY) {
+                        for (uint32_t w = 0; w < wide; ++w)
+                            tc::copy_in(to + kBlock + w * (kBlock / 2),
+                                        from_right + part * low_right +
+                                            (uint64_t(d / 2) * a.x_blocks + right * 2 + w) * kBlock + (d & 1) * (kBlock / 2),
+                                        kBlock / 2, &st.full[at]);
+                    } else if (has_right) {
+                        tc::copy_in(to + kBlock, from_right + part * low_right + (uint64_t(right) * left_across + d) * kBlock,
+                                    kBlock, &st.full[at]);
+                    }
+                }
+                if (++at == S) at = 0, phase ^= 1;
+            }
+        }
+        // nothing may still be on its way in when the block ends: every stage that was filled has been read,
+        // or (after a wait that ran out) its copies are waited for
+        if (!on) {
+            uint32_t none = 0;
+            for (uint32_t s = 0; s < S; ++s) wait_for(&st.full[s], s < at ? phase : phase ^ 1, &none);
+        }
+    } else if (warp == 1 && rank == 0 && lane == 0 && !broken) { // issues the products
+        constexpr uint32_t instr = tc::instruction(SIZE, SIZE, PHASE == APPLY);
+        constexpr uint32_t STEP = PHASE == APPLY ? 2048 / 16 : 32 / 16; // of the right operand, 16 of depth
+        uint32_t at = 0, phase = 0, n = 0;
+        bool on = true;
+        for (uint32_t t = unit; t < tiles && on; t += units, ++n) {
+            const uint32_t depth = tile_of<PHASE, SIZE>(g, t).depth, half = n & 1;
+            if (!wait_for(&st.taken[half], (n >> 1 & 1) ^ 1, &st.stop)) break;
+            tc::fence_after();
+            const uint32_t sums = tmem + half * SIZE;
+            for (uint32_t d = 0; d < depth; ++d) {
+                if (!(on = wait_for(&st.full[at], phase, &st.stop))) break;
+                if constexpr (CG == 2)
+                    if (!(on = wait_for(&st.peer[at], phase, &st.stop))) break;
+                tc::fence_after();
+                const uint32_t base = tc::shared_address(shared + at * STAGE);
+                const uint64_t left = tc::descriptor(base, 16);
+                const uint64_t right = tc::descriptor(base + kBlock, PHASE == APPLY ? kBlock / 2 : 16);
+#pragma unroll
+                for (uint32_t s = 0; s < kDepth / 16; ++s) {
+                    tc::mma<CG>(sums, left + s * 2, right + s * STEP, instr, d != 0 || s != 0);
+                    if constexpr (SPLIT) {
+                        constexpr uint32_t LOW = kStageBytes / 16;
+                        tc::mma<CG>(sums, left + s * 2, right + LOW + s * STEP, instr, true);
+                        tc::mma<CG>(sums, left + LOW + s * 2, right + s * STEP, instr, true);
+                    }
+                }
+                tc::commit<CG>(&st.empty[at]);
+                if (++at == S) at = 0, phase ^= 1;
+            }
+            if (on) tc::commit<CG>(&st.done[half]);
+        }
+    } else if (CG == 2 && warp == 2 && rank == 1 && lane == 0 && !broken) { // tells the first block of its operands
+        uint32_t at = 0, phase = 0;
+        bool on = true;
+        for (uint32_t t = unit; t < tiles && on; t += units) {
+            const uint32_t depth = tile_of<PHASE, SIZE>(g, t).depth;
+            for (uint32_t d = 0; d < depth; ++d) {
+                if (!(on = wait_for(&st.full[at], phase, &st.stop))) break;
+                tc::barrier_arrive_at(tc::in_block(&st.peer[at], 0));
+                if (++at == S) at = 0, phase ^= 1;
+            }
+        }
+    } else if (warp >= 4 && !broken) { // takes the sums out: a thread has a row
+        uint32_t n = 0;
+        for (uint32_t t = unit; t < tiles; t += units, ++n) {
+            const Tile tile = tile_of<PHASE, SIZE>(g, t);
+            const Matrix &a = *tile.a;
+            const uint32_t half = n & 1;
+            if (!__all_sync(0xffffffffu, wait_for(&st.done[half], n >> 1 & 1, &st.stop))) break;
+            tc::fence_after();
+            const uint32_t row = tile.i * SIZE + rank * kRows + (warp - 4) * 32 + lane;
+            const uint32_t sums = tmem + half * SIZE + ((warp - 4) * 32 << 16);
+            const uint32_t width = PHASE == APPLY ? a.n : a.m;
+            const int shift = max(0, g.shift[tile.index] - 2 * int(step)), next = max(0, shift - 2);
+            // of the sum and of what is added to it
+            const float of_sum = PHASE == GRAM         ? 1.0f / kScaleX
+                                 : PHASE == POLYNOMIAL ? ldexpf(0.5f * kC / kScaleX, -4 * shift)
+                                                       : ldexpf(2.0f / kScaleX, next - shift);
+            const float of_old = PHASE == POLYNOMIAL ? ldexpf(0.5f * kB, -2 * shift) : ldexpf(kA, next - shift);
+            // rows and columns up to the end of their block: behind the matrix they are zero
+            const uint32_t rows_end = a.down_blocks * kRows, columns_end = (PHASE == APPLY ? a.x_blocks : a.a_blocks) * kDepth;
+            for (uint32_t c = 0; c < SIZE; c += 32) {
+                const uint32_t column = tile.j * SIZE + c;
+                if (column >= columns_end) break;
+                float v[32];
+                __syncwarp();
+                tc::tmem_load(v, sums + c);
+                if (row >= rows_end) continue;
+                if constexpr (PHASE == APPLY) {
+                    const uint64_t low = bytes_of(a.down_blocks, a.x_blocks);
+                    const char *old = g.scratch + a.x[current];
+                    char *to = g.scratch + a.x[current ^ 1];
+#pragma unroll
+                    for (uint32_t q = 0; q < 32; q += 8) {
+                        const uint64_t place = place_of(row, column + q, a.x_blocks);
+                        float x[8];
+                        load_operand<SPLIT>(x, old + place, low);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[q + e] = of_old * x[e] + v[q + e] * of_sum;
+                        if (!last) {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) x[e] = v[q + e];
+                            store_operand<SPLIT>(to + place, low, x);
+                        }
+                    }
+                    if (last && row < a.m) {
+                        const float rate = ldexpf(a.momentum ? -a.rate / kScaleX : 1.0f / kScaleX, -next);
+                        if (a.flip) { // neighbouring lanes have neighbouring elements
+#pragma unroll
+                            for (uint32_t q = 0; q < 32; ++q) {
+                                if (column + q >= width) break;
+                                const uint64_t i = uint64_t(column + q) * a.m + row;
+                                const float y = v[q] * rate;
+                                store1(a.out, a.out_type, i, a.momentum ? fmaf(a.down, load1(a.out, a.out_type, i), y) : y);
+                            }
+                        } else {
+#pragma unroll
+                            for (uint32_t q = 0; q < 32; q += 8) {
+                                if (column + q >= width) break;
+                                const uint64_t i = uint64_t(row) * a.n + column + q;
+                                const uint32_t count = min(8u, width - column - q);
+                                float y[8], old_p[8];
+                                if (a.momentum) load8(old_p, a.out, a.out_type, i, count);
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) {
+                                    y[e] = v[q + e] * rate;
+                                    if (a.momentum) y[e] = fmaf(a.down, old_p[e], y[e]);
+                                }
+                                store8(y, a.out, a.out_type, i, count);
+                            }
+                        }
+                    }
+                } else {
+                    const uint64_t low = bytes_of(a.down_blocks, a.a_blocks);
+                    char *to = g.scratch + (PHASE == GRAM ? a.a : a.p);
+#pragma unroll
+                    for (uint32_t q = 0; q < 32; q += 8) {
+                        const uint64_t place = place_of(row, column + q, a.a_blocks);
+                        float x[8];
+                        if constexpr (PHASE == GRAM) {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) x[e] = v[q + e] = v[q + e] * of_sum;
+                        } else {
+                            load_operand<SPLIT>(x, g.scratch + a.a + place, low);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) x[e] = v[q + e] = of_old * x[e] + v[q + e] * of_sum;
+                        }
+                        store_operand<SPLIT>(to + place, low, x);
+                    }
+                    if (tile.i != tile.j) { // the mirror image: lanes in pairs, each with two rows of one column
+#pragma unroll
+                        for (uint32_t q = 0; q < 32; q += 2) {
+                            const float other = __shfl_xor_sync(0xffffffffu, lane & 1 ? v[q] : v[q + 1], 1);
+                            const float first = lane & 1 ? other : v[q], second = lane & 1 ? v[q + 1] : other;
+                            const uint32_t r = column + q + (lane & 1), to_column = row & ~1u;
+                            const __half2 h = __floats2half2_rn(first, second);
+                            char *at = to + place_of(r, to_column, a.a_blocks) + to_column % 8 * 2;
+                            *reinterpret_cast<__half2 *>(at) = h;
+                            if constexpr (SPLIT) {
+                                const float2 y = __half22float2(h);
+                                *reinterpret_cast<__half2 *>(at + low) = __floats2half2_rn(first - y.x, second - y.y);
+                            }
+                        }
+                    }
+                }
+            }
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) tc::barrier_arrive_at(CG == 2 ? tc::in_block(&st.taken[half], 0) : tc::shared_address(&st.taken[half]));
+        }
+    }
+    __syncwarp();
+    tc::fence_before();
+    __syncthreads();
+    if constexpr (CG == 2) tc::cluster_sync();
+    tc::fence_after();
+    if (threadIdx.x == 0 && st.stop) *g.fault = 1;
+    if (warp == 1) tc::tmem_free<CG>(tmem, 2 * SIZE);
+}
+
+// A wait that ran out left the products unfinished: everything that the call was to write is NaN.
+__global__ void __launch_bounds__(kThreads) k_check_fault(const __grid_constant__ Group g) {
+    cudaGridDependencySynchronize();
+    if (!*g.fault) return;
+    for (uint32_t k = 0; k < g.count; ++k) {
+        const Matrix &a = g.matrix[k];
+        const uint64_t n = uint64_t(a.m) * a.n;
+        for (uint64_t i = uint64_t(blockIdx.x) * kThreads + threadIdx.x; i < n; i += uint64_t(gridDim.x) * kThreads)
+            store1(a.out, a.out_type, i, __int_as_float(0x7fffffff));
     }
 }
 
@@ -137,7 +614,8 @@ void check_list(const ArcqmlMatrix *list, size_t count, const char *name) {
         if (a.dtype > ARCQML_NO_TENSOR) refuse(name, i, "has an unknown type");
         if (a.reserved != 0) refuse(name, i, "has a nonzero reserved field");
         if (!present(a)) continue;
-        if (a.rows >> 24 || a.columns >> 24 || (a.rows * a.columns) >> 36) refuse(name, i, "is too large");
+        if (a.rows >> 24 || a.columns >> 24 || (a.rows * a.columns) >> 36 || std::min(a.rows, a.columns) >> 17)
+            refuse(name, i, "is too large");
         if (!a.data) refuse(name, i, "is null");
         if (reinterpret_cast<uintptr_t>(a.data) % bytes_of_element(a.dtype)) refuse(name, i, "is not aligned to its elements");
     }
@@ -155,11 +633,21 @@ void check_scratch(const double *ws, size_t len, size_t need) {
 }
 
 template <class... P, class... A>
-void start(void (*kernel)(P...), dim3 blocks, uint32_t threads, double bytes, cudaStream_t s, const A &...args) {
+void start(void (*kernel)(P...), uint32_t blocks, uint32_t threads, uint32_t cluster, uint32_t shared, bool follows,
+           double bytes, cudaStream_t s, const A &...args) {
     cudaLaunchConfig_t c{};
-    c.gridDim = blocks;
+    cudaLaunchAttribute at[2]{};
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = follows;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    c.gridDim = dim3(blocks);
     c.blockDim = dim3(threads);
+    c.dynamicSmemBytes = shared;
     c.stream = s;
+    c.attrs = at;
+    c.numAttrs = cluster > 1 ? 2 : 1;
     std::tuple<P...> held{P(args)...};
     const ProfToken tok = prof_begin(PROF_OTHER, s);
     const cudaError_t e = std::apply([&](auto &...x) { return cudaLaunchKernelEx(&c, kernel, x...); }, held);
@@ -167,29 +655,159 @@ void start(void (*kernel)(P...), dim3 blocks, uint32_t threads, double bytes, cu
     prof_end(tok, s, bytes);
 }
 
-// Scratch of one matrix: sums, X twice, A, P.
-size_t scratch_of(const ArcqmlMatrix &a) {
-    if (!present(a)) return 0;
+// Types of 11 bits and more take operands of 22.
+bool is_split(uint32_t type) { return type != ARCQML_BF16; }
+
+constexpr size_t kHeadBytes = 512; // the fault, and from 256 on the shifts
+size_t sums_bytes() { return size_t(kMatrices) * kSumBlocks * sizeof(double); }
+
+// Scratch bytes of a matrix's X (twice), A and P.
+uint64_t operand_bytes(const ArcqmlMatrix &a, bool split) {
     const uint64_t m = std::min(a.rows, a.columns), n = std::max(a.rows, a.columns);
-    return kSumBlocks + size_t(m * n + m * m) + 8;
+    const uint32_t down = uint32_t((m + kRows - 1) / kRows), across = 2 * uint32_t((n + kRows - 1) / kRows);
+    return (2 * bytes_of(down, across) + 2 * bytes_of(down, 2 * down)) * (split ? 2 : 1);
 }
 
-void run_job(const Job &j, int steps, double eps, double *ws, cudaStream_t s) {
-    const uint64_t m = std::min(j.rows, j.columns), n = std::max(j.rows, j.columns), all = m * n;
-    const uint32_t blocks = uint32_t(std::min<uint64_t>(kSumBlocks, (all + kThreads - 1) / kThreads));
-    start(k_update_squares, blocks, kThreads, 4.0 * double(all), s, j, ws);
-    float *x = reinterpret_cast<float *>(ws + kSumBlocks), *y = x + all, *a = y + all, *p = a + m * m;
-    const uint32_t grid = uint32_t(std::min<uint64_t>(148 * 8, (all + kThreads - 1) / kThreads));
-    start(k_scale_update, grid, kThreads, 4.0 * double(all), s, j, ws, blocks, eps, x);
-    const auto tiles = [](uint64_t v) { return uint32_t((v + 15) / 16); };
-    const float *none = nullptr;
-    for (int i = 0; i < steps; ++i) {
-        start(k_product, dim3(tiles(m), tiles(m)), 256, 0.0, s, x, x, none, a, m, m, n, true, 0.0f, 1.0f);
-        start(k_product, dim3(tiles(m), tiles(m)), 256, 0.0, s, a, a, a, p, m, m, m, true, kB, kC);
-        start(k_product, dim3(tiles(n), tiles(m)), 256, 0.0, s, p, x, x, y, m, n, m, false, kA, 1.0f);
-        std::swap(x, y);
+// The scratch of a launch's matrices: what one needs, and more of them while that stays below 2 GB.
+constexpr uint64_t kGroupBytes = uint64_t(2) << 30;
+
+template <class F>
+void for_groups(const ArcqmlMatrix *list, const ArcqmlMatrix *kinds, size_t count, uint64_t most, F &&f) {
+    std::vector<size_t> members;
+    for (int split = 1; split >= 0; --split) {
+        uint64_t bytes = 0;
+        const auto flush = [&] {
+            if (!members.empty()) f(members, bytes, split != 0);
+            members.clear();
+            bytes = 0;
+        };
+        for (size_t i = 0; i < count; ++i) {
+            if (!present(list[i]) || is_split(kinds[i].dtype) != (split != 0)) continue;
+            const uint64_t need = operand_bytes(list[i], split != 0);
+            if (members.size() == kMatrices || (bytes && bytes + need > most)) flush();
+            members.push_back(i);
+            bytes += need;
+        }
+        flush();
     }
-    start(k_finish, grid, kThreads, 4.0 * double(all), s, j, x);
+}
+
+template <int PHASE, bool SPLIT, int CG>
+void product(Group &g, uint32_t tiles, uint32_t step, bool last, cudaStream_t s) {
+    static std::atomic<uint64_t> set{0}; // the devices on which the kernel may have that much shared memory
+    int device = 0;
+    check_cuda(cudaGetDevice(&device), "cudaGetDevice");
+    if (device >= 64 || !(set.load() >> device & 1)) {
+        check_cuda(cudaFuncSetAttribute(k_product<PHASE, SPLIT, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        int(kProductShared<SPLIT>)),
+                   "orthogonalisation kernel attribute");
+        if (device < 64) set |= uint64_t(1) << device;
+    }
+    start(k_product<PHASE, SPLIT, CG>, std::min(tiles * CG, kSMs), kProductThreads, CG, kProductShared<SPLIT>, true, 0.0, s, g,
+          step, uint32_t(last));
+}
+
+template <int PHASE> uint32_t tiles_of(const Matrix &a, uint32_t size) {
+    const uint32_t down = (a.m + size - 1) / size, across = (a.n + size - 1) / size;
+    return PHASE == APPLY ? down * across : down * (down + 1) / 2;
+}
+
+template <int PHASE, bool SPLIT> void phase(Group &g, uint32_t step, bool last, cudaStream_t s) {
+    // time of the phase in steps of 64 of a block's depth, on pairs of blocks and on single ones: all of the
+    // work spread over the GPU and half of its longest tile behind it
+    double cost[2];
+    for (int pair = 0; pair < 2; ++pair) {
+        double all = 0.0, longest = 0.0;
+        for (uint32_t i = 0; i < g.count; ++i) {
+            const Matrix &a = g.matrix[i];
+            const double depth = ((PHASE == GRAM ? a.n : a.m) + kDepth - 1) / kDepth * (pair ? 2.0 : 1.0) + 8;
+            const uint32_t tiles = tiles_of<PHASE>(a, kRows << pair);
+            all += tiles * depth;
+            longest = std::max(longest, depth);
+        }
+        const double units = pair ? kSMs / 2 : kSMs;
+        cost[pair] = std::max(longest, all / units + longest / 2);
+    }
+    const bool pair = cost[1] <= cost[0];
+    uint32_t tiles = 0;
+    for (uint32_t i = 0; i < g.count; ++i) {
+        g.first[i] = tiles;
+        tiles += tiles_of<PHASE>(g.matrix[i], pair ? 2 * kRows : kRows);
+    }
+    g.first[g.count] = tiles;
+    if (pair) product<PHASE, SPLIT, 2>(g, tiles, step, last, s);
+    else product<PHASE, SPLIT, 1>(g, tiles, step, last, s);
+}
+
+// The members' `out`, `in` and step are set; shapes and places are filled in here.
+template <bool SPLIT> void run_group(Group &g, int steps, cudaStream_t s) {
+    uint32_t blocks = 0, spread = 0;
+    double elements = 0.0;
+    uint64_t at = kHeadBytes + sums_bytes();
+    static thread_local Group tiles;
+    for (uint32_t i = 0; i < g.count; ++i) {
+        Matrix &a = g.matrix[i];
+        a.down_blocks = (a.m + kRows - 1) / kRows;
+        a.x_blocks = 2 * ((a.n + kRows - 1) / kRows);
+        a.a_blocks = 2 * a.down_blocks;
+        const uint64_t x = bytes_of(a.down_blocks, a.x_blocks) * (SPLIT ? 2 : 1);
+        const uint64_t square = bytes_of(a.down_blocks, a.a_blocks) * (SPLIT ? 2 : 1);
+        a.x[0] = at;
+        a.x[1] = at + x;
+        a.a = at + 2 * x;
+        a.p = a.a + square;
+        at = a.p + square;
+        const uint64_t all = uint64_t(a.m) * a.n;
+        g.first[i] = blocks;
+        tiles.first[i] = spread;
+        blocks += uint32_t(std::min<uint64_t>(kSumBlocks, (all + kThreads * 8 - 1) / (kThreads * 8)));
+        spread += a.down_blocks * a.x_blocks;
+        elements += double(all);
+    }
+    g.first[g.count] = blocks;
+    tiles.first[g.count] = spread;
+    start(k_update_squares, blocks, kThreads, 1, 0, false, 8.0 * elements, s, g);
+    std::copy(g.matrix, g.matrix + g.count, tiles.matrix);
+    tiles.count = g.count;
+    tiles.scratch = g.scratch;
+    tiles.fault = g.fault;
+    tiles.shift = g.shift;
+    tiles.sums = g.sums;
+    tiles.eps = g.eps;
+    start(k_spread<SPLIT>, spread, kThreads, 1, 0, true, 8.0 * elements, s, tiles, g);
+    for (int i = 0; i < steps; ++i) {
+        phase<GRAM, SPLIT>(g, i, false, s);
+        phase<POLYNOMIAL, SPLIT>(g, i, false, s);
+        phase<APPLY, SPLIT>(g, i, i + 1 == steps, s);
+    }
+    start(k_check_fault, 8, kThreads, 1, 0, true, 0.0, s, g);
+}
+
+// fill(matrix, place) sets what the call does to a place of the list.
+template <class F>
+void run(const ArcqmlMatrix *list, const ArcqmlMatrix *kinds, size_t count, int steps, double eps, double *ws, size_t ws_len,
+         cudaStream_t s, F &&fill) {
+    const uint64_t have = ws_len * sizeof(double), head = kHeadBytes + sums_bytes();
+    for_groups(list, kinds, count, have > head ? have - head : 0, [&](const std::vector<size_t> &members, uint64_t, bool split) {
+        static thread_local Group g;
+        g.count = uint32_t(members.size());
+        g.scratch = reinterpret_cast<char *>(ws);
+        g.fault = reinterpret_cast<uint32_t *>(ws);
+        g.shift = reinterpret_cast<int *>(g.scratch + kHeadBytes / 2);
+        g.sums = reinterpret_cast<double *>(g.scratch + kHeadBytes);
+        g.eps = eps;
+        for (uint32_t i = 0; i < g.count; ++i) {
+            const ArcqmlMatrix &a = list[members[i]];
+            Matrix &m = g.matrix[i];
+            m = Matrix{};
+            m.flip = a.rows > a.columns;
+            m.m = uint32_t(std::min(a.rows, a.columns));
+            m.n = uint32_t(std::max(a.rows, a.columns));
+            fill(m, members[i]);
+        }
+        if (split) run_group<true>(g, steps, s);
+        else run_group<false>(g, steps, s);
+    });
 }
 
 void check_steps(int steps, double eps) {
@@ -200,9 +818,11 @@ void check_steps(int steps, double eps) {
 }  // namespace
 
 size_t orthogonalize_workspace(const ArcqmlMatrix *list, size_t count) {
-    size_t most = 0;
-    for (size_t i = 0; list && i < count; ++i) most = std::max(most, scratch_of(list[i]));
-    return most;
+    if (!list) return 0;
+    uint64_t most = 0;
+    for_groups(list, list, count, kGroupBytes,
+               [&](const std::vector<size_t> &, uint64_t bytes, bool) { most = std::max(most, bytes); });
+    return most ? size_t((kHeadBytes + sums_bytes() + most) / sizeof(double)) : 0;
 }
 
 void orthogonalize_device(const ArcqmlMatrix *in, const ArcqmlMatrix *out, size_t count, int steps, double eps,
@@ -214,10 +834,12 @@ void orthogonalize_device(const ArcqmlMatrix *in, const ArcqmlMatrix *out, size_
         if (in[i].dtype != out[i].dtype || in[i].rows != out[i].rows || in[i].columns != out[i].columns)
             refuse("output", i, "differs from its input in type or shape");
     check_scratch(ws, ws_len, orthogonalize_workspace(in, count));
-    for (size_t i = 0; i < count; ++i) {
-        if (!present(in[i])) continue;
-        run_job({out[i].data, in[i].data, nullptr, in[i].rows, in[i].columns, out[i].dtype, in[i].dtype}, steps, eps, ws, s);
-    }
+    run(in, in, count, steps, eps, ws, ws_len, s, [&](Matrix &m, size_t i) {
+        m.out = out[i].data;
+        m.in = in[i].data;
+        m.out_type = uint8_t(out[i].dtype);
+        m.in_type = uint8_t(in[i].dtype);
+    });
 }
 
 void muon_step_device(const ArcqmlMatrix *params, const ArcqmlMatrix *grads, const ArcqmlMatrix *momenta, size_t count,
@@ -238,15 +860,18 @@ void muon_step_device(const ArcqmlMatrix *params, const ArcqmlMatrix *grads, con
             refuse("momentum", i, "differs in shape from its parameter, or is not f32");
     }
     check_scratch(ws, ws_len, orthogonalize_workspace(params, count));
-    for (size_t i = 0; i < count; ++i) {
-        if (!present(grads[i])) continue;
-        const double ratio = double(params[i].rows) / double(params[i].columns);
-        run_job({params[i].data, grads[i].data, static_cast<float *>(momenta[i].data), params[i].rows, params[i].columns,
-                 params[i].dtype, grads[i].dtype, float(o.momentum), float(1.0 - o.momentum),
-                 float(1.0 - o.learning_rate * o.weight_decay),
-                 float(o.learning_rate * std::sqrt(std::max(1.0, ratio))), uint32_t(o.nesterov)},
-                o.steps, o.epsilon, ws, s);
-    }
+    run(grads, params, count, o.steps, o.epsilon, ws, ws_len, s, [&](Matrix &m, size_t i) {
+        m.out = params[i].data;
+        m.in = grads[i].data;
+        m.momentum = static_cast<float *>(momenta[i].data);
+        m.out_type = uint8_t(params[i].dtype);
+        m.in_type = uint8_t(grads[i].dtype);
+        m.nesterov = uint8_t(o.nesterov);
+        m.beta = float(o.momentum);
+        m.keep = float(1.0 - o.momentum);
+        m.down = float(1.0 - o.learning_rate * o.weight_decay);
+        m.rate = float(o.learning_rate * std::sqrt(std::max(1.0, double(params[i].rows) / double(params[i].columns))));
+    });
 }
 
 }  // namespace arcqml
