@@ -119,11 +119,6 @@ template <class T> __device__ __forceinline__ void store8_as(const float (&v)[8]
             if (uint32_t(i) < count) p[i] = to_element<T>(v[i]);
     }
 }
-__device__ __forceinline__ void store8(const float (&v)[8], void *p, uint32_t type, uint64_t i, uint32_t count) {
-    if (type == ARCQML_F32) store8_as(v, static_cast<float *>(p) + i, count);
-    else if (type == ARCQML_BF16) store8_as(v, static_cast<__nv_bfloat16 *>(p) + i, count);
-    else store8_as(v, static_cast<__half *>(p) + i, count);
-}
 __device__ __forceinline__ float load1(const void *p, uint32_t type, uint64_t i) {
     if (type == ARCQML_F32) return static_cast<const float *>(p)[i];
     if (type == ARCQML_BF16) return to_wide(static_cast<const __nv_bfloat16 *>(p)[i]);
@@ -290,11 +285,19 @@ template <bool SPLIT> __global__ void __launch_bounds__(kThreads) k_spread(const
 
 enum Phase { GRAM, POLYNOMIAL, APPLY };
 constexpr uint32_t kStageBytes = 32768; // one depth of 64: 128 rows of the left operand, 128 of the right
-constexpr uint32_t kProductThreads = 256;
+constexpr uint32_t kTakers = 8; // warps that take sums out: each has a quarter of the rows, half of the columns
+constexpr uint32_t kProductThreads = 128 + kTakers * 32;
 
-// Stages of a block: 192 KB of operands.
+// Stages of a block: 192 KB of operands. Behind them a square of 32 x 32 for each taker.
 template <bool SPLIT> constexpr uint32_t kStages = SPLIT ? 3 : 6;
-template <bool SPLIT> constexpr uint32_t kProductShared = 1024 + kStages<SPLIT> * (SPLIT ? 2 : 1) * kStageBytes + 256;
+constexpr uint32_t kSquare = 32 * 33 * sizeof(float);
+template <bool SPLIT> constexpr uint32_t kProductShared =
+    1024 + kStages<SPLIT> * (SPLIT ? 2 : 1) * kStageBytes + 256 + kTakers * kSquare;
+// The tensor cores cut what falls behind the last bit of a running sum (they do not round): a chain of k
+// steps of 16 loses up to k 2^-24 of it, always towards 0. Operands of 22 bits would show that (a matrix of
+// 4096 x 8191 came out 4.4e-5 off, 7e-6 with f32 operations), so their sums leave tensor memory every 512 of
+// depth and go on in registers. Steps of 64:
+template <bool SPLIT> constexpr uint32_t kChain = SPLIT ? 8 : 0xffffffffu;
 
 struct ProductState {
     uint64_t full[6], empty[6], peer[6], done[2], taken[2];
@@ -343,6 +346,82 @@ template <int PHASE, uint32_t SIZE> __device__ __forceinline__ Tile tile_of(cons
     return r;
 }
 
+// 32 neighbouring sums of a row, for each thread of a warp, become what the phase stores.
+template <int PHASE, bool SPLIT>
+__device__ __forceinline__ void take_sums(const Group &g, const Matrix &a, float (&v)[32], uint32_t row, uint32_t column,
+                                          bool mirrored, int shift, uint32_t current, bool last, float *square) {
+    // rows and columns up to the end of their block: behind the matrix they are zero
+    const uint32_t across = PHASE == APPLY ? a.x_blocks : a.a_blocks;
+    if (row >= a.down_blocks * kRows || column >= across * kDepth) return; // the same for the whole warp
+    const uint32_t lane = threadIdx.x & 31;
+    const int next = max(0, shift - 2);
+    // of the sum and of what is added to it
+    const float of_sum = PHASE == GRAM         ? 1.0f / kScaleX
+                         : PHASE == POLYNOMIAL ? ldexpf(0.5f * kC / kScaleX, -4 * shift)
+                                               : ldexpf(2.0f / kScaleX, next - shift);
+    const float of_old = PHASE == POLYNOMIAL ? ldexpf(0.5f * kB, -2 * shift) : ldexpf(kA, next - shift);
+    const uint64_t low = bytes_of(a.down_blocks, across);
+    const char *old = g.scratch + (PHASE == APPLY ? a.x[current] : a.a);
+    char *to = g.scratch + (PHASE == APPLY ? a.x[current ^ 1] : PHASE == GRAM ? a.a : a.p);
+#pragma unroll
+    for (uint32_t q = 0; q < 32; q += 8) {
+        const uint64_t place = place_of(row, column + q, across);
+        float x[8];
+        if constexpr (PHASE != GRAM) load_operand<SPLIT>(x, old + place, low);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = v[q + e] = PHASE == GRAM ? v[q + e] * of_sum : of_old * x[e] + v[q + e] * of_sum;
+        if (PHASE != APPLY || !last) store_operand<SPLIT>(to + place, low, x);
+    }
+    if (PHASE != APPLY && mirrored) { // lanes in pairs, each with two rows of one column
+#pragma unroll
+        for (uint32_t q = 0; q < 32; q += 2) {
+            const float other = __shfl_xor_sync(0xffffffffu, lane & 1 ? v[q] : v[q + 1], 1);
+            const float one = lane & 1 ? other : v[q], two = lane & 1 ? v[q + 1] : other;
+            const uint32_t r = column + q + (lane & 1), to_column = row & ~1u;
+            const __half2 h = __floats2half2_rn(one, two);
+            char *at = to + place_of(r, to_column, across) + to_column % 8 * 2;
+            *reinterpret_cast<__half2 *>(at) = h;
+            if constexpr (SPLIT) {
+                const float2 y = __half22float2(h);
+                *reinterpret_cast<__half2 *>(at + low) = __floats2half2_rn(one - y.x, two - y.y);
+            }
+        }
+    }
+    if (PHASE == APPLY && last) {
+        const float rate = ldexpf(a.momentum ? -a.rate / kScaleX : 1.0f / kScaleX, -next);
+        const uint32_t row0 = row - lane;
+        if (!a.flip) { // turned in shared memory, so that neighbouring lanes have neighbouring elements
+            __syncwarp();
+#pragma unroll
+            for (uint32_t q = 0; q < 32; ++q) square[lane * 33 + q] = v[q];
+            __syncwarp();
+#pragma unroll
+            for (uint32_t q = 0; q < 32; ++q) v[q] = square[q * 33 + lane];
+        }
+        // v[q]: element `at` + q * pitch
+        const uint32_t along = a.flip ? column : row0, count = a.flip ? a.n - min(a.n, along) : a.m - min(a.m, along);
+        const uint32_t pitch = a.flip ? a.m : a.n, mine = a.flip ? row : column + lane;
+        if (mine < pitch) {
+            const uint64_t at = uint64_t(along) * pitch + mine;
+            if (a.momentum) {
+                float p[32];
+#pragma unroll
+                for (uint32_t q = 0; q < 32; ++q)
+                    if (q < count) p[q] = load1(a.out, a.out_type, at + uint64_t(q) * pitch);
+#pragma unroll
+                for (uint32_t q = 0; q < 32; ++q) v[q] = fmaf(a.down, p[q], v[q] * rate);
+            } else {
+#pragma unroll
+                for (uint32_t q = 0; q < 32; ++q) v[q] *= rate;
+            }
+#pragma unroll
+            for (uint32_t q = 0; q < 32; ++q)
+                if (q < count) store1(a.out, a.out_type, at + uint64_t(q) * pitch, v[q]);
+        }
+        __syncwarp();
+    }
+}
+
 // One phase for all matrices of a group: D = L R^T in tiles of 128 CG x 128 CG, a pair of blocks a tile with
 // CG = 2 (each has half of the tile's rows, and brings half of the right operand's).
 template <int PHASE, bool SPLIT, int CG>
@@ -362,7 +441,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         }
         for (uint32_t s = 0; s < 2; ++s) {
             tc::barrier_init(&st.done[s], 1);
-            tc::barrier_init(&st.taken[s], 4 * CG);
+            tc::barrier_init(&st.taken[s], kTakers * CG);
         }
         st.stop = 0;
         tc::barrier_init_fence();
@@ -378,6 +457,10 @@ __global__ void __launch_bounds__(kProductThreads, 1)
     const uint32_t units = gridDim.x / CG, unit = blockIdx.x / CG, tiles = g.first[g.count];
     const bool broken = *reinterpret_cast<volatile uint32_t *>(g.fault) != 0;
 
+    // the sums of a tile in registers take more of them than a thread's share: 384 x 168 registers as
+    // 128 x 56 and 256 x 216
+    if (warp < 4) {
+        if constexpr (SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 0 && lane == 0 && !broken) { // copies operands in
         uint32_t at = 0, phase = 0;
         bool on = true;
@@ -428,32 +511,36 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         constexpr uint32_t STEP = PHASE == APPLY ? 2048 / 16 : 32 / 16; // of the right operand, 16 of depth
         uint32_t at = 0, phase = 0, n = 0;
         bool on = true;
-        for (uint32_t t = unit; t < tiles && on; t += units, ++n) {
-            const uint32_t depth = tile_of<PHASE, SIZE>(g, t).depth, half = n & 1;
-            if (!wait_for(&st.taken[half], (n >> 1 & 1) ^ 1, &st.stop)) break;
-            tc::fence_after();
-            const uint32_t sums = tmem + half * SIZE;
-            for (uint32_t d = 0; d < depth; ++d) {
-                if (!(on = wait_for(&st.full[at], phase, &st.stop))) break;
-                if constexpr (CG == 2)
-                    if (!(on = wait_for(&st.peer[at], phase, &st.stop))) break;
+        for (uint32_t t = unit; t < tiles && on; t += units) {
+            const uint32_t depth = tile_of<PHASE, SIZE>(g, t).depth;
+            for (uint32_t d = 0; d < depth && on; ++n) {
+                const uint32_t half = n & 1, end = min(depth - d, kChain<SPLIT>) + d;
+                if (!(on = wait_for(&st.taken[half], (n >> 1 & 1) ^ 1, &st.stop))) break;
                 tc::fence_after();
-                const uint32_t base = tc::shared_address(shared + at * STAGE);
-                const uint64_t left = tc::descriptor(base, 16);
-                const uint64_t right = tc::descriptor(base + kBlock, PHASE == APPLY ? kBlock / 2 : 16);
+                const uint32_t sums = tmem + half * SIZE;
+                for (bool add = false; d < end; ++d) {
+                    if (!(on = wait_for(&st.full[at], phase, &st.stop))) break;
+                    if constexpr (CG == 2)
+                        if (!(on = wait_for(&st.peer[at], phase, &st.stop))) break;
+                    tc::fence_after();
+                    const uint32_t base = tc::shared_address(shared + at * STAGE);
+                    const uint64_t left = tc::descriptor(base, 16);
+                    const uint64_t right = tc::descriptor(base + kBlock, PHASE == APPLY ? kBlock / 2 : 16);
 #pragma unroll
-                for (uint32_t s = 0; s < kDepth / 16; ++s) {
-                    tc::mma<CG>(sums, left + s * 2, right + s * STEP, instr, d != 0 || s != 0);
-                    if constexpr (SPLIT) {
-                        constexpr uint32_t LOW = kStageBytes / 16;
-                        tc::mma<CG>(sums, left + s * 2, right + LOW + s * STEP, instr, true);
-                        tc::mma<CG>(sums, left + LOW + s * 2, right + s * STEP, instr, true);
+                    for (uint32_t s = 0; s < kDepth / 16; ++s) {
+                        tc::mma<CG>(sums, left + s * 2, right + s * STEP, instr, add);
+                        add = true;
+                        if constexpr (SPLIT) {
+                            constexpr uint32_t LOW = kStageBytes / 16;
+                            tc::mma<CG>(sums, left + s * 2, right + LOW + s * STEP, instr, true);
+                            tc::mma<CG>(sums, left + LOW + s * 2, right + s * STEP, instr, true);
+                        }
                     }
+                    tc::commit<CG>(&st.empty[at]);
+                    if (++at == S) at = 0, phase ^= 1;
                 }
-                tc::commit<CG>(&st.empty[at]);
-                if (++at == S) at = 0, phase ^= 1;
+                if (on) tc::commit<CG>(&st.done[half]);
             }
-            if (on) tc::commit<CG>(&st.done[half]);
         }
     } else if (CG == 2 && warp == 2 && rank == 1 && lane == 0 && !broken) { // tells the first block of its operands
         uint32_t at = 0, phase = 0;
@@ -466,114 +553,71 @@ __global__ void __launch_bounds__(kProductThreads, 1)
                 if (++at == S) at = 0, phase ^= 1;
             }
         }
-    } else if (warp >= 4 && !broken) { // takes the sums out: a thread has a row
+    }
+    } else {
+        if constexpr (SPLIT) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    if (!broken) { // takes the sums out: a thread has a row
+        constexpr uint32_t COLUMNS = SIZE / 2;
+        const uint32_t quarter = warp & 3, first = (warp - 4) / 4 * COLUMNS;
+        float *square = reinterpret_cast<float *>(reinterpret_cast<char *>(&st) + 256) + (warp - 4) * (kSquare / 4);
         uint32_t n = 0;
-        for (uint32_t t = unit; t < tiles; t += units, ++n) {
-            const Tile tile = tile_of<PHASE, SIZE>(g, t);
-            const Matrix &a = *tile.a;
-            const uint32_t half = n & 1;
-            if (!__all_sync(0xffffffffu, wait_for(&st.done[half], n >> 1 & 1, &st.stop))) break;
-            tc::fence_after();
-            const uint32_t row = tile.i * SIZE + rank * kRows + (warp - 4) * 32 + lane;
-            const uint32_t sums = tmem + half * SIZE + ((warp - 4) * 32 << 16);
-            const uint32_t width = PHASE == APPLY ? a.n : a.m;
-            const int shift = max(0, g.shift[tile.index] - 2 * int(step)), next = max(0, shift - 2);
-            // of the sum and of what is added to it
-            const float of_sum = PHASE == GRAM         ? 1.0f / kScaleX
-                                 : PHASE == POLYNOMIAL ? ldexpf(0.5f * kC / kScaleX, -4 * shift)
-                                                       : ldexpf(2.0f / kScaleX, next - shift);
-            const float of_old = PHASE == POLYNOMIAL ? ldexpf(0.5f * kB, -2 * shift) : ldexpf(kA, next - shift);
-            // rows and columns up to the end of their block: behind the matrix they are zero
-            const uint32_t rows_end = a.down_blocks * kRows, columns_end = (PHASE == APPLY ? a.x_blocks : a.a_blocks) * kDepth;
-            for (uint32_t c = 0; c < SIZE; c += 32) {
-                const uint32_t column = tile.j * SIZE + c;
-                if (column >= columns_end) break;
-                float v[32];
-                __syncwarp();
-                tc::tmem_load(v, sums + c);
-                if (row >= rows_end) continue;
-                if constexpr (PHASE == APPLY) {
-                    const uint64_t low = bytes_of(a.down_blocks, a.x_blocks);
-                    const char *old = g.scratch + a.x[current];
-                    char *to = g.scratch + a.x[current ^ 1];
-#pragma unroll
-                    for (uint32_t q = 0; q < 32; q += 8) {
-                        const uint64_t place = place_of(row, column + q, a.x_blocks);
-                        float x[8];
-                        load_operand<SPLIT>(x, old + place, low);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) v[q + e] = of_old * x[e] + v[q + e] * of_sum;
-                        if (!last) {
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) x[e] = v[q + e];
-                            store_operand<SPLIT>(to + place, low, x);
-                        }
-                    }
-                    if (last && row < a.m) {
-                        const float rate = ldexpf(a.momentum ? -a.rate / kScaleX : 1.0f / kScaleX, -next);
-                        if (a.flip) { // neighbouring lanes have neighbouring elements
-#pragma unroll
-                            for (uint32_t q = 0; q < 32; ++q) {
-                                if (column + q >= width) break;
-                                const uint64_t i = uint64_t(column + q) * a.m + row;
-                                const float y = v[q] * rate;
-                                store1(a.out, a.out_type, i, a.momentum ? fmaf(a.down, load1(a.out, a.out_type, i), y) : y);
-                            }
-                        } else {
-#pragma unroll
-                            for (uint32_t q = 0; q < 32; q += 8) {
-                                if (column + q >= width) break;
-                                const uint64_t i = uint64_t(row) * a.n + column + q;
-                                const uint32_t count = min(8u, width - column - q);
-                                float y[8], old_p[8];
-                                if (a.momentum) load8(old_p, a.out, a.out_type, i, count);
-#pragma unroll
-                                for (int e = 0; e < 8; ++e) {
-                                    y[e] = v[q + e] * rate;
-                                    if (a.momentum) y[e] = fmaf(a.down, old_p[e], y[e]);
-                                }
-                                store8(y, a.out, a.out_type, i, count);
-                            }
-                        }
-                    }
-                } else {
-                    const uint64_t low = bytes_of(a.down_blocks, a.a_blocks);
-                    char *to = g.scratch + (PHASE == GRAM ? a.a : a.p);
-#pragma unroll
-                    for (uint32_t q = 0; q < 32; q += 8) {
-                        const uint64_t place = place_of(row, column + q, a.a_blocks);
-                        float x[8];
-                        if constexpr (PHASE == GRAM) {
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) x[e] = v[q + e] = v[q + e] * of_sum;
-                        } else {
-                            load_operand<SPLIT>(x, g.scratch + a.a + place, low);
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) x[e] = v[q + e] = of_old * x[e] + v[q + e] * of_sum;
-                        }
-                        store_operand<SPLIT>(to + place, low, x);
-                    }
-                    if (tile.i != tile.j) { // the mirror image: lanes in pairs, each with two rows of one column
-#pragma unroll
-                        for (uint32_t q = 0; q < 32; q += 2) {
-                            const float other = __shfl_xor_sync(0xffffffffu, lane & 1 ? v[q] : v[q + 1], 1);
-                            const float first = lane & 1 ? other : v[q], second = lane & 1 ? v[q + 1] : other;
-                            const uint32_t r = column + q + (lane & 1), to_column = row & ~1u;
-                            const __half2 h = __floats2half2_rn(first, second);
-                            char *at = to + place_of(r, to_column, a.a_blocks) + to_column % 8 * 2;
-                            *reinterpret_cast<__half2 *>(at) = h;
-                            if constexpr (SPLIT) {
-                                const float2 y = __half22float2(h);
-                                *reinterpret_cast<__half2 *>(at + low) = __floats2half2_rn(first - y.x, second - y.y);
-                            }
-                        }
-                    }
-                }
-            }
+        bool on = true;
+        const auto release = [&](uint32_t half) {
             tc::fence_before();
             __syncwarp();
-            if (lane == 0) tc::barrier_arrive_at(CG == 2 ? tc::in_block(&st.taken[half], 0) : tc::shared_address(&st.taken[half]));
+            if (lane == 0)
+                tc::barrier_arrive_at(CG == 2 ? tc::in_block(&st.taken[half], 0) : tc::shared_address(&st.taken[half]));
+        };
+        const auto wait_done = [&](uint32_t half) {
+            on = __all_sync(0xffffffffu, wait_for(&st.done[half], n >> 1 & 1, &st.stop));
+            tc::fence_after();
+            return on;
+        };
+        for (uint32_t t = unit; t < tiles && on; t += units) {
+            const Tile tile = tile_of<PHASE, SIZE>(g, t);
+            const Matrix &a = *tile.a;
+            const uint32_t row = tile.i * SIZE + rank * kRows + quarter * 32 + lane;
+            const uint32_t lanes = quarter * 32 << 16;
+            const int shift = max(0, g.shift[tile.index] - 2 * int(step));
+            const auto take = [&](float (&v)[32], uint32_t c) {
+                take_sums<PHASE, SPLIT>(g, a, v, row, tile.j * SIZE + first + c, tile.i != tile.j, shift, current, last != 0,
+                                        square);
+            };
+            if constexpr (SPLIT) {
+                float sum[COLUMNS];
+#pragma unroll
+                for (uint32_t c = 0; c < COLUMNS; ++c) sum[c] = 0.0f;
+#pragma unroll 1
+                for (uint32_t d = 0; d < tile.depth; d += kChain<SPLIT>, ++n) {
+                    const uint32_t half = n & 1;
+                    if (!wait_done(half)) break;
+#pragma unroll
+                    for (uint32_t c = 0; c < COLUMNS; c += 16) tc::tmem_add(sum + c, tmem + half * SIZE + lanes + first + c);
+                    release(half);
+                }
+                if (!on) break;
+#pragma unroll
+                for (uint32_t c = 0; c < COLUMNS; c += 32) {
+                    float v[32];
+#pragma unroll
+                    for (uint32_t e = 0; e < 32; ++e) v[e] = sum[c + e];
+                    take(v, c);
+                }
+            } else {
+                const uint32_t half = n & 1;
+                if (!wait_done(half)) break;
+#pragma unroll 1
+                for (uint32_t c = 0; c < COLUMNS; c += 32) {
+                    float v[32];
+                    __syncwarp();
+                    tc::tmem_load(v, tmem + half * SIZE + lanes + first + c);
+                    take(v, c);
+                }
+                release(half);
+                ++n;
+            }
         }
+    }
     }
     __syncwarp();
     tc::fence_before();
@@ -720,7 +764,7 @@ template <int PHASE, bool SPLIT> void phase(Group &g, uint32_t step, bool last, 
         double all = 0.0, longest = 0.0;
         for (uint32_t i = 0; i < g.count; ++i) {
             const Matrix &a = g.matrix[i];
-            const double depth = ((PHASE == GRAM ? a.n : a.m) + kDepth - 1) / kDepth * (pair ? 2.0 : 1.0) + 8;
+            const double depth = ((PHASE == GRAM ? a.n : a.m) + kDepth - 1) / kDepth * (pair ? 1.3 : 1.0) + 8;
             const uint32_t tiles = tiles_of<PHASE>(a, kRows << pair);
             all += tiles * depth;
             longest = std::max(longest, depth);

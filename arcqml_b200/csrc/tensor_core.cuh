@@ -23,13 +23,15 @@ __device__ __forceinline__ uint32_t in_block(const void *b, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(shared_address(b)), "r"(rank));
     return at;
 }
+// What these barriers order is read and written by copies and tensor cores alone, not by threads: a block's
+// scope is enough, and a cluster's costs a fence for each arrival (a stage of a pair took 1300 cycles with it).
 __device__ __forceinline__ void barrier_arrive_at(uint32_t cluster_address) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_address) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_address) : "memory");
 }
 __device__ __forceinline__ bool barrier_try(uint64_t *b, uint32_t parity) {
     uint32_t done;
     asm volatile("{\n .reg .pred p;\n"
-                 " mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+                 " mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
                  " selp.u32 %0, 1, 0, p;\n}"
                  : "=r"(done)
                  : "r"(shared_address(b)), "r"(parity)
@@ -100,6 +102,20 @@ __device__ __forceinline__ void tmem_load(float (&v)[32], uint32_t at) {
                  : "memory");
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// 16 columns, added to v.
+__device__ __forceinline__ void tmem_add(float *v, uint32_t at) {
+    uint32_t r[16];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
+                 " tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(at)
+                 : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] += __uint_as_float(r[i]);
 }
 
 // ------------------------------------------------------------------ tcgen05.mma
