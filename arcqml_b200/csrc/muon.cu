@@ -119,11 +119,6 @@ template <class T> __device__ __forceinline__ void store8_as(const float (&v)[8]
             if (uint32_t(i) < count) p[i] = to_element<T>(v[i]);
     }
 }
-__device__ __forceinline__ float load1(const void *p, uint32_t type, uint64_t i) {
-    if (type == ARCQML_F32) return static_cast<const float *>(p)[i];
-    if (type == ARCQML_BF16) return to_wide(static_cast<const __nv_bfloat16 *>(p)[i]);
-    return to_wide(static_cast<const __half *>(p)[i]);
-}
 __device__ __forceinline__ void store1(void *p, uint32_t type, uint64_t i, float x) {
     if (type == ARCQML_F32) static_cast<float *>(p)[i] = x;
     else if (type == ARCQML_BF16) static_cast<__nv_bfloat16 *>(p)[i] = to_element<__nv_bfloat16>(x);
@@ -346,6 +341,24 @@ template <int PHASE, uint32_t SIZE> __device__ __forceinline__ Tile tile_of(cons
     return r;
 }
 
+// Up to 32 elements, `pitch` apart: the result as it is, or the step with it. All are loaded before the first
+// is used.
+template <class T>
+__device__ __forceinline__ void finish(T *at, uint64_t pitch, uint32_t count, const Matrix &a, float rate, const float (&v)[32]) {
+    if (!a.momentum) {
+#pragma unroll
+        for (uint32_t q = 0; q < 32; ++q)
+            if (q < count) at[q * pitch] = to_element<T>(v[q] * rate);
+        return;
+    }
+    T p[32];
+#pragma unroll
+    for (uint32_t q = 0; q < 32; ++q) p[q] = at[min(q, count - 1) * pitch];
+#pragma unroll
+    for (uint32_t q = 0; q < 32; ++q)
+        if (q < count) at[q * pitch] = to_element<T>(fmaf(a.down, to_wide(p[q]), v[q] * rate));
+}
+
 // 32 neighbouring sums of a row, for each thread of a warp, become what the phase stores.
 template <int PHASE, bool SPLIT>
 __device__ __forceinline__ void take_sums(const Group &g, const Matrix &a, float (&v)[32], uint32_t row, uint32_t column,
@@ -401,22 +414,11 @@ __device__ __forceinline__ void take_sums(const Group &g, const Matrix &a, float
         // v[q]: element `at` + q * pitch
         const uint32_t along = a.flip ? column : row0, count = a.flip ? a.n - min(a.n, along) : a.m - min(a.m, along);
         const uint32_t pitch = a.flip ? a.m : a.n, mine = a.flip ? row : column + lane;
-        if (mine < pitch) {
+        if (mine < pitch && count) {
             const uint64_t at = uint64_t(along) * pitch + mine;
-            if (a.momentum) {
-                float p[32];
-#pragma unroll
-                for (uint32_t q = 0; q < 32; ++q)
-                    if (q < count) p[q] = load1(a.out, a.out_type, at + uint64_t(q) * pitch);
-#pragma unroll
-                for (uint32_t q = 0; q < 32; ++q) v[q] = fmaf(a.down, p[q], v[q] * rate);
-            } else {
-#pragma unroll
-                for (uint32_t q = 0; q < 32; ++q) v[q] *= rate;
-            }
-#pragma unroll
-            for (uint32_t q = 0; q < 32; ++q)
-                if (q < count) store1(a.out, a.out_type, at + uint64_t(q) * pitch, v[q]);
+            if (a.out_type == ARCQML_F32) finish(static_cast<float *>(a.out) + at, pitch, count, a, rate, v);
+            else if (a.out_type == ARCQML_BF16) finish(static_cast<__nv_bfloat16 *>(a.out) + at, pitch, count, a, rate, v);
+            else finish(static_cast<__half *>(a.out) + at, pitch, count, a, rate, v);
         }
         __syncwarp();
     }
