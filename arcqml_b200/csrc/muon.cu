@@ -140,6 +140,24 @@ __device__ __forceinline__ void update8(float (&u)[8], const Matrix &a, uint64_t
     for (int e = 0; e < 8; ++e) u[e] = a.beta * m[e] + a.keep * u[e];
 }
 
+// The momentum's update in memory, and u of 8 elements.
+__device__ __forceinline__ void new_update8(float (&u)[8], const Matrix &a, uint64_t i, uint32_t count) {
+    load8(u, a.in, a.in_type, i, count);
+    if (!a.momentum) return;
+    float m[8];
+    load8_as(m, a.momentum + i, count);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m[e] = a.beta * m[e] + a.keep * u[e];
+    store8_as(m, a.momentum + i, count);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) u[e] = a.nesterov ? a.beta * m[e] + a.keep * u[e] : m[e];
+}
+
+// |X| 2^shift lies in [1/2, 1]; a norm of zero, infinity or NaN has no shift.
+__device__ __forceinline__ int shift_of(double norm, double whole) {
+    return norm > 0.0 && norm < whole && whole < INFINITY ? max(0, ilogb(whole) - ilogb(norm) - 1) : 0;
+}
+
 // ------------------------------------------------------------------ the update and its norm
 
 // The sum over a block of kThreads, the same in every thread.
@@ -164,16 +182,8 @@ __global__ void __launch_bounds__(kThreads) k_update_squares(const __grid_consta
     for (uint64_t i = (uint64_t(blockIdx.x - g.first[k]) * kThreads + threadIdx.x) * 8; i < n;
          i += uint64_t(blocks) * kThreads * 8) {
         const uint32_t count = uint32_t(min(uint64_t(8), n - i));
-        float u[8], m[8];
-        load8(u, a.in, a.in_type, i, count);
-        if (a.momentum) {
-            load8_as(m, a.momentum + i, count);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) m[e] = a.beta * m[e] + a.keep * u[e];
-            store8_as(m, a.momentum + i, count);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) u[e] = a.nesterov ? a.beta * m[e] + a.keep * u[e] : m[e];
-        }
+        float u[8];
+        new_update8(u, a, i, count);
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum = fma(double(u[e]), double(u[e]), sum);
     }
@@ -236,8 +246,7 @@ template <bool SPLIT> __global__ void __launch_bounds__(kThreads) k_spread(const
     double sum = 0.0;
     for (uint32_t b = sums.first[k] + threadIdx.x; b < sums.first[k + 1]; b += kThreads) sum += g.sums[b];
     const double norm = sqrt(block_sum(sum)), whole = norm + g.eps;
-    // |X| 2^shift lies in [1/2, 1]; a norm of zero, infinity or NaN has no shift
-    const int shift = norm > 0.0 && norm < whole && whole < INFINITY ? max(0, ilogb(whole) - ilogb(norm) - 1) : 0;
+    const int shift = shift_of(norm, whole);
     if (block == 0 && threadIdx.x == 0) g.shift[k] = shift;
     const double factor = ldexp(double(kScaleX) / whole, shift);
     const uint32_t row0 = block / a.x_blocks * kRows, column0 = block % a.x_blocks * kDepth;
@@ -341,22 +350,58 @@ template <int PHASE, uint32_t SIZE> __device__ __forceinline__ Tile tile_of(cons
     return r;
 }
 
-// Up to 32 elements, `pitch` apart: the result as it is, or the step with it. All are loaded before the first
+// Up to N elements, `pitch` apart: the result as it is, or the step with it. All are loaded before the first
 // is used.
-template <class T>
-__device__ __forceinline__ void finish(T *at, uint64_t pitch, uint32_t count, const Matrix &a, float rate, const float (&v)[32]) {
+template <class T, int N>
+__device__ __forceinline__ void finish(T *at, uint64_t pitch, uint32_t count, const Matrix &a, float rate, const float (&v)[N]) {
     if (!a.momentum) {
 #pragma unroll
-        for (uint32_t q = 0; q < 32; ++q)
+        for (uint32_t q = 0; q < N; ++q)
             if (q < count) at[q * pitch] = to_element<T>(v[q] * rate);
         return;
     }
-    T p[32];
+    T p[N];
 #pragma unroll
-    for (uint32_t q = 0; q < 32; ++q) p[q] = at[min(q, count - 1) * pitch];
+    for (uint32_t q = 0; q < N; ++q) p[q] = at[min(q, count - 1) * pitch];
 #pragma unroll
-    for (uint32_t q = 0; q < 32; ++q)
+    for (uint32_t q = 0; q < N; ++q)
         if (q < count) at[q * pitch] = to_element<T>(fmaf(a.down, to_wide(p[q]), v[q] * rate));
+}
+
+// N neighbouring values of X's row for each thread of a warp, stored 2^shift kScaleX times as large as they
+// are, go out. Rows of the matrix are turned in shared memory (`square`), so that neighbouring lanes have
+// neighbouring elements; X's rows are the columns of a flipped matrix and lie that way already.
+template <int N>
+__device__ __forceinline__ void give_result(const Matrix &a, float (&v)[N], uint32_t row, uint32_t column, int shift,
+                                            float *square) {
+    constexpr uint32_t ROWS = 32 / N; // of the matrix side by side
+    const float rate = ldexpf(a.momentum ? -a.rate / kScaleX : 1.0f / kScaleX, -shift);
+    const uint32_t lane = threadIdx.x & 31;
+    uint32_t along, mine, step; // v[q] belongs to place (along + q step, mine) of rows of `pitch`
+    const uint32_t pitch = a.flip ? a.m : a.n, rows = a.flip ? a.n : a.m;
+    if (a.flip) {
+        along = column;
+        mine = row;
+        step = 1;
+    } else {
+        __syncwarp();
+#pragma unroll
+        for (uint32_t q = 0; q < N; ++q) square[lane * (N + 1) + q] = v[q];
+        __syncwarp();
+#pragma unroll
+        for (uint32_t q = 0; q < N; ++q) v[q] = square[(q * ROWS + lane / N) * (N + 1) + lane % N];
+        along = row - lane + lane / N;
+        mine = column + lane % N;
+        step = ROWS;
+    }
+    if (mine < pitch && along < rows) {
+        const uint32_t count = (rows - along + step - 1) / step;
+        const uint64_t at = uint64_t(along) * pitch + mine, apart = uint64_t(step) * pitch;
+        if (a.out_type == ARCQML_F32) finish(static_cast<float *>(a.out) + at, apart, count, a, rate, v);
+        else if (a.out_type == ARCQML_BF16) finish(static_cast<__nv_bfloat16 *>(a.out) + at, apart, count, a, rate, v);
+        else finish(static_cast<__half *>(a.out) + at, apart, count, a, rate, v);
+    }
+    __syncwarp();
 }
 
 // 32 neighbouring sums of a row, for each thread of a warp, become what the phase stores.
@@ -400,28 +445,7 @@ __device__ __forceinline__ void take_sums(const Group &g, const Matrix &a, float
             }
         }
     }
-    if (PHASE == APPLY && last) {
-        const float rate = ldexpf(a.momentum ? -a.rate / kScaleX : 1.0f / kScaleX, -next);
-        const uint32_t row0 = row - lane;
-        if (!a.flip) { // turned in shared memory, so that neighbouring lanes have neighbouring elements
-            __syncwarp();
-#pragma unroll
-            for (uint32_t q = 0; q < 32; ++q) square[lane * 33 + q] = v[q];
-            __syncwarp();
-#pragma unroll
-            for (uint32_t q = 0; q < 32; ++q) v[q] = square[q * 33 + lane];
-        }
-        // v[q]: element `at` + q * pitch
-        const uint32_t along = a.flip ? column : row0, count = a.flip ? a.n - min(a.n, along) : a.m - min(a.m, along);
-        const uint32_t pitch = a.flip ? a.m : a.n, mine = a.flip ? row : column + lane;
-        if (mine < pitch && count) {
-            const uint64_t at = uint64_t(along) * pitch + mine;
-            if (a.out_type == ARCQML_F32) finish(static_cast<float *>(a.out) + at, pitch, count, a, rate, v);
-            else if (a.out_type == ARCQML_BF16) finish(static_cast<__nv_bfloat16 *>(a.out) + at, pitch, count, a, rate, v);
-            else finish(static_cast<__half *>(a.out) + at, pitch, count, a, rate, v);
-        }
-        __syncwarp();
-    }
+    if (PHASE == APPLY && last) give_result(a, v, row, column, next, square);
 }
 
 // One phase for all matrices of a group: D = L R^T in tiles of 128 CG x 128 CG, a pair of blocks a tile with
@@ -642,6 +666,161 @@ __global__ void __launch_bounds__(kThreads) k_check_fault(const __grid_constant_
     }
 }
 
+// ------------------------------------------------------------------ small matrices
+
+// A matrix of at most 128 rows of X whose operands fit into a block's shared memory is orthogonalised by
+// that block from its update to its result: one launch for a list, 15 rounds of a few hundred cycles each.
+constexpr uint32_t kSmallThreads = 256;
+template <bool SPLIT> constexpr uint32_t kSmallBlocks = SPLIT ? 4 : 8; // of X: 256 or 512 columns
+template <bool SPLIT> constexpr uint32_t kSmallShared =
+    1024 + (kSmallBlocks<SPLIT> + 2) * (SPLIT ? 2 : 1) * kBlock + 256 + kSmallThreads / 32 * 32 * 17 * sizeof(float);
+
+struct SmallState {
+    uint64_t done;
+    uint32_t tmem, stop;
+};
+
+__device__ __forceinline__ void shared_writes_to_tensor_cores() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+template <bool SPLIT> __global__ void __launch_bounds__(kSmallThreads, 1)
+    k_small(const __grid_constant__ Group g, int steps) {
+    constexpr uint32_t LOW = kSmallBlocks<SPLIT> * kBlock; // X's low parts behind its high ones
+    extern __shared__ char raw[];
+    char *x = raw + (1024 - (tc::shared_address(raw) & 1023)) % 1024;
+    char *p = x + LOW * (SPLIT ? 2 : 1); // A, then P; low parts 2 blocks behind
+    SmallState &st = *reinterpret_cast<SmallState *>(p + 2 * kBlock * (SPLIT ? 2 : 1));
+    const Matrix &a = g.matrix[blockIdx.x];
+    const uint32_t thread = threadIdx.x, warp = thread / 32, lane = thread % 32;
+    float *square = reinterpret_cast<float *>(reinterpret_cast<char *>(&st) + 256) + warp * 32 * 17;
+    if (thread == 0) {
+        tc::barrier_init(&st.done, 1);
+        st.stop = 0;
+        tc::barrier_init_fence();
+    }
+    if (warp == 1) tc::tmem_alloc<1>(&st.tmem, 512);
+    tc::fence_before();
+
+    // the update, its norm, and X
+    const uint64_t all = uint64_t(a.m) * a.n;
+    double sum = 0.0;
+    for (uint64_t i = thread * 8; i < all; i += kSmallThreads * 8) {
+        const uint32_t count = uint32_t(min(uint64_t(8), all - i));
+        float u[8];
+        new_update8(u, a, i, count);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = fma(double(u[e]), double(u[e]), sum);
+    }
+    const uint32_t m16 = (a.m + 15) / 16 * 16, n16 = (a.n + 15) / 16 * 16, used = (a.n + kDepth - 1) / kDepth * kBlock;
+    for (uint32_t i = thread * 16; i < used; i += kSmallThreads * 16) {
+        *reinterpret_cast<uint4 *>(x + i) = make_uint4(0, 0, 0, 0);
+        if constexpr (SPLIT) *reinterpret_cast<uint4 *>(x + LOW + i) = make_uint4(0, 0, 0, 0);
+    }
+    const double norm = sqrt(block_sum(sum)), whole = norm + g.eps; // (and a barrier)
+    int shift = shift_of(norm, whole);
+    const double factor = ldexp(double(kScaleX) / whole, shift);
+    const uint32_t pitch = a.flip ? a.m : a.n;
+    for (uint64_t i = thread * 8; i < all; i += kSmallThreads * 8) {
+        const uint32_t count = uint32_t(min(uint64_t(8), all - i));
+        float u[8];
+        update8(u, a, i, count);
+        uint32_t r = uint32_t(i / pitch), c = uint32_t(i % pitch);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (uint32_t(e) < count) {
+                const uint32_t row = a.flip ? c : r, column = a.flip ? r : c;
+                char *at = x + place_of(row, column, kSmallBlocks<SPLIT>) + column % 8 * 2;
+                const float v = float(double(u[e]) * factor);
+                const __half h = __float2half_rn(v);
+                *reinterpret_cast<__half *>(at) = h;
+                if constexpr (SPLIT) *reinterpret_cast<__half *>(at + LOW) = __float2half_rn(v - __half2float(h));
+            }
+            if (++c == pitch) c = 0, ++r;
+        }
+    }
+    shared_writes_to_tensor_cores();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = st.tmem, mine = tmem + ((warp & 3) * 32 << 16), row = (warp & 3) * 32 + lane;
+    const uint32_t x_at = tc::shared_address(x), p_at = tc::shared_address(p);
+    uint32_t parity = 0;
+    bool broken = false;
+    // steps of 16 of the depth; operands by depth, or the right one by width
+    const auto multiply = [&](uint32_t sums, uint32_t left, uint32_t left_low, uint32_t right, uint32_t right_low,
+                              uint32_t depth, uint32_t columns, bool by_width) {
+        const uint32_t instr = tc::instruction(128, columns, by_width);
+        for (uint32_t k = 0; k < depth / 16; ++k) {
+            const uint32_t by_depth = k / 4 * kBlock + k % 4 * 32, along = by_width ? k * 2048 : by_depth;
+            const uint32_t apart = by_width ? kBlock : 16;
+            tc::mma<1>(sums, tc::descriptor(left + by_depth, 16), tc::descriptor(right + along, apart), instr, k != 0);
+            if constexpr (SPLIT) {
+                tc::mma<1>(sums, tc::descriptor(left + by_depth, 16), tc::descriptor(right_low + along, apart), instr, true);
+                tc::mma<1>(sums, tc::descriptor(left_low + by_depth, 16), tc::descriptor(right + along, apart), instr, true);
+            }
+        }
+    };
+    const auto sums_ready = [&] {
+        const bool ok = wait_for(&st.done, parity, &st.stop);
+        parity ^= 1;
+        broken = __syncthreads_or(!ok);
+        tc::fence_after();
+        return !broken;
+    };
+    const auto operands_ready = [&] {
+        shared_writes_to_tensor_cores();
+        tc::fence_before();
+        __syncthreads();
+        tc::fence_after();
+    };
+    for (int step = 0; step < steps; ++step) {
+        const int next = max(0, shift - 2);
+        for (int phase = GRAM; phase <= APPLY; ++phase) {
+            const uint32_t columns = phase == APPLY ? n16 : m16;
+            if (thread == 0) {
+                if (phase == GRAM) multiply(tmem, x_at, x_at + LOW, x_at, x_at + LOW, n16, m16, false);
+                else if (phase == POLYNOMIAL) multiply(tmem, p_at, p_at + 2 * kBlock, p_at, p_at + 2 * kBlock, m16, m16, false);
+                else
+                    for (uint32_t c = 0; c < n16; c += 256)
+                        multiply(tmem + c, p_at, p_at + 2 * kBlock, x_at + c / kDepth * kBlock, x_at + LOW + c / kDepth * kBlock,
+                                 m16, min(256u, n16 - c), true);
+                tc::commit<1>(&st.done);
+            }
+            if (!sums_ready()) break;
+            const float of_sum = phase == GRAM         ? 1.0f / kScaleX
+                                 : phase == POLYNOMIAL ? ldexpf(0.5f * kC / kScaleX, -4 * shift)
+                                                       : ldexpf(2.0f / kScaleX, next - shift);
+            const float of_old = phase == GRAM ? 0.0f : phase == POLYNOMIAL ? ldexpf(0.5f * kB, -2 * shift) : ldexpf(kA, next - shift);
+            char *to = phase == APPLY ? x : p;
+            const uint64_t low = phase == APPLY ? LOW : 2 * kBlock;
+            const uint32_t across = phase == APPLY ? kSmallBlocks<SPLIT> : 2;
+#pragma unroll 1
+            for (uint32_t c = warp / 4 * 16; c < columns; c += 32) {
+                float v[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) v[e] = 0.0f;
+                tc::tmem_add(v, mine + c);
+#pragma unroll
+                for (uint32_t q = 0; q < 16; q += 8) {
+                    char *at = to + place_of(row, c + q, across);
+                    float y[8];
+                    if (phase != GRAM) load_operand<SPLIT>(y, at, low);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        y[e] = v[q + e] = phase == GRAM ? v[q + e] * of_sum : of_old * y[e] + v[q + e] * of_sum;
+                    store_operand<SPLIT>(at, low, y);
+                }
+                if (phase == APPLY && step + 1 == steps) give_result(a, v, row, c, next, square);
+            }
+            operands_ready();
+        }
+        if (broken) break;
+        shift = next;
+    }
+    if (broken)
+        for (uint64_t i = thread; i < all; i += kSmallThreads) store1(a.out, a.out_type, i, __int_as_float(0x7fffffff));
+    __syncthreads();
+    if (warp == 1) tc::tmem_free<1>(tmem, 512);
+}
+
 // ------------------------------------------------------------------ host
 
 [[noreturn]] void refuse(const char *list, size_t i, const char *why) {
@@ -707,6 +886,12 @@ bool is_split(uint32_t type) { return type != ARCQML_BF16; }
 constexpr size_t kHeadBytes = 512; // the fault, and from 256 on the shifts
 size_t sums_bytes() { return size_t(kMatrices) * kSumBlocks * sizeof(double); }
 
+// Matrices that one block takes whole.
+bool is_small(const ArcqmlMatrix &a, bool split) {
+    const uint64_t m = std::min(a.rows, a.columns), n = std::max(a.rows, a.columns);
+    return m <= kRows && n <= (split ? kSmallBlocks<true> : kSmallBlocks<false>) * kDepth;
+}
+
 // Scratch bytes of a matrix's X (twice), A and P.
 uint64_t operand_bytes(const ArcqmlMatrix &a, bool split) {
     const uint64_t m = std::min(a.rows, a.columns), n = std::max(a.rows, a.columns);
@@ -720,16 +905,17 @@ constexpr uint64_t kGroupBytes = uint64_t(2) << 30;
 template <class F>
 void for_groups(const ArcqmlMatrix *list, const ArcqmlMatrix *kinds, size_t count, uint64_t most, F &&f) {
     std::vector<size_t> members;
-    for (int split = 1; split >= 0; --split) {
+    for (int kind = 0; kind < 4; ++kind) {
+        const bool split = kind & 1, small = kind & 2;
         uint64_t bytes = 0;
         const auto flush = [&] {
-            if (!members.empty()) f(members, bytes, split != 0);
+            if (!members.empty()) f(members, bytes, split, small);
             members.clear();
             bytes = 0;
         };
         for (size_t i = 0; i < count; ++i) {
-            if (!present(list[i]) || is_split(kinds[i].dtype) != (split != 0)) continue;
-            const uint64_t need = operand_bytes(list[i], split != 0);
+            if (!present(list[i]) || is_split(kinds[i].dtype) != split || is_small(list[i], split) != small) continue;
+            const uint64_t need = small ? 0 : operand_bytes(list[i], split);
             if (members.size() == kMatrices || (bytes && bytes + need > most)) flush();
             members.push_back(i);
             bytes += need;
@@ -738,17 +924,20 @@ void for_groups(const ArcqmlMatrix *list, const ArcqmlMatrix *kinds, size_t coun
     }
 }
 
-template <int PHASE, bool SPLIT, int CG>
-void product(Group &g, uint32_t tiles, uint32_t step, bool last, cudaStream_t s) {
-    static std::atomic<uint64_t> set{0}; // the devices on which the kernel may have that much shared memory
+// Lets a kernel have `bytes` of shared memory, once on each device.
+template <auto KERNEL> void allow_shared(uint32_t bytes) {
+    static std::atomic<uint64_t> set{0};
     int device = 0;
     check_cuda(cudaGetDevice(&device), "cudaGetDevice");
-    if (device >= 64 || !(set.load() >> device & 1)) {
-        check_cuda(cudaFuncSetAttribute(k_product<PHASE, SPLIT, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        int(kProductShared<SPLIT>)),
-                   "orthogonalisation kernel attribute");
-        if (device < 64) set |= uint64_t(1) << device;
-    }
+    if (device < 64 && (set.load() >> device & 1)) return;
+    check_cuda(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)),
+               "orthogonalisation kernel attribute");
+    if (device < 64) set |= uint64_t(1) << device;
+}
+
+template <int PHASE, bool SPLIT, int CG>
+void product(Group &g, uint32_t tiles, uint32_t step, bool last, cudaStream_t s) {
+    allow_shared<k_product<PHASE, SPLIT, CG>>(kProductShared<SPLIT>);
     start(k_product<PHASE, SPLIT, CG>, std::min(tiles * CG, kSMs), kProductThreads, CG, kProductShared<SPLIT>, true, 0.0, s, g,
           step, uint32_t(last));
 }
@@ -829,12 +1018,17 @@ template <bool SPLIT> void run_group(Group &g, int steps, cudaStream_t s) {
     start(k_check_fault, 8, kThreads, 1, 0, true, 0.0, s, g);
 }
 
+template <bool SPLIT> void run_small(Group &g, int steps, cudaStream_t s) {
+    allow_shared<k_small<SPLIT>>(kSmallShared<SPLIT>);
+    start(k_small<SPLIT>, g.count, kSmallThreads, 1, kSmallShared<SPLIT>, false, 0.0, s, g, steps);
+}
+
 // fill(matrix, place) sets what the call does to a place of the list.
 template <class F>
 void run(const ArcqmlMatrix *list, const ArcqmlMatrix *kinds, size_t count, int steps, double eps, double *ws, size_t ws_len,
          cudaStream_t s, F &&fill) {
     const uint64_t have = ws_len * sizeof(double), head = kHeadBytes + sums_bytes();
-    for_groups(list, kinds, count, have > head ? have - head : 0, [&](const std::vector<size_t> &members, uint64_t, bool split) {
+    for_groups(list, kinds, count, have > head ? have - head : 0, [&](const std::vector<size_t> &members, uint64_t, bool split, bool small) {
         static thread_local Group g;
         g.count = uint32_t(members.size());
         g.scratch = reinterpret_cast<char *>(ws);
@@ -851,7 +1045,9 @@ void run(const ArcqmlMatrix *list, const ArcqmlMatrix *kinds, size_t count, int 
             m.n = uint32_t(std::max(a.rows, a.columns));
             fill(m, members[i]);
         }
-        if (split) run_group<true>(g, steps, s);
+        if (small && split) run_small<true>(g, steps, s);
+        else if (small) run_small<false>(g, steps, s);
+        else if (split) run_group<true>(g, steps, s);
         else run_group<false>(g, steps, s);
     });
 }
@@ -867,7 +1063,7 @@ size_t orthogonalize_workspace(const ArcqmlMatrix *list, size_t count) {
     if (!list) return 0;
     uint64_t most = 0;
     for_groups(list, list, count, kGroupBytes,
-               [&](const std::vector<size_t> &, uint64_t bytes, bool) { most = std::max(most, bytes); });
+               [&](const std::vector<size_t> &, uint64_t bytes, bool, bool) { most = std::max(most, bytes); });
     return most ? size_t((kHeadBytes + sums_bytes() + most) / sizeof(double)) : 0;
 }
 
