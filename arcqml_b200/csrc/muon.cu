@@ -46,6 +46,7 @@ constexpr uint32_t kSumBlocks = 148 * 8; // partial sums of a matrix, at most
 constexpr uint32_t kRows = 128, kDepth = 64;         // of a block
 constexpr uint32_t kBlock = kRows * kDepth * 2;      // bytes
 constexpr uint32_t kSMs = 148;
+constexpr uint32_t kTakers = 8; // warps that take sums out: each has a quarter of the rows, half of the columns
 
 // One matrix of a launch. The update u is the matrix `in`, or follows from the momentum and the gradient.
 struct Matrix {
@@ -62,16 +63,20 @@ struct Matrix {
 
 struct Group {
     Matrix matrix[kMatrices];
-    uint32_t first[kMatrices + 1]; // of the launch's blocks or tiles
+    uint32_t first[kMatrices + 1]; // of the launch's blocks or tiles, by place
+    uint8_t order[kMatrices];      // the matrix at each place
     uint32_t count;
     char *scratch;
-    uint32_t *fault; // set by a wait that ran out
+    uint32_t *fault;   // set by a wait that ran out
+    uint32_t *arrived; // parts of a tile that are done, for each warp of the units that begin one
+    float *partial;
     int *shift;      // of each matrix: X is stored 2^shift times as large at first
     double *sums;
     double eps;
 };
 
-__device__ __forceinline__ uint32_t matrix_of(const Group &g, uint32_t c) {
+// The place of the matrix that has the launch's block or tile c.
+__device__ __forceinline__ uint32_t place_with(const Group &g, uint32_t c) {
     uint32_t lo = 0, hi = g.count;
     while (hi - lo > 1) {
         const uint32_t mid = (lo + hi) / 2;
@@ -174,8 +179,11 @@ __device__ __forceinline__ double block_sum(double v) {
 // The momentum's update, and the squares of u: an f64 sum for each block.
 __global__ void __launch_bounds__(kThreads) k_update_squares(const __grid_constant__ Group g) {
     cudaTriggerProgrammaticLaunchCompletion();
-    if (blockIdx.x == 0 && threadIdx.x == 0) *g.fault = 0;
-    const uint32_t k = matrix_of(g, blockIdx.x), blocks = g.first[k + 1] - g.first[k];
+    if (blockIdx.x == 0) {
+        if (threadIdx.x == 0) *g.fault = 0;
+        for (uint32_t i = threadIdx.x; i < kSMs * kTakers * 2; i += kThreads) g.arrived[i] = 0;
+    }
+    const uint32_t k = place_with(g, blockIdx.x), blocks = g.first[k + 1] - g.first[k];
     const Matrix &a = g.matrix[k];
     const uint64_t n = uint64_t(a.m) * a.n;
     double sum = 0.0;
@@ -240,7 +248,7 @@ template <bool SPLIT> __global__ void __launch_bounds__(kThreads) k_spread(const
                                                                            const __grid_constant__ Group sums) {
     __shared__ float turned[kDepth][kRows + 1];
     cudaTriggerProgrammaticLaunchCompletion();
-    const uint32_t k = matrix_of(g, blockIdx.x), block = blockIdx.x - g.first[k];
+    const uint32_t k = place_with(g, blockIdx.x), block = blockIdx.x - g.first[k];
     const Matrix &a = g.matrix[k];
     cudaGridDependencySynchronize();
     double sum = 0.0;
@@ -289,7 +297,6 @@ template <bool SPLIT> __global__ void __launch_bounds__(kThreads) k_spread(const
 
 enum Phase { GRAM, POLYNOMIAL, APPLY };
 constexpr uint32_t kStageBytes = 32768; // one depth of 64: 128 rows of the left operand, 128 of the right
-constexpr uint32_t kTakers = 8; // warps that take sums out: each has a quarter of the rows, half of the columns
 constexpr uint32_t kProductThreads = 128 + kTakers * 32;
 
 // Stages of a block: 192 KB of operands. Behind them a square of 32 x 32 for each taker.
@@ -325,13 +332,14 @@ __device__ __forceinline__ bool wait_for(uint64_t *b, uint32_t parity, uint32_t 
 // The tile t of a phase.
 struct Tile {
     const Matrix *a;
-    uint32_t index, i, j, depth; // rows and columns in tiles; steps of 64 of the depth
+    uint32_t index, i, j; // rows and columns in tiles
 };
 template <int PHASE, uint32_t SIZE> __device__ __forceinline__ Tile tile_of(const Group &g, uint32_t t) {
     Tile r;
-    r.index = matrix_of(g, t);
+    const uint32_t place = place_with(g, t);
+    r.index = g.order[place];
     r.a = &g.matrix[r.index];
-    t -= g.first[r.index];
+    t -= g.first[place];
     if constexpr (PHASE == APPLY) {
         const uint32_t across = (r.a->n + SIZE - 1) / SIZE;
         r.i = t / across;
@@ -346,9 +354,73 @@ template <int PHASE, uint32_t SIZE> __device__ __forceinline__ Tile tile_of(cons
         }
         r.j = r.i + t;
     }
-    r.depth = ((PHASE == GRAM ? r.a->n : r.a->m) + kDepth - 1) / kDepth;
     return r;
 }
+
+// Who does which tile. Units (blocks, or pairs of them) take the tiles of each depth, deepest first, in whole
+// rounds: neighbouring tiles at a time, which share their operands in L2. The steps that are left of all depths
+// are cut into equal runs, one for each unit. Cuts move to the next tile's edge, or (where it is worth what
+// it costs, see product()) go through a tile, which the unit that finishes last then sums up in the order of
+// its depth.
+struct Plan {
+    uint32_t classes; // of depth
+    uint32_t tile[kMatrices + 1], rounds[kMatrices], depth[kMatrices];
+    uint32_t left[kMatrices + 1]; // steps left before the class; a tile counts for kLeast of them at least
+    uint32_t runs;                // units that share the steps left
+    uint32_t snap;                // a cut this near to a tile's edge moves there
+};
+
+constexpr uint32_t kLeast = 16; // taking a tile's sums out takes as long
+__host__ __device__ inline uint32_t weight(uint32_t depth) { return depth > kLeast ? depth : kLeast; }
+
+// The class that step `at` of those left belongs to.
+__host__ __device__ inline uint32_t class_of(const Plan &p, uint32_t at) {
+    uint32_t c = 0;
+    while (p.left[c + 1] <= at) ++c;
+    return c;
+}
+// Where the unit's run of the steps left begins.
+__host__ __device__ inline uint32_t cut(const Plan &p, uint32_t unit) {
+    const uint32_t all = p.left[p.classes];
+    if (unit >= p.runs) return all;
+    const uint32_t at = uint32_t(uint64_t(unit) * all / p.runs);
+    if (at == 0) return 0;
+    const uint32_t c = class_of(p, at), w = weight(p.depth[c]), past = (at - p.left[c]) % w, behind = w - past;
+    return past < p.snap && past < behind          ? at - past
+           : past < p.snap || past + p.snap > p.depth[c] || past + p.snap < past ? at + behind
+                                                                                 : at;
+}
+struct Part {
+    uint32_t tile, begin, end, depth; // steps of the tile's depth
+    uint32_t start;                   // the tile's first step among those left
+    __device__ __forceinline__ bool whole() const { return begin == 0 && end == depth; }
+};
+struct Walk {
+    const Plan &p;
+    uint32_t unit, units, c = 0, round = 0, at, end;
+    __device__ __forceinline__ Walk(const Plan &plan, uint32_t u, uint32_t n) : p(plan), unit(u), units(n) {
+        at = cut(p, unit);
+        end = cut(p, unit + 1);
+    }
+    __device__ __forceinline__ bool next(Part &r) {
+        for (; c < p.classes; ++c, round = 0)
+            if (round < p.rounds[c]) {
+                r.tile = p.tile[c] + round++ * units + unit;
+                r.begin = 0;
+                r.end = r.depth = p.depth[c];
+                return true;
+            }
+        if (at >= end) return false;
+        const uint32_t k = class_of(p, at), w = weight(p.depth[k]), n = (at - p.left[k]) / w;
+        r.depth = p.depth[k];
+        r.start = p.left[k] + n * w;
+        r.tile = p.tile[k] + p.rounds[k] * units + n;
+        r.begin = at - r.start;
+        r.end = min(r.depth, end - r.start);
+        at = r.start + (r.end == r.depth ? w : r.end);
+        return true;
+    }
+};
 
 // Up to N elements, `pitch` apart: the result as it is, or the step with it. All are loaded before the first
 // is used.
@@ -452,7 +524,7 @@ __device__ __forceinline__ void take_sums(const Group &g, const Matrix &a, float
 // CG = 2 (each has half of the tile's rows, and brings half of the right operand's).
 template <int PHASE, bool SPLIT, int CG>
 __global__ void __launch_bounds__(kProductThreads, 1)
-    k_product(const __grid_constant__ Group g, uint32_t step, uint32_t last) {
+    k_product(const __grid_constant__ Group g, const __grid_constant__ Plan plan, uint32_t step, uint32_t last) {
     constexpr uint32_t SIZE = kRows * CG, S = kStages<SPLIT>, STAGE = kStageBytes * (SPLIT ? 2 : 1);
     extern __shared__ char raw[];
     char *shared = raw + (1024 - (tc::shared_address(raw) & 1023)) % 1024;
@@ -480,7 +552,9 @@ __global__ void __launch_bounds__(kProductThreads, 1)
     cudaTriggerProgrammaticLaunchCompletion();
     cudaGridDependencySynchronize();
     const uint32_t tmem = st.tmem;
-    const uint32_t units = gridDim.x / CG, unit = blockIdx.x / CG, tiles = g.first[g.count];
+    const uint32_t units = gridDim.x / CG, unit = blockIdx.x / CG;
+    Walk walk(plan, unit, units);
+    Part part;
     const bool broken = *reinterpret_cast<volatile uint32_t *>(g.fault) != 0;
 
     // the sums of a tile in registers take more of them than a thread's share: 384 x 168 registers as
@@ -490,8 +564,8 @@ __global__ void __launch_bounds__(kProductThreads, 1)
     if (warp == 0 && lane == 0 && !broken) { // copies operands in
         uint32_t at = 0, phase = 0;
         bool on = true;
-        for (uint32_t t = unit; t < tiles && on; t += units) {
-            const Tile tile = tile_of<PHASE, SIZE>(g, t);
+        while (on && walk.next(part)) {
+            const Tile tile = tile_of<PHASE, SIZE>(g, part.tile);
             const Matrix &a = *tile.a;
             const uint32_t left = tile.i * CG + rank, right = tile.j * CG + rank;
             const uint32_t left_across = PHASE == GRAM ? a.x_blocks : a.a_blocks;
@@ -505,7 +579,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
             const uint32_t wide = PHASE == APPLY ? min(2u, a.x_blocks - min(a.x_blocks, right * 2)) : 0;
             const bool has_right = right < a.down_blocks;
             const uint32_t bytes = parts * ((has_left ? kBlock : 0) + (PHASE == APPLY ? wide * (kBlock / 2) : has_right ? kBlock : 0));
-            for (uint32_t d = 0; d < tile.depth; ++d) {
+            for (uint32_t d = part.begin; d < part.end; ++d) {
                 if (!(on = wait_for(&st.empty[at], phase ^ 1, &st.stop))) break;
                 char *to = shared + at * STAGE;
                 tc::barrier_expect(&st.full[at], bytes);
@@ -537,10 +611,9 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         constexpr uint32_t STEP = PHASE == APPLY ? 2048 / 16 : 32 / 16; // of the right operand, 16 of depth
         uint32_t at = 0, phase = 0, n = 0;
         bool on = true;
-        for (uint32_t t = unit; t < tiles && on; t += units) {
-            const uint32_t depth = tile_of<PHASE, SIZE>(g, t).depth;
-            for (uint32_t d = 0; d < depth && on; ++n) {
-                const uint32_t half = n & 1, end = min(depth - d, kChain<SPLIT>) + d;
+        while (on && walk.next(part)) {
+            for (uint32_t d = part.begin; d < part.end && on; ++n) {
+                const uint32_t half = n & 1, end = min(part.end - d, kChain<SPLIT>) + d;
                 if (!(on = wait_for(&st.taken[half], (n >> 1 & 1) ^ 1, &st.stop))) break;
                 tc::fence_after();
                 const uint32_t sums = tmem + half * SIZE;
@@ -571,9 +644,8 @@ __global__ void __launch_bounds__(kProductThreads, 1)
     } else if (CG == 2 && warp == 2 && rank == 1 && lane == 0 && !broken) { // tells the first block of its operands
         uint32_t at = 0, phase = 0;
         bool on = true;
-        for (uint32_t t = unit; t < tiles && on; t += units) {
-            const uint32_t depth = tile_of<PHASE, SIZE>(g, t).depth;
-            for (uint32_t d = 0; d < depth; ++d) {
+        while (on && walk.next(part)) {
+            for (uint32_t d = part.begin; d < part.end; ++d) {
                 if (!(on = wait_for(&st.full[at], phase, &st.stop))) break;
                 tc::barrier_arrive_at(tc::in_block(&st.peer[at], 0));
                 if (++at == S) at = 0, phase ^= 1;
@@ -599,8 +671,12 @@ __global__ void __launch_bounds__(kProductThreads, 1)
             tc::fence_after();
             return on;
         };
-        for (uint32_t t = unit; t < tiles && on; t += units) {
-            const Tile tile = tile_of<PHASE, SIZE>(g, t);
+        const uint32_t from = walk.at, writer = rank * kTakers + warp - 4;
+        const auto slice = [&](uint32_t u, uint32_t slot) { // of a unit's parts: 0 of a tile that began earlier
+            return reinterpret_cast<float4 *>(g.partial) + ((uint64_t(u) * 2 + slot) * (kTakers * CG) + writer) * (COLUMNS * 8) + lane;
+        };
+        while (on && walk.next(part)) {
+            const Tile tile = tile_of<PHASE, SIZE>(g, part.tile);
             const Matrix &a = *tile.a;
             const uint32_t row = tile.i * SIZE + rank * kRows + quarter * 32 + lane;
             const uint32_t lanes = quarter * 32 << 16;
@@ -609,12 +685,14 @@ __global__ void __launch_bounds__(kProductThreads, 1)
                 take_sums<PHASE, SPLIT>(g, a, v, row, tile.j * SIZE + first + c, tile.i != tile.j, shift, current, last != 0,
                                         square);
             };
+            const bool whole = part.whole();
+            float4 *mine = whole ? nullptr : slice(unit, part.start < from ? 0 : 1);
             if constexpr (SPLIT) {
                 float sum[COLUMNS];
 #pragma unroll
                 for (uint32_t c = 0; c < COLUMNS; ++c) sum[c] = 0.0f;
 #pragma unroll 1
-                for (uint32_t d = 0; d < tile.depth; d += kChain<SPLIT>, ++n) {
+                for (uint32_t d = part.begin; d < part.end; d += kChain<SPLIT>, ++n) {
                     const uint32_t half = n & 1;
                     if (!wait_done(half)) break;
 #pragma unroll
@@ -622,13 +700,18 @@ __global__ void __launch_bounds__(kProductThreads, 1)
                     release(half);
                 }
                 if (!on) break;
+                if (whole) {
 #pragma unroll
-                for (uint32_t c = 0; c < COLUMNS; c += 32) {
-                    float v[32];
+                    for (uint32_t c = 0; c < COLUMNS; c += 32) {
+                        float v[32];
 #pragma unroll
-                    for (uint32_t e = 0; e < 32; ++e) v[e] = sum[c + e];
-                    take(v, c);
+                        for (uint32_t e = 0; e < 32; ++e) v[e] = sum[c + e];
+                        take(v, c);
+                    }
+                    continue;
                 }
+#pragma unroll
+                for (uint32_t c = 0; c < COLUMNS; c += 4) mine[c * 8] = make_float4(sum[c], sum[c + 1], sum[c + 2], sum[c + 3]);
             } else {
                 const uint32_t half = n & 1;
                 if (!wait_done(half)) break;
@@ -637,10 +720,51 @@ __global__ void __launch_bounds__(kProductThreads, 1)
                     float v[32];
                     __syncwarp();
                     tc::tmem_load(v, tmem + half * SIZE + lanes + first + c);
-                    take(v, c);
+                    if (whole) {
+                        take(v, c);
+                    } else {
+#pragma unroll
+                        for (uint32_t e = 0; e < 32; e += 4)
+                            mine[(c + e) * 8] = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                    }
                 }
                 release(half);
                 ++n;
+                if (whole) continue;
+            }
+            // a part: the warp that brings its rows and columns' last one puts them together
+            uint32_t u0 = uint32_t(uint64_t(part.start) * plan.runs / plan.left[plan.classes]); // has the tile's first step
+            while (cut(plan, u0) > part.start) --u0;
+            while (cut(plan, u0 + 1) <= part.start) ++u0;
+            uint32_t parts = 1;
+            while (cut(plan, u0 + parts) < part.start + part.depth) ++parts;
+            __threadfence();
+            __syncwarp();
+            uint32_t before = 0;
+            if (lane == 0) before = atomicAdd(&g.arrived[u0 * (kTakers * 2) + writer], 1u);
+            if (__shfl_sync(0xffffffffu, before, 0) + 1 != parts) continue;
+            if (lane == 0) g.arrived[u0 * (kTakers * 2) + writer] = 0;
+            __threadfence();
+#pragma unroll 1
+            for (uint32_t c = 0; c < COLUMNS; c += 32) {
+                float v[32];
+#pragma unroll
+                for (uint32_t e = 0; e < 32; ++e) v[e] = 0.0f;
+#pragma unroll 2
+                for (uint32_t u = 0; u < parts; ++u) {
+                    const float4 *from = slice(u0 + u, u ? 0 : 1) + c * 8;
+                    float4 w[8];
+#pragma unroll
+                    for (uint32_t e = 0; e < 8; ++e) w[e] = __ldcg(from + e * 32);
+#pragma unroll
+                    for (uint32_t e = 0; e < 8; ++e) {
+                        v[4 * e] += w[e].x;
+                        v[4 * e + 1] += w[e].y;
+                        v[4 * e + 2] += w[e].z;
+                        v[4 * e + 3] += w[e].w;
+                    }
+                }
+                take(v, c);
             }
         }
     }
@@ -883,8 +1007,11 @@ void start(void (*kernel)(P...), uint32_t blocks, uint32_t threads, uint32_t clu
 // Types of 11 bits and more take operands of 22.
 bool is_split(uint32_t type) { return type != ARCQML_BF16; }
 
-constexpr size_t kHeadBytes = 512; // the fault, and from 256 on the shifts
-size_t sums_bytes() { return size_t(kMatrices) * kSumBlocks * sizeof(double); }
+// The scratch: the fault, the shifts, the parts that arrived, sums of squares, parts of tiles, then operands.
+constexpr size_t kShiftsAt = 256, kArrivedAt = 512, kSumsAt = kArrivedAt + kSMs * kTakers * 2 * sizeof(uint32_t);
+constexpr size_t kPartialAt = (kSumsAt + size_t(kMatrices) * kSumBlocks * sizeof(double) + 1023) / 1024 * 1024;
+// two tiles for each pair of blocks (single blocks: half as much)
+constexpr size_t kOperandsAt = kPartialAt + size_t(kSMs / 2) * 2 * (2 * kRows) * (2 * kRows) * sizeof(float);
 
 // Matrices that one block takes whole.
 bool is_small(const ArcqmlMatrix &a, bool split) {
@@ -935,51 +1062,72 @@ template <auto KERNEL> void allow_shared(uint32_t bytes) {
     if (device < 64) set |= uint64_t(1) << device;
 }
 
-template <int PHASE, bool SPLIT, int CG>
-void product(Group &g, uint32_t tiles, uint32_t step, bool last, cudaStream_t s) {
-    allow_shared<k_product<PHASE, SPLIT, CG>>(kProductShared<SPLIT>);
-    start(k_product<PHASE, SPLIT, CG>, std::min(tiles * CG, kSMs), kProductThreads, CG, kProductShared<SPLIT>, true, 0.0, s, g,
-          step, uint32_t(last));
-}
-
 template <int PHASE> uint32_t tiles_of(const Matrix &a, uint32_t size) {
     const uint32_t down = (a.m + size - 1) / size, across = (a.n + size - 1) / size;
     return PHASE == APPLY ? down * across : down * (down + 1) / 2;
 }
+template <int PHASE> uint32_t depth_of(const Matrix &a) { return ((PHASE == GRAM ? a.n : a.m) + kDepth - 1) / kDepth; }
 
-template <int PHASE, bool SPLIT> void phase(Group &g, uint32_t step, bool last, cudaStream_t s) {
-    // time of the phase in steps of 64 of a block's depth, on pairs of blocks and on single ones: all of the
-    // work spread over the GPU and half of its longest tile behind it
-    double cost[2];
-    for (int pair = 0; pair < 2; ++pair) {
-        double all = 0.0, longest = 0.0;
-        for (uint32_t i = 0; i < g.count; ++i) {
-            const Matrix &a = g.matrix[i];
-            const double depth = ((PHASE == GRAM ? a.n : a.m) + kDepth - 1) / kDepth * (pair ? 1.3 : 1.0) + 8;
-            const uint32_t tiles = tiles_of<PHASE>(a, kRows << pair);
-            all += tiles * depth;
-            longest = std::max(longest, depth);
-        }
-        const double units = pair ? kSMs / 2 : kSMs;
-        cost[pair] = std::max(longest, all / units + longest / 2);
-    }
-    const bool pair = cost[1] <= cost[0];
+template <int PHASE, bool SPLIT, int CG> void product(Group &g, uint32_t step, bool last, cudaStream_t s) {
+    allow_shared<k_product<PHASE, SPLIT, CG>>(kProductShared<SPLIT>);
+    std::stable_sort(g.order, g.order + g.count, [&](uint8_t x, uint8_t y) {
+        return depth_of<PHASE>(g.matrix[x]) > depth_of<PHASE>(g.matrix[y]);
+    });
     uint32_t tiles = 0;
     for (uint32_t i = 0; i < g.count; ++i) {
         g.first[i] = tiles;
-        tiles += tiles_of<PHASE>(g.matrix[i], pair ? 2 * kRows : kRows);
+        tiles += tiles_of<PHASE>(g.matrix[g.order[i]], CG * kRows);
     }
     g.first[g.count] = tiles;
-    if (pair) product<PHASE, SPLIT, 2>(g, tiles, step, last, s);
-    else product<PHASE, SPLIT, 1>(g, tiles, step, last, s);
+    const uint32_t units = kSMs / CG;
+    Plan p;
+    p.classes = p.left[0] = 0;
+    for (uint32_t i = 0, next; i < g.count; i = next) {
+        const uint32_t c = p.classes++, depth = depth_of<PHASE>(g.matrix[g.order[i]]);
+        for (next = i; next < g.count && depth_of<PHASE>(g.matrix[g.order[next]]) == depth;) ++next;
+        const uint32_t has = g.first[next] - g.first[i];
+        p.tile[c] = g.first[i];
+        p.depth[c] = depth;
+        p.rounds[c] = has / units;
+        p.left[c + 1] = p.left[c] + has % units * weight(depth);
+    }
+    // whole tiles, or runs of equal length, of 16 steps and a sixth of a tile at least: writing parts and putting
+    // them together takes about 18 us, 40 steps of 11-bit operands and 20 of 22-bit ones
+    const uint32_t all = p.left[p.classes];
+    uint32_t longest[2];
+    for (int parts = 1; parts >= 0; --parts) {
+        p.snap = parts ? 8 : 0xffffffffu;
+        p.runs = parts ? std::max(1u, std::min(units, all / std::max(16u, (p.depth[0] + 5) / 6))) : units;
+        longest[parts] = parts ? (SPLIT ? 20 : 40) : 0;
+        uint32_t run = 0;
+        for (uint32_t u = 0; u < p.runs; ++u) run = std::max(run, cut(p, u + 1) - cut(p, u));
+        longest[parts] += run;
+    }
+    if (longest[1] < longest[0]) {
+        p.snap = 8;
+        p.runs = std::max(1u, std::min(units, all / std::max(16u, (p.depth[0] + 5) / 6)));
+    }
+    start(k_product<PHASE, SPLIT, CG>, kSMs, kProductThreads, CG, kProductShared<SPLIT>, true, 0.0, s, g, p, step, uint32_t(last));
+}
+
+template <int PHASE, bool SPLIT> void phase(Group &g, uint32_t step, bool last, cudaStream_t s) {
+    // steps of 64 of the depth, on pairs of blocks and on single ones: a pair's takes 1.3 times as long for
+    // up to four times the work
+    uint64_t steps[2] = {0, 0};
+    for (uint32_t i = 0; i < g.count; ++i)
+        for (int pair = 0; pair < 2; ++pair)
+            steps[pair] += uint64_t(tiles_of<PHASE>(g.matrix[i], kRows << pair)) * depth_of<PHASE>(g.matrix[i]);
+    if (1.3 * 2.0 * double(steps[1]) <= double(steps[0])) product<PHASE, SPLIT, 2>(g, step, last, s);
+    else product<PHASE, SPLIT, 1>(g, step, last, s);
 }
 
 // The members' `out`, `in` and step are set; shapes and places are filled in here.
 template <bool SPLIT> void run_group(Group &g, int steps, cudaStream_t s) {
     uint32_t blocks = 0, spread = 0;
     double elements = 0.0;
-    uint64_t at = kHeadBytes + sums_bytes();
+    uint64_t at = kOperandsAt;
     static thread_local Group tiles;
+    for (uint32_t i = 0; i < g.count; ++i) g.order[i] = tiles.order[i] = uint8_t(i);
     for (uint32_t i = 0; i < g.count; ++i) {
         Matrix &a = g.matrix[i];
         a.down_blocks = (a.m + kRows - 1) / kRows;
@@ -1027,14 +1175,16 @@ template <bool SPLIT> void run_small(Group &g, int steps, cudaStream_t s) {
 template <class F>
 void run(const ArcqmlMatrix *list, const ArcqmlMatrix *kinds, size_t count, int steps, double eps, double *ws, size_t ws_len,
          cudaStream_t s, F &&fill) {
-    const uint64_t have = ws_len * sizeof(double), head = kHeadBytes + sums_bytes();
+    const uint64_t have = ws_len * sizeof(double), head = kOperandsAt;
     for_groups(list, kinds, count, have > head ? have - head : 0, [&](const std::vector<size_t> &members, uint64_t, bool split, bool small) {
         static thread_local Group g;
         g.count = uint32_t(members.size());
         g.scratch = reinterpret_cast<char *>(ws);
         g.fault = reinterpret_cast<uint32_t *>(ws);
-        g.shift = reinterpret_cast<int *>(g.scratch + kHeadBytes / 2);
-        g.sums = reinterpret_cast<double *>(g.scratch + kHeadBytes);
+        g.shift = reinterpret_cast<int *>(g.scratch + kShiftsAt);
+        g.arrived = reinterpret_cast<uint32_t *>(g.scratch + kArrivedAt);
+        g.sums = reinterpret_cast<double *>(g.scratch + kSumsAt);
+        g.partial = reinterpret_cast<float *>(g.scratch + kPartialAt);
         g.eps = eps;
         for (uint32_t i = 0; i < g.count; ++i) {
             const ArcqmlMatrix &a = list[members[i]];
@@ -1064,7 +1214,7 @@ size_t orthogonalize_workspace(const ArcqmlMatrix *list, size_t count) {
     uint64_t most = 0;
     for_groups(list, list, count, kGroupBytes,
                [&](const std::vector<size_t> &, uint64_t bytes, bool, bool) { most = std::max(most, bytes); });
-    return most ? size_t((kHeadBytes + sums_bytes() + most) / sizeof(double)) : 0;
+    return most ? size_t((kOperandsAt + most) / sizeof(double)) : 0;
 }
 
 void orthogonalize_device(const ArcqmlMatrix *in, const ArcqmlMatrix *out, size_t count, int steps, double eps,
