@@ -11,9 +11,11 @@
 // places stay in order and equal inputs give equal bits without atomics on values); chunks of the sorted
 // places are then summed side by side, whatever rows they belong to, so a row that most places point to
 // costs no more than others; rows that cross chunks are put together from the chunks' partial sums.
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <sstream>
 #include <string>
@@ -24,6 +26,8 @@
 #include "embedding.h"
 #include "launch.h"
 #include "profile.h"
+
+namespace cg = cooperative_groups;
 
 namespace arcqml {
 namespace {
@@ -220,6 +224,7 @@ __device__ __forceinline__ uint32_t digit_of(uint32_t key, uint32_t shift, uint3
 // The first pass's counts; clears those of the passes behind it (`clear` words at s.next).
 __global__ void __launch_bounds__(kThreads) k_count_digits(const __grid_constant__ Sort s, uint64_t clear) {
     __shared__ uint32_t bins[kBins];
+    cudaTriggerProgrammaticLaunchCompletion();
     for (uint32_t b = threadIdx.x; b < kBins; b += kThreads) bins[b] = 0;
     for (uint64_t i = uint64_t(blockIdx.x) * kThreads + threadIdx.x; i < clear; i += uint64_t(gridDim.x) * kThreads)
         s.next[i] = 0;
@@ -235,6 +240,8 @@ __global__ void __launch_bounds__(kThreads) k_count_digits(const __grid_constant
 // A block takes 32 digits, 32 threads each.
 __global__ void __launch_bounds__(1024) k_prefix_counts(uint32_t *counts, uint32_t *totals, uint32_t blocks) {
     __shared__ uint32_t part[32][33];
+    cudaTriggerProgrammaticLaunchCompletion();
+    cudaGridDependencySynchronize();
     const uint32_t digit = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
     const uint32_t each = (blocks + 31) / 32, lo = slice * each, hi = min(blocks, lo + each);
     uint32_t sum = 0;
@@ -259,8 +266,10 @@ __global__ void __launch_bounds__(kThreads) k_sort_pass(const __grid_constant__ 
     __shared__ uint32_t base[kBins];
     __shared__ uint32_t warp_sum[kWarps];
     const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    cudaTriggerProgrammaticLaunchCompletion();
     for (uint32_t b = t; b < kWarps * kBins; b += kThreads) (&hist[0][0])[b] = 0;
     __syncthreads();
+    cudaGridDependencySynchronize();
     uint32_t key[kKeysPerThread], rank[kKeysPerThread];
     const uint32_t first = blockIdx.x * kSortKeys + warp * (kSortKeys / kWarps) + lane;
 #pragma unroll
@@ -333,6 +342,127 @@ __global__ void __launch_bounds__(kThreads) k_sort_pass(const __grid_constant__ 
     }
 }
 
+// Up to 16 blocks of a cluster sort up to 131072 keys in one launch: keys and places stay in shared memory,
+// the blocks' counts and each pass's scatter go through distributed shared memory. The other clusters of the
+// launch clear the output meanwhile: most of its rows are often absent, and it is written twice only where
+// a row is present.
+constexpr uint32_t kClusterThreads = 1024, kClusterKeys = 8192, kPerThread = kClusterKeys / kClusterThreads;
+constexpr uint32_t kClusterWarps = kClusterThreads / 32, kMostCluster = 16;
+
+struct ClusterSort {
+    Indices index;
+    uint32_t *out_keys, *out_places;
+    char *clear;
+    uint64_t clear_bytes;
+    uint32_t places, passes, bits;
+};
+struct ClusterShared {
+    uint32_t key[2][kClusterKeys], place[2][kClusterKeys];
+    uint16_t hist[kClusterWarps][kBins];
+    uint32_t total[2][kBins]; // of this block, by parity of the pass
+    uint32_t base[kBins];
+    uint32_t warp_sum[kClusterWarps];
+};
+
+__device__ __forceinline__ void clear_share(char *to, uint64_t bytes, uint64_t thread, uint64_t threads) {
+    const uint64_t head = min(bytes, uint64_t(-reinterpret_cast<uintptr_t>(to) & 15)), body = (bytes - head) / 16;
+    if (thread < head) to[thread] = 0;
+    uint4 *v = reinterpret_cast<uint4 *>(to + head);
+    for (uint64_t i = thread; i < body; i += threads) v[i] = make_uint4(0, 0, 0, 0);
+    const uint64_t tail = head + body * 16;
+    if (thread < bytes - tail) to[tail + thread] = 0;
+}
+
+__global__ void __launch_bounds__(kClusterThreads, 1) k_sort_cluster(const __grid_constant__ ClusterSort s) {
+    extern __shared__ char raw[];
+    ClusterShared &sh = *reinterpret_cast<ClusterShared *>(raw);
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t size = cluster.num_blocks(), me = cluster.block_rank();
+    const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    cudaTriggerProgrammaticLaunchCompletion();
+    if (blockIdx.x >= size) {
+        clear_share(s.clear, s.clear_bytes, uint64_t(blockIdx.x - size) * kClusterThreads + t,
+                    uint64_t(gridDim.x - size) * kClusterThreads);
+        return;
+    }
+    // every block has kClusterKeys slots of the sorted order; those behind the last place hold kAbsent, which
+    // sorts last and keeps them there
+    for (uint32_t j = 0; j < kPerThread; ++j) {
+        const uint32_t k = j * kClusterThreads + t, i = me * kClusterKeys + k;
+        sh.key[0][k] = i < s.places ? key_at(s.index, i) : kAbsent;
+        sh.place[0][k] = i;
+    }
+    __syncthreads();
+    for (uint32_t p = 0; p < s.passes; ++p) {
+        const uint32_t shift = p * s.bits, from = p & 1, to = from ^ 1;
+        for (uint32_t b = t; b < kClusterWarps * kBins / 2; b += kClusterThreads)
+            reinterpret_cast<uint32_t *>(&sh.hist[0][0])[b] = 0;
+        __syncthreads();
+        uint32_t key[kPerThread], rank[kPerThread];
+#pragma unroll
+        for (uint32_t j = 0; j < kPerThread; ++j) {
+            key[j] = sh.key[from][warp * (kClusterKeys / kClusterWarps) + j * 32 + lane];
+            const uint32_t d = digit_of(key[j], shift, s.bits), same = __match_any_sync(0xffffffffu, d);
+            const uint32_t before = __popc(same & ((1u << lane) - 1));
+            rank[j] = sh.hist[warp][d] + before;
+            __syncwarp();
+            if (before == 0) sh.hist[warp][d] = uint16_t(rank[j] + __popc(same));
+            __syncwarp();
+        }
+        __syncthreads();
+        if (t < kBins) { // a thread for each digit
+            uint32_t sum = 0;
+#pragma unroll 8
+            for (uint32_t w = 0; w < kClusterWarps; ++w) {
+                const uint32_t c = sh.hist[w][t];
+                sh.hist[w][t] = uint16_t(sum);
+                sum += c;
+            }
+            sh.total[from][t] = sum;
+        }
+        cluster.sync();
+        uint32_t all = 0, mine = 0;
+        if (t < kBins) {
+            for (uint32_t b = 0; b < size; ++b) {
+                const uint32_t c = cluster.map_shared_rank(&sh, b)->total[from][t];
+                if (b < me) mine += c;
+                all += c;
+            }
+        }
+        uint32_t scan = all;
+        for (uint32_t o = 1; o < 32; o *= 2) {
+            const uint32_t up = __shfl_up_sync(0xffffffffu, scan, o);
+            if (lane >= o) scan += up;
+        }
+        if (lane == 31) sh.warp_sum[warp] = scan;
+        __syncthreads();
+        if (t < kBins) {
+            uint32_t before = scan - all + mine;
+            for (uint32_t w = 0; w < warp; ++w) before += sh.warp_sum[w];
+            sh.base[t] = before;
+        }
+        __syncthreads();
+        const bool last = p + 1 == s.passes;
+#pragma unroll
+        for (uint32_t j = 0; j < kPerThread; ++j) {
+            const uint32_t d = digit_of(key[j], shift, s.bits);
+            const uint32_t at = sh.base[d] + sh.hist[warp][d] + rank[j];
+            const uint32_t place = sh.place[from][warp * (kClusterKeys / kClusterWarps) + j * 32 + lane];
+            if (last) {
+                if (at < s.places) {
+                    s.out_keys[at] = key[j];
+                    s.out_places[at] = place;
+                }
+            } else {
+                ClusterShared *there = cluster.map_shared_rank(&sh, at / kClusterKeys);
+                there->key[to][at % kClusterKeys] = key[j];
+                there->place[to][at % kClusterKeys] = place;
+            }
+        }
+        cluster.sync(); // the next pass's keys are there, and nobody reads this block's counts any more
+    }
+}
+
 // ------------------------------------------------------------------ sums of the rows' places
 
 struct Sums {
@@ -370,10 +500,12 @@ __global__ void __launch_bounds__(kThreads) k_sum_chunks(const __grid_constant__
     using T = Element<DT>;
     using O = Element<OT>;
     using W = WideElement<DT>;
+    cudaTriggerProgrammaticLaunchCompletion();
     const uint64_t unit = (uint64_t(blockIdx.x) * kThreads + threadIdx.x) / a.lanes;
     const uint32_t c = uint32_t(unit / a.tiles);
     const uint32_t vector = uint32_t(unit % a.tiles) * a.lanes + (threadIdx.x & (a.lanes - 1));
     if (c >= a.chunks || vector >= a.vectors) return;
+    cudaGridDependencySynchronize();
     const uint32_t i0 = c * a.chunk, i1 = min(a.places, i0 + a.chunk);
     uint32_t row = a.keys[i0], begin = i0;
     if (row == kAbsent) return;
@@ -391,25 +523,36 @@ __global__ void __launch_bounds__(kThreads) k_sum_chunks(const __grid_constant__
             for (int e = 0; e < N; ++e) p[e] = sum[e];
         }
     };
-    for (uint32_t i = i0; i < i1; i += kAhead) {
-        uint32_t key[kAhead];
-        VectorOf<T, N> v[kAhead];
+    // the keys and places of the next group are loaded while this one's rows are on their way
+    uint32_t key[kAhead], at[kAhead];
+    const auto group = [&](uint32_t i) {
 #pragma unroll
         for (uint32_t j = 0; j < kAhead; ++j) {
             key[j] = i + j < i1 ? a.keys[i + j] : kAbsent;
-            if (key[j] != kAbsent)
-                v[j] = load_vector<T, N>(a.gradient + uint64_t(a.at[i + j]) * a.stride + uint64_t(vector) * sizeof(v[j]));
+            at[j] = i + j < i1 ? a.at[i + j] : 0;
         }
+    };
+    group(i0);
+    const char *column = a.gradient + uint64_t(vector) * sizeof(VectorOf<T, N>);
+    for (uint32_t i = i0; i < i1; i += kAhead) {
+        VectorOf<T, N> v[kAhead];
+        uint32_t now[kAhead];
 #pragma unroll
         for (uint32_t j = 0; j < kAhead; ++j) {
-            if (key[j] != row) {
+            if (key[j] != kAbsent) v[j] = load_vector<T, N>(column + uint64_t(at[j]) * a.stride);
+            now[j] = key[j];
+        }
+        group(i + kAhead);
+#pragma unroll
+        for (uint32_t j = 0; j < kAhead; ++j) {
+            if (now[j] != row) {
                 if (row != kAbsent) flush(i + j);
-                row = key[j];
+                row = now[j];
                 begin = i + j;
 #pragma unroll
                 for (int e = 0; e < N; ++e) sum[e] = W(0);
             }
-            if (key[j] == kAbsent) break;
+            if (now[j] == kAbsent) break;
 #pragma unroll
             for (int e = 0; e < N; ++e) sum[e] += to_wide(v[j].x[e]);
         }
@@ -429,28 +572,44 @@ __device__ __forceinline__ uint32_t first_not_below(const uint32_t *keys, uint32
     return lo;
 }
 
-// Rows that began in a chunk and went on: its partial sums in order.
+// Rows that began in a chunk and went on: a block for each chunk and 32 vectors. Its warps add up an eighth
+// of the row's partial sums each, in order, then the first one the eighths.
 template <uint32_t DT, uint32_t OT, int N>
 __global__ void __launch_bounds__(kThreads) k_join_chunks(const __grid_constant__ Sums a) {
     using T = Element<DT>;
     using O = Element<OT>;
     using W = WideElement<DT>;
-    const uint64_t unit = (uint64_t(blockIdx.x) * kThreads + threadIdx.x) / a.lanes;
-    const uint32_t c = uint32_t(unit / a.tiles);
-    const uint32_t vector = uint32_t(unit % a.tiles) * a.lanes + (threadIdx.x & (a.lanes - 1));
-    if (c + 1 >= a.chunks || vector >= a.vectors) return;
+    __shared__ W part[kWarps][32][N];
+    const uint32_t groups = (a.vectors + 31) / 32, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t c = blockIdx.x / groups, vector = blockIdx.x % groups * 32 + lane;
+    cudaTriggerProgrammaticLaunchCompletion();
+    cudaGridDependencySynchronize();
     const uint32_t i0 = c * a.chunk, i1 = i0 + a.chunk, row = a.keys[i1 - 1];
     if (row == kAbsent || a.keys[i1] != row) return;
     if (a.keys[i0] == row && i0 != 0 && a.keys[i0 - 1] == row) return; // it began earlier
     const uint32_t last = (first_not_below(a.keys, a.places, row + 1) - 1) / a.chunk;
+    // the first partial is 2c + 1, the others 2d for d = c + 1 .. last
+    const uint32_t count = last - c, each = (count + kWarps - 1) / kWarps, lo = c + 1 + warp * each, hi = min(last + 1, lo + each);
     W sum[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) sum[e] = W(0);
+    const bool on = vector < a.vectors;
     const W *p = static_cast<const W *>(a.partial) + uint64_t(vector) * N;
+    if (on && warp == 0)
 #pragma unroll
-    for (int e = 0; e < N; ++e) sum[e] = p[(uint64_t(2) * c + 1) * a.width + e];
+        for (int e = 0; e < N; ++e) sum[e] = p[(uint64_t(2) * c + 1) * a.width + e];
+    if (on)
 #pragma unroll 8
-    for (uint32_t d = c + 1; d <= last; ++d)
+        for (uint32_t d = lo; d < hi; ++d)
 #pragma unroll
-        for (int e = 0; e < N; ++e) sum[e] += p[uint64_t(2) * d * a.width + e];
+            for (int e = 0; e < N; ++e) sum[e] += p[uint64_t(2) * d * a.width + e];
+#pragma unroll
+    for (int e = 0; e < N; ++e) part[warp][lane][e] = sum[e];
+    __syncthreads();
+    if (warp != 0 || !on) return;
+    for (uint32_t w = 1; w < kWarps; ++w)
+#pragma unroll
+        for (int e = 0; e < N; ++e) sum[e] += part[w][lane][e];
     write_sum<T, O, W, N>(a, row, vector, sum);
 }
 
@@ -459,7 +618,9 @@ template <uint32_t OT> __global__ void __launch_bounds__(kThreads) k_zero_rows(c
     using O = Element<OT>;
     const uint32_t lane = threadIdx.x & 31;
     const uint64_t first = (uint64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5)) * 32;
+    cudaTriggerProgrammaticLaunchCompletion();
     if (first >= a.rows) return;
+    cudaGridDependencySynchronize();
     bool absent = false;
     if (first + lane < a.rows) {
         const uint32_t key = uint32_t(first) + lane, at = first_not_below(a.keys, a.places, key);
@@ -478,7 +639,7 @@ struct Project {
     char *out;
     const uint32_t *keys;
     uint64_t table_stride, width, rows;
-    uint32_t places;
+    uint32_t places, cleared; // rows without places are zero already
 };
 template <uint32_t DT>
 __global__ void __launch_bounds__(kThreads) k_project(const __grid_constant__ Project a) {
@@ -486,9 +647,11 @@ __global__ void __launch_bounds__(kThreads) k_project(const __grid_constant__ Pr
     using W = WideElement<DT>;
     __shared__ double part[2][kWarps];
     const uint32_t row = blockIdx.x;
+    cudaGridDependencySynchronize();
     const uint32_t at = first_not_below(a.keys, a.places, row);
     T *out = reinterpret_cast<T *>(a.out) + uint64_t(row) * a.width;
     if (at == a.places || a.keys[at] != row) {
+        if (a.cleared) return;
         for (uint64_t k = threadIdx.x; k < a.width; k += kThreads) out[k] = to_element<T>(W(0));
         return;
     }
@@ -519,6 +682,150 @@ __global__ void __launch_bounds__(kThreads) k_project(const __grid_constant__ Pr
 #pragma unroll 4
     for (uint64_t k = threadIdx.x; k < a.width; k += kThreads)
         out[k] = to_element<T>(W((double(g[k]) - double(to_wide(t[k])) * along) * inverse));
+}
+
+// ------------------------------------------------------------------ few places: everything in one launch
+
+// A block has `group` rows of the table. It lists the places that point to them, in order, and then a warp
+// (a block for wide rows) sums each row's places, takes the sum through the norm, and writes the row,
+// zeros where there is no place.
+constexpr uint32_t kFewPlaces = 1024, kDirectVectors = 4;
+
+struct Direct {
+    const char *gradient, *table; // table: null unless rows are normalised
+    char *out;
+    Indices index;
+    uint64_t stride, table_stride, row_bytes;
+    double scale;
+    uint32_t places, rows, group, vectors;
+    uint32_t aligned; // vectors start on their size; otherwise they are moved by elements
+};
+
+template <class T, int N> __device__ __forceinline__ VectorOf<T, N> load_any(const char *p, uint32_t aligned) {
+    if (aligned) return load_vector<T, N>(p);
+    VectorOf<T, N> v;
+#pragma unroll
+    for (int e = 0; e < N; ++e) v.x[e] = reinterpret_cast<const T *>(p)[e];
+    return v;
+}
+
+template <uint32_t DT, int N, bool BLOCK>
+__global__ void __launch_bounds__(kThreads) k_direct(const __grid_constant__ Direct a) {
+    using T = Element<DT>;
+    using W = WideElement<DT>;
+    __shared__ uint32_t list[kFewPlaces]; // the row within the group << 16 | the place
+    __shared__ uint32_t count[kWarps + 1];
+    const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const uint32_t row0 = blockIdx.x * a.group, rows = min(a.group, a.rows - row0);
+    const uint32_t each = (a.places + kThreads - 1) / kThreads * 32, lo = warp * each; // places of a warp
+    constexpr uint32_t ROUNDS = kFewPlaces / kThreads;
+    uint32_t mine[ROUNDS], found = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < ROUNDS; ++j) {
+        const uint32_t i = lo + j * 32 + lane;
+        mine[j] = j * 32 < each && i < a.places ? key_at(a.index, i) - row0 : kAbsent;
+        found += __popc(__ballot_sync(0xffffffffu, mine[j] < rows));
+    }
+    if (lane == 0) count[warp] = found;
+    __syncthreads();
+    uint32_t at = 0, all = 0;
+    for (uint32_t w = 0; w < kWarps; ++w) {
+        if (w == warp) at = all;
+        all += count[w];
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < ROUNDS; ++j) {
+        const uint32_t here = __ballot_sync(0xffffffffu, mine[j] < rows);
+        if (mine[j] < rows) list[at + __popc(here & ((1u << lane) - 1))] = mine[j] << 16 | (lo + j * 32 + lane);
+        at += __popc(here);
+    }
+    __syncthreads();
+    constexpr uint32_t THREADS = BLOCK ? kThreads : 32;
+    const uint32_t thread = BLOCK ? t : lane, vector0 = blockIdx.y * (THREADS * kDirectVectors) + thread;
+    for (uint32_t r = BLOCK ? 0 : warp; r < rows; r += BLOCK ? 1 : kWarps) {
+        W sum[kDirectVectors][N];
+#pragma unroll
+        for (uint32_t j = 0; j < kDirectVectors; ++j)
+#pragma unroll
+            for (int e = 0; e < N; ++e) sum[j][e] = W(0);
+        bool any = false;
+        for (uint32_t b = 0; b < all; b += 32) {
+            const uint32_t entry = b + lane < all ? list[b + lane] : kAbsent;
+            uint32_t same = __ballot_sync(0xffffffffu, b + lane < all && entry >> 16 == r);
+            any = any || same;
+            while (same) { // up to four places at a time
+                VectorOf<T, N> v[4][kDirectVectors];
+                uint32_t n = 0;
+#pragma unroll
+                for (uint32_t q = 0; q < 4; ++q) {
+                    if (!same) break;
+                    const uint32_t place = __shfl_sync(0xffffffffu, entry, __ffs(int(same)) - 1) & 0xffff;
+                    same &= same - 1;
+                    ++n;
+                    const char *from = a.gradient + uint64_t(place) * a.stride;
+#pragma unroll
+                    for (uint32_t j = 0; j < kDirectVectors; ++j) {
+                        const uint32_t k = vector0 + j * THREADS;
+                        if (k < a.vectors) v[q][j] = load_any<T, N>(from + uint64_t(k) * sizeof(v[q][j]), a.aligned);
+                    }
+                }
+#pragma unroll
+                for (uint32_t q = 0; q < 4; ++q)
+                    if (q < n)
+#pragma unroll
+                        for (uint32_t j = 0; j < kDirectVectors; ++j)
+                            if (vector0 + j * THREADS < a.vectors)
+#pragma unroll
+                                for (int e = 0; e < N; ++e) sum[j][e] += to_wide(v[q][j].x[e]);
+            }
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < kDirectVectors; ++j)
+#pragma unroll
+            for (int e = 0; e < N; ++e) sum[j][e] *= W(a.scale);
+        const uint64_t row = uint64_t(row0) + r;
+        double along = 0.0, inverse = 1.0;
+        VectorOf<T, N> unit[kDirectVectors];
+        if (a.table && any) { // the same in all threads of the row
+            const char *from = a.table + row * a.table_stride;
+            double tt = 0.0, ts = 0.0;
+#pragma unroll
+            for (uint32_t j = 0; j < kDirectVectors; ++j) {
+                const uint32_t k = vector0 + j * THREADS;
+                if (k >= a.vectors) continue;
+                unit[j] = load_any<T, N>(from + uint64_t(k) * sizeof(unit[j]), a.aligned);
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const double x = to_wide(unit[j].x[e]);
+                    tt = fma(x, x, tt);
+                    ts = fma(x, double(sum[j][e]), ts);
+                }
+            }
+            tt = sum_over<BLOCK>(tt, 32);
+            if constexpr (BLOCK) __syncthreads(); // the first sum's shared memory
+            ts = sum_over<BLOCK>(ts, 32);
+            if constexpr (BLOCK) __syncthreads();
+            inverse = tt == 0.0 ? 0.0 : 1.0 / sqrt(tt);
+            along = tt == 0.0 ? 0.0 : ts / tt;
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < kDirectVectors; ++j) {
+            const uint32_t k = vector0 + j * THREADS;
+            if (k >= a.vectors) continue;
+            VectorOf<T, N> y;
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                W x = sum[j][e];
+                if (a.table && any) x = W((double(x) - double(to_wide(unit[j].x[e])) * along) * inverse);
+                y.x[e] = to_element<T>(x);
+            }
+            char *to = a.out + row * a.row_bytes + uint64_t(k) * sizeof(y);
+            if (a.aligned) store_vector<T, N>(to, y);
+            else
+#pragma unroll
+                for (int e = 0; e < N; ++e) reinterpret_cast<T *>(to)[e] = y.x[e];
+        }
+    }
 }
 
 // ------------------------------------------------------------------ host
@@ -596,18 +903,47 @@ template <class F> void for_access(uint32_t dtype, uint32_t bytes, F &&f) {
     }
 }
 
+struct Shape {
+    uint64_t blocks;
+    uint32_t threads;
+    bool follows = false; // may start while the call's last launch ends
+    uint32_t cluster = 1, shared = 0, across = 1;
+};
+
 template <class... P, class... A>
-void start(void (*kernel)(P...), uint64_t blocks, uint32_t threads, double bytes, cudaStream_t s, const A &...args) {
-    if (blocks >> 31) fail("the embedding call is too large for one launch");
+void start(void (*kernel)(P...), const Shape &shape, double bytes, cudaStream_t s, const A &...args) {
+    if (shape.blocks >> 31) fail("the embedding call is too large for one launch");
     cudaLaunchConfig_t c{};
-    c.gridDim = dim3(uint32_t(blocks));
-    c.blockDim = dim3(threads);
+    cudaLaunchAttribute at[2]{};
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = shape.cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    c.attrs = shape.follows ? at : at + 1;
+    c.numAttrs = (shape.follows ? 1 : 0) + (shape.cluster > 1 ? 1 : 0);
+    c.gridDim = dim3(uint32_t(shape.blocks), shape.across);
+    c.blockDim = dim3(shape.threads);
+    c.dynamicSmemBytes = shape.shared;
     c.stream = s;
     std::tuple<P...> held{P(args)...};
     const ProfToken tok = prof_begin(PROF_OTHER, s);
     const cudaError_t e = std::apply([&](auto &...x) { return cudaLaunchKernelEx(&c, kernel, x...); }, held);
     check_cuda(e, "embedding kernel launch");
     prof_end(tok, s, bytes);
+}
+
+// Lets the sort have clusters of 16 blocks and their shared memory, once on each device.
+void allow_cluster() {
+    static std::atomic<uint64_t> set{0};
+    int device = 0;
+    check_cuda(cudaGetDevice(&device), "cudaGetDevice");
+    if (device < 64 && (set.load() >> device & 1)) return;
+    check_cuda(cudaFuncSetAttribute(k_sort_cluster, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(ClusterShared))),
+               "embedding kernel attribute");
+    check_cuda(cudaFuncSetAttribute(k_sort_cluster, cudaFuncAttributeNonPortableClusterSizeAllowed, 1),
+               "embedding kernel attribute");
+    if (device < 64) set |= uint64_t(1) << device;
 }
 
 uint64_t blocks_for(uint64_t threads) { return (threads + kThreads - 1) / kThreads; }
@@ -629,6 +965,10 @@ struct GradientScratch {
 GradientScratch gradient_scratch(const ArcqmlRows &g, uint64_t rows, const ArcqmlEmbeddingOptions &o) {
     GradientScratch s{};
     const uint64_t n = g.rows;
+    // few places, and not many to a row: one launch. A row that goes through its norm has to fit into a block.
+    const uint64_t row = g.width * bytes_of_element(g.dtype);
+    if (n <= kFewPlaces && n <= 16 * rows && (!o.normalize || row / access_bytes(row | 16) <= kThreads * kDirectVectors))
+        return s;
     const auto take = [&](uint64_t words) {
         const uint64_t at = s.words;
         s.words += (words + 3) / 4 * 4;
@@ -639,12 +979,15 @@ GradientScratch gradient_scratch(const ArcqmlRows &g, uint64_t rows, const Arcqm
     s.passes = (bits + 8) / 9;
     s.bits = (bits + s.passes - 1) / s.passes;
     s.blocks = uint32_t((n + kSortKeys - 1) / kSortKeys);
-    for (int i = 0; i < 2; ++i) {
+    const bool in_cluster = n <= kClusterKeys * kMostCluster;
+    for (int i = 0; i < (in_cluster ? 1 : 2); ++i) {
         s.keys[i] = take(n);
         s.places[i] = take(n);
     }
-    s.counts = take(uint64_t(s.passes) * s.blocks * kBins);
-    s.totals = take(kBins);
+    if (!in_cluster) {
+        s.counts = take(uint64_t(s.passes) * s.blocks * kBins);
+        s.totals = take(kBins);
+    }
     // chunks: enough of them to fill the GPU, 128 places at most
     const uint64_t tiles = std::max<uint64_t>(1, g.width * bytes_of_element(g.dtype) / 512);
     s.chunk = 8;
@@ -695,20 +1038,20 @@ void embedding_lookup_device(const ArcqmlRows &table, const void *indices, size_
     for_access(table.dtype, bytes, [&](auto type, auto n) {
         constexpr uint32_t DT = type;
         constexpr int N = n;
-        if (held && vectors > 32 * kRowVectors) return start(k_lookup_row<DT, N, true>, count, kThreads, moved, s, a);
+        if (held && vectors > 32 * kRowVectors) return start(k_lookup_row<DT, N, true>, {count, kThreads}, moved, s, a);
         if (held) {
             a.lanes = power_of_two_from((vectors + 1) / 2);
             while (a.lanes * kRowVectors < vectors) a.lanes *= 2;
-            return start(k_lookup_row<DT, N, false>, blocks_for(count * a.lanes), kThreads, moved, s, a);
+            return start(k_lookup_row<DT, N, false>, {blocks_for(count * a.lanes), kThreads}, moved, s, a);
         }
         if (o.normalize) {
             a.pieces = uint32_t((vectors + kPieceVectors - 1) / kPieceVectors);
-            start(k_row_squares<DT, N>, count * a.pieces, kThreads, moved / 2, s, a, ws);
+            start(k_row_squares<DT, N>, {count * a.pieces, kThreads}, moved / 2, s, a, ws);
             a.squares = ws;
         }
         a.lanes = power_of_two_from((vectors + kTileVectors - 1) / kTileVectors);
         a.tiles = uint32_t((vectors + a.lanes * kTileVectors - 1) / (a.lanes * kTileVectors));
-        start(k_lookup<DT, N>, blocks_for(count * a.tiles * a.lanes), kThreads, moved, s, a);
+        start(k_lookup<DT, N>, {blocks_for(count * a.tiles * a.lanes), kThreads}, moved, s, a);
     });
 }
 
@@ -728,22 +1071,72 @@ void embedding_gradient_device(const ArcqmlRows &gradient, const void *indices, 
         if (table->dtype != out.dtype || table->width != out.width || table->rows != out.rows)
             refuse("table", "does not have the output's type and shape");
     }
+    const uint64_t size = bytes_of_element(gradient.dtype), n = gradient.rows, row = out.width * size;
     const GradientScratch w = gradient_scratch(gradient, out.rows, o);
     check_scratch(ws, ws_len, size_t((w.words + 1) / 2));
     if (!out.rows) return;
-    const uint64_t size = bytes_of_element(gradient.dtype), n = gradient.rows;
+    const uint64_t starts = address(gradient.data) | address(out.data) | gradient.stride * size | row | 16;
+    const uint32_t bytes = access_bytes(table ? starts | address(table->data) | table->stride * size : starts);
+    const Indices index{indices, out.rows, o.padding, o.index_bytes == 8};
+    const double moved = double(n) * double(row);
+    if (!w.words) {
+        Direct a{};
+        a.gradient = static_cast<const char *>(gradient.data);
+        a.table = table ? static_cast<const char *>(table->data) : nullptr;
+        a.out = static_cast<char *>(out.data);
+        a.index = index;
+        a.stride = gradient.stride * size;
+        a.table_stride = table ? table->stride * size : 0;
+        a.row_bytes = row;
+        a.scale = o.scale;
+        a.places = uint32_t(n);
+        a.rows = uint32_t(out.rows);
+        const uint32_t whole = access_bytes(row | 16);
+        a.aligned = bytes == whole;
+        a.vectors = uint32_t(row / whole);
+        const bool wide = a.vectors > 32 * kDirectVectors;
+        const uint32_t across = wide ? (a.vectors + kThreads * kDirectVectors - 1) / (kThreads * kDirectVectors) : 1;
+        // blocks for each place on the GPU; warps take the rows of a block in turn
+        a.group = uint32_t(std::min<uint64_t>(65535, (out.rows + 148 * 6 - 1) / (148 * 6)));
+        if (!wide) a.group = std::max(a.group, kWarps);
+        const Shape shape{(out.rows + a.group - 1) / a.group, kThreads, false, 1, 0, across};
+        return for_access(gradient.dtype, whole, [&](auto type, auto nn) {
+            constexpr uint32_t DT = type;
+            constexpr int N = nn;
+            if (wide) start(k_direct<DT, N, true>, shape, moved, s, a);
+            else start(k_direct<DT, N, false>, shape, moved, s, a);
+        });
+    }
     uint32_t *base = reinterpret_cast<uint32_t *>(ws);
-    const uint32_t *keys = base + w.keys[w.passes & 1], *places = base + w.places[w.passes & 1];
-    if (n) {
+    const bool in_cluster = n <= kClusterKeys * kMostCluster;
+    const uint32_t *keys = base + w.keys[in_cluster ? 0 : w.passes & 1], *places = base + w.places[in_cluster ? 0 : w.passes & 1];
+    if (in_cluster) {
+        ClusterSort a{};
+        a.index = index;
+        a.out_keys = base + w.keys[0];
+        a.out_places = base + w.places[0];
+        a.clear = static_cast<char *>(out.data);
+        a.clear_bytes = out.rows * row;
+        a.places = uint32_t(n);
+        a.passes = w.passes;
+        a.bits = w.bits;
+        uint32_t cluster = 1;
+        while (cluster * kClusterKeys < n) cluster *= 2;
+        allow_cluster();
+        // as many blocks clear as the GPU takes beside the sort, at least 64 KB each
+        const uint64_t clears = std::min<uint64_t>((112 - cluster) / cluster, a.clear_bytes / (uint64_t(cluster) << 16) + 1);
+        start(k_sort_cluster, {cluster * (1 + clears), kClusterThreads, false, cluster, sizeof(ClusterShared)},
+              double(a.clear_bytes), s, a);
+    } else {
         Sort a{};
-        a.index = {indices, out.rows, o.padding, o.index_bytes == 8};
+        a.index = index;
         a.places = uint32_t(n);
         a.blocks = w.blocks;
         a.bits = w.bits;
         const uint64_t each = uint64_t(w.blocks) * kBins;
         a.counts = base + w.counts;
         a.next = a.counts + each;
-        start(k_count_digits, w.blocks, kThreads, 8.0 * double(n), s, a, each * (w.passes - 1));
+        start(k_count_digits, {w.blocks, kThreads}, 8.0 * double(n), s, a, each * (w.passes - 1));
         for (uint32_t p = 0; p < w.passes; ++p) {
             a.shift = p * w.bits;
             a.next_shift = a.shift + w.bits;
@@ -756,9 +1149,9 @@ void embedding_gradient_device(const ArcqmlRows &gradient, const void *indices, 
             a.totals = nullptr;
             if (w.blocks > 128) {
                 a.totals = base + w.totals;
-                start(k_prefix_counts, kBins / 32, 1024, 8.0 * double(each), s, a.counts, a.totals, w.blocks);
+                start(k_prefix_counts, {kBins / 32, 1024, true}, 8.0 * double(each), s, a.counts, a.totals, w.blocks);
             }
-            start(k_sort_pass, w.blocks, kThreads, 16.0 * double(n), s, a);
+            start(k_sort_pass, {w.blocks, kThreads, true}, 16.0 * double(n), s, a);
         }
     }
     Sums a{};
@@ -775,22 +1168,19 @@ void embedding_gradient_device(const ArcqmlRows &gradient, const void *indices, 
     a.chunks = w.chunks;
     const bool apart = o.normalize && size == 2; // the sums keep 32 bits until the norm is through
     a.out = apart ? reinterpret_cast<char *>(base + w.sums) : static_cast<char *>(out.data);
-    const uint64_t row = a.width * size;
-    const uint32_t bytes = access_bytes(address(gradient.data) | (apart ? 0 : address(out.data)) | a.stride | row | 16);
     a.vectors = uint32_t(row / bytes);
     a.lanes = power_of_two_from(a.vectors);
     a.tiles = (a.vectors + a.lanes - 1) / a.lanes;
-    const double moved = double(n) * double(row);
     for_access(gradient.dtype, bytes, [&](auto type, auto nn) {
         constexpr uint32_t DT = type;
         constexpr int N = nn;
         constexpr uint32_t WIDE = DT == ARCQML_F64 ? ARCQML_F64 : ARCQML_F32;
-        const uint64_t blocks = blocks_for(uint64_t(a.chunks) * a.tiles * a.lanes);
         const auto sums = [&](auto kind) {
             constexpr uint32_t OT = kind;
             if (!n) return;
-            start(k_sum_chunks<DT, OT, N>, blocks, kThreads, moved, s, a);
-            if (a.chunks > 1) start(k_join_chunks<DT, OT, N>, blocks, kThreads, 0.0, s, a);
+            start(k_sum_chunks<DT, OT, N>, {blocks_for(uint64_t(a.chunks) * a.tiles * a.lanes), kThreads, true}, moved, s, a);
+            if (a.chunks > 1)
+                start(k_join_chunks<DT, OT, N>, {uint64_t(a.chunks - 1) * ((a.vectors + 31) / 32), kThreads, true}, 0.0, s, a);
         };
         if constexpr (WIDE != DT) {
             if (apart) sums(std::integral_constant<uint32_t, WIDE>{});
@@ -801,8 +1191,10 @@ void embedding_gradient_device(const ArcqmlRows &gradient, const void *indices, 
     });
     for_access(out.dtype, 16, [&](auto type, auto) {
         constexpr uint32_t DT = type;
-        if (!o.normalize)
-            return start(k_zero_rows<DT>, (out.rows + kWarps * 32 - 1) / (kWarps * 32), kThreads, 0.0, s, a);
+        if (!o.normalize) {
+            if (!in_cluster) start(k_zero_rows<DT>, {(out.rows + kWarps * 32 - 1) / (kWarps * 32), kThreads, true}, 0.0, s, a);
+            return;
+        }
         Project p{};
         p.table = static_cast<const char *>(table->data);
         p.sums = a.out;
@@ -812,7 +1204,8 @@ void embedding_gradient_device(const ArcqmlRows &gradient, const void *indices, 
         p.width = out.width;
         p.rows = out.rows;
         p.places = uint32_t(n);
-        start(k_project<DT>, out.rows, kThreads, 3.0 * double(row) * double(out.rows), s, p);
+        p.cleared = in_cluster;
+        start(k_project<DT>, {out.rows, kThreads, true}, 3.0 * double(row) * double(out.rows), s, p);
     });
 }
 
