@@ -73,4 +73,50 @@ template <class T, int N> __device__ __forceinline__ void store_vector(void *p, 
     else *static_cast<uint16_t *>(p) = *reinterpret_cast<const uint16_t *>(&v);
 }
 
+// N elements as the words that one access moves. 16-bit elements stay in pairs until they are used: a register
+// each would double those of a load in flight.
+template <class T, int N> struct Packed {
+    using W = decltype(to_wide(T()));
+    static constexpr int BYTES = sizeof(T) * N, WORDS = BYTES < 4 ? 1 : BYTES / 4; // in memory; here 4 at least
+    uint32_t w[WORDS];
+    __device__ __forceinline__ W wide(int e) const {
+        if constexpr (sizeof(T) == 8) return __hiloint2double(int(w[2 * e + 1]), int(w[2 * e]));
+        else if constexpr (sizeof(T) == 4) return __uint_as_float(w[e]);
+        else if constexpr (sizeof(T) == 2 && __is_same(T, __nv_bfloat16))
+            return __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+        else return __half2float(__ushort_as_half(uint16_t(e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xffffu)));
+    }
+    __device__ __forceinline__ void set(int e, W x) { // 16-bit elements in turn, the even ones first
+        if constexpr (sizeof(T) == 8) {
+            w[2 * e] = uint32_t(__double2loint(x));
+            w[2 * e + 1] = uint32_t(__double2hiint(x));
+        } else if constexpr (sizeof(T) == 4) {
+            w[e] = __float_as_uint(x);
+        } else {
+            const T y = to_element<T>(x);
+            const uint32_t bits = *reinterpret_cast<const uint16_t *>(&y);
+            w[e / 2] = e & 1 ? w[e / 2] | bits << 16 : bits;
+        }
+    }
+    __device__ __forceinline__ void load(const void *p) {
+        if constexpr (BYTES == 16) {
+            const uint4 v = *static_cast<const uint4 *>(p);
+            w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+        } else if constexpr (BYTES == 8) {
+            const uint2 v = *static_cast<const uint2 *>(p);
+            w[0] = v.x, w[1] = v.y;
+        } else if constexpr (BYTES == 4) {
+            w[0] = *static_cast<const uint32_t *>(p);
+        } else {
+            w[0] = *static_cast<const uint16_t *>(p);
+        }
+    }
+    __device__ __forceinline__ void store(void *p) const {
+        if constexpr (BYTES == 16) *static_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+        else if constexpr (BYTES == 8) *static_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
+        else if constexpr (BYTES == 4) *static_cast<uint32_t *>(p) = w[0];
+        else *static_cast<uint16_t *>(p) = uint16_t(w[0]);
+    }
+};
+
 }  // namespace arcqml

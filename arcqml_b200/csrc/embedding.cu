@@ -67,9 +67,7 @@ constexpr uint32_t kPieceVectors = 2048;
 
 // ------------------------------------------------------------------ lookup
 
-template <class T> __device__ __forceinline__ T not_a_number() {
-    return to_element<T>(WideElement<ARCQML_F32>(__int_as_float(0x7fffffff)));
-}
+template <class W> __device__ __forceinline__ W not_a_number() { return W(__int_as_float(0x7fffffff)); }
 
 // Rows in tiles of 4 vectors a thread, a tile taken by `lanes` threads.
 template <uint32_t DT, int N>
@@ -85,11 +83,11 @@ __global__ void __launch_bounds__(kThreads) k_lookup(const __grid_constant__ Loo
     const bool inside = a.index.inside(row), padding = a.index.is_padding(row);
     const char *from = a.table + (inside ? uint64_t(row) : 0) * a.stride;
     char *to = a.out + place * a.row_bytes;
-    VectorOf<T, N> v[kTileVectors];
+    Packed<T, N> v[kTileVectors];
 #pragma unroll
     for (uint32_t j = 0; j < kTileVectors; ++j) {
         const uint32_t k = first + j * a.lanes;
-        if (inside && k < a.vectors) v[j] = load_vector<T, N>(from + uint64_t(k) * sizeof(v[j]));
+        if (inside && k < a.vectors) v[j].load(from + uint64_t(k) * Packed<T, N>::BYTES);
     }
     double factor = a.scale;
     if (a.squares) {
@@ -102,14 +100,15 @@ __global__ void __launch_bounds__(kThreads) k_lookup(const __grid_constant__ Loo
     for (uint32_t j = 0; j < kTileVectors; ++j) {
         const uint32_t k = first + j * a.lanes;
         if (k >= a.vectors) continue;
+        Packed<T, N> y;
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-            if (padding) v[j].x[e] = to_element<T>(W(0));
-            else if (!inside) v[j].x[e] = not_a_number<T>();
-            else if (a.squares) v[j].x[e] = to_element<T>(W(double(to_wide(v[j].x[e])) * factor));
-            else v[j].x[e] = to_element<T>(to_wide(v[j].x[e]) * W(factor));
+            if (padding) y.set(e, W(0));
+            else if (!inside) y.set(e, not_a_number<W>());
+            else if (a.squares) y.set(e, W(double(v[j].wide(e)) * factor));
+            else y.set(e, v[j].wide(e) * W(factor));
         }
-        store_vector<T, N>(to + uint64_t(k) * sizeof(v[j]), v[j]);
+        y.store(to + uint64_t(k) * Packed<T, N>::BYTES);
     }
 }
 
@@ -139,21 +138,21 @@ __global__ void __launch_bounds__(kThreads) k_lookup_row(const __grid_constant__
     const int64_t row = on ? a.index[place] : -1;
     const bool inside = a.index.inside(row), padding = a.index.is_padding(row);
     const char *from = a.table + (inside ? uint64_t(row) : 0) * a.stride;
-    VectorOf<T, N> v[kRowVectors];
+    Packed<T, N> v[kRowVectors];
 #pragma unroll
     for (uint32_t j = 0; j < kRowVectors; ++j) {
         const uint32_t k = lane + j * lanes;
-        if (inside && !padding && k < a.vectors) v[j] = load_vector<T, N>(from + uint64_t(k) * sizeof(v[j]));
+        if (inside && !padding && k < a.vectors) v[j].load(from + uint64_t(k) * Packed<T, N>::BYTES);
         else
 #pragma unroll
-            for (int e = 0; e < N; ++e) v[j].x[e] = to_element<T>(W(0));
+            for (int e = 0; e < N; ++e) v[j].set(e, W(0));
     }
     double sum = 0.0;
 #pragma unroll
     for (uint32_t j = 0; j < kRowVectors; ++j)
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-            const double x = to_wide(v[j].x[e]);
+            const double x = v[j].wide(e);
             sum = fma(x, x, sum);
         }
     sum = sum_over<BLOCK>(sum, lanes);
@@ -163,11 +162,11 @@ __global__ void __launch_bounds__(kThreads) k_lookup_row(const __grid_constant__
     for (uint32_t j = 0; j < kRowVectors; ++j) {
         const uint32_t k = lane + j * lanes;
         if (!on || k >= a.vectors) continue;
+        Packed<T, N> y;
 #pragma unroll
         for (int e = 0; e < N; ++e)
-            v[j].x[e] = padding || inside ? to_element<T>(W(double(to_wide(v[j].x[e])) * factor))
-                                          : not_a_number<T>();
-        store_vector<T, N>(to + uint64_t(k) * sizeof(v[j]), v[j]);
+            y.set(e, padding || inside ? W(double(v[j].wide(e)) * factor) : not_a_number<W>());
+        y.store(to + uint64_t(k) * Packed<T, N>::BYTES);
     }
 }
 
@@ -184,10 +183,11 @@ __global__ void __launch_bounds__(kThreads) k_row_squares(const __grid_constant_
         const uint32_t end = min(a.vectors, (piece + 1) * kPieceVectors);
 #pragma unroll 8
         for (uint32_t k = piece * kPieceVectors + threadIdx.x; k < end; k += kThreads) {
-            const auto v = load_vector<T, N>(from + uint64_t(k) * sizeof(VectorOf<T, N>));
+            Packed<T, N> v;
+            v.load(from + uint64_t(k) * Packed<T, N>::BYTES);
 #pragma unroll
             for (int e = 0; e < N; ++e) {
-                const double x = to_wide(v.x[e]);
+                const double x = v.wide(e);
                 sum = fma(x, x, sum);
             }
         }
@@ -205,8 +205,8 @@ constexpr uint32_t kWarps = kThreads / 32;
 
 struct Sort {
     Indices index;
-    const uint32_t *keys, *from; // null in the first pass, which reads the indices
-    uint32_t *out_keys, *out_places;
+    const uint2 *from; // keys with their places; null in the first pass, which reads the indices
+    uint2 *out;
     uint32_t *counts; // [blocks][kBins] of this pass, as prefixes over the blocks if `totals` is not null
     uint32_t *totals; // [kBins]
     uint32_t *next;   // counts of the next pass, zero so far; null in the last one
@@ -219,6 +219,19 @@ __device__ __forceinline__ uint32_t key_at(const Indices &x, uint64_t i) {
 }
 __device__ __forceinline__ uint32_t digit_of(uint32_t key, uint32_t shift, uint32_t bits) {
     return key >> shift & ((1u << bits) - 1);
+}
+
+// The lanes whose digit is this lane's, a ballot for each bit (a match instruction takes about 100 cycles: the
+// sort of 131071 places took 40 us with it).
+__device__ __forceinline__ uint32_t lanes_alike(uint32_t digit, uint32_t bits) {
+    uint32_t same = 0xffffffffu;
+#pragma unroll
+    for (uint32_t b = 0; b < 9; ++b) {
+        if (b >= bits) break;
+        const uint32_t all = uint32_t(int32_t(digit << (31 - b)) >> 31); // the bit, everywhere
+        same &= ~(__ballot_sync(0xffffffffu, all != 0) ^ all);
+    }
+    return same;
 }
 
 // The first pass's counts; clears those of the passes behind it (`clear` words at s.next).
@@ -270,18 +283,21 @@ __global__ void __launch_bounds__(kThreads) k_sort_pass(const __grid_constant__ 
     for (uint32_t b = t; b < kWarps * kBins; b += kThreads) (&hist[0][0])[b] = 0;
     __syncthreads();
     cudaGridDependencySynchronize();
-    uint32_t key[kKeysPerThread], rank[kKeysPerThread];
+    uint32_t key[kKeysPerThread], place[kKeysPerThread], rank[kKeysPerThread];
     const uint32_t first = blockIdx.x * kSortKeys + warp * (kSortKeys / kWarps) + lane;
 #pragma unroll
     for (uint32_t j = 0; j < kKeysPerThread; ++j) {
         const uint32_t i = first + j * 32;
-        key[j] = i >= s.places ? kAbsent : s.keys ? s.keys[i] : key_at(s.index, i);
+        place[j] = i;
+        key[j] = kAbsent;
+        if (i < s.places && s.from) key[j] = s.from[i].x, place[j] = s.from[i].y;
+        else if (i < s.places) key[j] = key_at(s.index, i);
     }
 #pragma unroll
     for (uint32_t j = 0; j < kKeysPerThread; ++j) {
         const bool on = first + j * 32 < s.places; // the warp's first lanes, all of it but at the end
-        const uint32_t d = on ? digit_of(key[j], s.shift, s.bits) : kBins; // kBins: matches no digit
-        const uint32_t same = __match_any_sync(0xffffffffu, d);
+        const uint32_t d = digit_of(key[j], s.shift, s.bits);
+        const uint32_t same = lanes_alike(d, s.bits) & __ballot_sync(0xffffffffu, on);
         const uint32_t before = __popc(same & ((1u << lane) - 1));
         if (on) rank[j] = hist[warp][d] + before;
         __syncwarp();
@@ -336,31 +352,29 @@ __global__ void __launch_bounds__(kThreads) k_sort_pass(const __grid_constant__ 
         if (i >= s.places) continue;
         const uint32_t d = digit_of(key[j], s.shift, s.bits);
         const uint32_t to = base[d] + hist[warp][d] + rank[j];
-        s.out_keys[to] = key[j];
-        s.out_places[to] = s.from ? s.from[i] : i;
+        s.out[to] = make_uint2(key[j], place[j]);
         if (s.next) atomicAdd(&s.next[uint64_t(to / kSortKeys) * kBins + digit_of(key[j], s.next_shift, s.bits)], 1u);
     }
 }
 
-// Up to 16 blocks of a cluster sort up to 131072 keys in one launch: keys and places stay in shared memory,
-// the blocks' counts and each pass's scatter go through distributed shared memory. The other clusters of the
-// launch clear the output meanwhile: most of its rows are often absent, and it is written twice only where
-// a row is present.
+// Up to 16 blocks of a cluster sort up to 131072 keys in one launch; their counts go through distributed
+// shared memory, the keys through L2 (stores into other blocks' shared memory took no less). A pass takes about
+// 25,000 cycles, 8,000 of them for the ballots of the ranks. The other clusters of the launch clear the output
+// meanwhile: most of its rows are often absent, and it is written twice only where a row is present.
 constexpr uint32_t kClusterThreads = 1024, kClusterKeys = 8192, kPerThread = kClusterKeys / kClusterThreads;
 constexpr uint32_t kClusterWarps = kClusterThreads / 32, kMostCluster = 16;
 
 struct ClusterSort {
     Indices index;
-    uint32_t *out_keys, *out_places;
+    uint2 *out[2]; // the sorted keys, and room for a pass before the last
     char *clear;
     uint64_t clear_bytes;
     uint32_t places, passes, bits;
 };
 struct ClusterShared {
-    uint32_t key[2][kClusterKeys], place[2][kClusterKeys];
     uint16_t hist[kClusterWarps][kBins];
     uint32_t total[2][kBins]; // of this block, by parity of the pass
-    uint32_t base[kBins];
+    uint32_t base[kBins]; // where this block's keys of a digit begin
     uint32_t warp_sum[kClusterWarps];
 };
 
@@ -385,24 +399,31 @@ __global__ void __launch_bounds__(kClusterThreads, 1) k_sort_cluster(const __gri
                     uint64_t(gridDim.x - size) * kClusterThreads);
         return;
     }
-    // every block has kClusterKeys slots of the sorted order; those behind the last place hold kAbsent, which
-    // sorts last and keeps them there
-    for (uint32_t j = 0; j < kPerThread; ++j) {
-        const uint32_t k = j * kClusterThreads + t, i = me * kClusterKeys + k;
-        sh.key[0][k] = i < s.places ? key_at(s.index, i) : kAbsent;
-        sh.place[0][k] = i;
-    }
-    __syncthreads();
     for (uint32_t p = 0; p < s.passes; ++p) {
-        const uint32_t shift = p * s.bits, from = p & 1, to = from ^ 1;
+        const uint32_t shift = p * s.bits, parity = p & 1;
+        const bool last = p + 1 == s.passes;
+        // the last pass writes out[0]
+        uint2 *to = s.out[(s.passes - 1 - p) & 1];
+        const uint2 *from = s.out[(s.passes - p) & 1];
         for (uint32_t b = t; b < kClusterWarps * kBins / 2; b += kClusterThreads)
             reinterpret_cast<uint32_t *>(&sh.hist[0][0])[b] = 0;
         __syncthreads();
-        uint32_t key[kPerThread], rank[kPerThread];
+        uint2 key[kPerThread];
+        uint32_t rank[kPerThread];
+        const uint32_t first = me * kClusterKeys + warp * (kClusterKeys / kClusterWarps) + lane;
 #pragma unroll
         for (uint32_t j = 0; j < kPerThread; ++j) {
-            key[j] = sh.key[from][warp * (kClusterKeys / kClusterWarps) + j * 32 + lane];
-            const uint32_t d = digit_of(key[j], shift, s.bits), same = __match_any_sync(0xffffffffu, d);
+            // keys behind the last place sort behind all others and stay where they are
+            const uint32_t i = first + j * 32;
+            key[j] = make_uint2(kAbsent, i);
+            if (i < s.places) {
+                if (p) key[j] = __ldcg(from + i);
+                else key[j].x = key_at(s.index, i);
+            }
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < kPerThread; ++j) {
+            const uint32_t d = digit_of(key[j].x, shift, s.bits), same = lanes_alike(d, s.bits);
             const uint32_t before = __popc(same & ((1u << lane) - 1));
             rank[j] = sh.hist[warp][d] + before;
             __syncwarp();
@@ -418,13 +439,13 @@ __global__ void __launch_bounds__(kClusterThreads, 1) k_sort_cluster(const __gri
                 sh.hist[w][t] = uint16_t(sum);
                 sum += c;
             }
-            sh.total[from][t] = sum;
+            sh.total[parity][t] = sum;
         }
         cluster.sync();
         uint32_t all = 0, mine = 0;
         if (t < kBins) {
             for (uint32_t b = 0; b < size; ++b) {
-                const uint32_t c = cluster.map_shared_rank(&sh, b)->total[from][t];
+                const uint32_t c = cluster.map_shared_rank(&sh, b)->total[parity][t];
                 if (b < me) mine += c;
                 all += c;
             }
@@ -442,24 +463,20 @@ __global__ void __launch_bounds__(kClusterThreads, 1) k_sort_cluster(const __gri
             sh.base[t] = before;
         }
         __syncthreads();
-        const bool last = p + 1 == s.passes;
+        // (the last pass: nobody reads this block's counts any more; it need not wait for its own stores)
+        if (last) cluster.barrier_arrive();
 #pragma unroll
         for (uint32_t j = 0; j < kPerThread; ++j) {
-            const uint32_t d = digit_of(key[j], shift, s.bits);
+            const uint32_t d = digit_of(key[j].x, shift, s.bits);
             const uint32_t at = sh.base[d] + sh.hist[warp][d] + rank[j];
-            const uint32_t place = sh.place[from][warp * (kClusterKeys / kClusterWarps) + j * 32 + lane];
-            if (last) {
-                if (at < s.places) {
-                    s.out_keys[at] = key[j];
-                    s.out_places[at] = place;
-                }
-            } else {
-                ClusterShared *there = cluster.map_shared_rank(&sh, at / kClusterKeys);
-                there->key[to][at % kClusterKeys] = key[j];
-                there->place[to][at % kClusterKeys] = place;
-            }
+            if (at < s.places) to[at] = key[j];
         }
-        cluster.sync(); // the next pass's keys are there, and nobody reads this block's counts any more
+        if (last) {
+            cluster.barrier_wait();
+        } else {
+            __threadfence();
+            cluster.sync(); // the next pass's keys are there
+        }
     }
 }
 
@@ -468,7 +485,7 @@ __global__ void __launch_bounds__(kClusterThreads, 1) k_sort_cluster(const __gri
 struct Sums {
     const char *gradient;
     char *out;
-    const uint32_t *keys, *at; // sorted: the row, and the place
+    const uint2 *sorted; // the rows with their places
     void *partial;             // [2 chunks][width] of the wide type: rows that cross chunks
     uint64_t stride;           // bytes between the gradient's rows
     uint64_t width, rows;
@@ -486,17 +503,17 @@ __device__ __forceinline__ void write_sum(const Sums &a, uint32_t row, uint32_t 
     char *to = a.out + (uint64_t(row) * a.width + uint64_t(vector) * N) * sizeof(O);
 #pragma unroll
     for (int p = 0; p < N; p += PART) {
-        VectorOf<O, PART> v;
+        Packed<O, PART> v;
 #pragma unroll
-        for (int e = 0; e < PART; ++e) v.x[e] = to_element<O>(sum[p + e] * W(a.scale));
-        store_vector<O, PART>(to + p * sizeof(O), v);
+        for (int e = 0; e < PART; ++e) v.set(e, sum[p + e] * W(a.scale));
+        v.store(to + p * sizeof(O));
     }
 }
 
 // One vector of a row for each thread, over the places of one chunk. A row that lies inside the chunk is
 // done; the part of one that began earlier goes to partial 2c, of one that goes on to 2c + 1.
 template <uint32_t DT, uint32_t OT, int N>
-__global__ void __launch_bounds__(kThreads) k_sum_chunks(const __grid_constant__ Sums a) {
+__global__ void __launch_bounds__(kThreads, 3) k_sum_chunks(const __grid_constant__ Sums a) {
     using T = Element<DT>;
     using O = Element<OT>;
     using W = WideElement<DT>;
@@ -507,14 +524,17 @@ __global__ void __launch_bounds__(kThreads) k_sum_chunks(const __grid_constant__
     if (c >= a.chunks || vector >= a.vectors) return;
     cudaGridDependencySynchronize();
     const uint32_t i0 = c * a.chunk, i1 = min(a.places, i0 + a.chunk);
-    uint32_t row = a.keys[i0], begin = i0;
+    uint32_t row = a.sorted[i0].x, begin = i0;
     if (row == kAbsent) return;
     W sum[N];
+    const auto clear = [&] {
 #pragma unroll
-    for (int e = 0; e < N; ++e) sum[e] = W(0);
+        for (int e = 0; e < N; ++e) sum[e] = W(0);
+    };
+    clear();
     const auto flush = [&](uint32_t end) {
-        const bool starts = begin > i0 || i0 == 0 || a.keys[i0 - 1] != row;
-        const bool ends = end < i1 || i1 == a.places || a.keys[i1] != row;
+        const bool starts = begin > i0 || i0 == 0 || a.sorted[i0 - 1].x != row;
+        const bool ends = end < i1 || i1 == a.places || a.sorted[i1].x != row;
         if (starts && ends) {
             write_sum<T, O, W, N>(a, row, vector, sum);
         } else {
@@ -523,38 +543,27 @@ __global__ void __launch_bounds__(kThreads) k_sum_chunks(const __grid_constant__
             for (int e = 0; e < N; ++e) p[e] = sum[e];
         }
     };
-    // the keys and places of the next group are loaded while this one's rows are on their way
-    uint32_t key[kAhead], at[kAhead];
-    const auto group = [&](uint32_t i) {
-#pragma unroll
-        for (uint32_t j = 0; j < kAhead; ++j) {
-            key[j] = i + j < i1 ? a.keys[i + j] : kAbsent;
-            at[j] = i + j < i1 ? a.at[i + j] : 0;
-        }
-    };
-    group(i0);
-    const char *column = a.gradient + uint64_t(vector) * sizeof(VectorOf<T, N>);
+    const char *column = a.gradient + uint64_t(vector) * Packed<T, N>::BYTES;
     for (uint32_t i = i0; i < i1; i += kAhead) {
-        VectorOf<T, N> v[kAhead];
-        uint32_t now[kAhead];
+        Packed<T, N> v[kAhead];
+        uint32_t key[kAhead];
 #pragma unroll
         for (uint32_t j = 0; j < kAhead; ++j) {
-            if (key[j] != kAbsent) v[j] = load_vector<T, N>(column + uint64_t(at[j]) * a.stride);
-            now[j] = key[j];
+            const uint2 p = i + j < i1 ? a.sorted[i + j] : make_uint2(kAbsent, 0);
+            key[j] = p.x;
+            if (key[j] != kAbsent) v[j].load(column + uint64_t(p.y) * a.stride);
         }
-        group(i + kAhead);
 #pragma unroll
         for (uint32_t j = 0; j < kAhead; ++j) {
-            if (now[j] != row) {
+            if (key[j] != row) {
                 if (row != kAbsent) flush(i + j);
-                row = now[j];
+                row = key[j];
                 begin = i + j;
-#pragma unroll
-                for (int e = 0; e < N; ++e) sum[e] = W(0);
+                clear();
             }
-            if (now[j] == kAbsent) break;
+            if (key[j] == kAbsent) break;
 #pragma unroll
-            for (int e = 0; e < N; ++e) sum[e] += to_wide(v[j].x[e]);
+            for (int e = 0; e < N; ++e) sum[e] += v[j].wide(e);
         }
         if (row == kAbsent) return;
     }
@@ -562,11 +571,11 @@ __global__ void __launch_bounds__(kThreads) k_sum_chunks(const __grid_constant__
 }
 
 // The first place in the sorted keys that is not below `key`.
-__device__ __forceinline__ uint32_t first_not_below(const uint32_t *keys, uint32_t n, uint32_t key) {
+__device__ __forceinline__ uint32_t first_not_below(const uint2 *sorted, uint32_t n, uint32_t key) {
     uint32_t lo = 0, hi = n;
     while (lo < hi) {
         const uint32_t mid = lo + (hi - lo) / 2;
-        if (keys[mid] < key) lo = mid + 1;
+        if (sorted[mid].x < key) lo = mid + 1;
         else hi = mid;
     }
     return lo;
@@ -584,10 +593,17 @@ __global__ void __launch_bounds__(kThreads) k_join_chunks(const __grid_constant_
     const uint32_t c = blockIdx.x / groups, vector = blockIdx.x % groups * 32 + lane;
     cudaTriggerProgrammaticLaunchCompletion();
     cudaGridDependencySynchronize();
-    const uint32_t i0 = c * a.chunk, i1 = i0 + a.chunk, row = a.keys[i1 - 1];
-    if (row == kAbsent || a.keys[i1] != row) return;
-    if (a.keys[i0] == row && i0 != 0 && a.keys[i0 - 1] == row) return; // it began earlier
-    const uint32_t last = (first_not_below(a.keys, a.places, row + 1) - 1) / a.chunk;
+    const uint32_t i0 = c * a.chunk, i1 = i0 + a.chunk, row = a.sorted[i1 - 1].x;
+    if (row == kAbsent || a.sorted[i1].x != row) return;
+    if (a.sorted[i0].x == row && i0 != 0 && a.sorted[i0 - 1].x == row) return; // it began earlier
+    uint32_t last = c; // the chunk in which the row ends: the first one that does not end with it, or the last of all
+    for (bool on = true; on;) {
+        const uint32_t d = last + 1 + lane, end = (d + 1) * a.chunk;
+        const bool goes_on = d + 1 < a.chunks && a.sorted[end - 1].x == row && a.sorted[end].x == row;
+        const uint32_t stops = __ballot_sync(0xffffffffu, !goes_on);
+        on = stops == 0;
+        last += on ? 32 : __ffs(int(stops));
+    }
     // the first partial is 2c + 1, the others 2d for d = c + 1 .. last
     const uint32_t count = last - c, each = (count + kWarps - 1) / kWarps, lo = c + 1 + warp * each, hi = min(last + 1, lo + each);
     W sum[N];
@@ -623,8 +639,8 @@ template <uint32_t OT> __global__ void __launch_bounds__(kThreads) k_zero_rows(c
     cudaGridDependencySynchronize();
     bool absent = false;
     if (first + lane < a.rows) {
-        const uint32_t key = uint32_t(first) + lane, at = first_not_below(a.keys, a.places, key);
-        absent = at == a.places || a.keys[at] != key;
+        const uint32_t key = uint32_t(first) + lane, at = first_not_below(a.sorted, a.places, key);
+        absent = at == a.places || a.sorted[at].x != key;
     }
     O *out = reinterpret_cast<O *>(a.out);
     for (uint32_t m = __ballot_sync(0xffffffffu, absent); m; m &= m - 1) {
@@ -637,7 +653,7 @@ template <uint32_t OT> __global__ void __launch_bounds__(kThreads) k_zero_rows(c
 struct Project {
     const char *table, *sums;
     char *out;
-    const uint32_t *keys;
+    const uint2 *sorted;
     uint64_t table_stride, width, rows;
     uint32_t places, cleared; // rows without places are zero already
 };
@@ -648,9 +664,9 @@ __global__ void __launch_bounds__(kThreads) k_project(const __grid_constant__ Pr
     __shared__ double part[2][kWarps];
     const uint32_t row = blockIdx.x;
     cudaGridDependencySynchronize();
-    const uint32_t at = first_not_below(a.keys, a.places, row);
+    const uint32_t at = first_not_below(a.sorted, a.places, row);
     T *out = reinterpret_cast<T *>(a.out) + uint64_t(row) * a.width;
-    if (at == a.places || a.keys[at] != row) {
+    if (at == a.places || a.sorted[at].x != row) {
         if (a.cleared) return;
         for (uint64_t k = threadIdx.x; k < a.width; k += kThreads) out[k] = to_element<T>(W(0));
         return;
@@ -701,12 +717,10 @@ struct Direct {
     uint32_t aligned; // vectors start on their size; otherwise they are moved by elements
 };
 
-template <class T, int N> __device__ __forceinline__ VectorOf<T, N> load_any(const char *p, uint32_t aligned) {
-    if (aligned) return load_vector<T, N>(p);
-    VectorOf<T, N> v;
+template <class T, int N> __device__ __forceinline__ void load_any(Packed<T, N> &v, const char *p, uint32_t aligned) {
+    if (aligned) return v.load(p);
 #pragma unroll
-    for (int e = 0; e < N; ++e) v.x[e] = reinterpret_cast<const T *>(p)[e];
-    return v;
+    for (int e = 0; e < N; ++e) v.set(e, to_wide(reinterpret_cast<const T *>(p)[e]));
 }
 
 template <uint32_t DT, int N, bool BLOCK>
@@ -754,7 +768,7 @@ __global__ void __launch_bounds__(kThreads) k_direct(const __grid_constant__ Dir
             uint32_t same = __ballot_sync(0xffffffffu, b + lane < all && entry >> 16 == r);
             any = any || same;
             while (same) { // up to four places at a time
-                VectorOf<T, N> v[4][kDirectVectors];
+                Packed<T, N> v[4][kDirectVectors];
                 uint32_t n = 0;
 #pragma unroll
                 for (uint32_t q = 0; q < 4; ++q) {
@@ -766,7 +780,7 @@ __global__ void __launch_bounds__(kThreads) k_direct(const __grid_constant__ Dir
 #pragma unroll
                     for (uint32_t j = 0; j < kDirectVectors; ++j) {
                         const uint32_t k = vector0 + j * THREADS;
-                        if (k < a.vectors) v[q][j] = load_any<T, N>(from + uint64_t(k) * sizeof(v[q][j]), a.aligned);
+                        if (k < a.vectors) load_any<T, N>(v[q][j], from + uint64_t(k) * Packed<T, N>::BYTES, a.aligned);
                     }
                 }
 #pragma unroll
@@ -776,7 +790,7 @@ __global__ void __launch_bounds__(kThreads) k_direct(const __grid_constant__ Dir
                         for (uint32_t j = 0; j < kDirectVectors; ++j)
                             if (vector0 + j * THREADS < a.vectors)
 #pragma unroll
-                                for (int e = 0; e < N; ++e) sum[j][e] += to_wide(v[q][j].x[e]);
+                                for (int e = 0; e < N; ++e) sum[j][e] += v[q][j].wide(e);
             }
         }
 #pragma unroll
@@ -785,7 +799,7 @@ __global__ void __launch_bounds__(kThreads) k_direct(const __grid_constant__ Dir
             for (int e = 0; e < N; ++e) sum[j][e] *= W(a.scale);
         const uint64_t row = uint64_t(row0) + r;
         double along = 0.0, inverse = 1.0;
-        VectorOf<T, N> unit[kDirectVectors];
+        Packed<T, N> unit[kDirectVectors];
         if (a.table && any) { // the same in all threads of the row
             const char *from = a.table + row * a.table_stride;
             double tt = 0.0, ts = 0.0;
@@ -793,10 +807,10 @@ __global__ void __launch_bounds__(kThreads) k_direct(const __grid_constant__ Dir
             for (uint32_t j = 0; j < kDirectVectors; ++j) {
                 const uint32_t k = vector0 + j * THREADS;
                 if (k >= a.vectors) continue;
-                unit[j] = load_any<T, N>(from + uint64_t(k) * sizeof(unit[j]), a.aligned);
+                load_any<T, N>(unit[j], from + uint64_t(k) * Packed<T, N>::BYTES, a.aligned);
 #pragma unroll
                 for (int e = 0; e < N; ++e) {
-                    const double x = to_wide(unit[j].x[e]);
+                    const double x = unit[j].wide(e);
                     tt = fma(x, x, tt);
                     ts = fma(x, double(sum[j][e]), ts);
                 }
@@ -812,18 +826,18 @@ __global__ void __launch_bounds__(kThreads) k_direct(const __grid_constant__ Dir
         for (uint32_t j = 0; j < kDirectVectors; ++j) {
             const uint32_t k = vector0 + j * THREADS;
             if (k >= a.vectors) continue;
-            VectorOf<T, N> y;
+            Packed<T, N> y;
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 W x = sum[j][e];
-                if (a.table && any) x = W((double(x) - double(to_wide(unit[j].x[e])) * along) * inverse);
-                y.x[e] = to_element<T>(x);
+                if (a.table && any) x = W((double(x) - double(unit[j].wide(e)) * along) * inverse);
+                y.set(e, x);
             }
-            char *to = a.out + row * a.row_bytes + uint64_t(k) * sizeof(y);
-            if (a.aligned) store_vector<T, N>(to, y);
+            char *to = a.out + row * a.row_bytes + uint64_t(k) * Packed<T, N>::BYTES;
+            if (a.aligned) y.store(to);
             else
 #pragma unroll
-                for (int e = 0; e < N; ++e) reinterpret_cast<T *>(to)[e] = y.x[e];
+                for (int e = 0; e < N; ++e) reinterpret_cast<T *>(to)[e] = to_element<T>(y.wide(e));
         }
     }
 }
@@ -958,7 +972,7 @@ uint32_t most_pieces(const ArcqmlRows &t, const ArcqmlEmbeddingOptions &o) {
 
 // Scratch of the gradient, in 4-byte words from its start.
 struct GradientScratch {
-    uint64_t keys[2], places[2], counts, totals, partial, sums, words;
+    uint64_t sorted[2], counts, totals, partial, sums, words;
     uint32_t blocks, passes, bits, chunk, chunks;
 };
 
@@ -980,9 +994,8 @@ GradientScratch gradient_scratch(const ArcqmlRows &g, uint64_t rows, const Arcqm
     s.bits = (bits + s.passes - 1) / s.passes;
     s.blocks = uint32_t((n + kSortKeys - 1) / kSortKeys);
     const bool in_cluster = n <= kClusterKeys * kMostCluster;
-    for (int i = 0; i < (in_cluster ? 1 : 2); ++i) {
-        s.keys[i] = take(n);
-        s.places[i] = take(n);
+    for (int i = 0; i < 2; ++i) {
+        s.sorted[i] = take(2 * n);
     }
     if (!in_cluster) {
         s.counts = take(uint64_t(s.passes) * s.blocks * kBins);
@@ -1109,12 +1122,13 @@ void embedding_gradient_device(const ArcqmlRows &gradient, const void *indices, 
     }
     uint32_t *base = reinterpret_cast<uint32_t *>(ws);
     const bool in_cluster = n <= kClusterKeys * kMostCluster;
-    const uint32_t *keys = base + w.keys[in_cluster ? 0 : w.passes & 1], *places = base + w.places[in_cluster ? 0 : w.passes & 1];
+    uint2 *buffers[2] = {reinterpret_cast<uint2 *>(base + w.sorted[0]), reinterpret_cast<uint2 *>(base + w.sorted[1])};
+    const uint2 *sorted = buffers[in_cluster ? 0 : w.passes & 1];
     if (in_cluster) {
         ClusterSort a{};
         a.index = index;
-        a.out_keys = base + w.keys[0];
-        a.out_places = base + w.places[0];
+        a.out[0] = buffers[0];
+        a.out[1] = buffers[1];
         a.clear = static_cast<char *>(out.data);
         a.clear_bytes = out.rows * row;
         a.places = uint32_t(n);
@@ -1142,10 +1156,8 @@ void embedding_gradient_device(const ArcqmlRows &gradient, const void *indices, 
             a.next_shift = a.shift + w.bits;
             a.counts = base + w.counts + p * each;
             a.next = p + 1 < w.passes ? a.counts + each : nullptr;
-            a.keys = p ? base + w.keys[p & 1] : nullptr;
-            a.from = p ? base + w.places[p & 1] : nullptr;
-            a.out_keys = base + w.keys[(p + 1) & 1];
-            a.out_places = base + w.places[(p + 1) & 1];
+            a.from = p ? buffers[p & 1] : nullptr;
+            a.out = buffers[(p + 1) & 1];
             a.totals = nullptr;
             if (w.blocks > 128) {
                 a.totals = base + w.totals;
@@ -1156,8 +1168,7 @@ void embedding_gradient_device(const ArcqmlRows &gradient, const void *indices, 
     }
     Sums a{};
     a.gradient = static_cast<const char *>(gradient.data);
-    a.keys = keys;
-    a.at = places;
+    a.sorted = sorted;
     a.partial = base + w.partial;
     a.stride = gradient.stride * size;
     a.width = out.width;
@@ -1178,7 +1189,8 @@ void embedding_gradient_device(const ArcqmlRows &gradient, const void *indices, 
         const auto sums = [&](auto kind) {
             constexpr uint32_t OT = kind;
             if (!n) return;
-            start(k_sum_chunks<DT, OT, N>, {blocks_for(uint64_t(a.chunks) * a.tiles * a.lanes), kThreads, true}, moved, s, a);
+            const Shape shape{blocks_for(uint64_t(a.chunks) * a.tiles * a.lanes), kThreads, true};
+            start(k_sum_chunks<DT, OT, N>, shape, moved, s, a);
             if (a.chunks > 1)
                 start(k_join_chunks<DT, OT, N>, {uint64_t(a.chunks - 1) * ((a.vectors + 31) / 32), kThreads, true}, 0.0, s, a);
         };
@@ -1199,7 +1211,7 @@ void embedding_gradient_device(const ArcqmlRows &gradient, const void *indices, 
         p.table = static_cast<const char *>(table->data);
         p.sums = a.out;
         p.out = static_cast<char *>(out.data);
-        p.keys = keys;
+        p.sorted = sorted;
         p.table_stride = table->stride * size;
         p.width = out.width;
         p.rows = out.rows;
