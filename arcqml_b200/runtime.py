@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from bisect import bisect_left
 from typing import Optional, Sequence
 
@@ -1012,15 +1013,19 @@ def orthogonalize_device(matrices, steps: int = 5, eps: float = 1e-7, out=None, 
         if [a is None for a in x.tensors] != [b is None for b in y.tensors]:
             raise ValueError("outputs and matrices must have the same empty places")
     on, ws = _scratch(torch, device, x._matrix_words, stream)
-    if not given:
-        y = TensorList(_on_stream(torch, stream, lambda: [
-            None if t is None else torch.empty_like(t) for t in x.tensors]))
-    _status(load().arcqml_rt_v2_orthogonalize(
-        table, y._as_matrices("the outputs"), len(x), int(steps), float(eps),
-        None if ws is None else ws.data_ptr(), x._matrix_words, on))
+    if given:
+        outputs, to = list(y.tensors), y._as_matrices("the outputs")
+    else:  # of the matrices' shapes and types: their table with other addresses
+        outputs = _on_stream(torch, stream, lambda: [
+            None if t is None else torch.empty_like(t) for t in x.tensors])
+        rows = x._matrices.copy()
+        rows["data"][:len(outputs)] = [0 if t is None else t.data_ptr() for t in outputs]
+        to = rows.ctypes.data
+    _status(load().arcqml_rt_v2_orthogonalize(table, to, len(x), int(steps), float(eps),
+                                              None if ws is None else ws.data_ptr(), x._matrix_words, on))
     if given:
         y._written(torch)
-    return list(y.tensors)
+    return outputs
 
 
 class DeviceMuonState:
@@ -1122,56 +1127,60 @@ def _scratch(torch, device: int, words: int, stream):
 # ------------------------------------------------------------------ tables looked up by index
 
 
-class EmbeddingRows(C.Structure):
-    _fields_ = [("data", C.c_void_p), ("rows", C.c_uint64), ("width", C.c_uint64), ("stride", C.c_uint64),
-                ("dtype", C.c_uint32), ("reserved", C.c_uint32)]
-
-
-class EmbeddingOptions(C.Structure):
-    _fields_ = [("scale", C.c_double), ("padding", C.c_int64), ("normalize", C.c_int32),
-                ("index_bytes", C.c_int32)]
+# ArcqmlRows and ArcqmlEmbeddingOptions as bytes: a ctypes structure costs three times as much to fill
+_EMBEDDING_ROWS, _EMBEDDING_OPTIONS = struct.Struct("=QQQQII").pack, struct.Struct("=dqii").pack
 
 
 def _embedding_rows(torch, t, outer: int, name: str, device: int):
-    """A tensor as rows: its first `outer` dimensions count them, the others are a row."""
+    """A tensor as rows, its first `outer` dimensions counting them, the others a row: (rows, elements of a
+    row, the tensor as ArcqmlRows)."""
     kind = _tensor_kinds().get(t.dtype) if isinstance(t, torch.Tensor) else None
     if kind is None or not t.is_cuda or t.layout != torch.strided or t.is_conj() or t.is_neg():
         raise TypeError(f"{name} must be a dense float64, float32, bfloat16, float16 or complex CUDA tensor: "
                         f"got {_kind_of(torch, t)}")
     if t.get_device() != device:
         raise RuntimeError(f"{name} is on cuda:{t.get_device()} and the current device is cuda:{device}")
-    if t.dim() <= outer:
-        raise TypeError(f"{name} has no dimension for its rows' elements: its shape is {list(t.shape)}")
-    shape, strides = t.shape, t.stride()
-    width, rows = 1, 1
-    fits = True
-    for n, st in zip(reversed(shape[outer:]), reversed(strides[outer:])):
-        fits = fits and (n == 1 or st == width)
-        width *= n
-    step = None  # between one row and the next
-    for n, st in zip(reversed(shape[:outer]), reversed(strides[:outer])):
-        if n != 1:
-            fits = fits and (step is None or st == step * rows)
-            step = st if step is None else step
-        rows *= n
-    if not fits and rows and width:
-        raise TypeError(f"{name} must have rows without gaps at equal distances: got shape {list(shape)} with "
-                        f"strides {list(strides)}")
-    return EmbeddingRows(t.data_ptr(), rows, width * kind[1], (width if step is None else step) * kind[1],
-                         kind[0], 0)
+    shape = t.shape
+    if len(shape) <= outer:
+        raise TypeError(f"{name} has no dimension for its rows' elements: its shape is {list(shape)}")
+    width, rows, step = 1, 1, None
+    if t.is_contiguous():
+        for n in shape[:outer]:
+            rows *= n
+        for n in shape[outer:]:
+            width *= n
+        step = width
+    else:
+        strides, fits = t.stride(), True
+        for n, st in zip(reversed(shape[outer:]), reversed(strides[outer:])):
+            fits = fits and (n == 1 or st == width)
+            width *= n
+        for n, st in zip(reversed(shape[:outer]), reversed(strides[:outer])):
+            if n != 1:
+                fits = fits and (step is None or st == step * rows)
+                step = st if step is None else step
+            rows *= n
+        if not fits and rows and width:
+            raise TypeError(f"{name} must have rows without gaps at equal distances: got shape {list(shape)} "
+                            f"with strides {list(strides)}")
+        step = width if step is None else step
+    code, parts, _ = kind
+    return rows, width * parts, _EMBEDDING_ROWS(t.data_ptr(), rows, width * parts, step * parts, code, 0)
 
 
 def _embedding_call(torch, indices, scale, normalize, padding, device: int):
-    if not (isinstance(indices, torch.Tensor) and indices.is_cuda
-            and indices.dtype in (torch.int64, torch.int32)):
+    """(options, indices next to each other)"""
+    kind = indices.dtype if isinstance(indices, torch.Tensor) and indices.is_cuda else None
+    if kind != torch.int64 and kind != torch.int32:
         raise TypeError("indices must be an int64 or int32 CUDA tensor")
     if indices.get_device() != device:
         raise RuntimeError(f"the indices are on cuda:{indices.get_device()} and the current device is "
                            f"cuda:{device}")
-    if padding is not None and int(padding) < 0:
+    if padding is None:
+        padding = -1
+    elif padding < 0:
         raise ValueError("the padding index must not be negative")
-    return EmbeddingOptions(float(scale), -1 if padding is None else int(padding), bool(normalize),
-                            8 if indices.dtype == torch.int64 else 4)
+    return _EMBEDDING_OPTIONS(scale, padding, bool(normalize), 8 if kind == torch.int64 else 4)
 
 
 def embedding_lookup_device(table, indices, scale: float = 1.0, normalize: bool = False, padding=None,
@@ -1182,20 +1191,25 @@ def embedding_lookup_device(table, indices, scale: float = 1.0, normalize: bool 
     whose index is `padding` are zero. An index outside the table gives NaN: refusing it would wait for the
     device."""
     import torch
+    if stream is not None:
+        with torch.cuda.stream(torch.cuda.ExternalStream(int(stream))):
+            return embedding_lookup_device(table, indices, scale, normalize, padding)
     device = torch.cuda.current_device()
-    rows = _embedding_rows(torch, table, 1, "the table", device)
+    _, width, rows = _embedding_rows(torch, table, 1, "the table", device)
     options = _embedding_call(torch, indices, scale, normalize, padding, device)
-    make = lambda: (indices.contiguous(), table.new_empty(indices.shape + table.shape[1:]))  # noqa: E731
-    x, out = _on_stream(torch, stream, make)
-    n = x.numel()
-    if out.numel():
-        to = EmbeddingRows(out.data_ptr(), n, rows.width, rows.width, rows.dtype, 0)
-        lib = load()
-        words = lib.arcqml_rt_v2_embedding_lookup_workspace(C.byref(rows), n, C.byref(options)) if normalize else 0
-        on, ws = _scratch(torch, device, words, stream)
+    if not indices.is_contiguous():
+        indices = indices.contiguous()
+    out = table.new_empty(indices.shape + table.shape[1:])
+    n = indices.numel()
+    if n and width:
+        lib, ws, words = load(), None, 0
+        if normalize:
+            words = lib.arcqml_rt_v2_embedding_lookup_workspace(rows, n, options)
+            ws = torch.empty(words, dtype=torch.float64, device=table.device) if words else None
+        kind = _tensor_kinds()[out.dtype][0]
         _status(lib.arcqml_rt_v2_embedding_lookup(
-            C.byref(rows), x.data_ptr(), n, C.byref(options), C.byref(to),
-            None if ws is None else ws.data_ptr(), words, on))
+            rows, indices.data_ptr(), n, options, _EMBEDDING_ROWS(out.data_ptr(), n, width, width, kind, 0),
+            None if ws is None else ws.data_ptr(), words, torch._C._cuda_getCurrentRawStream(device)))
     return out
 
 
@@ -1206,30 +1220,35 @@ def embedding_gradient_device(gradient, indices, rows: int, scale: float = 1.0, 
     zeros where there is none. With `table` the lookup was a normalised one of that table, and the sum is
     taken through the rows' norms. A row's places are added in their order: equal inputs give equal bits."""
     import torch
+    if stream is not None:
+        with torch.cuda.stream(torch.cuda.ExternalStream(int(stream))):
+            return embedding_gradient_device(gradient, indices, rows, scale, table, padding)
     device = torch.cuda.current_device()
     options = _embedding_call(torch, indices, scale, table is not None, padding, device)
-    if not isinstance(gradient, torch.Tensor) or gradient.shape[:indices.dim()] != indices.shape:
+    outer = indices.dim()
+    if not isinstance(gradient, torch.Tensor) or gradient.shape[:outer] != indices.shape:
         raise ValueError("the gradient must have a row for each index")
-    g = _embedding_rows(torch, gradient, indices.dim(), "the gradient", device)
+    _, width, g = _embedding_rows(torch, gradient, outer, "the gradient", device)
     rows = int(rows)
     if rows < 0:
         raise ValueError("a table has no negative number of rows")
-    inner = gradient.shape[indices.dim():]
+    shape = (rows,) + gradient.shape[outer:]
     t = None
     if table is not None:
-        t = _embedding_rows(torch, table, 1, "the table", device)
-        if table.dtype != gradient.dtype or table.shape != (rows,) + tuple(inner):
-            raise ValueError(f"the table must be {gradient.dtype} of shape {[rows, *inner]}")
-    make = lambda: (indices.contiguous(), gradient.new_empty((rows,) + tuple(inner)))  # noqa: E731
-    x, out = _on_stream(torch, stream, make)
-    if out.numel():
-        to = EmbeddingRows(out.data_ptr(), rows, g.width, g.width, g.dtype, 0)
+        _, _, t = _embedding_rows(torch, table, 1, "the table", device)
+        if table.dtype != gradient.dtype or table.shape != shape:
+            raise ValueError(f"the table must be {gradient.dtype} of shape {list(shape)}")
+    if not indices.is_contiguous():
+        indices = indices.contiguous()
+    out = gradient.new_empty(shape)
+    if rows and width:
         lib = load()
-        words = lib.arcqml_rt_v2_embedding_gradient_workspace(C.byref(g), rows, C.byref(options))
-        on, ws = _scratch(torch, device, words, stream)
+        words = lib.arcqml_rt_v2_embedding_gradient_workspace(g, rows, options)
+        ws = torch.empty(words, dtype=torch.float64, device=out.device) if words else None
+        kind = _tensor_kinds()[out.dtype][0]
         _status(lib.arcqml_rt_v2_embedding_gradient(
-            C.byref(g), x.data_ptr(), C.byref(options), None if t is None else C.byref(t), C.byref(to),
-            None if ws is None else ws.data_ptr(), words, on))
+            g, indices.data_ptr(), options, t, _EMBEDDING_ROWS(out.data_ptr(), rows, width, width, kind, 0),
+            None if ws is None else ws.data_ptr(), words, torch._C._cuda_getCurrentRawStream(device)))
     return out
 
 
