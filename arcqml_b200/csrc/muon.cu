@@ -12,6 +12,11 @@
 // the sums' own rounding). An update far below epsilon makes a small X, which grows by at most 3.4445 a step:
 // it is stored 2^k times as large, k from its norm, and k falls by 2 a step until it is 0.
 //
+// The diagonals of A and P, by far their largest entries, stay in f32 beside the operands, which hold zeros
+// there: with A = D + O, A^2 = O^2 + D O + O D + D^2, and the last terms, like diag(P) X, are formed where
+// sums are taken out. With the diagonals rounded to 11 bits, results of bf16 matrices were 1.3e-3 to 5.8e-3
+// off before their own rounding (a 4 x 266 matrix), without them 6e-4 to 9e-4 (a model of the roundings).
+//
 // Layout in the scratch: X, A and P in blocks of 128 rows x 64 columns, 16 KB each, row by row with their
 // 16-byte pieces permuted as the tensor cores want them in shared memory. So every copy is one run of 8 or
 // 16 KB that needs no tensor map, matrices of any size and address share a launch, and one block of X
@@ -26,6 +31,7 @@
 #include <sstream>
 #include <string>
 #include <tuple>
+#include <type_traits>
 #include <vector>
 
 #include "elements.cuh"
@@ -54,6 +60,7 @@ struct Matrix {
     const void *in;  // the matrix, or the gradient
     float *momentum; // null without a step
     uint64_t x[2], a, p; // offsets in the scratch; low parts lie behind their high parts
+    uint64_t diagonal;   // of A, and behind it of P: f32, as large as the operands are stored
     uint32_t m, n;       // of X
     uint32_t down_blocks, x_blocks, a_blocks; // blocks of X down, and across X and A
     uint8_t flip, out_type, in_type, nesterov;
@@ -476,6 +483,12 @@ __device__ __forceinline__ void give_result(const Matrix &a, float (&v)[N], uint
     __syncwarp();
 }
 
+// An entry of P from that of A off its diagonal (x), the sum of products off the diagonal, and the diagonal's
+// entries of its row and column.
+__device__ __forceinline__ float combine(float x, float sum, float row, float column, bool diagonal, float of_old, float of_sum) {
+    return diagonal ? of_old * row + of_sum * (sum + row * row) : of_old * x + of_sum * (sum + (row + column) * x);
+}
+
 // 32 neighbouring sums of a row, for each thread of a warp, become what the phase stores.
 template <int PHASE, bool SPLIT>
 __device__ __forceinline__ void take_sums(const Group &g, const Matrix &a, float (&v)[32], uint32_t row, uint32_t column,
@@ -493,13 +506,32 @@ __device__ __forceinline__ void take_sums(const Group &g, const Matrix &a, float
     const uint64_t low = bytes_of(a.down_blocks, across);
     const char *old = g.scratch + (PHASE == APPLY ? a.x[current] : a.a);
     char *to = g.scratch + (PHASE == APPLY ? a.x[current ^ 1] : PHASE == GRAM ? a.a : a.p);
+    float *of_a = reinterpret_cast<float *>(g.scratch + a.diagonal), *of_p = of_a + a.down_blocks * kRows;
+    const float mine = PHASE == GRAM ? 0.0f : PHASE == POLYNOMIAL ? of_a[row] : of_old + of_p[row] * of_sum;
+    const uint32_t own = row - column; // the diagonal's place among the 32, if below that
 #pragma unroll
     for (uint32_t q = 0; q < 32; q += 8) {
         const uint64_t place = place_of(row, column + q, across);
         float x[8];
         if constexpr (PHASE != GRAM) load_operand<SPLIT>(x, old + place, low);
+        if constexpr (PHASE == POLYNOMIAL) {
+            const float4 d[2] = {*reinterpret_cast<const float4 *>(of_a + column + q),
+                                 *reinterpret_cast<const float4 *>(of_a + column + q + 4)};
+            const float *other = &d[0].x;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = v[q + e] = PHASE == GRAM ? v[q + e] * of_sum : of_old * x[e] + v[q + e] * of_sum;
+            for (int e = 0; e < 8; ++e) v[q + e] = combine(x[e], v[q + e], mine, other[e], q + e == own, of_old, of_sum);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[q + e] = PHASE == GRAM ? v[q + e] * of_sum : mine * x[e] + v[q + e] * of_sum;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (PHASE != APPLY && q + e == own) {
+                (PHASE == GRAM ? of_a : of_p)[row] = v[q + e];
+                v[q + e] = 0.0f;
+            }
+            x[e] = v[q + e];
+        }
         if (PHASE != APPLY || !last) store_operand<SPLIT>(to + place, low, x);
     }
     if (PHASE != APPLY && mirrored) { // lanes in pairs, each with two rows of one column
@@ -795,9 +827,11 @@ __global__ void __launch_bounds__(kThreads) k_check_fault(const __grid_constant_
 // A matrix of at most 128 rows of X whose operands fit into a block's shared memory is orthogonalised by
 // that block from its update to its result: one launch for a list, 15 rounds of a few hundred cycles each.
 constexpr uint32_t kSmallThreads = 256;
+static_assert(kSmallThreads == 2 * kRows, "a thread for each diagonal entry of A and P");
 template <bool SPLIT> constexpr uint32_t kSmallBlocks = SPLIT ? 4 : 8; // of X: 256 or 512 columns
 template <bool SPLIT> constexpr uint32_t kSmallShared =
-    1024 + (kSmallBlocks<SPLIT> + 2) * (SPLIT ? 2 : 1) * kBlock + 256 + kSmallThreads / 32 * 32 * 17 * sizeof(float);
+    1024 + (kSmallBlocks<SPLIT> + 2) * (SPLIT ? 2 : 1) * kBlock + 256 + kSmallThreads / 32 * 32 * 17 * sizeof(float) +
+    2 * kRows * sizeof(float);
 
 struct SmallState {
     uint64_t done;
@@ -816,6 +850,8 @@ template <bool SPLIT> __global__ void __launch_bounds__(kSmallThreads, 1)
     const Matrix &a = g.matrix[blockIdx.x];
     const uint32_t thread = threadIdx.x, warp = thread / 32, lane = thread % 32;
     float *square = reinterpret_cast<float *>(reinterpret_cast<char *>(&st) + 256) + warp * 32 * 17;
+    float *of_a = reinterpret_cast<float *>(reinterpret_cast<char *>(&st) + 256) + kSmallThreads / 32 * 32 * 17, *of_p = of_a + kRows;
+    of_a[thread] = 0.0f; // both: rows behind the matrix keep it
     if (thread == 0) {
         tc::barrier_init(&st.done, 1);
         st.stop = 0;
@@ -868,7 +904,9 @@ template <bool SPLIT> __global__ void __launch_bounds__(kSmallThreads, 1)
     const uint32_t x_at = tc::shared_address(x), p_at = tc::shared_address(p);
     uint32_t parity = 0;
     bool broken = false;
-    // steps of 16 of the depth; operands by depth, or the right one by width
+    // steps of 16 of the depth; operands by depth, or the right one by width. Products with low parts have sums
+    // of their own: a long chain of additions to the high parts' would cost as much again (see kChain)
+    constexpr uint32_t CROSS = 256;
     const auto multiply = [&](uint32_t sums, uint32_t left, uint32_t left_low, uint32_t right, uint32_t right_low,
                               uint32_t depth, uint32_t columns, bool by_width) {
         const uint32_t instr = tc::instruction(128, columns, by_width);
@@ -877,8 +915,8 @@ template <bool SPLIT> __global__ void __launch_bounds__(kSmallThreads, 1)
             const uint32_t apart = by_width ? kBlock : 16;
             tc::mma<1>(sums, tc::descriptor(left + by_depth, 16), tc::descriptor(right + along, apart), instr, k != 0);
             if constexpr (SPLIT) {
-                tc::mma<1>(sums, tc::descriptor(left + by_depth, 16), tc::descriptor(right_low + along, apart), instr, true);
-                tc::mma<1>(sums, tc::descriptor(left_low + by_depth, 16), tc::descriptor(right + along, apart), instr, true);
+                tc::mma<1>(sums + CROSS, tc::descriptor(left + by_depth, 16), tc::descriptor(right_low + along, apart), instr, k != 0);
+                tc::mma<1>(sums + CROSS, tc::descriptor(left_low + by_depth, 16), tc::descriptor(right + along, apart), instr, true);
             }
         }
     };
@@ -895,49 +933,68 @@ template <bool SPLIT> __global__ void __launch_bounds__(kSmallThreads, 1)
         __syncthreads();
         tc::fence_after();
     };
-    for (int step = 0; step < steps; ++step) {
+    int step = 0;
+    const auto run_phase = [&](auto which) {
+        constexpr int PHASE = which;
         const int next = max(0, shift - 2);
-        for (int phase = GRAM; phase <= APPLY; ++phase) {
-            const uint32_t columns = phase == APPLY ? n16 : m16;
-            if (thread == 0) {
-                if (phase == GRAM) multiply(tmem, x_at, x_at + LOW, x_at, x_at + LOW, n16, m16, false);
-                else if (phase == POLYNOMIAL) multiply(tmem, p_at, p_at + 2 * kBlock, p_at, p_at + 2 * kBlock, m16, m16, false);
-                else
-                    for (uint32_t c = 0; c < n16; c += 256)
-                        multiply(tmem + c, p_at, p_at + 2 * kBlock, x_at + c / kDepth * kBlock, x_at + LOW + c / kDepth * kBlock,
-                                 m16, min(256u, n16 - c), true);
-                tc::commit<1>(&st.done);
-            }
-            if (!sums_ready()) break;
-            const float of_sum = phase == GRAM         ? 1.0f / kScaleX
-                                 : phase == POLYNOMIAL ? ldexpf(0.5f * kC / kScaleX, -4 * shift)
-                                                       : ldexpf(2.0f / kScaleX, next - shift);
-            const float of_old = phase == GRAM ? 0.0f : phase == POLYNOMIAL ? ldexpf(0.5f * kB, -2 * shift) : ldexpf(kA, next - shift);
-            char *to = phase == APPLY ? x : p;
-            const uint64_t low = phase == APPLY ? LOW : 2 * kBlock;
-            const uint32_t across = phase == APPLY ? kSmallBlocks<SPLIT> : 2;
+        const uint32_t columns = PHASE == APPLY ? n16 : m16;
+        if (thread == 0) {
+            if (PHASE == GRAM) multiply(tmem, x_at, x_at + LOW, x_at, x_at + LOW, n16, m16, false);
+            else if (PHASE == POLYNOMIAL) multiply(tmem, p_at, p_at + 2 * kBlock, p_at, p_at + 2 * kBlock, m16, m16, false);
+            else
+                for (uint32_t c = 0; c < n16; c += 256)
+                    multiply(tmem + c, p_at, p_at + 2 * kBlock, x_at + c / kDepth * kBlock, x_at + LOW + c / kDepth * kBlock,
+                             m16, min(256u, n16 - c), true);
+            tc::commit<1>(&st.done);
+        }
+        const float of_sum = PHASE == GRAM         ? 1.0f / kScaleX
+                             : PHASE == POLYNOMIAL ? ldexpf(0.5f * kC / kScaleX, -4 * shift)
+                                                   : ldexpf(2.0f / kScaleX, next - shift);
+        const float of_old = PHASE == GRAM ? 0.0f : PHASE == POLYNOMIAL ? ldexpf(0.5f * kB, -2 * shift) : ldexpf(kA, next - shift);
+        const float diagonal = PHASE == GRAM ? 0.0f : PHASE == POLYNOMIAL ? of_a[row] : of_old + of_p[row] * of_sum;
+        char *to = PHASE == APPLY ? x : p;
+        constexpr uint64_t low = PHASE == APPLY ? LOW : 2 * kBlock;
+        constexpr uint32_t across = PHASE == APPLY ? kSmallBlocks<SPLIT> : 2;
+        if (!sums_ready()) return;
 #pragma unroll 1
-            for (uint32_t c = warp / 4 * 16; c < columns; c += 32) {
-                float v[16];
+        for (uint32_t c = warp / 4 * 16; c < columns; c += 32) {
+            float v[16];
+            if constexpr (SPLIT) {
+                tc::tmem_load2(v, mine + c, mine + CROSS + c);
+            } else {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) v[e] = 0.0f;
                 tc::tmem_add(v, mine + c);
-#pragma unroll
-                for (uint32_t q = 0; q < 16; q += 8) {
-                    char *at = to + place_of(row, c + q, across);
-                    float y[8];
-                    if (phase != GRAM) load_operand<SPLIT>(y, at, low);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        y[e] = v[q + e] = phase == GRAM ? v[q + e] * of_sum : of_old * y[e] + v[q + e] * of_sum;
-                    store_operand<SPLIT>(at, low, y);
-                }
-                if (phase == APPLY && step + 1 == steps) give_result(a, v, row, c, next, square);
             }
-            operands_ready();
+            const uint32_t own = row - c;
+#pragma unroll
+            for (uint32_t q = 0; q < 16; q += 8) {
+                char *at = to + place_of(row, c + q, across);
+                float y[8];
+                if constexpr (PHASE != GRAM) load_operand<SPLIT>(y, at, low);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    float &z = v[q + e];
+                    if constexpr (PHASE == GRAM) z *= of_sum;
+                    else if constexpr (PHASE == APPLY) z = diagonal * y[e] + z * of_sum;
+                    else z = combine(y[e], z, diagonal, of_a[c + q + e], q + e == own, of_old, of_sum);
+                    if (PHASE != APPLY && q + e == own) {
+                        (PHASE == GRAM ? of_a : of_p)[row] = z;
+                        z = 0.0f;
+                    }
+                    y[e] = z;
+                }
+                store_operand<SPLIT>(at, low, y);
+            }
+            if (PHASE == APPLY && step + 1 == steps) give_result(a, v, row, c, next, square);
         }
-        if (broken) break;
-        shift = next;
+        operands_ready();
+    };
+    for (; step < steps && !broken; ++step) {
+        run_phase(std::integral_constant<int, GRAM>{});
+        if (!broken) run_phase(std::integral_constant<int, POLYNOMIAL>{});
+        if (!broken) run_phase(std::integral_constant<int, APPLY>{});
+        shift = max(0, shift - 2);
     }
     if (broken)
         for (uint64_t i = thread; i < all; i += kSmallThreads) store1(a.out, a.out_type, i, __int_as_float(0x7fffffff));
@@ -1019,11 +1076,11 @@ bool is_small(const ArcqmlMatrix &a, bool split) {
     return m <= kRows && n <= (split ? kSmallBlocks<true> : kSmallBlocks<false>) * kDepth;
 }
 
-// Scratch bytes of a matrix's X (twice), A and P.
+// Scratch bytes of a matrix's X (twice), A, P and their diagonals.
 uint64_t operand_bytes(const ArcqmlMatrix &a, bool split) {
     const uint64_t m = std::min(a.rows, a.columns), n = std::max(a.rows, a.columns);
     const uint32_t down = uint32_t((m + kRows - 1) / kRows), across = 2 * uint32_t((n + kRows - 1) / kRows);
-    return (2 * bytes_of(down, across) + 2 * bytes_of(down, 2 * down)) * (split ? 2 : 1);
+    return (2 * bytes_of(down, across) + 2 * bytes_of(down, 2 * down)) * (split ? 2 : 1) + uint64_t(down) * kRows * 8;
 }
 
 // The scratch of a launch's matrices: what one needs, and more of them while that stays below 2 GB.
@@ -1139,7 +1196,8 @@ template <bool SPLIT> void run_group(Group &g, int steps, cudaStream_t s) {
         a.x[1] = at + x;
         a.a = at + 2 * x;
         a.p = a.a + square;
-        at = a.p + square;
+        a.diagonal = a.p + square;
+        at = a.diagonal + uint64_t(a.down_blocks) * kRows * 8;
         const uint64_t all = uint64_t(a.m) * a.n;
         g.first[i] = blocks;
         tiles.first[i] = spread;

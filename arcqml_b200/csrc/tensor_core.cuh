@@ -118,6 +118,24 @@ __device__ __forceinline__ void tmem_add(float *v, uint32_t at) {
     for (int i = 0; i < 16; ++i) v[i] += __uint_as_float(r[i]);
 }
 
+// The sum of 16 columns at two places.
+__device__ __forceinline__ void tmem_load2(float (&v)[16], uint32_t at, uint32_t too) {
+    uint32_t r[32];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%32];\n"
+                 " tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+                 "{%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%33];\n"
+                 " tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+                   "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(at), "r"(too)
+                 : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]) + __uint_as_float(r[i + 16]);
+}
+
 // ------------------------------------------------------------------ tcgen05.mma
 
 // Operands lie in atoms of 8 rows of 128 bytes (1024 bytes, aligned to them) whose 16-byte pieces are
