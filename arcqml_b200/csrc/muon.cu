@@ -170,6 +170,10 @@ __device__ __forceinline__ int shift_of(double norm, double whole) {
     return norm > 0.0 && norm < whole && whole < INFINITY ? max(0, ilogb(whole) - ilogb(norm) - 1) : 0;
 }
 
+// 2^-n; 0 below f32's normal range, where what it scales is nothing beside what it joins. (ldexpf takes some
+// 300 cycles, in every phase.)
+__device__ __forceinline__ float power(int n) { return n > 126 ? 0.0f : __int_as_float((127 - n) << 23); }
+
 // ------------------------------------------------------------------ the update and its norm
 
 // The sum over a block of kThreads, the same in every thread.
@@ -500,9 +504,9 @@ __device__ __forceinline__ void take_sums(const Group &g, const Matrix &a, float
     const int next = max(0, shift - 2);
     // of the sum and of what is added to it
     const float of_sum = PHASE == GRAM         ? 1.0f / kScaleX
-                         : PHASE == POLYNOMIAL ? ldexpf(0.5f * kC / kScaleX, -4 * shift)
-                                               : ldexpf(2.0f / kScaleX, next - shift);
-    const float of_old = PHASE == POLYNOMIAL ? ldexpf(0.5f * kB, -2 * shift) : ldexpf(kA, next - shift);
+                         : PHASE == POLYNOMIAL ? 0.5f * kC / kScaleX * power(4 * shift)
+                                               : 2.0f / kScaleX * power(shift - next);
+    const float of_old = PHASE == POLYNOMIAL ? 0.5f * kB * power(2 * shift) : kA * power(shift - next);
     const uint64_t low = bytes_of(a.down_blocks, across);
     const char *old = g.scratch + (PHASE == APPLY ? a.x[current] : a.a);
     char *to = g.scratch + (PHASE == APPLY ? a.x[current ^ 1] : PHASE == GRAM ? a.a : a.p);
@@ -861,12 +865,14 @@ template <bool SPLIT> __global__ void __launch_bounds__(kSmallThreads, 1)
     tc::fence_before();
 
     // the update, its norm, and X
-    const uint64_t all = uint64_t(a.m) * a.n;
+    const uint32_t all = a.m * a.n;
     double sum = 0.0;
-    for (uint64_t i = thread * 8; i < all; i += kSmallThreads * 8) {
-        const uint32_t count = uint32_t(min(uint64_t(8), all - i));
+    for (uint32_t i = thread * 8; i < all; i += kSmallThreads * 8) {
+        const uint32_t count = min(8u, all - i);
         float u[8];
         new_update8(u, a, i, count);
+        if (a.momentum) // the parameter, which the last step will want
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char *>(a.out) + uint64_t(i) * (a.out_type == ARCQML_F32 ? 4 : 2)));
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum = fma(double(u[e]), double(u[e]), sum);
     }
@@ -879,11 +885,11 @@ template <bool SPLIT> __global__ void __launch_bounds__(kSmallThreads, 1)
     int shift = shift_of(norm, whole);
     const double factor = ldexp(double(kScaleX) / whole, shift);
     const uint32_t pitch = a.flip ? a.m : a.n;
-    for (uint64_t i = thread * 8; i < all; i += kSmallThreads * 8) {
-        const uint32_t count = uint32_t(min(uint64_t(8), all - i));
+    for (uint32_t i = thread * 8; i < all; i += kSmallThreads * 8) {
+        const uint32_t count = min(8u, all - i);
         float u[8];
         update8(u, a, i, count);
-        uint32_t r = uint32_t(i / pitch), c = uint32_t(i % pitch);
+        uint32_t r = i / pitch, c = i % pitch;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             if (uint32_t(e) < count) {
@@ -948,9 +954,9 @@ template <bool SPLIT> __global__ void __launch_bounds__(kSmallThreads, 1)
             tc::commit<1>(&st.done);
         }
         const float of_sum = PHASE == GRAM         ? 1.0f / kScaleX
-                             : PHASE == POLYNOMIAL ? ldexpf(0.5f * kC / kScaleX, -4 * shift)
-                                                   : ldexpf(2.0f / kScaleX, next - shift);
-        const float of_old = PHASE == GRAM ? 0.0f : PHASE == POLYNOMIAL ? ldexpf(0.5f * kB, -2 * shift) : ldexpf(kA, next - shift);
+                             : PHASE == POLYNOMIAL ? 0.5f * kC / kScaleX * power(4 * shift)
+                                                   : 2.0f / kScaleX * power(shift - next);
+        const float of_old = PHASE == GRAM ? 0.0f : PHASE == POLYNOMIAL ? 0.5f * kB * power(2 * shift) : kA * power(shift - next);
         const float diagonal = PHASE == GRAM ? 0.0f : PHASE == POLYNOMIAL ? of_a[row] : of_old + of_p[row] * of_sum;
         char *to = PHASE == APPLY ? x : p;
         constexpr uint64_t low = PHASE == APPLY ? LOW : 2 * kBlock;
@@ -997,7 +1003,7 @@ template <bool SPLIT> __global__ void __launch_bounds__(kSmallThreads, 1)
         shift = max(0, shift - 2);
     }
     if (broken)
-        for (uint64_t i = thread; i < all; i += kSmallThreads) store1(a.out, a.out_type, i, __int_as_float(0x7fffffff));
+        for (uint32_t i = thread; i < all; i += kSmallThreads) store1(a.out, a.out_type, i, __int_as_float(0x7fffffff));
     __syncthreads();
     if (warp == 1) tc::tmem_free<1>(tmem, 512);
 }
