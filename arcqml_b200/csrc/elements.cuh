@@ -86,17 +86,32 @@ template <class T, int N> struct Packed {
             return __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
         else return __half2float(__ushort_as_half(uint16_t(e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xffffu)));
     }
-    __device__ __forceinline__ void set(int e, W x) { // 16-bit elements in turn, the even ones first
-        if constexpr (sizeof(T) == 8) {
-            w[2 * e] = uint32_t(__double2loint(x));
-            w[2 * e + 1] = uint32_t(__double2hiint(x));
-        } else if constexpr (sizeof(T) == 4) {
-            w[e] = __float_as_uint(x);
-        } else {
-            const T y = to_element<T>(x);
-            const uint32_t bits = *reinterpret_cast<const uint16_t *>(&y);
-            w[e / 2] = e & 1 ? w[e / 2] | bits << 16 : bits;
+    // 16-bit elements in pairs: converted one by one and put together, they bound a copy of 2 KB rows
+    __device__ __forceinline__ void pack(const W (&x)[N]) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            if constexpr (sizeof(T) == 8) {
+                w[2 * e] = uint32_t(__double2loint(x[e]));
+                w[2 * e + 1] = uint32_t(__double2hiint(x[e]));
+            } else if constexpr (sizeof(T) == 4) {
+                w[e] = __float_as_uint(x[e]);
+            } else if constexpr (N == 1) {
+                const T y = to_element<T>(x[0]);
+                w[0] = *reinterpret_cast<const uint16_t *>(&y);
+            } else if constexpr (__is_same(T, __nv_bfloat16)) {
+                if (e & 1) {
+                    const __nv_bfloat162 y = __floats2bfloat162_rn(x[e - 1], x[e]);
+                    w[e / 2] = *reinterpret_cast<const uint32_t *>(&y);
+                }
+            } else if (e & 1) {
+                const __half2 y = __floats2half2_rn(x[e - 1], x[e]);
+                w[e / 2] = *reinterpret_cast<const uint32_t *>(&y);
+            }
         }
+    }
+    __device__ __forceinline__ void fill(uint32_t word) {
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) w[i] = word;
     }
     __device__ __forceinline__ void load(const void *p) {
         if constexpr (BYTES == 16) {

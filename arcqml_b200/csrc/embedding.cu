@@ -67,7 +67,7 @@ constexpr uint32_t kPieceVectors = 2048;
 
 // ------------------------------------------------------------------ lookup
 
-template <class W> __device__ __forceinline__ W not_a_number() { return W(__int_as_float(0x7fffffff)); }
+constexpr uint32_t kNotANumber = 0x7fffffff; // as every word of a vector: NaN in each type
 
 // Rows in tiles of 4 vectors a thread, a tile taken by `lanes` threads.
 template <uint32_t DT, int N>
@@ -96,17 +96,20 @@ __global__ void __launch_bounds__(kThreads) k_lookup(const __grid_constant__ Loo
             for (uint32_t p = 0; p < a.pieces; ++p) sum += a.squares[place * a.pieces + p];
         factor = sum == 0.0 ? 0.0 : a.scale / sqrt(sum);
     }
+    const bool plain = !a.squares && factor == 1.0; // the rows as they are
 #pragma unroll
     for (uint32_t j = 0; j < kTileVectors; ++j) {
         const uint32_t k = first + j * a.lanes;
         if (k >= a.vectors) continue;
-        Packed<T, N> y;
+        Packed<T, N> y = v[j];
+        if (padding || !inside) {
+            y.fill(padding ? 0 : kNotANumber);
+        } else if (!plain) {
+            W x[N];
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-            if (padding) y.set(e, W(0));
-            else if (!inside) y.set(e, not_a_number<W>());
-            else if (a.squares) y.set(e, W(double(v[j].wide(e)) * factor));
-            else y.set(e, v[j].wide(e) * W(factor));
+            for (int e = 0; e < N; ++e)
+                x[e] = a.squares ? W(double(v[j].wide(e)) * factor) : v[j].wide(e) * W(factor);
+            y.pack(x);
         }
         y.store(to + uint64_t(k) * Packed<T, N>::BYTES);
     }
@@ -145,7 +148,7 @@ __global__ void __launch_bounds__(kThreads) k_lookup_row(const __grid_constant__
         if (inside && !padding && k < a.vectors) v[j].load(from + uint64_t(k) * Packed<T, N>::BYTES);
         else
 #pragma unroll
-            for (int e = 0; e < N; ++e) v[j].set(e, W(0));
+            for (int i = 0; i < Packed<T, N>::WORDS; ++i) v[j].w[i] = 0;
     }
     double sum = 0.0;
 #pragma unroll
@@ -163,9 +166,14 @@ __global__ void __launch_bounds__(kThreads) k_lookup_row(const __grid_constant__
         const uint32_t k = lane + j * lanes;
         if (!on || k >= a.vectors) continue;
         Packed<T, N> y;
+        if (padding || !inside) {
+            y.fill(padding ? 0 : kNotANumber);
+        } else {
+            W x[N];
 #pragma unroll
-        for (int e = 0; e < N; ++e)
-            y.set(e, padding || inside ? W(double(v[j].wide(e)) * factor) : not_a_number<W>());
+            for (int e = 0; e < N; ++e) x[e] = W(double(v[j].wide(e)) * factor);
+            y.pack(x);
+        }
         y.store(to + uint64_t(k) * Packed<T, N>::BYTES);
     }
 }
@@ -504,8 +512,10 @@ __device__ __forceinline__ void write_sum(const Sums &a, uint32_t row, uint32_t 
 #pragma unroll
     for (int p = 0; p < N; p += PART) {
         Packed<O, PART> v;
+        W x[PART];
 #pragma unroll
-        for (int e = 0; e < PART; ++e) v.set(e, sum[p + e] * W(a.scale));
+        for (int e = 0; e < PART; ++e) x[e] = sum[p + e] * W(a.scale);
+        v.pack(x);
         v.store(to + p * sizeof(O));
     }
 }
@@ -719,8 +729,10 @@ struct Direct {
 
 template <class T, int N> __device__ __forceinline__ void load_any(Packed<T, N> &v, const char *p, uint32_t aligned) {
     if (aligned) return v.load(p);
+    typename Packed<T, N>::W x[N];
 #pragma unroll
-    for (int e = 0; e < N; ++e) v.set(e, to_wide(reinterpret_cast<const T *>(p)[e]));
+    for (int e = 0; e < N; ++e) x[e] = to_wide(reinterpret_cast<const T *>(p)[e]);
+    v.pack(x);
 }
 
 template <uint32_t DT, int N, bool BLOCK>
@@ -827,12 +839,11 @@ __global__ void __launch_bounds__(kThreads) k_direct(const __grid_constant__ Dir
             const uint32_t k = vector0 + j * THREADS;
             if (k >= a.vectors) continue;
             Packed<T, N> y;
+            W x[N];
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-                W x = sum[j][e];
-                if (a.table && any) x = W((double(x) - double(unit[j].wide(e)) * along) * inverse);
-                y.set(e, x);
-            }
+            for (int e = 0; e < N; ++e)
+                x[e] = a.table && any ? W((double(sum[j][e]) - double(unit[j].wide(e)) * along) * inverse) : sum[j][e];
+            y.pack(x);
             char *to = a.out + row * a.row_bytes + uint64_t(k) * Packed<T, N>::BYTES;
             if (a.aligned) y.store(to);
             else
