@@ -331,10 +331,10 @@ static_assert(sizeof(ProductState) <= 256, "the end of the shared memory");
 __device__ __forceinline__ bool wait_for(uint64_t *b, uint32_t parity, uint32_t *stop) {
     if (tc::barrier_try(b, parity)) return true;
     const long long begin = clock64();
-    for (uint32_t i = 0; i < (1u << 26); ++i) {
+    for (uint32_t i = 0; i < (1u << 30); ++i) { // ten seconds at most
         if (tc::barrier_try(b, parity)) return true;
         if (*reinterpret_cast<volatile uint32_t *>(stop)) return false;
-        if (clock64() - begin > 4000000000ll) break;
+        if (clock64() - begin > 20000000000ll) break;
     }
     *reinterpret_cast<volatile uint32_t *>(stop) = 1;
     return false;
@@ -597,213 +597,213 @@ __global__ void __launch_bounds__(kProductThreads, 1)
     // 128 x 56 and 256 x 216
     if (warp < 4) {
         if constexpr (SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 0 && lane == 0 && !broken) { // copies operands in
-        uint32_t at = 0, phase = 0;
-        bool on = true;
-        while (on && walk.next(part)) {
-            const Tile tile = tile_of<PHASE, SIZE>(g, part.tile);
-            const Matrix &a = *tile.a;
-            const uint32_t left = tile.i * CG + rank, right = tile.j * CG + rank;
-            const uint32_t left_across = PHASE == GRAM ? a.x_blocks : a.a_blocks;
-            const char *from = g.scratch + (PHASE == GRAM ? a.x[current] : PHASE == POLYNOMIAL ? a.a : a.p);
-            const char *from_right = PHASE == APPLY ? g.scratch + a.x[current] : from;
-            const uint64_t low = bytes_of(a.down_blocks, left_across);
-            const uint64_t low_right = PHASE == APPLY ? bytes_of(a.down_blocks, a.x_blocks) : low;
-            const uint32_t parts = SPLIT ? 2 : 1;
-            // blocks behind the edges are not read: the sums that they would enter are not stored
-            const bool has_left = left < a.down_blocks;
-            const uint32_t wide = PHASE == APPLY ? min(2u, a.x_blocks - min(a.x_blocks, right * 2)) : 0;
-            const bool has_right = right < a.down_blocks;
-            const uint32_t bytes = parts * ((has_left ? kBlock : 0) + (PHASE == APPLY ? wide * (kBlock / 2) : has_right ? kBlock : 0));
-            for (uint32_t d = part.begin; d < part.end; ++d) {
-                if (!(on = wait_for(&st.empty[at], phase ^ 1, &st.stop))) break;
-                char *to = shared + at * STAGE;
-                tc::barrier_expect(&st.full[at], bytes);
-                for (uint32_t part = 0; part < parts; ++part, to += kStageBytes) {
-                    if (has_left)
-                        tc::copy_in(to, from + part * low + (uint64_t(left) * left_across + d) * kBlock, kBlock, &st.full[at]);
-                    if constexpr (PHASE == APPLY) {
-                        for (uint32_t w = 0; w < wide; ++w)
-                            tc::copy_in(to + kBlock + w * (kBlock / 2),
-                                        from_right + part * low_right +
-                                            (uint64_t(d / 2) * a.x_blocks + right * 2 + w) * kBlock + (d & 1) * (kBlock / 2),
-                                        kBlock / 2, &st.full[at]);
-                    } else if (has_right) {
-                        tc::copy_in(to + kBlock, from_right + part * low_right + (uint64_t(right) * left_across + d) * kBlock,
-                                    kBlock, &st.full[at]);
-                    }
-                }
-                if (++at == S) at = 0, phase ^= 1;
-            }
-        }
-        // nothing may still be on its way in when the block ends: every stage that was filled has been read,
-        // or (after a wait that ran out) its copies are waited for
-        if (!on) {
-            uint32_t none = 0;
-            for (uint32_t s = 0; s < S; ++s) wait_for(&st.full[s], s < at ? phase : phase ^ 1, &none);
-        }
-    } else if (warp == 1 && rank == 0 && lane == 0 && !broken) { // issues the products
-        constexpr uint32_t instr = tc::instruction(SIZE, SIZE, PHASE == APPLY);
-        constexpr uint32_t STEP = PHASE == APPLY ? 2048 / 16 : 32 / 16; // of the right operand, 16 of depth
-        uint32_t at = 0, phase = 0, n = 0;
-        bool on = true;
-        while (on && walk.next(part)) {
-            for (uint32_t d = part.begin; d < part.end && on; ++n) {
-                const uint32_t half = n & 1, end = min(part.end - d, kChain<SPLIT>) + d;
-                if (!(on = wait_for(&st.taken[half], (n >> 1 & 1) ^ 1, &st.stop))) break;
-                tc::fence_after();
-                const uint32_t sums = tmem + half * SIZE;
-                for (bool add = false; d < end; ++d) {
-                    if (!(on = wait_for(&st.full[at], phase, &st.stop))) break;
-                    if constexpr (CG == 2)
-                        if (!(on = wait_for(&st.peer[at], phase, &st.stop))) break;
-                    tc::fence_after();
-                    const uint32_t base = tc::shared_address(shared + at * STAGE);
-                    const uint64_t left = tc::descriptor(base, 16);
-                    const uint64_t right = tc::descriptor(base + kBlock, PHASE == APPLY ? kBlock / 2 : 16);
-#pragma unroll
-                    for (uint32_t s = 0; s < kDepth / 16; ++s) {
-                        tc::mma<CG>(sums, left + s * 2, right + s * STEP, instr, add);
-                        add = true;
-                        if constexpr (SPLIT) {
-                            constexpr uint32_t LOW = kStageBytes / 16;
-                            tc::mma<CG>(sums, left + s * 2, right + LOW + s * STEP, instr, true);
-                            tc::mma<CG>(sums, left + LOW + s * 2, right + s * STEP, instr, true);
+        if (warp == 0 && lane == 0 && !broken) { // copies operands in
+            uint32_t at = 0, phase = 0;
+            bool on = true;
+            while (on && walk.next(part)) {
+                const Tile tile = tile_of<PHASE, SIZE>(g, part.tile);
+                const Matrix &a = *tile.a;
+                const uint32_t left = tile.i * CG + rank, right = tile.j * CG + rank;
+                const uint32_t left_across = PHASE == GRAM ? a.x_blocks : a.a_blocks;
+                const char *from = g.scratch + (PHASE == GRAM ? a.x[current] : PHASE == POLYNOMIAL ? a.a : a.p);
+                const char *from_right = PHASE == APPLY ? g.scratch + a.x[current] : from;
+                const uint64_t low = bytes_of(a.down_blocks, left_across);
+                const uint64_t low_right = PHASE == APPLY ? bytes_of(a.down_blocks, a.x_blocks) : low;
+                const uint32_t parts = SPLIT ? 2 : 1;
+                // blocks behind the edges are not read: the sums that they would enter are not stored
+                const bool has_left = left < a.down_blocks;
+                const uint32_t wide = PHASE == APPLY ? min(2u, a.x_blocks - min(a.x_blocks, right * 2)) : 0;
+                const bool has_right = right < a.down_blocks;
+                const uint32_t bytes = parts * ((has_left ? kBlock : 0) + (PHASE == APPLY ? wide * (kBlock / 2) : has_right ? kBlock : 0));
+                for (uint32_t d = part.begin; d < part.end; ++d) {
+                    if (!(on = wait_for(&st.empty[at], phase ^ 1, &st.stop))) break;
+                    char *to = shared + at * STAGE;
+                    tc::barrier_expect(&st.full[at], bytes);
+                    for (uint32_t part = 0; part < parts; ++part, to += kStageBytes) {
+                        if (has_left)
+                            tc::copy_in(to, from + part * low + (uint64_t(left) * left_across + d) * kBlock, kBlock, &st.full[at]);
+                        if constexpr (PHASE == APPLY) {
+                            for (uint32_t w = 0; w < wide; ++w)
+                                tc::copy_in(to + kBlock + w * (kBlock / 2),
+                                            from_right + part * low_right +
+                                                (uint64_t(d / 2) * a.x_blocks + right * 2 + w) * kBlock + (d & 1) * (kBlock / 2),
+                                            kBlock / 2, &st.full[at]);
+                        } else if (has_right) {
+                            tc::copy_in(to + kBlock, from_right + part * low_right + (uint64_t(right) * left_across + d) * kBlock,
+                                        kBlock, &st.full[at]);
                         }
                     }
-                    tc::commit<CG>(&st.empty[at]);
                     if (++at == S) at = 0, phase ^= 1;
                 }
-                if (on) tc::commit<CG>(&st.done[half]);
+            }
+            // nothing may still be on its way in when the block ends: every stage that was filled has been read,
+            // or (after a wait that ran out) its copies are waited for
+            if (!on) {
+                uint32_t none = 0;
+                for (uint32_t s = 0; s < S; ++s) wait_for(&st.full[s], s < at ? phase : phase ^ 1, &none);
+            }
+        } else if (warp == 1 && rank == 0 && lane == 0 && !broken) { // issues the products
+            constexpr uint32_t instr = tc::instruction(SIZE, SIZE, PHASE == APPLY);
+            constexpr uint32_t STEP = PHASE == APPLY ? 2048 / 16 : 32 / 16; // of the right operand, 16 of depth
+            uint32_t at = 0, phase = 0, n = 0;
+            bool on = true;
+            while (on && walk.next(part)) {
+                for (uint32_t d = part.begin; d < part.end && on; ++n) {
+                    const uint32_t half = n & 1, end = min(part.end - d, kChain<SPLIT>) + d;
+                    if (!(on = wait_for(&st.taken[half], (n >> 1 & 1) ^ 1, &st.stop))) break;
+                    tc::fence_after();
+                    const uint32_t sums = tmem + half * SIZE;
+                    for (bool add = false; d < end; ++d) {
+                        if (!(on = wait_for(&st.full[at], phase, &st.stop))) break;
+                        if constexpr (CG == 2)
+                            if (!(on = wait_for(&st.peer[at], phase, &st.stop))) break;
+                        tc::fence_after();
+                        const uint32_t base = tc::shared_address(shared + at * STAGE);
+                        const uint64_t left = tc::descriptor(base, 16);
+                        const uint64_t right = tc::descriptor(base + kBlock, PHASE == APPLY ? kBlock / 2 : 16);
+#pragma unroll
+                        for (uint32_t s = 0; s < kDepth / 16; ++s) {
+                            tc::mma<CG>(sums, left + s * 2, right + s * STEP, instr, add);
+                            add = true;
+                            if constexpr (SPLIT) {
+                                constexpr uint32_t LOW = kStageBytes / 16;
+                                tc::mma<CG>(sums, left + s * 2, right + LOW + s * STEP, instr, true);
+                                tc::mma<CG>(sums, left + LOW + s * 2, right + s * STEP, instr, true);
+                            }
+                        }
+                        tc::commit<CG>(&st.empty[at]);
+                        if (++at == S) at = 0, phase ^= 1;
+                    }
+                    if (on) tc::commit<CG>(&st.done[half]);
+                }
+            }
+        } else if (CG == 2 && warp == 2 && rank == 1 && lane == 0 && !broken) { // tells the first block of its operands
+            uint32_t at = 0, phase = 0;
+            bool on = true;
+            while (on && walk.next(part)) {
+                for (uint32_t d = part.begin; d < part.end; ++d) {
+                    if (!(on = wait_for(&st.full[at], phase, &st.stop))) break;
+                    tc::barrier_arrive_at(tc::in_block(&st.peer[at], 0));
+                    if (++at == S) at = 0, phase ^= 1;
+                }
             }
         }
-    } else if (CG == 2 && warp == 2 && rank == 1 && lane == 0 && !broken) { // tells the first block of its operands
-        uint32_t at = 0, phase = 0;
-        bool on = true;
-        while (on && walk.next(part)) {
-            for (uint32_t d = part.begin; d < part.end; ++d) {
-                if (!(on = wait_for(&st.full[at], phase, &st.stop))) break;
-                tc::barrier_arrive_at(tc::in_block(&st.peer[at], 0));
-                if (++at == S) at = 0, phase ^= 1;
-            }
-        }
-    }
     } else {
         if constexpr (SPLIT) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-    if (!broken) { // takes the sums out: a thread has a row
-        constexpr uint32_t COLUMNS = SIZE / 2;
-        const uint32_t quarter = warp & 3, first = (warp - 4) / 4 * COLUMNS;
-        float *square = reinterpret_cast<float *>(reinterpret_cast<char *>(&st) + 256) + (warp - 4) * (kSquare / 4);
-        uint32_t n = 0;
-        bool on = true;
-        const auto release = [&](uint32_t half) {
-            tc::fence_before();
-            __syncwarp();
-            if (lane == 0)
-                tc::barrier_arrive_at(CG == 2 ? tc::in_block(&st.taken[half], 0) : tc::shared_address(&st.taken[half]));
-        };
-        const auto wait_done = [&](uint32_t half) {
-            on = __all_sync(0xffffffffu, wait_for(&st.done[half], n >> 1 & 1, &st.stop));
-            tc::fence_after();
-            return on;
-        };
-        const uint32_t from = walk.at, writer = rank * kTakers + warp - 4;
-        const auto slice = [&](uint32_t u, uint32_t slot) { // of a unit's parts: 0 of a tile that began earlier
-            return reinterpret_cast<float4 *>(g.partial) + ((uint64_t(u) * 2 + slot) * (kTakers * CG) + writer) * (COLUMNS * 8) + lane;
-        };
-        while (on && walk.next(part)) {
-            const Tile tile = tile_of<PHASE, SIZE>(g, part.tile);
-            const Matrix &a = *tile.a;
-            const uint32_t row = tile.i * SIZE + rank * kRows + quarter * 32 + lane;
-            const uint32_t lanes = quarter * 32 << 16;
-            const int shift = max(0, g.shift[tile.index] - 2 * int(step));
-            const auto take = [&](float (&v)[32], uint32_t c) {
-                take_sums<PHASE, SPLIT>(g, a, v, row, tile.j * SIZE + first + c, tile.i != tile.j, shift, current, last != 0,
-                                        square);
+        if (!broken) { // takes the sums out: a thread has a row
+            constexpr uint32_t COLUMNS = SIZE / 2;
+            const uint32_t quarter = warp & 3, first = (warp - 4) / 4 * COLUMNS;
+            float *square = reinterpret_cast<float *>(reinterpret_cast<char *>(&st) + 256) + (warp - 4) * (kSquare / 4);
+            uint32_t n = 0;
+            bool on = true;
+            const auto release = [&](uint32_t half) {
+                tc::fence_before();
+                __syncwarp();
+                if (lane == 0)
+                    tc::barrier_arrive_at(CG == 2 ? tc::in_block(&st.taken[half], 0) : tc::shared_address(&st.taken[half]));
             };
-            const bool whole = part.whole();
-            float4 *mine = whole ? nullptr : slice(unit, part.start < from ? 0 : 1);
-            if constexpr (SPLIT) {
-                float sum[COLUMNS];
+            const auto wait_done = [&](uint32_t half) {
+                on = __all_sync(0xffffffffu, wait_for(&st.done[half], n >> 1 & 1, &st.stop));
+                tc::fence_after();
+                return on;
+            };
+            const uint32_t from = walk.at, writer = rank * kTakers + warp - 4;
+            const auto slice = [&](uint32_t u, uint32_t slot) { // of a unit's parts: 0 of a tile that began earlier
+                return reinterpret_cast<float4 *>(g.partial) + ((uint64_t(u) * 2 + slot) * (kTakers * CG) + writer) * (COLUMNS * 8) + lane;
+            };
+            while (on && walk.next(part)) {
+                const Tile tile = tile_of<PHASE, SIZE>(g, part.tile);
+                const Matrix &a = *tile.a;
+                const uint32_t row = tile.i * SIZE + rank * kRows + quarter * 32 + lane;
+                const uint32_t lanes = quarter * 32 << 16;
+                const int shift = max(0, g.shift[tile.index] - 2 * int(step));
+                const auto take = [&](float (&v)[32], uint32_t c) {
+                    take_sums<PHASE, SPLIT>(g, a, v, row, tile.j * SIZE + first + c, tile.i != tile.j, shift, current, last != 0,
+                                            square);
+                };
+                const bool whole = part.whole();
+                float4 *mine = whole ? nullptr : slice(unit, part.start < from ? 0 : 1);
+                if constexpr (SPLIT) {
+                    float sum[COLUMNS];
 #pragma unroll
-                for (uint32_t c = 0; c < COLUMNS; ++c) sum[c] = 0.0f;
+                    for (uint32_t c = 0; c < COLUMNS; ++c) sum[c] = 0.0f;
 #pragma unroll 1
-                for (uint32_t d = part.begin; d < part.end; d += kChain<SPLIT>, ++n) {
+                    for (uint32_t d = part.begin; d < part.end; d += kChain<SPLIT>, ++n) {
+                        const uint32_t half = n & 1;
+                        if (!wait_done(half)) break;
+#pragma unroll
+                        for (uint32_t c = 0; c < COLUMNS; c += 16) tc::tmem_add(sum + c, tmem + half * SIZE + lanes + first + c);
+                        release(half);
+                    }
+                    if (!on) break;
+                    if (whole) {
+#pragma unroll
+                        for (uint32_t c = 0; c < COLUMNS; c += 32) {
+                            float v[32];
+#pragma unroll
+                            for (uint32_t e = 0; e < 32; ++e) v[e] = sum[c + e];
+                            take(v, c);
+                        }
+                        continue;
+                    }
+#pragma unroll
+                    for (uint32_t c = 0; c < COLUMNS; c += 4) mine[c * 8] = make_float4(sum[c], sum[c + 1], sum[c + 2], sum[c + 3]);
+                } else {
                     const uint32_t half = n & 1;
                     if (!wait_done(half)) break;
-#pragma unroll
-                    for (uint32_t c = 0; c < COLUMNS; c += 16) tc::tmem_add(sum + c, tmem + half * SIZE + lanes + first + c);
-                    release(half);
-                }
-                if (!on) break;
-                if (whole) {
-#pragma unroll
+#pragma unroll 1
                     for (uint32_t c = 0; c < COLUMNS; c += 32) {
                         float v[32];
+                        __syncwarp();
+                        tc::tmem_load(v, tmem + half * SIZE + lanes + first + c);
+                        if (whole) {
+                            take(v, c);
+                        } else {
 #pragma unroll
-                        for (uint32_t e = 0; e < 32; ++e) v[e] = sum[c + e];
-                        take(v, c);
+                            for (uint32_t e = 0; e < 32; e += 4)
+                                mine[(c + e) * 8] = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                        }
                     }
-                    continue;
+                    release(half);
+                    ++n;
+                    if (whole) continue;
                 }
-#pragma unroll
-                for (uint32_t c = 0; c < COLUMNS; c += 4) mine[c * 8] = make_float4(sum[c], sum[c + 1], sum[c + 2], sum[c + 3]);
-            } else {
-                const uint32_t half = n & 1;
-                if (!wait_done(half)) break;
+                // a part: the warp that brings its rows and columns' last one puts them together
+                uint32_t u0 = uint32_t(uint64_t(part.start) * plan.runs / plan.left[plan.classes]); // has the tile's first step
+                while (cut(plan, u0) > part.start) --u0;
+                while (cut(plan, u0 + 1) <= part.start) ++u0;
+                uint32_t parts = 1;
+                while (cut(plan, u0 + parts) < part.start + part.depth) ++parts;
+                __threadfence();
+                __syncwarp();
+                uint32_t before = 0;
+                if (lane == 0) before = atomicAdd(&g.arrived[u0 * (kTakers * 2) + writer], 1u);
+                if (__shfl_sync(0xffffffffu, before, 0) + 1 != parts) continue;
+                if (lane == 0) g.arrived[u0 * (kTakers * 2) + writer] = 0;
+                __threadfence();
 #pragma unroll 1
                 for (uint32_t c = 0; c < COLUMNS; c += 32) {
                     float v[32];
-                    __syncwarp();
-                    tc::tmem_load(v, tmem + half * SIZE + lanes + first + c);
-                    if (whole) {
-                        take(v, c);
-                    } else {
 #pragma unroll
-                        for (uint32_t e = 0; e < 32; e += 4)
-                            mine[(c + e) * 8] = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-                    }
-                }
-                release(half);
-                ++n;
-                if (whole) continue;
-            }
-            // a part: the warp that brings its rows and columns' last one puts them together
-            uint32_t u0 = uint32_t(uint64_t(part.start) * plan.runs / plan.left[plan.classes]); // has the tile's first step
-            while (cut(plan, u0) > part.start) --u0;
-            while (cut(plan, u0 + 1) <= part.start) ++u0;
-            uint32_t parts = 1;
-            while (cut(plan, u0 + parts) < part.start + part.depth) ++parts;
-            __threadfence();
-            __syncwarp();
-            uint32_t before = 0;
-            if (lane == 0) before = atomicAdd(&g.arrived[u0 * (kTakers * 2) + writer], 1u);
-            if (__shfl_sync(0xffffffffu, before, 0) + 1 != parts) continue;
-            if (lane == 0) g.arrived[u0 * (kTakers * 2) + writer] = 0;
-            __threadfence();
-#pragma unroll 1
-            for (uint32_t c = 0; c < COLUMNS; c += 32) {
-                float v[32];
-#pragma unroll
-                for (uint32_t e = 0; e < 32; ++e) v[e] = 0.0f;
+                    for (uint32_t e = 0; e < 32; ++e) v[e] = 0.0f;
 #pragma unroll 2
-                for (uint32_t u = 0; u < parts; ++u) {
-                    const float4 *from = slice(u0 + u, u ? 0 : 1) + c * 8;
-                    float4 w[8];
+                    for (uint32_t u = 0; u < parts; ++u) {
+                        const float4 *from = slice(u0 + u, u ? 0 : 1) + c * 8;
+                        float4 w[8];
 #pragma unroll
-                    for (uint32_t e = 0; e < 8; ++e) w[e] = __ldcg(from + e * 32);
+                        for (uint32_t e = 0; e < 8; ++e) w[e] = __ldcg(from + e * 32);
 #pragma unroll
-                    for (uint32_t e = 0; e < 8; ++e) {
-                        v[4 * e] += w[e].x;
-                        v[4 * e + 1] += w[e].y;
-                        v[4 * e + 2] += w[e].z;
-                        v[4 * e + 3] += w[e].w;
+                        for (uint32_t e = 0; e < 8; ++e) {
+                            v[4 * e] += w[e].x;
+                            v[4 * e + 1] += w[e].y;
+                            v[4 * e + 2] += w[e].z;
+                            v[4 * e + 3] += w[e].w;
+                        }
                     }
+                    take(v, c);
                 }
-                take(v, c);
             }
         }
-    }
     }
     __syncwarp();
     tc::fence_before();

@@ -77,8 +77,9 @@ def gradient64(g, index, rows, scale, table, padding):
 
 def polynomial64(u, steps=5, eps=1e-7, rounded=None, seed=0):
     """The definition in 64 bits; with `rounded` = (bits of the products' operands) a model of a computation
-    that rounds X, A and P to that many bits and sums products in f32 with an error of one f32 step per 16
-    terms of a chain (of a running sum that grows evenly: half of it on average, in one direction)."""
+    that rounds X, A and P to that many bits, the diagonals of A and P to 24, and sums products in f32 with an
+    error of one f32 step per 16 terms of a chain (of a running sum that grows evenly: half of it on average, in
+    one direction)."""
     gen = torch.Generator().manual_seed(seed)
     u = u.to(torch.float64)
     flip = u.shape[0] > u.shape[1]
@@ -100,9 +101,18 @@ def polynomial64(u, steps=5, eps=1e-7, rounded=None, seed=0):
 
     x = operand(x / (x.square().sum().sqrt() + eps))
     for _ in range(steps):
-        a = operand(product(x, x.mT))
-        p = operand(B * a + C * product(a, a))
-        x = operand(A * x + product(p, x))
+        if rounded is None:
+            a = x @ x.mT
+            x = A * x + (B * a + C * (a @ a)) @ x
+            continue
+        a = product(x, x.mT)
+        d = a.diagonal().clone()
+        a = operand(a - torch.diag(d))
+        s = product(a, a)
+        p = B * a + C * (s + (d[:, None] + d) * a)
+        e = B * d + C * (s.diagonal() + d * d)
+        p = operand(p - torch.diag(p.diagonal()))
+        x = operand((A + e)[:, None] * x + product(p, x))
     return x.mT if flip else x
 
 

@@ -79,11 +79,28 @@ def test_gradient_of_many_rows(runtime, rows):
     check_gradient(runtime, g, torch.full((3000,), rows - 1), rows, padding=0)
 
 
-@pytest.mark.parametrize("n", [2048, 2049, 70_000, 300_000])
+@pytest.mark.parametrize("n", [1024, 1025, 8192, 8193, 20_000, 131_072, 131_073, 300_000])
 def test_gradient_of_many_places(runtime, n):
     g = make((n, 3), torch.float32, n)
     check_gradient(runtime, g, indices(n, 700, n, skewed=True), 700, 0.5)
     check_gradient(runtime, g, torch.zeros(n, dtype=torch.int64), 3)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.complex64])
+@pytest.mark.parametrize("n", [40, 3000])
+def test_rows_that_start_anywhere(runtime, dtype, n):
+    """Views whose rows start off the accesses' boundaries, through the norm too, against their copies."""
+    wide, g = make((20, 300), dtype, 1).cuda(), make((n, 300), dtype, 2).cuda()
+    x = indices(n, 20, 3).cuda()
+    for start, width in ((1, 64), (3, 128), (5, 200), (1, 7)):
+        t, v = wide[:, start:start + width], g[:, start:start + width]
+        for table in (None, t):
+            got = runtime.embedding_gradient_device(v, x, 20, table=table)
+            assert torch.equal(got, runtime.embedding_gradient_device(
+                v.contiguous(), x, 20, table=None if table is None else table.contiguous()))
+        index = x.cpu().long()
+        check_gradient(runtime, v.cpu(), index, 20, table=t.cpu().contiguous())
+        check_lookup(runtime, t.cpu().contiguous(), index, 0.5, True)
 
 
 def test_indices_outside_and_padding(runtime):
