@@ -317,9 +317,10 @@ template <bool SPLIT> constexpr uint32_t kProductShared =
     1024 + kStages<SPLIT> * (SPLIT ? 2 : 1) * kStageBytes + 256 + kTakers * kSquare;
 // The tensor cores cut what falls behind the last bit of a running sum (they do not round): a chain of k
 // steps of 16 loses up to k 2^-24 of it, always towards 0. Operands of 22 bits would show that (a matrix of
-// 4096 x 8191 came out 4.4e-5 off, 7e-6 with f32 operations), so their sums leave tensor memory every 512 of
-// depth and go on in registers. Steps of 64:
-template <bool SPLIT> constexpr uint32_t kChain = SPLIT ? 8 : 0xffffffffu;
+// 4096 x 8191 came out 4.4e-5 off), so their sums leave tensor memory and go on in registers: every 128 of
+// depth for A, whose diagonal adds up squares (every 512: 130 x 8000 4.9e-6 off instead of 1.0e-6, f32
+// operations 1.3e-6; it takes 4 % of the whole), every 512 for sums of both signs. Steps of 64:
+template <int PHASE, bool SPLIT> constexpr uint32_t kChain = !SPLIT ? 0xffffffffu : PHASE == 0 ? 2 : 8;
 
 struct ProductState {
     uint64_t full[6], empty[6], peer[6], done[2], taken[2];
@@ -649,7 +650,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
             bool on = true;
             while (on && walk.next(part)) {
                 for (uint32_t d = part.begin; d < part.end && on; ++n) {
-                    const uint32_t half = n & 1, end = min(part.end - d, kChain<SPLIT>) + d;
+                    const uint32_t half = n & 1, end = min(part.end - d, kChain<PHASE, SPLIT>) + d;
                     if (!(on = wait_for(&st.taken[half], (n >> 1 & 1) ^ 1, &st.stop))) break;
                     tc::fence_after();
                     const uint32_t sums = tmem + half * SIZE;
@@ -728,7 +729,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
 #pragma unroll
                     for (uint32_t c = 0; c < COLUMNS; ++c) sum[c] = 0.0f;
 #pragma unroll 1
-                    for (uint32_t d = part.begin; d < part.end; d += kChain<SPLIT>, ++n) {
+                    for (uint32_t d = part.begin; d < part.end; d += kChain<PHASE, SPLIT>, ++n) {
                         const uint32_t half = n & 1;
                         if (!wait_done(half)) break;
 #pragma unroll
