@@ -369,7 +369,9 @@ __global__ void __launch_bounds__(kThreads) k_sort_pass(const __grid_constant__ 
 // shared memory, the keys through L2 (stores into other blocks' shared memory took no less). A pass takes about
 // 25,000 cycles, 8,000 of them for the ballots of the ranks. The other clusters of the launch clear the output
 // meanwhile: most of its rows are often absent, and it is written twice only where a row is present.
-constexpr uint32_t kClusterThreads = 1024, kClusterKeys = 8192, kPerThread = kClusterKeys / kClusterThreads;
+// Each thread has 1, 2, 4 or 8 keys: as few as 16 blocks leave it, since ranking takes 1000 cycles for each
+// (8192 places: 25 us in one block, see the call's times for more).
+constexpr uint32_t kClusterThreads = 1024, kMostPerThread = 8;
 constexpr uint32_t kClusterWarps = kClusterThreads / 32, kMostCluster = 16;
 
 struct ClusterSort {
@@ -395,7 +397,9 @@ __device__ __forceinline__ void clear_share(char *to, uint64_t bytes, uint64_t t
     if (thread < bytes - tail) to[tail + thread] = 0;
 }
 
+template <uint32_t PER_THREAD>
 __global__ void __launch_bounds__(kClusterThreads, 1) k_sort_cluster(const __grid_constant__ ClusterSort s) {
+    constexpr uint32_t KEYS = PER_THREAD * kClusterThreads;
     extern __shared__ char raw[];
     ClusterShared &sh = *reinterpret_cast<ClusterShared *>(raw);
     cg::cluster_group cluster = cg::this_cluster();
@@ -416,11 +420,11 @@ __global__ void __launch_bounds__(kClusterThreads, 1) k_sort_cluster(const __gri
         for (uint32_t b = t; b < kClusterWarps * kBins / 2; b += kClusterThreads)
             reinterpret_cast<uint32_t *>(&sh.hist[0][0])[b] = 0;
         __syncthreads();
-        uint2 key[kPerThread];
-        uint32_t rank[kPerThread];
-        const uint32_t first = me * kClusterKeys + warp * (kClusterKeys / kClusterWarps) + lane;
+        uint2 key[PER_THREAD];
+        uint32_t rank[PER_THREAD];
+        const uint32_t first = me * KEYS + warp * (KEYS / kClusterWarps) + lane;
 #pragma unroll
-        for (uint32_t j = 0; j < kPerThread; ++j) {
+        for (uint32_t j = 0; j < PER_THREAD; ++j) {
             // keys behind the last place sort behind all others and stay where they are
             const uint32_t i = first + j * 32;
             key[j] = make_uint2(kAbsent, i);
@@ -430,7 +434,7 @@ __global__ void __launch_bounds__(kClusterThreads, 1) k_sort_cluster(const __gri
             }
         }
 #pragma unroll
-        for (uint32_t j = 0; j < kPerThread; ++j) {
+        for (uint32_t j = 0; j < PER_THREAD; ++j) {
             const uint32_t d = digit_of(key[j].x, shift, s.bits), same = lanes_alike(d, s.bits);
             const uint32_t before = __popc(same & ((1u << lane) - 1));
             rank[j] = sh.hist[warp][d] + before;
@@ -474,7 +478,7 @@ __global__ void __launch_bounds__(kClusterThreads, 1) k_sort_cluster(const __gri
         // (the last pass: nobody reads this block's counts any more; it need not wait for its own stores)
         if (last) cluster.barrier_arrive();
 #pragma unroll
-        for (uint32_t j = 0; j < kPerThread; ++j) {
+        for (uint32_t j = 0; j < PER_THREAD; ++j) {
             const uint32_t d = digit_of(key[j].x, shift, s.bits);
             const uint32_t at = sh.base[d] + sh.hist[warp][d] + rank[j];
             if (at < s.places) to[at] = key[j];
@@ -958,16 +962,13 @@ void start(void (*kernel)(P...), const Shape &shape, double bytes, cudaStream_t 
     prof_end(tok, s, bytes);
 }
 
-// Lets the sort have clusters of 16 blocks and their shared memory, once on each device.
-void allow_cluster() {
+// Lets the sort have clusters of 16 blocks, once on each device.
+template <auto KERNEL> void allow_cluster() {
     static std::atomic<uint64_t> set{0};
     int device = 0;
     check_cuda(cudaGetDevice(&device), "cudaGetDevice");
     if (device < 64 && (set.load() >> device & 1)) return;
-    check_cuda(cudaFuncSetAttribute(k_sort_cluster, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(ClusterShared))),
-               "embedding kernel attribute");
-    check_cuda(cudaFuncSetAttribute(k_sort_cluster, cudaFuncAttributeNonPortableClusterSizeAllowed, 1),
-               "embedding kernel attribute");
+    check_cuda(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "embedding kernel attribute");
     if (device < 64) set |= uint64_t(1) << device;
 }
 
@@ -1004,7 +1005,7 @@ GradientScratch gradient_scratch(const ArcqmlRows &g, uint64_t rows, const Arcqm
     s.passes = (bits + 8) / 9;
     s.bits = (bits + s.passes - 1) / s.passes;
     s.blocks = uint32_t((n + kSortKeys - 1) / kSortKeys);
-    const bool in_cluster = n <= kClusterKeys * kMostCluster;
+    const bool in_cluster = n <= kMostPerThread * kClusterThreads * kMostCluster;
     for (int i = 0; i < 2; ++i) {
         s.sorted[i] = take(2 * n);
     }
@@ -1012,10 +1013,12 @@ GradientScratch gradient_scratch(const ArcqmlRows &g, uint64_t rows, const Arcqm
         s.counts = take(uint64_t(s.passes) * s.blocks * kBins);
         s.totals = take(kBins);
     }
-    // chunks: enough of them to fill the GPU, 128 places at most
+    // chunks of 8 to 128 places: enough of them to fill the GPU, and not more than 2048 beyond that, since a row
+    // that many places point to is put together from its chunks (131071 places of 128 bytes took 46 us for
+    // that in chunks of 8, 27 us in chunks of 32)
     const uint64_t tiles = std::max<uint64_t>(1, g.width * bytes_of_element(g.dtype) / 512);
     s.chunk = 8;
-    while (s.chunk < 128 && n * tiles / (s.chunk * 2) >= 148 * 32) s.chunk *= 2;
+    while (s.chunk < 128 && (n * tiles / (s.chunk * 2) >= 148 * 32 || n / s.chunk > 2048)) s.chunk *= 2;
     s.chunks = uint32_t((n + s.chunk - 1) / s.chunk);
     const uint64_t wide = g.dtype == ARCQML_F64 ? 2 : 1;
     s.partial = take(2 * uint64_t(s.chunks) * g.width * wide);
@@ -1132,7 +1135,7 @@ void embedding_gradient_device(const ArcqmlRows &gradient, const void *indices, 
         });
     }
     uint32_t *base = reinterpret_cast<uint32_t *>(ws);
-    const bool in_cluster = n <= kClusterKeys * kMostCluster;
+    const bool in_cluster = n <= kMostPerThread * kClusterThreads * kMostCluster;
     uint2 *buffers[2] = {reinterpret_cast<uint2 *>(base + w.sorted[0]), reinterpret_cast<uint2 *>(base + w.sorted[1])};
     const uint2 *sorted = buffers[in_cluster ? 0 : w.passes & 1];
     if (in_cluster) {
@@ -1145,13 +1148,21 @@ void embedding_gradient_device(const ArcqmlRows &gradient, const void *indices, 
         a.places = uint32_t(n);
         a.passes = w.passes;
         a.bits = w.bits;
-        uint32_t cluster = 1;
-        while (cluster * kClusterKeys < n) cluster *= 2;
-        allow_cluster();
-        // as many blocks clear as the GPU takes beside the sort, at least 64 KB each
-        const uint64_t clears = std::min<uint64_t>((112 - cluster) / cluster, a.clear_bytes / (uint64_t(cluster) << 16) + 1);
-        start(k_sort_cluster, {cluster * (1 + clears), kClusterThreads, false, cluster, sizeof(ClusterShared)},
-              double(a.clear_bytes), s, a);
+        const auto sort = [&](auto per_thread) {
+            constexpr uint32_t P = per_thread;
+            uint32_t cluster = 1;
+            while (cluster * P * kClusterThreads < n) cluster *= 2;
+            allow_cluster<k_sort_cluster<P>>();
+            // as many blocks clear as the GPU takes beside the sort, at least 64 KB each
+            const uint64_t clears = std::min<uint64_t>((112 - cluster) / cluster, a.clear_bytes / (uint64_t(cluster) << 16) + 1);
+            start(k_sort_cluster<P>, {cluster * (1 + clears), kClusterThreads, false, cluster, sizeof(ClusterShared)},
+                  double(a.clear_bytes), s, a);
+        };
+        const uint32_t each = kClusterThreads * kMostCluster;
+        if (n <= each) sort(std::integral_constant<uint32_t, 1>{});
+        else if (n <= 2 * each) sort(std::integral_constant<uint32_t, 2>{});
+        else if (n <= 4 * each) sort(std::integral_constant<uint32_t, 4>{});
+        else sort(std::integral_constant<uint32_t, 8>{});
     } else {
         Sort a{};
         a.index = index;
