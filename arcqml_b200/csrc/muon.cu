@@ -1132,19 +1132,20 @@ template <int PHASE> uint32_t tiles_of(const Matrix &a, uint32_t size) {
 }
 template <int PHASE> uint32_t depth_of(const Matrix &a) { return ((PHASE == GRAM ? a.n : a.m) + kDepth - 1) / kDepth; }
 
-template <int PHASE, bool SPLIT, int CG> void product(Group &g, uint32_t step, bool last, cudaStream_t s) {
-    allow_shared<k_product<PHASE, SPLIT, CG>>(kProductShared<SPLIT>);
+// Who does which tile of 128 CG x 128 CG, and how many steps of 64 of the depth the longest unit has. g's
+// matrices are put in order.
+template <int PHASE> uint32_t make_plan(Group &g, Plan &p, uint32_t cg, bool split) {
     std::stable_sort(g.order, g.order + g.count, [&](uint8_t x, uint8_t y) {
         return depth_of<PHASE>(g.matrix[x]) > depth_of<PHASE>(g.matrix[y]);
     });
     uint32_t tiles = 0;
     for (uint32_t i = 0; i < g.count; ++i) {
         g.first[i] = tiles;
-        tiles += tiles_of<PHASE>(g.matrix[g.order[i]], CG * kRows);
+        tiles += tiles_of<PHASE>(g.matrix[g.order[i]], cg * kRows);
     }
     g.first[g.count] = tiles;
-    const uint32_t units = kSMs / CG;
-    Plan p;
+    const uint32_t units = kSMs / cg;
+    uint32_t whole = 0;
     p.classes = p.left[0] = 0;
     for (uint32_t i = 0, next; i < g.count; i = next) {
         const uint32_t c = p.classes++, depth = depth_of<PHASE>(g.matrix[g.order[i]]);
@@ -1154,35 +1155,42 @@ template <int PHASE, bool SPLIT, int CG> void product(Group &g, uint32_t step, b
         p.depth[c] = depth;
         p.rounds[c] = has / units;
         p.left[c + 1] = p.left[c] + has % units * weight(depth);
+        whole += p.rounds[c] * weight(depth);
     }
     // whole tiles, or runs of equal length, of 16 steps and a sixth of a tile at least: writing parts and putting
     // them together takes about 18 us, 40 steps of 11-bit operands and 20 of 22-bit ones
     const uint32_t all = p.left[p.classes];
     uint32_t longest[2];
-    for (int parts = 1; parts >= 0; --parts) {
+    const auto cut_up = [&](bool parts) {
         p.snap = parts ? 8 : 0xffffffffu;
         p.runs = parts ? std::max(1u, std::min(units, all / std::max(16u, (p.depth[0] + 5) / 6))) : units;
-        longest[parts] = parts ? (SPLIT ? 20 : 40) : 0;
+    };
+    for (int parts = 0; parts < 2; ++parts) {
+        cut_up(parts != 0);
         uint32_t run = 0;
         for (uint32_t u = 0; u < p.runs; ++u) run = std::max(run, cut(p, u + 1) - cut(p, u));
-        longest[parts] += run;
+        longest[parts] = run + (parts ? (split ? 20 : 40) : 0);
     }
-    if (longest[1] < longest[0]) {
-        p.snap = 8;
-        p.runs = std::max(1u, std::min(units, all / std::max(16u, (p.depth[0] + 5) / 6)));
-    }
+    const bool parts = longest[1] < longest[0];
+    cut_up(parts);
+    return whole + longest[parts];
+}
+
+template <int PHASE, bool SPLIT, int CG> void product(const Group &g, const Plan &p, uint32_t step, bool last, cudaStream_t s) {
+    allow_shared<k_product<PHASE, SPLIT, CG>>(kProductShared<SPLIT>);
     start(k_product<PHASE, SPLIT, CG>, kSMs, kProductThreads, CG, kProductShared<SPLIT>, true, 0.0, s, g, p, step, uint32_t(last));
 }
 
 template <int PHASE, bool SPLIT> void phase(Group &g, uint32_t step, bool last, cudaStream_t s) {
-    // steps of 64 of the depth, on pairs of blocks and on single ones: a pair's takes 1.3 times as long for
-    // up to four times the work
-    uint64_t steps[2] = {0, 0};
-    for (uint32_t i = 0; i < g.count; ++i)
-        for (int pair = 0; pair < 2; ++pair)
-            steps[pair] += uint64_t(tiles_of<PHASE>(g.matrix[i], kRows << pair)) * depth_of<PHASE>(g.matrix[i]);
-    if (1.3 * 2.0 * double(steps[1]) <= double(steps[0])) product<PHASE, SPLIT, 2>(g, step, last, s);
-    else product<PHASE, SPLIT, 1>(g, step, last, s);
+    // A pair's step is four times the work of a single block's and takes 1.4 times as long (11-bit operands 0.45
+    // and 0.32 us, 22-bit ones 0.85 and 0.62): pairs for many tiles (4096 x 4096: 107 and 179 us for the last
+    // phase), single blocks where whole tiles of pairs are too few (the second phase of 2048 x 2048 has 36 for
+    // 74 pairs: 25.6 and 20.5 us).
+    Plan pairs, singles;
+    const uint32_t single = make_plan<PHASE>(g, singles, 1, SPLIT), pair = make_plan<PHASE>(g, pairs, 2, SPLIT);
+    if (7 * pair <= 5 * single) return product<PHASE, SPLIT, 2>(g, pairs, step, last, s);
+    make_plan<PHASE>(g, singles, 1, SPLIT);
+    product<PHASE, SPLIT, 1>(g, singles, step, last, s);
 }
 
 // The members' `out`, `in` and step are set; shapes and places are filled in here.
