@@ -233,25 +233,35 @@ template <bool SPLIT> __device__ __forceinline__ void store_operand(char *at, ui
     *reinterpret_cast<uint4 *>(at) = make_uint4(h[0], h[1], h[2], h[3]);
     if constexpr (SPLIT) *reinterpret_cast<uint4 *>(at + low) = make_uint4(l[0], l[1], l[2], l[3]);
 }
-template <bool SPLIT> __device__ __forceinline__ void load_operand(float (&v)[8], const char *at, uint64_t low) {
-    const uint4 h = *reinterpret_cast<const uint4 *>(at);
-    const uint32_t w[4] = {h.x, h.y, h.z, h.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-        v[2 * i] = y.x;
-        v[2 * i + 1] = y.y;
+template <bool SPLIT> struct OperandWords {
+    uint4 high, low;
+    __device__ __forceinline__ void load(const char *at, uint64_t apart) {
+        high = *reinterpret_cast<const uint4 *>(at);
+        if constexpr (SPLIT) low = *reinterpret_cast<const uint4 *>(at + apart);
     }
-    if constexpr (SPLIT) {
-        const uint4 l = *reinterpret_cast<const uint4 *>(at + low);
-        const uint32_t z[4] = {l.x, l.y, l.z, l.w};
+    __device__ __forceinline__ void unpack(float (&v)[8]) const {
+        const uint32_t w[4] = {high.x, high.y, high.z, high.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&z[i]));
-            v[2 * i] += y.x;
-            v[2 * i + 1] += y.y;
+            const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+            v[2 * i] = y.x;
+            v[2 * i + 1] = y.y;
+        }
+        if constexpr (SPLIT) {
+            const uint32_t z[4] = {low.x, low.y, low.z, low.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&z[i]));
+                v[2 * i] += y.x;
+                v[2 * i + 1] += y.y;
+            }
         }
     }
+};
+template <bool SPLIT> __device__ __forceinline__ void load_operand(float (&v)[8], const char *at, uint64_t low) {
+    OperandWords<SPLIT> w;
+    w.load(at, low);
+    w.unpack(v);
 }
 
 // X = u / (|u| + eps) in blocks, one for each thread block; zeros behind the matrix's edges.
@@ -514,30 +524,41 @@ __device__ __forceinline__ void take_sums(const Group &g, const Matrix &a, float
     float *of_a = reinterpret_cast<float *>(g.scratch + a.diagonal), *of_p = of_a + a.down_blocks * kRows;
     const float mine = PHASE == GRAM ? 0.0f : PHASE == POLYNOMIAL ? of_a[row] : of_old + of_p[row] * of_sum;
     const uint32_t own = row - column; // the diagonal's place among the 32, if below that
+    // what is read is read before the first store, which it might otherwise have to wait for: a round trip to L2
+    // for 32 columns, or 16 where registers are short
+    constexpr uint32_t BATCH = SPLIT ? 16 : 32;
 #pragma unroll
-    for (uint32_t q = 0; q < 32; q += 8) {
-        const uint64_t place = place_of(row, column + q, across);
-        float x[8];
-        if constexpr (PHASE != GRAM) load_operand<SPLIT>(x, old + place, low);
-        if constexpr (PHASE == POLYNOMIAL) {
-            const float4 d[2] = {*reinterpret_cast<const float4 *>(of_a + column + q),
-                                 *reinterpret_cast<const float4 *>(of_a + column + q + 4)};
-            const float *other = &d[0].x;
+    for (uint32_t q0 = 0; q0 < 32; q0 += BATCH) {
+        OperandWords<SPLIT> was[BATCH / 8];
+        float4 other[BATCH / 4];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[q + e] = combine(x[e], v[q + e], mine, other[e], q + e == own, of_old, of_sum);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[q + e] = PHASE == GRAM ? v[q + e] * of_sum : mine * x[e] + v[q + e] * of_sum;
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            if (PHASE != APPLY && q + e == own) {
-                (PHASE == GRAM ? of_a : of_p)[row] = v[q + e];
-                v[q + e] = 0.0f;
+        for (uint32_t q = 0; q < BATCH; q += 8) {
+            if constexpr (PHASE != GRAM) was[q / 8].load(old + place_of(row, column + q0 + q, across), low);
+            if constexpr (PHASE == POLYNOMIAL) {
+                other[q / 4] = *reinterpret_cast<const float4 *>(of_a + column + q0 + q);
+                other[q / 4 + 1] = *reinterpret_cast<const float4 *>(of_a + column + q0 + q + 4);
             }
-            x[e] = v[q + e];
         }
-        if (PHASE != APPLY || !last) store_operand<SPLIT>(to + place, low, x);
+#pragma unroll
+        for (uint32_t i = 0; i < BATCH; i += 8) {
+            const uint32_t q = q0 + i;
+            float x[8];
+            if constexpr (PHASE != GRAM) was[i / 8].unpack(x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if constexpr (PHASE == GRAM) v[q + e] *= of_sum;
+                else if constexpr (PHASE == APPLY) v[q + e] = mine * x[e] + v[q + e] * of_sum;
+                else
+                    v[q + e] = combine(x[e], v[q + e], mine, reinterpret_cast<const float *>(other)[i + e], q + e == own, of_old,
+                                       of_sum);
+                if (PHASE != APPLY && q + e == own) {
+                    (PHASE == GRAM ? of_a : of_p)[row] = v[q + e];
+                    v[q + e] = 0.0f;
+                }
+                x[e] = v[q + e];
+            }
+            if (PHASE != APPLY || !last) store_operand<SPLIT>(to + place_of(row, column + q, across), low, x);
+        }
     }
     if (PHASE != APPLY && mirrored) { // lanes in pairs, each with two rows of one column
 #pragma unroll
@@ -587,21 +608,29 @@ __global__ void __launch_bounds__(kProductThreads, 1)
     if constexpr (CG == 2) tc::cluster_sync();
     tc::fence_after();
     cudaTriggerProgrammaticLaunchCompletion();
-    cudaGridDependencySynchronize();
+    // The first tile is found, and its matrix's entries are read, before the last phase's results are waited
+    // for: the launch's parameters come from L2 the first time, some 5000 cycles for all of them.
     const uint32_t tmem = st.tmem;
     const uint32_t units = gridDim.x / CG, unit = blockIdx.x / CG;
     Walk walk(plan, unit, units);
     Part part;
-    const bool broken = *reinterpret_cast<volatile uint32_t *>(g.fault) != 0;
+    bool more = walk.next(part);
+    if (more) {
+        const Matrix &a = *tile_of<PHASE, SIZE>(g, part.tile).a;
+        asm volatile("" ::"l"(a.x[current]), "l"(a.x[current ^ 1]), "l"(a.a), "l"(a.p), "l"(a.diagonal), "l"(a.out), "r"(a.m),
+                     "r"(a.n), "r"(a.down_blocks), "r"(a.x_blocks), "r"(a.a_blocks), "f"(a.rate), "l"(g.scratch), "l"(g.shift),
+                     "l"(g.fault), "l"(g.partial));
+    }
+    cudaGridDependencySynchronize();
 
     // the sums of a tile in registers take more of them than a thread's share: 384 x 168 registers as
     // 128 x 56 and 256 x 216
     if (warp < 4) {
         if constexpr (SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        if (warp == 0 && lane == 0 && !broken) { // copies operands in
+        if (warp == 0 && lane == 0) { // copies operands in
             uint32_t at = 0, phase = 0;
             bool on = true;
-            while (on && walk.next(part)) {
+            for (; on && more; more = walk.next(part)) {
                 const Tile tile = tile_of<PHASE, SIZE>(g, part.tile);
                 const Matrix &a = *tile.a;
                 const uint32_t left = tile.i * CG + rank, right = tile.j * CG + rank;
@@ -643,12 +672,12 @@ __global__ void __launch_bounds__(kProductThreads, 1)
                 uint32_t none = 0;
                 for (uint32_t s = 0; s < S; ++s) wait_for(&st.full[s], s < at ? phase : phase ^ 1, &none);
             }
-        } else if (warp == 1 && rank == 0 && lane == 0 && !broken) { // issues the products
+        } else if (warp == 1 && rank == 0 && lane == 0) { // issues the products
             constexpr uint32_t instr = tc::instruction(SIZE, SIZE, PHASE == APPLY);
             constexpr uint32_t STEP = PHASE == APPLY ? 2048 / 16 : 32 / 16; // of the right operand, 16 of depth
             uint32_t at = 0, phase = 0, n = 0;
             bool on = true;
-            while (on && walk.next(part)) {
+            for (; on && more; more = walk.next(part)) {
                 for (uint32_t d = part.begin; d < part.end && on; ++n) {
                     const uint32_t half = n & 1, end = min(part.end - d, kChain<PHASE, SPLIT>) + d;
                     if (!(on = wait_for(&st.taken[half], (n >> 1 & 1) ^ 1, &st.stop))) break;
@@ -678,10 +707,10 @@ __global__ void __launch_bounds__(kProductThreads, 1)
                     if (on) tc::commit<CG>(&st.done[half]);
                 }
             }
-        } else if (CG == 2 && warp == 2 && rank == 1 && lane == 0 && !broken) { // tells the first block of its operands
+        } else if (CG == 2 && warp == 2 && rank == 1 && lane == 0) { // tells the first block of its operands
             uint32_t at = 0, phase = 0;
             bool on = true;
-            while (on && walk.next(part)) {
+            for (; on && more; more = walk.next(part)) {
                 for (uint32_t d = part.begin; d < part.end; ++d) {
                     if (!(on = wait_for(&st.full[at], phase, &st.stop))) break;
                     tc::barrier_arrive_at(tc::in_block(&st.peer[at], 0));
@@ -691,118 +720,118 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         }
     } else {
         if constexpr (SPLIT) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-        if (!broken) { // takes the sums out: a thread has a row
-            constexpr uint32_t COLUMNS = SIZE / 2;
-            const uint32_t quarter = warp & 3, first = (warp - 4) / 4 * COLUMNS;
-            float *square = reinterpret_cast<float *>(reinterpret_cast<char *>(&st) + 256) + (warp - 4) * (kSquare / 4);
-            uint32_t n = 0;
-            bool on = true;
-            const auto release = [&](uint32_t half) {
-                tc::fence_before();
-                __syncwarp();
-                if (lane == 0)
-                    tc::barrier_arrive_at(CG == 2 ? tc::in_block(&st.taken[half], 0) : tc::shared_address(&st.taken[half]));
+        // takes the sums out: a thread has a row
+        Walk tiles(plan, unit, units);
+        constexpr uint32_t COLUMNS = SIZE / 2;
+        const uint32_t quarter = warp & 3, first = (warp - 4) / 4 * COLUMNS;
+        float *square = reinterpret_cast<float *>(reinterpret_cast<char *>(&st) + 256) + (warp - 4) * (kSquare / 4);
+        uint32_t n = 0;
+        bool on = true;
+        const auto release = [&](uint32_t half) {
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0)
+                tc::barrier_arrive_at(CG == 2 ? tc::in_block(&st.taken[half], 0) : tc::shared_address(&st.taken[half]));
+        };
+        const auto wait_done = [&](uint32_t half) {
+            on = __all_sync(0xffffffffu, wait_for(&st.done[half], n >> 1 & 1, &st.stop));
+            tc::fence_after();
+            return on;
+        };
+        const uint32_t from = cut(plan, unit), writer = rank * kTakers + warp - 4;
+        const auto slice = [&](uint32_t u, uint32_t slot) { // of a unit's parts: 0 of a tile that began earlier
+            return reinterpret_cast<float4 *>(g.partial) + ((uint64_t(u) * 2 + slot) * (kTakers * CG) + writer) * (COLUMNS * 8) + lane;
+        };
+        while (on && tiles.next(part)) {
+            const Tile tile = tile_of<PHASE, SIZE>(g, part.tile);
+            const Matrix &a = *tile.a;
+            const uint32_t row = tile.i * SIZE + rank * kRows + quarter * 32 + lane;
+            const uint32_t lanes = quarter * 32 << 16;
+            const int shift = max(0, g.shift[tile.index] - 2 * int(step));
+            const auto take = [&](float (&v)[32], uint32_t c) {
+                take_sums<PHASE, SPLIT>(g, a, v, row, tile.j * SIZE + first + c, tile.i != tile.j, shift, current, last != 0,
+                                        square);
             };
-            const auto wait_done = [&](uint32_t half) {
-                on = __all_sync(0xffffffffu, wait_for(&st.done[half], n >> 1 & 1, &st.stop));
-                tc::fence_after();
-                return on;
-            };
-            const uint32_t from = walk.at, writer = rank * kTakers + warp - 4;
-            const auto slice = [&](uint32_t u, uint32_t slot) { // of a unit's parts: 0 of a tile that began earlier
-                return reinterpret_cast<float4 *>(g.partial) + ((uint64_t(u) * 2 + slot) * (kTakers * CG) + writer) * (COLUMNS * 8) + lane;
-            };
-            while (on && walk.next(part)) {
-                const Tile tile = tile_of<PHASE, SIZE>(g, part.tile);
-                const Matrix &a = *tile.a;
-                const uint32_t row = tile.i * SIZE + rank * kRows + quarter * 32 + lane;
-                const uint32_t lanes = quarter * 32 << 16;
-                const int shift = max(0, g.shift[tile.index] - 2 * int(step));
-                const auto take = [&](float (&v)[32], uint32_t c) {
-                    take_sums<PHASE, SPLIT>(g, a, v, row, tile.j * SIZE + first + c, tile.i != tile.j, shift, current, last != 0,
-                                            square);
-                };
-                const bool whole = part.whole();
-                float4 *mine = whole ? nullptr : slice(unit, part.start < from ? 0 : 1);
-                if constexpr (SPLIT) {
-                    float sum[COLUMNS];
+            const bool whole = part.whole();
+            float4 *mine = whole ? nullptr : slice(unit, part.start < from ? 0 : 1);
+            if constexpr (SPLIT) {
+                float sum[COLUMNS];
 #pragma unroll
-                    for (uint32_t c = 0; c < COLUMNS; ++c) sum[c] = 0.0f;
+                for (uint32_t c = 0; c < COLUMNS; ++c) sum[c] = 0.0f;
 #pragma unroll 1
-                    for (uint32_t d = part.begin; d < part.end; d += kChain<PHASE, SPLIT>, ++n) {
-                        const uint32_t half = n & 1;
-                        if (!wait_done(half)) break;
-#pragma unroll
-                        for (uint32_t c = 0; c < COLUMNS; c += 16) tc::tmem_add(sum + c, tmem + half * SIZE + lanes + first + c);
-                        release(half);
-                    }
-                    if (!on) break;
-                    if (whole) {
-#pragma unroll
-                        for (uint32_t c = 0; c < COLUMNS; c += 32) {
-                            float v[32];
-#pragma unroll
-                            for (uint32_t e = 0; e < 32; ++e) v[e] = sum[c + e];
-                            take(v, c);
-                        }
-                        continue;
-                    }
-#pragma unroll
-                    for (uint32_t c = 0; c < COLUMNS; c += 4) mine[c * 8] = make_float4(sum[c], sum[c + 1], sum[c + 2], sum[c + 3]);
-                } else {
+                for (uint32_t d = part.begin; d < part.end; d += kChain<PHASE, SPLIT>, ++n) {
                     const uint32_t half = n & 1;
                     if (!wait_done(half)) break;
-#pragma unroll 1
+#pragma unroll
+                    for (uint32_t c = 0; c < COLUMNS; c += 16) tc::tmem_add(sum + c, tmem + half * SIZE + lanes + first + c);
+                    release(half);
+                }
+                if (!on) break;
+                if (whole) {
+#pragma unroll
                     for (uint32_t c = 0; c < COLUMNS; c += 32) {
                         float v[32];
-                        __syncwarp();
-                        tc::tmem_load(v, tmem + half * SIZE + lanes + first + c);
-                        if (whole) {
-                            take(v, c);
-                        } else {
 #pragma unroll
-                            for (uint32_t e = 0; e < 32; e += 4)
-                                mine[(c + e) * 8] = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-                        }
+                        for (uint32_t e = 0; e < 32; ++e) v[e] = sum[c + e];
+                        take(v, c);
                     }
-                    release(half);
-                    ++n;
-                    if (whole) continue;
+                    continue;
                 }
-                // a part: the warp that brings its rows and columns' last one puts them together
-                uint32_t u0 = uint32_t(uint64_t(part.start) * plan.runs / plan.left[plan.classes]); // has the tile's first step
-                while (cut(plan, u0) > part.start) --u0;
-                while (cut(plan, u0 + 1) <= part.start) ++u0;
-                uint32_t parts = 1;
-                while (cut(plan, u0 + parts) < part.start + part.depth) ++parts;
-                __threadfence();
-                __syncwarp();
-                uint32_t before = 0;
-                if (lane == 0) before = atomicAdd(&g.arrived[u0 * (kTakers * 2) + writer], 1u);
-                if (__shfl_sync(0xffffffffu, before, 0) + 1 != parts) continue;
-                if (lane == 0) g.arrived[u0 * (kTakers * 2) + writer] = 0;
-                __threadfence();
+#pragma unroll
+                for (uint32_t c = 0; c < COLUMNS; c += 4) mine[c * 8] = make_float4(sum[c], sum[c + 1], sum[c + 2], sum[c + 3]);
+            } else {
+                const uint32_t half = n & 1;
+                if (!wait_done(half)) break;
 #pragma unroll 1
                 for (uint32_t c = 0; c < COLUMNS; c += 32) {
                     float v[32];
+                    __syncwarp();
+                    tc::tmem_load(v, tmem + half * SIZE + lanes + first + c);
+                    if (whole) {
+                        take(v, c);
+                    } else {
 #pragma unroll
-                    for (uint32_t e = 0; e < 32; ++e) v[e] = 0.0f;
-#pragma unroll 2
-                    for (uint32_t u = 0; u < parts; ++u) {
-                        const float4 *from = slice(u0 + u, u ? 0 : 1) + c * 8;
-                        float4 w[8];
-#pragma unroll
-                        for (uint32_t e = 0; e < 8; ++e) w[e] = __ldcg(from + e * 32);
-#pragma unroll
-                        for (uint32_t e = 0; e < 8; ++e) {
-                            v[4 * e] += w[e].x;
-                            v[4 * e + 1] += w[e].y;
-                            v[4 * e + 2] += w[e].z;
-                            v[4 * e + 3] += w[e].w;
-                        }
+                        for (uint32_t e = 0; e < 32; e += 4)
+                            mine[(c + e) * 8] = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
                     }
-                    take(v, c);
                 }
+                release(half);
+                ++n;
+                if (whole) continue;
+            }
+            // a part: the warp that brings its rows and columns' last one puts them together
+            uint32_t u0 = uint32_t(uint64_t(part.start) * plan.runs / plan.left[plan.classes]); // has the tile's first step
+            while (cut(plan, u0) > part.start) --u0;
+            while (cut(plan, u0 + 1) <= part.start) ++u0;
+            uint32_t parts = 1;
+            while (cut(plan, u0 + parts) < part.start + part.depth) ++parts;
+            __threadfence();
+            __syncwarp();
+            uint32_t before = 0;
+            if (lane == 0) before = atomicAdd(&g.arrived[u0 * (kTakers * 2) + writer], 1u);
+            if (__shfl_sync(0xffffffffu, before, 0) + 1 != parts) continue;
+            if (lane == 0) g.arrived[u0 * (kTakers * 2) + writer] = 0;
+            __threadfence();
+#pragma unroll 1
+            for (uint32_t c = 0; c < COLUMNS; c += 32) {
+                float v[32];
+#pragma unroll
+                for (uint32_t e = 0; e < 32; ++e) v[e] = 0.0f;
+#pragma unroll 2
+                for (uint32_t u = 0; u < parts; ++u) {
+                    const float4 *from = slice(u0 + u, u ? 0 : 1) + c * 8;
+                    float4 w[8];
+#pragma unroll
+                    for (uint32_t e = 0; e < 8; ++e) w[e] = __ldcg(from + e * 32);
+#pragma unroll
+                    for (uint32_t e = 0; e < 8; ++e) {
+                        v[4 * e] += w[e].x;
+                        v[4 * e + 1] += w[e].y;
+                        v[4 * e + 2] += w[e].z;
+                        v[4 * e + 3] += w[e].w;
+                    }
+                }
+                take(v, c);
             }
         }
     }
