@@ -753,6 +753,13 @@ __global__ void __launch_bounds__(kProductThreads, 1)
                                         square);
             };
             const bool whole = part.whole();
+            uint32_t u0 = 0, parts = 1; // the unit with the tile's first step, and how many have parts of it
+            if (!whole) {
+                u0 = uint32_t(uint64_t(part.start) * plan.runs / plan.left[plan.classes]);
+                while (cut(plan, u0) > part.start) --u0;
+                while (cut(plan, u0 + 1) <= part.start) ++u0;
+                while (cut(plan, u0 + parts) < part.start + part.depth) ++parts;
+            }
             float4 *mine = whole ? nullptr : slice(unit, part.start < from ? 0 : 1);
             if constexpr (SPLIT) {
                 float sum[COLUMNS];
@@ -800,11 +807,6 @@ __global__ void __launch_bounds__(kProductThreads, 1)
                 if (whole) continue;
             }
             // a part: the warp that brings its rows and columns' last one puts them together
-            uint32_t u0 = uint32_t(uint64_t(part.start) * plan.runs / plan.left[plan.classes]); // has the tile's first step
-            while (cut(plan, u0) > part.start) --u0;
-            while (cut(plan, u0 + 1) <= part.start) ++u0;
-            uint32_t parts = 1;
-            while (cut(plan, u0 + parts) < part.start + part.depth) ++parts;
             __threadfence();
             __syncwarp();
             uint32_t before = 0;
