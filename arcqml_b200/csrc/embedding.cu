@@ -11,6 +11,18 @@
 // places stay in order and equal inputs give equal bits without atomics on values); chunks of the sorted
 // places are then summed side by side, whatever rows they belong to, so a row that most places point to
 // costs no more than others; rows that cross chunks are put together from the chunks' partial sums.
+//
+//   k_lookup, k_lookup_row, k_row_squares   rows as they are; normalised in registers; in pieces
+//   k_direct                                the gradient of few places, in one launch
+//   k_sort_cluster                          up to 131072 places sorted, the output cleared beside that
+//   k_count_digits, k_prefix_counts,
+//   k_sort_pass, k_zero_rows                more places
+//   k_sum_chunks, k_join_chunks, k_project  sums of chunks, rows across them, the norm
+//
+// Measured on a B200 (copy rate 6543 GB/s): 65,536 bf16 rows of 2 KB at random, scaled, 36 us a call (4.6 TB/s of
+// algorithmic bytes); 1024 normalised rows of 16 KB 8.9 us in the kernel, 11 us a call (the host's time);
+// the gradient of 131,071 bf16 places in 50,021 rows of 2 KB 120 us a call: 32 us the sort, 66 us the sums
+// (4.1 TB/s), 19 us the rows across chunks; of 1024 places in 509 normalised rows of 16 KB 13.5 us a call.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
@@ -69,7 +81,8 @@ constexpr uint32_t kPieceVectors = 2048;
 
 constexpr uint32_t kNotANumber = 0x7fffffff; // as every word of a vector: NaN in each type
 
-// Rows in tiles of 4 vectors a thread, a tile taken by `lanes` threads.
+// Rows in tiles of 4 vectors a thread, a tile taken by `lanes` threads: 2 KB a warp, four loads in flight for
+// each thread. Bound by HBM for rows of 512 bytes and more (34 us for 65,536 rows of 2 KB, 243 MB).
 template <uint32_t DT, int N>
 __global__ void __launch_bounds__(kThreads) k_lookup(const __grid_constant__ Lookup a) {
     using T = Element<DT>;
@@ -129,7 +142,8 @@ template <bool BLOCK> __device__ __forceinline__ double sum_over(double v, uint3
     return v;
 }
 
-// Normalised rows that their threads hold: `lanes` threads of a warp, or a block, for each place.
+// Normalised rows that their threads hold (read once): `lanes` threads of a warp up to 4 KB a row, or a block
+// up to 32 KB, for each place. 8.9 us for 1024 rows of 16 KB from and to HBM: latency of one round.
 template <uint32_t DT, int N, bool BLOCK>
 __global__ void __launch_bounds__(kThreads) k_lookup_row(const __grid_constant__ Lookup a) {
     using T = Element<DT>;
@@ -524,7 +538,9 @@ __device__ __forceinline__ void write_sum(const Sums &a, uint32_t row, uint32_t 
     }
 }
 
-// One vector of a row for each thread, over the places of one chunk. A row that lies inside the chunk is
+// One vector of a row for each thread, over the places of one chunk, eight of them in flight: what bounds it is
+// the latency of rows at random (66 us for 131,071 rows of 2 KB, 4.1 TB/s; vectors through slots of shared
+// memory by cp.async, 16 in flight, took 76 us; whole rows of 2 KB a warp 126 us, for want of registers). A row that lies inside the chunk is
 // done; the part of one that began earlier goes to partial 2c, of one that goes on to 2c + 1.
 template <uint32_t DT, uint32_t OT, int N>
 __global__ void __launch_bounds__(kThreads, 3) k_sum_chunks(const __grid_constant__ Sums a) {
@@ -595,7 +611,8 @@ __device__ __forceinline__ uint32_t first_not_below(const uint2 *sorted, uint32_
     return lo;
 }
 
-// Rows that began in a chunk and went on: a block for each chunk and 32 vectors. Its warps add up an eighth
+// Rows that began in a chunk and went on: a block for each chunk and 32 vectors (19 us after 131,071 places, of
+// which 8,400 belong to one row). Its warps add up an eighth
 // of the row's partial sums each, in order, then the first one the eighths.
 template <uint32_t DT, uint32_t OT, int N>
 __global__ void __launch_bounds__(kThreads) k_join_chunks(const __grid_constant__ Sums a) {
@@ -663,7 +680,8 @@ template <uint32_t OT> __global__ void __launch_bounds__(kThreads) k_zero_rows(c
     }
 }
 
-// Sums through the norm of their rows, a block for each row; `sums` may be the output itself.
+// Sums through the norm of their rows, a block for each row, which reads both twice (the second time from L2):
+// one division and one root a row, f64. `sums` may be the output itself.
 struct Project {
     const char *table, *sums;
     char *out;
