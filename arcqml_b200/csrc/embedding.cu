@@ -680,37 +680,65 @@ template <uint32_t OT> __global__ void __launch_bounds__(kThreads) k_zero_rows(c
     }
 }
 
-// Sums through the norm of their rows, a block for each row, which reads both twice (the second time from L2):
-// one division and one root a row, f64. `sums` may be the output itself.
+// Sums through the norm of their rows: a cluster of 1 to 8 blocks for each row, 16 KB or more of it a block,
+// which read both twice (the second time from L2); one division and one root a row, f64. `sums` may be the
+// output itself. (Five rows of 512 KB among 138: a block each,
+// by elements, 192 us a call; now 33.)
+constexpr uint32_t kMostProject = 8;
 struct Project {
     const char *table, *sums;
     char *out;
     const uint2 *sorted;
-    uint64_t table_stride, width, rows;
+    uint64_t table_stride, width;
     uint32_t places, cleared; // rows without places are zero already
+    uint32_t vectors;         // of a row
 };
-template <uint32_t DT>
+
+// N values of the wide type, as wide accesses as they allow.
+template <class W, int N> __device__ __forceinline__ void load_values(W (&x)[N], const W *p) {
+    constexpr int PART = sizeof(W) * N > 16 ? 16 / int(sizeof(W)) : N;
+#pragma unroll
+    for (int i = 0; i < N; i += PART) {
+        Packed<W, PART> v;
+        v.load(p + i);
+#pragma unroll
+        for (int e = 0; e < PART; ++e) x[i + e] = v.wide(e);
+    }
+}
+
+template <uint32_t DT, int N>
 __global__ void __launch_bounds__(kThreads) k_project(const __grid_constant__ Project a) {
     using T = Element<DT>;
     using W = WideElement<DT>;
-    __shared__ double part[2][kWarps];
-    const uint32_t row = blockIdx.x;
+    __shared__ double part[2][kWarps], total[2];
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t size = cluster.num_blocks(), row = blockIdx.x / size;
     cudaGridDependencySynchronize();
     const uint32_t at = first_not_below(a.sorted, a.places, row);
-    T *out = reinterpret_cast<T *>(a.out) + uint64_t(row) * a.width;
-    if (at == a.places || a.sorted[at].x != row) {
+    const uint32_t each = (a.vectors + size - 1) / size, lo = cluster.block_rank() * each, hi = min(a.vectors, lo + each);
+    char *out = a.out + uint64_t(row) * a.width * sizeof(T);
+    if (at == a.places || a.sorted[at].x != row) { // the same for the whole cluster
         if (a.cleared) return;
-        for (uint64_t k = threadIdx.x; k < a.width; k += kThreads) out[k] = to_element<T>(W(0));
+        Packed<T, N> none;
+        none.fill(0);
+        for (uint32_t k = lo + threadIdx.x; k < hi; k += kThreads) none.store(out + uint64_t(k) * Packed<T, N>::BYTES);
         return;
     }
-    const T *t = reinterpret_cast<const T *>(a.table + uint64_t(row) * a.table_stride);
-    const W *g = reinterpret_cast<const W *>(a.sums) + uint64_t(row) * a.width;
+    const char *table = a.table + uint64_t(row) * a.table_stride;
+    const W *sums = reinterpret_cast<const W *>(a.sums) + uint64_t(row) * a.width;
     double tt = 0.0, tg = 0.0;
 #pragma unroll 4
-    for (uint64_t k = threadIdx.x; k < a.width; k += kThreads) {
-        const double x = to_wide(t[k]);
-        tt = fma(x, x, tt);
-        tg = fma(x, double(g[k]), tg);
+    for (uint32_t k = lo + threadIdx.x; k < hi; k += kThreads) {
+        Packed<T, N> t;
+        W g[N];
+        t.load(table + uint64_t(k) * Packed<T, N>::BYTES);
+        load_values<W, N>(g, sums + uint64_t(k) * N);
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const double x = t.wide(e);
+            tt = fma(x, x, tt);
+            tg = fma(x, double(g[e]), tg);
+        }
     }
     for (int o = 16; o > 0; o >>= 1) {
         tt += __shfl_xor_sync(0xffffffffu, tt, o);
@@ -721,15 +749,31 @@ __global__ void __launch_bounds__(kThreads) k_project(const __grid_constant__ Pr
         part[1][threadIdx.x >> 5] = tg;
     }
     __syncthreads();
-    tt = tg = 0.0;
-    for (uint32_t w = 0; w < kWarps; ++w) {
-        tt += part[0][w];
-        tg += part[1][w];
+    if (threadIdx.x < 2) {
+        double sum = 0.0;
+        for (uint32_t w = 0; w < kWarps; ++w) sum += part[threadIdx.x][w];
+        total[threadIdx.x] = sum;
     }
+    cluster.sync();
+    tt = tg = 0.0;
+    for (uint32_t b = 0; b < size; ++b) {
+        const double *there = cluster.map_shared_rank(total, b);
+        tt += there[0];
+        tg += there[1];
+    }
+    cluster.sync(); // nobody leaves while its sums are read
     const double inverse = tt == 0.0 ? 0.0 : 1.0 / sqrt(tt), along = tt == 0.0 ? 0.0 : tg / tt;
 #pragma unroll 4
-    for (uint64_t k = threadIdx.x; k < a.width; k += kThreads)
-        out[k] = to_element<T>(W((double(g[k]) - double(to_wide(t[k])) * along) * inverse));
+    for (uint32_t k = lo + threadIdx.x; k < hi; k += kThreads) {
+        Packed<T, N> t, y;
+        W g[N];
+        t.load(table + uint64_t(k) * Packed<T, N>::BYTES);
+        load_values<W, N>(g, sums + uint64_t(k) * N);
+#pragma unroll
+        for (int e = 0; e < N; ++e) g[e] = W((double(g[e]) - double(t.wide(e)) * along) * inverse);
+        y.pack(g);
+        y.store(out + uint64_t(k) * Packed<T, N>::BYTES);
+    }
 }
 
 // ------------------------------------------------------------------ few places: everything in one launch
@@ -1243,23 +1287,30 @@ void embedding_gradient_device(const ArcqmlRows &gradient, const void *indices, 
             sums(type);
         }
     });
-    for_access(out.dtype, 16, [&](auto type, auto) {
+    if (!o.normalize) {
+        if (!in_cluster)
+            for_access(out.dtype, 16, [&](auto type, auto) {
+                constexpr uint32_t DT = type;
+                start(k_zero_rows<DT>, {(out.rows + kWarps * 32 - 1) / (kWarps * 32), kThreads, true}, 0.0, s, a);
+            });
+        return;
+    }
+    Project p{};
+    p.table = static_cast<const char *>(table->data);
+    p.sums = a.out;
+    p.out = static_cast<char *>(out.data);
+    p.sorted = sorted;
+    p.table_stride = table->stride * size;
+    p.width = out.width;
+    p.places = uint32_t(n);
+    p.cleared = in_cluster;
+    p.vectors = uint32_t(row / bytes);
+    uint32_t cluster = 1;
+    while (cluster < kMostProject && row >= uint64_t(cluster) << 15) cluster *= 2;
+    for_access(out.dtype, bytes, [&](auto type, auto nn) {
         constexpr uint32_t DT = type;
-        if (!o.normalize) {
-            if (!in_cluster) start(k_zero_rows<DT>, {(out.rows + kWarps * 32 - 1) / (kWarps * 32), kThreads, true}, 0.0, s, a);
-            return;
-        }
-        Project p{};
-        p.table = static_cast<const char *>(table->data);
-        p.sums = a.out;
-        p.out = static_cast<char *>(out.data);
-        p.sorted = sorted;
-        p.table_stride = table->stride * size;
-        p.width = out.width;
-        p.rows = out.rows;
-        p.places = uint32_t(n);
-        p.cleared = in_cluster;
-        start(k_project<DT>, {out.rows, kThreads, true}, 3.0 * double(row) * double(out.rows), s, p);
+        constexpr int N = nn;
+        start(k_project<DT, N>, {out.rows * cluster, kThreads, true, cluster}, 3.0 * double(row) * double(out.rows), s, p);
     });
 }
 
