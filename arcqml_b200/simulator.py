@@ -339,6 +339,8 @@ class StateVectorSimulator:
 class BatchStateVectorSimulator:
     """[batch, 2^n] independent states sharing one circuit and observable."""
 
+    states = None  # of from_table: the batch as autograd knows it
+
     def __init__(self, num_qubits: int, batch_size: int, device=None):
         if batch_size <= 0:
             raise SimError("batch size must be non-zero")
@@ -378,8 +380,9 @@ class BatchStateVectorSimulator:
         """Rows of a complex128 CUDA table of amplitudes ([rows, 2^n]) picked by `indices` (one-dimensional
         int64 or int32 CUDA tensor) and normalised. ``states`` of the simulator is the batch as autograd knows
         it: ``sim.states.backward(initial_state_grad)`` gives the table its gradient after
-        ``RunResult.backward``. A row of zeros is no state and an index outside the table gives NaN; neither
-        is looked for."""
+        ``RunResult.backward``. ``apply_circuit`` leaves ``states`` as they are, and is refused where they
+        require a gradient. A row of zeros is no state and an index outside the table gives NaN; neither is
+        looked for."""
         from .embedding import lookup
         torch = _torch()
         if not isinstance(table, torch.Tensor) or table.dtype != torch.complex128 or table.dim() != 2 \
@@ -397,6 +400,12 @@ class BatchStateVectorSimulator:
 
     def apply_circuit(self, circuit: Circuit) -> None:
         plan = rt.CircuitPlan.create(circuit.compile_plan(0))
+        if self.states is not None:
+            if self.states.requires_grad:
+                raise SimError("the initial-state gradient of evolved states is not that of the table's rows: "
+                               "give run() the whole circuit, or make the batch under torch.no_grad()")
+            if self.state.data_ptr() == self.states.data_ptr():  # the rows stay what autograd knows
+                self.state = self.state.clone()
         rt.plan_apply_device(plan, self.state, self.num_qubits)
 
     def expectation(self, observable: SparsePauliOp) -> np.ndarray:
