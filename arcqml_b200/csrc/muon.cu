@@ -179,6 +179,10 @@ __device__ __forceinline__ void new_update8(float (&u)[8], const Matrix &a, uint
 __device__ __forceinline__ int shift_of(double norm, double whole) {
     return norm > 0.0 && norm < whole && whole < INFINITY ? max(0, ilogb(whole) - ilogb(norm) - 1) : 0;
 }
+// X as it is stored is u times this. Zeros stay zeros without an epsilon too, where X is 0 / 0.
+__device__ __forceinline__ double factor_of(double whole, int shift) {
+    return whole == 0.0 ? 0.0 : ldexp(double(kScaleX) / whole, shift);
+}
 
 // 2^-n; 0 below f32's normal range, where what it scales is nothing beside what it joins. (ldexpf takes some
 // 300 cycles, in every phase.)
@@ -289,7 +293,7 @@ template <bool SPLIT> __global__ void __launch_bounds__(kThreads) k_spread(const
     const double norm = sqrt(block_sum(sum)), whole = norm + g.eps;
     const int shift = shift_of(norm, whole);
     if (block == 0 && threadIdx.x == 0) g.shift[k] = shift;
-    const double factor = ldexp(double(kScaleX) / whole, shift);
+    const double factor = factor_of(whole, shift);
     const uint32_t row0 = block / a.x_blocks * kRows, column0 = block % a.x_blocks * kDepth;
     const uint64_t low = bytes_of(a.down_blocks, a.x_blocks);
     char *to = g.scratch + a.x[0];
@@ -931,7 +935,7 @@ template <bool SPLIT> __global__ void __launch_bounds__(kSmallThreads, 1)
     }
     const double norm = sqrt(block_sum(sum)), whole = norm + g.eps; // (and a barrier)
     int shift = shift_of(norm, whole);
-    const double factor = ldexp(double(kScaleX) / whole, shift);
+    const double factor = factor_of(whole, shift);
     const uint32_t pitch = a.flip ? a.m : a.n;
     for (uint32_t i = thread * 8; i < all; i += kSmallThreads * 8) {
         const uint32_t count = min(8u, all - i);

@@ -335,7 +335,8 @@ size_t arcqml_rt_v2_orthogonalize_workspace(const ArcqmlMatrix *matrices, size_t
 
 /* outputs[i] <- matrices[i] with its singular values pushed towards 1 by `steps` (1 to 20) steps of the
  * polynomial X <- a X + (b A + c A^2) X, A = X X^T (X^T X for more rows than columns),
- * (a, b, c) = (3.4445, -4.7750, 2.0315), from X = matrix / (its Frobenius norm + epsilon). Products of
+ * (a, b, c) = (3.4445, -4.7750, 2.0315), from X = matrix / (its Frobenius norm + epsilon); a matrix of
+ * zeros stays zero, with an epsilon of 0 too. Products of
  * f32 and f16 matrices are formed from operands of 22 bits, those of bf16 matrices from operands of 11,
  * sums in f32. outputs have the matrices' shapes and types; they are the matrices
  * themselves, place by place, or overlap none of them, nor one another. A NaN or infinity in a matrix makes that output NaN. */
