@@ -808,7 +808,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_direct(const __grid_constant__ 
     __shared__ uint32_t list[kFewPlaces]; // the row within the group << 16 | the place
     __shared__ uint32_t count[kWarps + 1];
     const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    const uint32_t row0 = blockIdx.x * a.group, rows = min(a.group, a.rows - row0);
+    const uint32_t row0 = blockIdx.y * a.group, rows = min(a.group, a.rows - row0);
     const uint32_t each = (a.places + kThreads - 1) / kThreads * 32, lo = warp * each; // places of a warp
     constexpr uint32_t ROUNDS = kFewPlaces / kThreads;
     uint32_t mine[ROUNDS], found = 0;
@@ -835,7 +835,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_direct(const __grid_constant__ 
     // places at a time: four in registers left one block on an SM (22 us instead of 17 for 1024 places of 509
     // rows of 16 KB)
     constexpr uint32_t THREADS = BLOCK ? kThreads : 32, PLACES = Packed<T, N>::BYTES == 16 ? 2 : 4;
-    const uint32_t thread = BLOCK ? t : lane, vector0 = blockIdx.y * (THREADS * kDirectVectors) + thread;
+    const uint32_t thread = BLOCK ? t : lane, vector0 = blockIdx.x * (THREADS * kDirectVectors) + thread;
     for (uint32_t r = BLOCK ? 0 : warp; r < rows; r += BLOCK ? 1 : kWarps) {
         W sum[kDirectVectors][N];
 #pragma unroll
@@ -1000,12 +1000,12 @@ struct Shape {
     uint64_t blocks;
     uint32_t threads;
     bool follows = false; // may start while the call's last launch ends
-    uint32_t cluster = 1, shared = 0, across = 1;
+    uint32_t cluster = 1, shared = 0, down = 1; // down: the grid's second dimension
 };
 
 template <class... P, class... A>
 void start(void (*kernel)(P...), const Shape &shape, double bytes, cudaStream_t s, const A &...args) {
-    if (shape.blocks >> 31) fail("the embedding call is too large for one launch");
+    if (shape.blocks >> 31 || shape.down > 65535) fail("the embedding call is too large for one launch");
     cudaLaunchConfig_t c{};
     cudaLaunchAttribute at[2]{};
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1015,7 +1015,7 @@ void start(void (*kernel)(P...), const Shape &shape, double bytes, cudaStream_t 
     at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     c.attrs = shape.follows ? at : at + 1;
     c.numAttrs = (shape.follows ? 1 : 0) + (shape.cluster > 1 ? 1 : 0);
-    c.gridDim = dim3(uint32_t(shape.blocks), shape.across);
+    c.gridDim = dim3(uint32_t(shape.blocks), shape.down);
     c.blockDim = dim3(shape.threads);
     c.dynamicSmemBytes = shape.shared;
     c.stream = s;
@@ -1187,10 +1187,11 @@ void embedding_gradient_device(const ArcqmlRows &gradient, const void *indices, 
         a.vectors = uint32_t(row / whole);
         const bool wide = a.vectors > 32 * kDirectVectors;
         const uint32_t across = wide ? (a.vectors + kThreads * kDirectVectors - 1) / (kThreads * kDirectVectors) : 1;
-        // blocks for each place on the GPU; warps take the rows of a block in turn
+        // blocks for each place on the GPU; warps take the rows of a block in turn. At most 32769 blocks of rows,
+        // in the grid's second dimension; the pieces of a row, up to 2^20, have the first one
         a.group = uint32_t(std::min<uint64_t>(65535, (out.rows + 148 * 6 - 1) / (148 * 6)));
         if (!wide) a.group = std::max(a.group, kWarps);
-        const Shape shape{(out.rows + a.group - 1) / a.group, kThreads, false, 1, 0, across};
+        const Shape shape{across, kThreads, false, 1, 0, uint32_t((out.rows + a.group - 1) / a.group)};
         return for_access(gradient.dtype, whole, [&](auto type, auto nn) {
             constexpr uint32_t DT = type;
             constexpr int N = nn;
