@@ -354,12 +354,13 @@ struct ProductState {
 };
 static_assert(sizeof(ProductState) <= 256, "the end of the shared memory");
 
-// Waits for a barrier's phase; false once a wait of this block has run out.
-__device__ __forceinline__ bool wait_for(uint64_t *b, uint32_t parity, uint32_t *stop) {
-    if (tc::barrier_try(b, parity)) return true;
+// Waits for a barrier's phase; false once a wait of this block has run out. CG: 2 if the other block of a pair
+// arrives there.
+template <int CG> __device__ __forceinline__ bool wait_for(uint64_t *b, uint32_t parity, uint32_t *stop) {
+    if (tc::barrier_try<CG>(b, parity)) return true;
     const long long begin = clock64();
     for (uint32_t i = 0; i < (1u << 30); ++i) { // ten seconds at most
-        if (tc::barrier_try(b, parity)) return true;
+        if (tc::barrier_try<CG>(b, parity)) return true;
         if (*reinterpret_cast<volatile uint32_t *>(stop)) return false;
         if (clock64() - begin > 20000000000ll) break;
     }
@@ -666,7 +667,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
                 const bool has_right = right < a.down_blocks;
                 const uint32_t bytes = parts * ((has_left ? kBlock : 0) + (PHASE == APPLY ? wide * (kBlock / 2) : has_right ? kBlock : 0));
                 for (uint32_t d = part.begin; d < part.end; ++d) {
-                    if (!(on = wait_for(&st.empty[at], phase ^ 1, &st.stop))) break;
+                    if (!(on = wait_for<CG>(&st.empty[at], phase ^ 1, &st.stop))) break;
                     char *to = shared + at * STAGE;
                     tc::barrier_expect(&st.full[at], bytes);
                     for (uint32_t part = 0; part < parts; ++part, to += kStageBytes) {
@@ -690,7 +691,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
             // or (after a wait that ran out) its copies are waited for
             if (!on) {
                 uint32_t none = 0;
-                for (uint32_t s = 0; s < S; ++s) wait_for(&st.full[s], s < at ? phase : phase ^ 1, &none);
+                for (uint32_t s = 0; s < S; ++s) wait_for<1>(&st.full[s], s < at ? phase : phase ^ 1, &none);
             }
         } else if (warp == 1 && rank == 0 && lane == 0) { // issues the products
             constexpr uint32_t instr = tc::instruction(SIZE, SIZE, PHASE == APPLY);
@@ -700,13 +701,13 @@ __global__ void __launch_bounds__(kProductThreads, 1)
             for (; on && more; more = walk.next(part)) {
                 for (uint32_t d = part.begin; d < part.end && on; ++n) {
                     const uint32_t half = n & 1, end = min(part.end - d, kChain<PHASE, SPLIT>) + d;
-                    if (!(on = wait_for(&st.taken[half], (n >> 1 & 1) ^ 1, &st.stop))) break;
+                    if (!(on = wait_for<CG>(&st.taken[half], (n >> 1 & 1) ^ 1, &st.stop))) break;
                     tc::fence_after();
                     const uint32_t sums = tmem + half * SIZE;
                     for (bool add = false; d < end; ++d) {
-                        if (!(on = wait_for(&st.full[at], phase, &st.stop))) break;
+                        if (!(on = wait_for<1>(&st.full[at], phase, &st.stop))) break;
                         if constexpr (CG == 2)
-                            if (!(on = wait_for(&st.peer[at], phase, &st.stop))) break;
+                            if (!(on = wait_for<CG>(&st.peer[at], phase, &st.stop))) break;
                         tc::fence_after();
                         const uint32_t base = tc::shared_address(shared + at * STAGE);
                         const uint64_t left = tc::descriptor(base, 16);
@@ -732,8 +733,8 @@ __global__ void __launch_bounds__(kProductThreads, 1)
             bool on = true;
             for (; on && more; more = walk.next(part)) {
                 for (uint32_t d = part.begin; d < part.end; ++d) {
-                    if (!(on = wait_for(&st.full[at], phase, &st.stop))) break;
-                    tc::barrier_arrive_at(tc::in_block(&st.peer[at], 0));
+                    if (!(on = wait_for<1>(&st.full[at], phase, &st.stop))) break;
+                    tc::barrier_arrive_at<CG>(tc::in_block(&st.peer[at], 0));
                     if (++at == S) at = 0, phase ^= 1;
                 }
             }
@@ -751,10 +752,10 @@ __global__ void __launch_bounds__(kProductThreads, 1)
             tc::fence_before();
             __syncwarp();
             if (lane == 0)
-                tc::barrier_arrive_at(CG == 2 ? tc::in_block(&st.taken[half], 0) : tc::shared_address(&st.taken[half]));
+                tc::barrier_arrive_at<CG>(CG == 2 ? tc::in_block(&st.taken[half], 0) : tc::shared_address(&st.taken[half]));
         };
         const auto wait_done = [&](uint32_t half) {
-            on = __all_sync(0xffffffffu, wait_for(&st.done[half], n >> 1 & 1, &st.stop));
+            on = __all_sync(0xffffffffu, wait_for<CG>(&st.done[half], n >> 1 & 1, &st.stop));
             tc::fence_after();
             return on;
         };
@@ -979,7 +980,7 @@ template <bool SPLIT> __global__ void __launch_bounds__(kSmallThreads, 1)
         }
     };
     const auto sums_ready = [&] {
-        const bool ok = wait_for(&st.done, parity, &st.stop);
+        const bool ok = wait_for<1>(&st.done, parity, &st.stop);
         parity ^= 1;
         broken = __syncthreads_or(!ok);
         tc::fence_after();

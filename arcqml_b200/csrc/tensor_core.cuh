@@ -23,19 +23,35 @@ __device__ __forceinline__ uint32_t in_block(const void *b, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(shared_address(b)), "r"(rank));
     return at;
 }
-// What these barriers order is read and written by copies and tensor cores alone, not by threads: a block's
-// scope is enough, and a cluster's costs a fence for each arrival (a stage of a pair took 1300 cycles with it).
-__device__ __forceinline__ void barrier_arrive_at(uint32_t cluster_address) {
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_address) : "memory");
+// Barriers of a pair of blocks (CG = 2) are arrived at by one block and waited for by the other, which orders what
+// the two have done only in the scope of their cluster. What an arrival releases lies in its own block's shared
+// memory (operands that copies have brought) or in tensor memory (ordered by fence_before): a fence of
+// shared memory alone is enough, and one of everything costs some 1000 cycles between a stage's arrival and its
+// products (8 large bf16 matrices 11.1 ms with it in one warp, 8.4 in three, 8.0 as it is).
+template <int CG> __device__ __forceinline__ void barrier_arrive_at(uint32_t cluster_address) {
+    if constexpr (CG == 1)
+        asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(cluster_address) : "memory");
+    else
+        asm volatile("fence.release.sync_restrict::shared::cta.cluster;\n"
+                     " mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_address)
+                     : "memory");
 }
-__device__ __forceinline__ bool barrier_try(uint64_t *b, uint32_t parity) {
+template <int CG> __device__ __forceinline__ bool barrier_try(uint64_t *b, uint32_t parity) {
     uint32_t done;
-    asm volatile("{\n .reg .pred p;\n"
-                 " mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-                 " selp.u32 %0, 1, 0, p;\n}"
-                 : "=r"(done)
-                 : "r"(shared_address(b)), "r"(parity)
-                 : "memory");
+    if constexpr (CG == 1)
+        asm volatile("{\n .reg .pred p;\n"
+                     " mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n"
+                     " selp.u32 %0, 1, 0, p;\n}"
+                     : "=r"(done)
+                     : "r"(shared_address(b)), "r"(parity)
+                     : "memory");
+    else
+        asm volatile("{\n .reg .pred p;\n"
+                     " mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+                     " selp.u32 %0, 1, 0, p;\n}"
+                     : "=r"(done)
+                     : "r"(shared_address(b)), "r"(parity)
+                     : "memory");
     return done != 0;
 }
 __device__ __forceinline__ void barrier_init_fence() {
