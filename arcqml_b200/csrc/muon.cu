@@ -687,11 +687,12 @@ __global__ void __launch_bounds__(kProductThreads, 1)
                     if (++at == S) at = 0, phase ^= 1;
                 }
             }
-            // nothing may still be on its way in when the block ends: every stage that was filled has been read,
-            // or (after a wait that ran out) its copies are waited for
-            if (!on) {
-                uint32_t none = 0;
-                for (uint32_t s = 0; s < S; ++s) wait_for<1>(&st.full[s], s < at ? phase : phase ^ 1, &none);
+            // nothing may still be on its way in when the block ends: neither the tensor cores' word that a stage has
+            // been read, nor (after a wait that ran out) copies
+            uint32_t none = 0;
+            for (uint32_t s = 0; s < S; ++s) {
+                if (on) wait_for<CG>(&st.empty[s], s < at ? phase : phase ^ 1, &st.stop);
+                else wait_for<1>(&st.full[s], s < at ? phase : phase ^ 1, &none);
             }
         } else if (warp == 1 && rank == 0 && lane == 0) { // issues the products
             constexpr uint32_t instr = tc::instruction(SIZE, SIZE, PHASE == APPLY);

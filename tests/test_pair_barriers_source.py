@@ -36,3 +36,28 @@ def test_barriers_of_a_pair_are_waited_for_in_its_scope():
         assert scope == ("<1>" if barrier == "full" else "<CG>"), (scope, barrier)
     arrivals = re.findall(r"barrier_arrive_at(<\w+>)?\(", kernel)
     assert arrivals and set(arrivals) == {"<CG>"}
+
+
+def test_a_block_stays_until_its_last_stages_are_read():
+    """The tensor cores arrive at `empty` of both blocks some time after the products were issued: the thread that
+    copies in waits for that behind its last stage, since a block that has ended has no shared memory to arrive in."""
+    text = source("muon.cu")
+    copies = text[text.index("if (warp == 0 && lane == 0) { // copies operands in"):text.index("// issues the products")]
+    loop = copies.index("for (; on && more; more = walk.next(part))")
+    behind = copies[copies.index("if (++at == S)", loop):]
+    assert re.search(r"if \(on\) wait_for<CG>\(&st\.empty\[s\], s < at \? phase : phase \^ 1", behind)
+
+
+def test_parities_behind_the_last_stage():
+    """`empty` of stage s has gone through as many phases as the stage was filled when what the test above looks for
+    passes: a barrier of n phases passes parity (n - 1) & 1, and a fresh one parity 1."""
+    for stages in (3, 6):
+        at, phase, filled = 0, 0, [0] * stages
+        for _ in range(40):
+            for s in range(stages):
+                parity = phase if s < at else phase ^ 1
+                assert parity == (filled[s] - 1) & 1
+            filled[at] += 1
+            at += 1
+            if at == stages:
+                at, phase = 0, phase ^ 1
