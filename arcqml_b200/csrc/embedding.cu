@@ -67,7 +67,9 @@ struct Lookup {
     Indices index;
     uint64_t places, stride, row_bytes; // stride: bytes between the table's rows
     double scale;
-    const double *squares; // of normalised rows in pieces: sums of squares, `pieces` for each place
+    // of normalised rows in pieces: sums of squares, `pieces` for each place; of f64, negative ones were formed of
+    // numbers 2^-n times as large, n lies `places * pieces` behind them
+    const double *squares;
     uint32_t vectors;      // of a row
     uint32_t lanes;        // a power of two: threads that share a tile
     uint32_t tiles, pieces;
@@ -80,6 +82,25 @@ constexpr uint32_t kPieceVectors = 2048;
 // ------------------------------------------------------------------ lookup
 
 constexpr uint32_t kNotANumber = 0x7fffffff; // as every word of a vector: NaN in each type
+
+// Squares of f64 leave its range long before the numbers do. A row whose sum of squares is near the range's ends
+// (what is lost below 2^-900 is 2^-174 of it or less) is gone through again with numbers 2^-n times as large, n the
+// exponent of its largest one; squares of the other types stay far inside. A NaN or an infinity stays what it is.
+template <class W> __device__ __forceinline__ bool out_of_range(double squares) {
+    return sizeof(W) == 8 && (squares < 0x1p-900 || squares > 0x1p900);
+}
+__device__ __forceinline__ int power_of(double largest) {
+    return largest > 0.0 && largest < INFINITY ? ilogb(largest) : 0;
+}
+// Numbers of a vector 2^-power times as large.
+template <class T, int N> __device__ __forceinline__ void rescale(Packed<T, N> &v, int power) {
+    if constexpr (sizeof(T) == 8) {
+        double x[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] = scalbn(v.wide(e), -power);
+        v.pack(x);
+    }
+}
 
 // Rows in tiles of 4 vectors a thread, a tile taken by `lanes` threads: 2 KB a warp, four loads in flight for
 // each thread. Bound by HBM for rows of 512 bytes and more (34 us for 65,536 rows of 2 KB, 243 MB).
@@ -105,8 +126,26 @@ __global__ void __launch_bounds__(kThreads) k_lookup(const __grid_constant__ Loo
     double factor = a.scale;
     if (a.squares) {
         double sum = 0.0;
-        if (inside && !padding)
-            for (uint32_t p = 0; p < a.pieces; ++p) sum += a.squares[place * a.pieces + p];
+        if (inside && !padding) {
+            const double *squares = a.squares + place * a.pieces, *powers = squares + a.places * a.pieces;
+            bool apart = false;
+            for (uint32_t p = 0; p < a.pieces; ++p) {
+                sum += squares[p];
+                apart = apart || squares[p] < 0.0;
+            }
+            if (sizeof(W) == 8 && apart) { // pieces of different powers: all by the largest one's
+                int power = -4096;
+#pragma unroll 1
+                for (uint32_t p = 0; p < a.pieces; ++p)
+                    if (squares[p] != 0.0) power = max(power, squares[p] < 0.0 ? int(powers[p]) : 0);
+                sum = 0.0;
+#pragma unroll 1
+                for (uint32_t p = 0; p < a.pieces; ++p)
+                    sum += scalbn(fabs(squares[p]), 2 * ((squares[p] < 0.0 ? int(powers[p]) : 0) - power));
+#pragma unroll
+                for (uint32_t j = 0; j < kTileVectors; ++j) rescale(v[j], power);
+            }
+        }
         factor = sum == 0.0 ? 0.0 : a.scale / sqrt(sum);
     }
     const bool plain = !a.squares && factor == 1.0; // the rows as they are
@@ -142,6 +181,20 @@ template <bool BLOCK> __device__ __forceinline__ double sum_over(double v, uint3
     return v;
 }
 
+// The largest over `lanes` threads.
+template <bool BLOCK> __device__ __forceinline__ double largest_over(double v, uint32_t lanes) {
+    const uint32_t within = BLOCK ? 32 : lanes;
+    for (uint32_t o = within / 2; o > 0; o >>= 1) v = fmax(v, __shfl_xor_sync(0xffffffffu, v, int(o)));
+    if constexpr (BLOCK) {
+        __shared__ double part[kThreads / 32];
+        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+        __syncthreads(); // (behind the last use of sum_over's shared memory, too)
+        v = 0.0;
+        for (int w = 0; w < kThreads / 32; ++w) v = fmax(v, part[w]);
+    }
+    return v;
+}
+
 // Normalised rows that their threads hold (read once): `lanes` threads of a warp up to 4 KB a row, or a block
 // up to 32 KB, for each place. 8.9 us for 1024 rows of 16 KB from and to HBM: latency of one round.
 template <uint32_t DT, int N, bool BLOCK>
@@ -173,6 +226,27 @@ __global__ void __launch_bounds__(kThreads) k_lookup_row(const __grid_constant__
             sum = fma(x, x, sum);
         }
     sum = sum_over<BLOCK>(sum, lanes);
+    const bool far = inside && !padding && out_of_range<W>(sum);
+    if (sizeof(W) == 8 && __any_sync(0xffffffffu, far)) { // one of the warp's rows; the block's one
+        double largest = 0.0;
+#pragma unroll
+        for (uint32_t j = 0; j < kRowVectors; ++j)
+#pragma unroll
+            for (int e = 0; e < N; ++e) largest = fmax(largest, fabs(double(v[j].wide(e))));
+        largest = largest_over<BLOCK>(largest, lanes);
+        const int power = far ? power_of(largest) : 0;
+        double again = 0.0;
+#pragma unroll
+        for (uint32_t j = 0; j < kRowVectors; ++j) {
+            rescale(v[j], power);
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const double x = v[j].wide(e);
+                again = fma(x, x, again);
+            }
+        }
+        sum = sum_over<BLOCK>(again, lanes); // a row in the range has the same one again
+    }
     const double factor = sum == 0.0 ? 0.0 : a.scale / sqrt(sum);
     char *to = a.out + place * a.row_bytes;
 #pragma unroll
@@ -199,23 +273,37 @@ __global__ void __launch_bounds__(kThreads) k_row_squares(const __grid_constant_
     const uint64_t place = blockIdx.x / a.pieces;
     const uint32_t piece = blockIdx.x % a.pieces;
     const int64_t row = a.index[place];
-    double sum = 0.0;
-    if (a.index.inside(row) && !a.index.is_padding(row)) {
-        const char *from = a.table + uint64_t(row) * a.stride;
-        const uint32_t end = min(a.vectors, (piece + 1) * kPieceVectors);
+    const char *from = a.table + (a.index.inside(row) ? uint64_t(row) : 0) * a.stride;
+    const uint32_t first = piece * kPieceVectors;
+    const uint32_t end = a.index.inside(row) && !a.index.is_padding(row) ? min(a.vectors, first + kPieceVectors) : first;
+    const auto over_row = [&](auto &&use) {
 #pragma unroll 8
-        for (uint32_t k = piece * kPieceVectors + threadIdx.x; k < end; k += kThreads) {
+        for (uint32_t k = first + threadIdx.x; k < end; k += kThreads) {
             Packed<T, N> v;
             v.load(from + uint64_t(k) * Packed<T, N>::BYTES);
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-                const double x = v.wide(e);
+            for (int e = 0; e < N; ++e) use(v.wide(e));
+        }
+    };
+    double sum = 0.0;
+    over_row([&](double x) { sum = fma(x, x, sum); });
+    sum = sum_over<true>(sum, kThreads);
+    const uint64_t at = place * a.pieces + piece;
+    if (end > first && out_of_range<WideElement<DT>>(sum)) { // the same in the whole block
+        double largest = 0.0;
+        over_row([&](double x) { largest = fmax(largest, fabs(x)); });
+        const int power = power_of(largest_over<true>(largest, kThreads));
+        if (power) {
+            sum = 0.0;
+            over_row([&](double x) {
+                x = scalbn(x, -power);
                 sum = fma(x, x, sum);
-            }
+            });
+            sum = -sum_over<true>(sum, kThreads);
+            if (threadIdx.x == 0) squares[a.places * a.pieces + at] = power;
         }
     }
-    sum = sum_over<true>(sum, kThreads);
-    if (threadIdx.x == 0) squares[uint64_t(place) * a.pieces + piece] = sum;
+    if (threadIdx.x == 0) squares[at] = sum;
 }
 
 // ------------------------------------------------------------------ sorting the places by their rows
@@ -727,6 +815,31 @@ __global__ void __launch_bounds__(kThreads) k_project(const __grid_constant__ Pr
     const char *table = a.table + uint64_t(row) * a.table_stride;
     const W *sums = reinterpret_cast<const W *>(a.sums) + uint64_t(row) * a.width;
     double tt = 0.0, tg = 0.0;
+    const auto over_cluster = [&](auto &&join) { // of tt and tg
+        for (int o = 16; o > 0; o >>= 1) {
+            tt = join(tt, __shfl_xor_sync(0xffffffffu, tt, o));
+            tg = join(tg, __shfl_xor_sync(0xffffffffu, tg, o));
+        }
+        if ((threadIdx.x & 31) == 0) {
+            part[0][threadIdx.x >> 5] = tt;
+            part[1][threadIdx.x >> 5] = tg;
+        }
+        __syncthreads();
+        if (threadIdx.x < 2) {
+            double all = 0.0;
+            for (uint32_t w = 0; w < kWarps; ++w) all = join(all, part[threadIdx.x][w]);
+            total[threadIdx.x] = all;
+        }
+        cluster.sync();
+        tt = tg = 0.0;
+        for (uint32_t b = 0; b < size; ++b) {
+            const double *there = cluster.map_shared_rank(total, b);
+            tt = join(tt, there[0]);
+            tg = join(tg, there[1]);
+        }
+        cluster.sync(); // nobody leaves, or writes anew, while its sums are read
+    };
+    const auto add = [](double x, double y) { return x + y; };
 #pragma unroll 4
     for (uint32_t k = lo + threadIdx.x; k < hi; k += kThreads) {
         Packed<T, N> t;
@@ -740,28 +853,30 @@ __global__ void __launch_bounds__(kThreads) k_project(const __grid_constant__ Pr
             tg = fma(x, double(g[e]), tg);
         }
     }
-    for (int o = 16; o > 0; o >>= 1) {
-        tt += __shfl_xor_sync(0xffffffffu, tt, o);
-        tg += __shfl_xor_sync(0xffffffffu, tg, o);
+    over_cluster(add);
+    if (out_of_range<W>(tt)) { // the same in the whole cluster
+        const T *x = reinterpret_cast<const T *>(table);
+        const uint32_t first = lo * N + threadIdx.x, end = hi * N;
+        tt = 0.0;
+#pragma unroll 1
+        for (uint32_t k = first; k < end; k += kThreads) tt = fmax(tt, fabs(double(to_wide(x[k]))));
+        over_cluster([](double v, double w) { return fmax(v, w); });
+        const int power = power_of(tt);
+        tt = tg = 0.0;
+#pragma unroll 1
+        for (uint32_t k = first; k < end; k += kThreads) {
+            const double t = scalbn(double(to_wide(x[k])), -power);
+            tt = fma(t, t, tt);
+            tg = fma(t, double(sums[k]), tg);
+        }
+        over_cluster(add);
+        const double inverse = tt == 0.0 ? 0.0 : 1.0 / sqrt(tt), along = tt == 0.0 ? 0.0 : tg / tt;
+#pragma unroll 1
+        for (uint32_t k = first; k < end; k += kThreads)
+            reinterpret_cast<T *>(out)[k] = to_element<T>(
+                W(scalbn((double(sums[k]) - scalbn(double(to_wide(x[k])), -power) * along) * inverse, -power)));
+        return;
     }
-    if ((threadIdx.x & 31) == 0) {
-        part[0][threadIdx.x >> 5] = tt;
-        part[1][threadIdx.x >> 5] = tg;
-    }
-    __syncthreads();
-    if (threadIdx.x < 2) {
-        double sum = 0.0;
-        for (uint32_t w = 0; w < kWarps; ++w) sum += part[threadIdx.x][w];
-        total[threadIdx.x] = sum;
-    }
-    cluster.sync();
-    tt = tg = 0.0;
-    for (uint32_t b = 0; b < size; ++b) {
-        const double *there = cluster.map_shared_rank(total, b);
-        tt += there[0];
-        tg += there[1];
-    }
-    cluster.sync(); // nobody leaves while its sums are read
     const double inverse = tt == 0.0 ? 0.0 : 1.0 / sqrt(tt), along = tt == 0.0 ? 0.0 : tg / tt;
 #pragma unroll 4
     for (uint32_t k = lo + threadIdx.x; k < hi; k += kThreads) {
@@ -899,6 +1014,32 @@ __global__ void __launch_bounds__(kThreads, 2) k_direct(const __grid_constant__ 
             if constexpr (BLOCK) __syncthreads(); // the first sum's shared memory
             ts = sum_over<BLOCK>(ts, 32);
             if constexpr (BLOCK) __syncthreads();
+            if (out_of_range<W>(tt)) {
+                double largest = 0.0;
+#pragma unroll
+                for (uint32_t j = 0; j < kDirectVectors; ++j)
+                    if (vector0 + j * THREADS < a.vectors)
+#pragma unroll
+                        for (int e = 0; e < N; ++e) largest = fmax(largest, fabs(double(unit[j].wide(e))));
+                const int power = power_of(largest_over<BLOCK>(largest, 32));
+                tt = ts = 0.0;
+#pragma unroll
+                for (uint32_t j = 0; j < kDirectVectors; ++j) {
+                    if (vector0 + j * THREADS >= a.vectors) continue;
+                    rescale(unit[j], power);
+#pragma unroll
+                    for (int e = 0; e < N; ++e) {
+                        const double x = unit[j].wide(e);
+                        sum[j][e] = W(scalbn(double(sum[j][e]), -power)); // what is over the norm goes on so
+                        tt = fma(x, x, tt);
+                        ts = fma(x, double(sum[j][e]), ts);
+                    }
+                }
+                tt = sum_over<BLOCK>(tt, 32);
+                if constexpr (BLOCK) __syncthreads();
+                ts = sum_over<BLOCK>(ts, 32);
+                if constexpr (BLOCK) __syncthreads();
+            }
             inverse = tt == 0.0 ? 0.0 : 1.0 / sqrt(tt);
             along = tt == 0.0 ? 0.0 : ts / tt;
         }
@@ -1094,7 +1235,7 @@ GradientScratch gradient_scratch(const ArcqmlRows &g, uint64_t rows, const Arcqm
 }  // namespace
 
 size_t embedding_lookup_workspace(const ArcqmlRows &table, size_t count, const ArcqmlEmbeddingOptions &o) {
-    return size_t(most_pieces(table, o)) * count;
+    return size_t(most_pieces(table, o)) * count * (table.dtype == ARCQML_F64 ? 2 : 1);
 }
 
 size_t embedding_gradient_workspace(const ArcqmlRows &gradient, uint64_t rows, const ArcqmlEmbeddingOptions &o) {

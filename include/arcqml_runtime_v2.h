@@ -276,8 +276,8 @@ int32_t arcqml_rt_v2_adam_step(const ArcqmlTensor *parameters, const ArcqmlTenso
 
 /* Rows of a table, looked up by index: token embeddings, or states made of trained amplitudes. A
  * complex table's row is its components. indices: device, `count` integers of index_bytes (4 or 8) each.
- * With `normalize` a row is divided by its 2-norm, which makes states of amplitudes; a row of zeros stays
- * zero. An index equal to `padding` (when it is not negative) gives a row of zeros. An index outside
+ * With `normalize` a row is divided by its 2-norm, which makes states of amplitudes, whatever the size of its
+ * finite numbers; a row of zeros stays zero. An index equal to `padding` (when it is not negative) gives a row of zeros. An index outside
  * [0, rows) gives a row of NaN, since refusing it would take a wait for the device. */
 typedef struct ArcqmlRows {
     void *data;       /* device pointer, aligned to the element's size */
