@@ -1075,10 +1075,10 @@ void check_rows(const ArcqmlRows &r, const char *what) {
     if (r.width == 0) refuse(what, "has rows without elements");
     if (r.width >> 30) refuse(what, "has rows that are too long (below 2^30 elements)");
     if (r.stride >> 40) refuse(what, "has rows too far apart");
-    if (!r.rows) return;
-    if (!r.data) refuse(what, "is null");
+    // (accesses are as wide as all addresses allow, so that of no rows has to start on an element too)
     if (reinterpret_cast<uintptr_t>(r.data) % bytes_of_element(r.dtype))
         refuse(what, "is not aligned to its elements");
+    if (r.rows && !r.data) refuse(what, "is null");
 }
 
 void check_options(const ArcqmlEmbeddingOptions &o) {
