@@ -1169,7 +1169,7 @@ def _embedding_rows(torch, t, outer: int, name: str, device: int):
 
 
 def _embedding_call(torch, indices, scale, normalize, padding, device: int):
-    """(options, indices next to each other)"""
+    """The options of a call (ArcqmlEmbeddingOptions), after a look at its indices."""
     kind = indices.dtype if isinstance(indices, torch.Tensor) and indices.is_cuda else None
     if kind != torch.int64 and kind != torch.int32:
         raise TypeError("indices must be an int64 or int32 CUDA tensor")
@@ -1178,8 +1178,8 @@ def _embedding_call(torch, indices, scale, normalize, padding, device: int):
                            f"cuda:{device}")
     if padding is None:
         padding = -1
-    elif padding < 0:
-        raise ValueError("the padding index must not be negative")
+    elif not 0 <= padding < 1 << 63:
+        raise ValueError("the padding index must not be negative, and fit into 8 bytes")
     return _EMBEDDING_OPTIONS(scale, padding, bool(normalize), 8 if kind == torch.int64 else 4)
 
 

@@ -20,3 +20,21 @@ def test_rows_that_are_none_start_on_an_element_too(call, dtype, data):
     wide = dict(width=40_000, dtype=dtype)
     call.message(call.gradient(gradient=call.rows(data=data, rows=0, **wide), options=call.options(normalize=1),
                                table=call.rows(**wide), output=call.rows(**wide)), "gradient is not aligned")
+
+
+def test_padding_that_is_no_index(runtime):
+    """The binding refuses what 8 bytes cannot hold as it refuses a negative one."""
+    from types import SimpleNamespace
+
+    class Indices:
+        is_cuda, dtype = True, "int64"
+
+        def get_device(self):
+            return 0
+
+    fake = SimpleNamespace(Tensor=Indices, int64="int64", int32="int32")
+    for padding in (-1, 2 ** 63, 2 ** 70):
+        with pytest.raises(ValueError, match="padding index"):
+            runtime._embedding_call(fake, Indices(), 1.0, False, padding, 0)
+    for padding in (None, 0, 2 ** 63 - 1):
+        assert len(runtime._embedding_call(fake, Indices(), 1.0, False, padding, 0)) == 24
