@@ -1071,7 +1071,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_direct(const __grid_constant__ 
 void check_rows(const ArcqmlRows &r, const char *what) {
     if (r.dtype > ARCQML_F16) refuse(what, "has an unknown type");
     if (r.reserved != 0) refuse(what, "has a nonzero reserved field");
-    if (r.rows >> 31) refuse(what, "has too many rows (2^31 at most)");
+    if (r.rows >> 31) refuse(what, "has too many rows (below 2^31)");
     if (r.width == 0) refuse(what, "has rows without elements");
     if (r.width >> 30) refuse(what, "has rows that are too long (below 2^30 elements)");
     if (r.stride >> 40) refuse(what, "has rows too far apart");

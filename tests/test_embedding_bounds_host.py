@@ -38,3 +38,10 @@ def test_padding_that_is_no_index(runtime):
             runtime._embedding_call(fake, Indices(), 1.0, False, padding, 0)
     for padding in (None, 0, 2 ** 63 - 1):
         assert len(runtime._embedding_call(fake, Indices(), 1.0, False, padding, 0)) == 24
+
+
+def test_messages_name_the_limits(call):
+    """2^31 rows are refused, one less is not."""
+    call.message(call.lookup(table=call.rows(rows=1 << 31)), "below 2^31")
+    # (the next check is reached)
+    call.message(call.lookup(table=call.rows(rows=(1 << 31) - 1), output=call.rows(rows=4)), "output")
