@@ -1057,7 +1057,7 @@ class DeviceMuonState:
         if x._shapes != like._shapes or len(x._present) != len(x):
             raise ValueError("the momentum must have the parameters' shapes")
         x._as_matrices("the momentum")
-        if any(t.dtype != like.tensors[0].new_empty(0).float().dtype for t in x.tensors):
+        if any(_tensor_kinds()[t.dtype][0] != 1 for t in x.tensors):  # (matrices of one component)
             raise TypeError("the momentum must be float32")
         return x
 
