@@ -42,7 +42,6 @@
 #include <string>
 #include <tuple>
 #include <type_traits>
-#include <vector>
 
 #include "elements.cuh"
 #include "launch.h"
@@ -1146,22 +1145,28 @@ uint64_t operand_bytes(const ArcqmlMatrix &a, bool split) {
 // The scratch of a launch's matrices: what one needs, and more of them while that stays below 2 GB.
 constexpr uint64_t kGroupBytes = uint64_t(2) << 30;
 
+// The places of a launch's matrices (of a fixed size: the workspace query allocates nothing, so it cannot throw).
+struct Members {
+    size_t at[kMatrices];
+    uint32_t count = 0;
+};
+
 template <class F>
 void for_groups(const ArcqmlMatrix *list, const ArcqmlMatrix *kinds, size_t count, uint64_t most, F &&f) {
-    std::vector<size_t> members;
+    Members members;
     for (int kind = 0; kind < 4; ++kind) {
         const bool split = kind & 1, small = kind & 2;
         uint64_t bytes = 0;
         const auto flush = [&] {
-            if (!members.empty()) f(members, bytes, split, small);
-            members.clear();
+            if (members.count) f(members, bytes, split, small);
+            members.count = 0;
             bytes = 0;
         };
         for (size_t i = 0; i < count; ++i) {
             if (!present(list[i]) || is_split(kinds[i].dtype) != split || is_small(list[i], split) != small) continue;
             const uint64_t need = small ? 0 : operand_bytes(list[i], split);
-            if (members.size() == kMatrices || (bytes && bytes + need > most)) flush();
-            members.push_back(i);
+            if (members.count == kMatrices || (bytes && bytes + need > most)) flush();
+            members.at[members.count++] = i;
             bytes += need;
         }
         flush();
@@ -1302,9 +1307,9 @@ template <class F>
 void run(const ArcqmlMatrix *list, const ArcqmlMatrix *kinds, size_t count, int steps, double eps, double *ws, size_t ws_len,
          cudaStream_t s, F &&fill) {
     const uint64_t have = ws_len * sizeof(double), head = kOperandsAt;
-    for_groups(list, kinds, count, have > head ? have - head : 0, [&](const std::vector<size_t> &members, uint64_t, bool split, bool small) {
+    for_groups(list, kinds, count, have > head ? have - head : 0, [&](const Members &members, uint64_t, bool split, bool small) {
         static thread_local Group g;
-        g.count = uint32_t(members.size());
+        g.count = members.count;
         g.scratch = reinterpret_cast<char *>(ws);
         g.fault = reinterpret_cast<uint32_t *>(ws);
         g.shift = reinterpret_cast<int *>(g.scratch + kShiftsAt);
@@ -1313,13 +1318,13 @@ void run(const ArcqmlMatrix *list, const ArcqmlMatrix *kinds, size_t count, int 
         g.partial = reinterpret_cast<float *>(g.scratch + kPartialAt);
         g.eps = eps;
         for (uint32_t i = 0; i < g.count; ++i) {
-            const ArcqmlMatrix &a = list[members[i]];
+            const ArcqmlMatrix &a = list[members.at[i]];
             Matrix &m = g.matrix[i];
             m = Matrix{};
             m.flip = a.rows > a.columns;
             m.m = uint32_t(std::min(a.rows, a.columns));
             m.n = uint32_t(std::max(a.rows, a.columns));
-            fill(m, members[i]);
+            fill(m, members.at[i]);
         }
         if (small && split) run_small<true>(g, steps, s);
         else if (small) run_small<false>(g, steps, s);
@@ -1339,7 +1344,7 @@ size_t orthogonalize_workspace(const ArcqmlMatrix *list, size_t count) {
     if (!list) return 0;
     uint64_t most = 0;
     for_groups(list, list, count, kGroupBytes,
-               [&](const std::vector<size_t> &, uint64_t bytes, bool, bool) { most = std::max(most, bytes); });
+               [&](const Members &, uint64_t bytes, bool, bool) { most = std::max(most, bytes); });
     return most ? size_t((kOperandsAt + most) / sizeof(double)) : 0;
 }
 
