@@ -46,6 +46,7 @@
 #include "elements.cuh"
 #include "launch.h"
 #include "muon.h"
+#include "muon_plan.h"
 #include "profile.h"
 #include "tensor_core.cuh"
 
@@ -56,7 +57,6 @@ constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
 // Scales of the stored values: the largest powers of two that keep them in f16.
 constexpr float kScaleX = 32768.0f; // of X and A; P has half of it
 constexpr int kThreads = 256;
-constexpr uint32_t kMatrices = 64;      // of a launch
 constexpr uint32_t kSumBlocks = 148 * 8; // partial sums of a matrix, at most
 constexpr uint32_t kRows = 128, kDepth = 64;         // of a block
 constexpr uint32_t kBlock = kRows * kDepth * 2;      // bytes
@@ -395,71 +395,6 @@ template <int PHASE, uint32_t SIZE> __device__ __forceinline__ Tile tile_of(cons
     return r;
 }
 
-// Who does which tile. Units (blocks, or pairs of them) take the tiles of each depth, deepest first, in whole
-// rounds: neighbouring tiles at a time, which share their operands in L2. The steps that are left of all depths
-// are cut into equal runs, one for each unit. Cuts move to the next tile's edge, or (where it is worth what
-// it costs, see product()) go through a tile, which the unit that finishes last then sums up in the order of
-// its depth.
-struct Plan {
-    uint32_t classes; // of depth
-    uint32_t tile[kMatrices + 1], rounds[kMatrices], depth[kMatrices];
-    uint32_t left[kMatrices + 1]; // steps left before the class; a tile counts for kLeast of them at least
-    uint32_t runs;                // units that share the steps left
-    uint32_t snap;                // a cut this near to a tile's edge moves there
-};
-
-constexpr uint32_t kLeast = 16; // taking a tile's sums out takes as long
-__host__ __device__ inline uint32_t weight(uint32_t depth) { return depth > kLeast ? depth : kLeast; }
-
-// The class that step `at` of those left belongs to.
-__host__ __device__ inline uint32_t class_of(const Plan &p, uint32_t at) {
-    uint32_t c = 0;
-    while (p.left[c + 1] <= at) ++c;
-    return c;
-}
-// Where the unit's run of the steps left begins.
-__host__ __device__ inline uint32_t cut(const Plan &p, uint32_t unit) {
-    const uint32_t all = p.left[p.classes];
-    if (unit >= p.runs) return all;
-    const uint32_t at = uint32_t(uint64_t(unit) * all / p.runs);
-    if (at == 0) return 0;
-    const uint32_t c = class_of(p, at), w = weight(p.depth[c]), past = (at - p.left[c]) % w, behind = w - past;
-    return past < p.snap && past < behind          ? at - past
-           : past < p.snap || past + p.snap > p.depth[c] || past + p.snap < past ? at + behind
-                                                                                 : at;
-}
-struct Part {
-    uint32_t tile, begin, end, depth; // steps of the tile's depth
-    uint32_t start;                   // the tile's first step among those left
-    __device__ __forceinline__ bool whole() const { return begin == 0 && end == depth; }
-};
-struct Walk {
-    const Plan &p;
-    uint32_t unit, units, c = 0, round = 0, at, end;
-    __device__ __forceinline__ Walk(const Plan &plan, uint32_t u, uint32_t n) : p(plan), unit(u), units(n) {
-        at = cut(p, unit);
-        end = cut(p, unit + 1);
-    }
-    __device__ __forceinline__ bool next(Part &r) {
-        for (; c < p.classes; ++c, round = 0)
-            if (round < p.rounds[c]) {
-                r.tile = p.tile[c] + round++ * units + unit;
-                r.begin = 0;
-                r.end = r.depth = p.depth[c];
-                return true;
-            }
-        if (at >= end) return false;
-        const uint32_t k = class_of(p, at), w = weight(p.depth[k]), n = (at - p.left[k]) / w;
-        r.depth = p.depth[k];
-        r.start = p.left[k] + n * w;
-        r.tile = p.tile[k] + p.rounds[k] * units + n;
-        r.begin = at - r.start;
-        r.end = min(r.depth, end - r.start);
-        at = r.start + (r.end == r.depth ? w : r.end);
-        return true;
-    }
-};
-
 // Up to N elements, `pitch` apart: the result as it is, or the step with it. All are loaded before the first
 // is used.
 template <class T, int N>
@@ -602,7 +537,7 @@ __device__ __forceinline__ void take_sums(const Group &g, const Matrix &a, float
 // held by what shared memory takes in (0.32 us).
 template <int PHASE, bool SPLIT, int CG>
 __global__ void __launch_bounds__(kProductThreads, 1)
-    k_product(const __grid_constant__ Group g, const __grid_constant__ Plan plan, uint32_t step, uint32_t last) {
+    k_product(const __grid_constant__ Group g, const __grid_constant__ TilePlan plan, uint32_t step, uint32_t last) {
     constexpr uint32_t SIZE = kRows * CG, S = kStages<SPLIT>, STAGE = kStageBytes * (SPLIT ? 2 : 1);
     extern __shared__ char raw[];
     char *shared = raw + (1024 - (tc::shared_address(raw) & 1023)) % 1024;
@@ -775,13 +710,8 @@ __global__ void __launch_bounds__(kProductThreads, 1)
             };
             const bool whole = part.whole();
             uint32_t u0 = 0, parts = 1; // the unit with the tile's first step, and how many have parts of it
-            if (!whole) {
-                u0 = uint32_t(uint64_t(part.start) * plan.runs / plan.left[plan.classes]);
-                while (cut(plan, u0) > part.start) --u0;
-                while (cut(plan, u0 + 1) <= part.start) ++u0;
-                while (cut(plan, u0 + parts) < part.start + part.depth) ++parts;
-            }
-            float4 *mine = whole ? nullptr : slice(unit, part.start < from ? 0 : 1);
+            if (!whole) sharers(plan, part, u0, parts);
+            float4 *mine = whole ? nullptr : slice(unit, slot_of(part, from));
             if constexpr (SPLIT) {
                 float sum[COLUMNS];
 #pragma unroll
@@ -1192,7 +1122,7 @@ template <int PHASE> uint32_t depth_of(const Matrix &a) { return ((PHASE == GRAM
 
 // Who does which tile of 128 CG x 128 CG, and how many steps of 64 of the depth the longest unit has. g's
 // matrices are put in order.
-template <int PHASE> uint32_t make_plan(Group &g, Plan &p, uint32_t cg, bool split) {
+template <int PHASE> uint32_t make_plan(Group &g, TilePlan &p, uint32_t cg, bool split) {
     std::stable_sort(g.order, g.order + g.count, [&](uint8_t x, uint8_t y) {
         return depth_of<PHASE>(g.matrix[x]) > depth_of<PHASE>(g.matrix[y]);
     });
@@ -1215,26 +1145,10 @@ template <int PHASE> uint32_t make_plan(Group &g, Plan &p, uint32_t cg, bool spl
         p.left[c + 1] = p.left[c] + has % units * weight(depth);
         whole += p.rounds[c] * weight(depth);
     }
-    // whole tiles, or runs of equal length, of 16 steps and a sixth of a tile at least: writing parts and putting
-    // them together takes about 18 us, 40 steps of 11-bit operands and 20 of 22-bit ones
-    const uint32_t all = p.left[p.classes];
-    uint32_t longest[2];
-    const auto cut_up = [&](bool parts) {
-        p.snap = parts ? 8 : 0xffffffffu;
-        p.runs = parts ? std::max(1u, std::min(units, all / std::max(16u, (p.depth[0] + 5) / 6))) : units;
-    };
-    for (int parts = 0; parts < 2; ++parts) {
-        cut_up(parts != 0);
-        uint32_t run = 0;
-        for (uint32_t u = 0; u < p.runs; ++u) run = std::max(run, cut(p, u + 1) - cut(p, u));
-        longest[parts] = run + (parts ? (split ? 20 : 40) : 0);
-    }
-    const bool parts = longest[1] < longest[0];
-    cut_up(parts);
-    return whole + longest[parts];
+    return whole + share_out(p, units, split);
 }
 
-template <int PHASE, bool SPLIT, int CG> void product(const Group &g, const Plan &p, uint32_t step, bool last, cudaStream_t s) {
+template <int PHASE, bool SPLIT, int CG> void product(const Group &g, const TilePlan &p, uint32_t step, bool last, cudaStream_t s) {
     allow_shared<k_product<PHASE, SPLIT, CG>>(kProductShared<SPLIT>);
     start(k_product<PHASE, SPLIT, CG>, kSMs, kProductThreads, CG, kProductShared<SPLIT>, true, 0.0, s, g, p, step, uint32_t(last));
 }
@@ -1244,7 +1158,7 @@ template <int PHASE, bool SPLIT> void phase(Group &g, uint32_t step, bool last, 
     // and 0.32 us, 22-bit ones 0.85 and 0.62): pairs for many tiles (4096 x 4096: 107 and 179 us for the last
     // phase), single blocks where whole tiles of pairs are too few (the second phase of 2048 x 2048 has 36 for
     // 74 pairs: 25.6 and 20.5 us).
-    Plan pairs, singles;
+    TilePlan pairs, singles;
     const uint32_t single = make_plan<PHASE>(g, singles, 1, SPLIT), pair = make_plan<PHASE>(g, pairs, 2, SPLIT);
     if (7 * pair <= 5 * single) return product<PHASE, SPLIT, 2>(g, pairs, step, last, s);
     make_plan<PHASE>(g, singles, 1, SPLIT);
