@@ -92,12 +92,17 @@ template <class W> __device__ __forceinline__ bool out_of_range(double squares) 
 __device__ __forceinline__ int power_of(double largest) {
     return largest > 0.0 && largest < INFINITY ? ilogb(largest) : 0;
 }
+// x 2^-power for powers of finite numbers, by two factors: one would leave the range.
+__device__ __forceinline__ double lowered(double x, int power) {
+    const int half = power / 2, rest = power - half;
+    return x * __hiloint2double((1023 - half) << 20, 0) * __hiloint2double((1023 - rest) << 20, 0);
+}
 // Numbers of a vector 2^-power times as large.
 template <class T, int N> __device__ __forceinline__ void rescale(Packed<T, N> &v, int power) {
     if constexpr (sizeof(T) == 8) {
         double x[N];
 #pragma unroll
-        for (int e = 0; e < N; ++e) x[e] = scalbn(v.wide(e), -power);
+        for (int e = 0; e < N; ++e) x[e] = lowered(v.wide(e), power);
         v.pack(x);
     }
 }
@@ -140,8 +145,11 @@ __global__ void __launch_bounds__(kThreads) k_lookup(const __grid_constant__ Loo
                     if (squares[p] != 0.0) power = max(power, squares[p] < 0.0 ? int(powers[p]) : 0);
                 sum = 0.0;
 #pragma unroll 1
-                for (uint32_t p = 0; p < a.pieces; ++p)
-                    sum += scalbn(fabs(squares[p]), 2 * ((squares[p] < 0.0 ? int(powers[p]) : 0) - power));
+                for (uint32_t p = 0; p < a.pieces; ++p) {
+                    const int below = power - (squares[p] < 0.0 ? int(powers[p]) : 0);
+                    // (2^-1200 times as large, a piece is nothing beside the largest)
+                    if (below < 600) sum += lowered(fabs(squares[p]), 2 * below);
+                }
 #pragma unroll
                 for (uint32_t j = 0; j < kTileVectors; ++j) rescale(v[j], power);
             }
@@ -296,7 +304,7 @@ __global__ void __launch_bounds__(kThreads) k_row_squares(const __grid_constant_
         if (power) {
             sum = 0.0;
             over_row([&](double x) {
-                x = scalbn(x, -power);
+                x = lowered(x, power);
                 sum = fma(x, x, sum);
             });
             sum = -sum_over<true>(sum, kThreads);
@@ -865,7 +873,7 @@ __global__ void __launch_bounds__(kThreads) k_project(const __grid_constant__ Pr
         tt = tg = 0.0;
 #pragma unroll 1
         for (uint32_t k = first; k < end; k += kThreads) {
-            const double t = scalbn(double(to_wide(x[k])), -power);
+            const double t = lowered(to_wide(x[k]), power);
             tt = fma(t, t, tt);
             tg = fma(t, double(sums[k]), tg);
         }
@@ -874,7 +882,7 @@ __global__ void __launch_bounds__(kThreads) k_project(const __grid_constant__ Pr
 #pragma unroll 1
         for (uint32_t k = first; k < end; k += kThreads)
             reinterpret_cast<T *>(out)[k] = to_element<T>(
-                W(scalbn((double(sums[k]) - scalbn(double(to_wide(x[k])), -power) * along) * inverse, -power)));
+                W(lowered((double(sums[k]) - lowered(to_wide(x[k]), power) * along) * inverse, power)));
         return;
     }
     const double inverse = tt == 0.0 ? 0.0 : 1.0 / sqrt(tt), along = tt == 0.0 ? 0.0 : tg / tt;
@@ -1030,7 +1038,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_direct(const __grid_constant__ 
 #pragma unroll
                     for (int e = 0; e < N; ++e) {
                         const double x = unit[j].wide(e);
-                        sum[j][e] = W(scalbn(double(sum[j][e]), -power)); // what is over the norm goes on so
+                        sum[j][e] = W(lowered(sum[j][e], power)); // what is over the norm goes on so
                         tt = fma(x, x, tt);
                         ts = fma(x, double(sum[j][e]), ts);
                     }
