@@ -6,8 +6,8 @@
 //             (G_v - u <u, G_v>) / |t_v| with u = t_v / |t_v|: every place of a row has the same u, so the
 //             sum is formed first and taken through the norm once
 //
-// Both move each number once and do next to nothing with it: HBM bounds them at real sizes, launches at
-// small ones. The gradient's places are sorted by their row first (a stable radix sort, so that a row's
+// Both move each number once and do next to nothing with it: the latency of index, row and store bounds them
+// at real sizes (at 60 to 70 % of the copy rate), launches at small ones. The gradient's places are sorted by their row first (a stable radix sort, so that a row's
 // places stay in order and equal inputs give equal bits without atomics on values); chunks of the sorted
 // places are then summed side by side, whatever rows they belong to, so a row that most places point to
 // costs no more than others; rows that cross chunks are put together from the chunks' partial sums.
@@ -108,7 +108,8 @@ template <class T, int N> __device__ __forceinline__ void rescale(Packed<T, N> &
 }
 
 // Rows in tiles of 4 vectors a thread, a tile taken by `lanes` threads: 2 KB a warp, four loads in flight for
-// each thread. Bound by HBM for rows of 512 bytes and more (34 us for 65,536 rows of 2 KB, 243 MB).
+// each thread. 34 us for 65,536 rows of 2 KB (243 MB, 112 of them from and to DRAM, the rest L2's) at half of what
+// memory and SMs take: a warp lives for one index -> row -> store, and waits for most of that.
 template <uint32_t DT, int N>
 __global__ void __launch_bounds__(kThreads) k_lookup(const __grid_constant__ Lookup a) {
     using T = Element<DT>;
@@ -636,8 +637,10 @@ __device__ __forceinline__ void write_sum(const Sums &a, uint32_t row, uint32_t 
 
 // One vector of a row for each thread, over the places of one chunk, eight of them in flight: what bounds it is
 // the latency of rows at random (66 us for 131,071 rows of 2 KB, 4.1 TB/s; vectors through slots of shared
-// memory by cp.async, 16 in flight, took 76 us; whole rows of 2 KB a warp 126 us, for want of registers). A row that lies inside the chunk is
-// done; the part of one that began earlier goes to partial 2c, of one that goes on to 2c + 1.
+// memory by cp.async, 16 in flight, took 76 us; whole rows of 2 KB a warp 126 us, for want of registers). Three
+// blocks an SM leave a thread 80 registers, and up to 80 bytes of what it holds are spilled (60 bytes for vectors
+// of 8 bf16 numbers). A row that lies inside the chunk is done; the part of one that began earlier goes to
+// partial 2c, of one that goes on to 2c + 1.
 template <uint32_t DT, uint32_t OT, int N>
 __global__ void __launch_bounds__(kThreads, 3) k_sum_chunks(const __grid_constant__ Sums a) {
     using T = Element<DT>;

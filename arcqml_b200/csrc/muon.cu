@@ -26,13 +26,15 @@
 //
 //   k_update_squares, k_spread   the momentum, the update's norm, X in blocks (HBM: 6.7 and 5.0 TB/s)
 //   k_product                    one of the three products of a step, for a whole list
-//   k_small                      small matrices from the update to the result
+//   k_small                      small matrices, and rows and columns, from the update to the result
 //
 // Measured on a B200 (cuBLAS bf16 1637 TFLOP/s in bursts, 1370 sustained): products of 4096 x 4096 and 8192 x 2048
-// bf16 matrices 1338 to 1420 TFLOP/s as issued; the three products of a 4096 x 4096 matrix 58 + 62 + 107 us in bf16
-// and 164 + 166 + 290 us in f32; a step over 8 bf16 matrices of 16M elements 7.85 ms, over 24
-// f32 ones of 1 to 4M 3.35 ms, over 5 of up to 80 x 64 33 us. Large sizes are bound by the tensor cores under the
-// power limit, middle ones by what surrounds a phase's products (some 8 us), small ones by 15 rounds' latency.
+// bf16 matrices 1338 to 1420 TFLOP/s as issued, launches timed one by one; the three products of a 4096 x 4096 matrix
+// 58 + 62 + 107 us in bf16 and 164 + 166 + 290 us in f32; a step over 8 bf16 matrices of 16M elements 7.9 ms, over 24
+// f32 ones of 1 to 4M 3.37 ms, over 5 of up to 80 x 64 33 us. In that first step the products run at 1.07 PFLOP/s as
+// issued, at 1365 MHz under the power limit (cuBLAS: 1.40 at 1335 MHz): a phase waits for its longest unit, and what
+// else it waits for is not known. Middle sizes lose 20 us and more of a phase so (4 matrices of up to 4M in 0.70 ms
+// at 1807 MHz), small ones are bound by 15 rounds' latency.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -174,7 +176,7 @@ __device__ __forceinline__ void new_update8(float (&u)[8], const Matrix &a, uint
     for (int e = 0; e < 8; ++e) u[e] = a.nesterov ? a.beta * m[e] + a.keep * u[e] : m[e];
 }
 
-// |X| 2^shift lies in [1/2, 1]; a norm of zero, infinity or NaN has no shift.
+// |X| 2^shift lies in (1/4, 1]: exponents are compared, not their numbers; a norm of zero, infinity or NaN has no shift.
 __device__ __forceinline__ int shift_of(double norm, double whole) {
     return norm > 0.0 && norm < whole && whole < INFINITY ? max(0, ilogb(whole) - ilogb(norm) - 1) : 0;
 }
@@ -812,7 +814,7 @@ __global__ void __launch_bounds__(kThreads) k_check_fault(const __grid_constant_
 // ------------------------------------------------------------------ small matrices
 
 // A matrix of at most 128 rows of X whose operands fit into a block's shared memory is orthogonalised by
-// that block from its update to its result: one launch for a list, 15 rounds of a few hundred cycles each.
+// that block from its update to its result: one launch for a list, 15 rounds of some 2900 cycles each.
 constexpr uint32_t kSmallThreads = 256;
 static_assert(kSmallThreads == 2 * kRows, "a thread for each diagonal entry of A and P");
 template <bool SPLIT> constexpr uint32_t kSmallBlocks = SPLIT ? 4 : 8; // of X: 256 or 512 columns

@@ -278,7 +278,8 @@ int32_t arcqml_rt_v2_adam_step(const ArcqmlTensor *parameters, const ArcqmlTenso
  * complex table's row is its components. indices: device, `count` integers of index_bytes (4 or 8) each.
  * With `normalize` a row is divided by its 2-norm, which makes states of amplitudes, whatever the size of its
  * finite numbers; a row of zeros stays zero. An index equal to `padding` (when it is not negative) gives a row of zeros. An index outside
- * [0, rows) gives a row of NaN, since refusing it would take a wait for the device. */
+ * [0, rows) gives a row of NaN, since refusing it would take a wait for the device. Counts of rows and indices
+ * are below 2^31, widths below 2^30, strides below 2^40. */
 typedef struct ArcqmlRows {
     void *data;       /* device pointer, aligned to the element's size */
     uint64_t rows;
@@ -312,8 +313,8 @@ int32_t arcqml_rt_v2_embedding_lookup(const ArcqmlRows *table, const void *indic
  * indices[i] = v, and with `normalize` that sum s through the norm of t = table[v]:
  * (s - u <u, s>) / |t|, u = t / |t| (0 for a row of zeros). Every row of the output is written, with zeros
  * where no index points; indices equal to `padding` or outside [0, rows) count nowhere. The places of a row
- * are added in their order, in groups that the count of indices fixes, in f64 for f64 and in f32 otherwise
- * and rounded once: equal inputs give equal bits. table: null unless `normalize` is set, then of the
+ * are added in their order, in groups that the shapes, the type and the options fix, in f64 for f64 and in f32
+ * otherwise and rounded once: equal inputs give equal bits. table: null unless `normalize` is set, then of the
  * output's rows, width and dtype. output: of the gradient's dtype. No two of them may overlap in memory but
  * that gradient rows may coincide (stride 0). */
 int32_t arcqml_rt_v2_embedding_gradient(const ArcqmlRows *gradient, const void *indices,
@@ -339,7 +340,10 @@ size_t arcqml_rt_v2_orthogonalize_workspace(const ArcqmlMatrix *matrices, size_t
  * zeros stays zero, with an epsilon of 0 too. Products of
  * f32 and f16 matrices are formed from operands of 22 bits, those of bf16 matrices from operands of 11,
  * sums in f32. outputs have the matrices' shapes and types; they are the matrices
- * themselves, place by place, or overlap none of them, nor one another. A NaN or infinity in a matrix makes that output NaN. */
+ * themselves, place by place, or overlap none of them, nor one another. A NaN or infinity in a matrix makes that
+ * output NaN. A matrix has less than 2^24 rows and columns, 2^36 elements, and 2^17 on its shorter side; a row or
+ * column is formed in f64. A list and its scratch give equal bits whenever they come; in another list, or with more
+ * scratch, the sums of a matrix's products may be split elsewhere along their depth, which moves their rounding. */
 int32_t arcqml_rt_v2_orthogonalize(const ArcqmlMatrix *matrices, const ArcqmlMatrix *outputs,
                                    size_t num_matrices, int32_t steps, double epsilon,
                                    double *workspace, size_t workspace_len, void *stream);
