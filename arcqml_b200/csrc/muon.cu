@@ -8,14 +8,19 @@
 // The products run on the tensor cores (tcgen05, f16 operands, f32 sums in tensor memory). X, A and P are
 // bounded in that iteration (entries of at most 1.203, 1.447 and 2.807), so f16 at a fixed scale holds
 // 11 bits of every entry down to 2^-29 of the largest: more than bf16 at the same rate. Types of 11 bits
-// and more take operands of 22 bits, as the sum of two f16 numbers, and three products (the fourth is below
-// the sums' own rounding). An update far below epsilon makes a small X, which grows by at most 3.4445 a step:
-// it is stored 2^k times as large, k from its norm, and k falls by 2 a step until it is 0.
+// and more, and small matrices, take operands of 22 bits, as the sum of two f16 numbers, and three products (the
+// fourth is below the sums' own rounding). Large bf16 matrices take products of 11 bits, but X keeps 22, for a X: what
+// its rounding leaves where u has no singular values grows up to 485 times in five steps. (With X in 11 bits, bf16
+// matrices of rank 1 to 64 came out 9.7e-2 to 1.7e-2 off, now 1.7e-3 to 2.4e-3, their own rounding 1.65e-3; full ones
+// 1.87e-3, now 1.78e-3. The low parts cost 9 % of 4 matrices' time, 5 % of 8 large ones'.) An update far below
+// epsilon makes a small X: see start_of.
 //
 // The diagonals of A and P, by far their largest entries, stay in f32 beside the operands, which hold zeros
 // there: with A = D + O, A^2 = O^2 + D O + O D + D^2, and the last terms, like diag(P) X, are formed where
-// sums are taken out. With the diagonals rounded to 11 bits, results of bf16 matrices were 1.3e-3 to 5.8e-3
-// off before their own rounding (a 4 x 266 matrix), without them 6e-4 to 9e-4 (a model of the roundings).
+// sums are taken out. With the diagonals rounded to 11 bits too, results of bf16 matrices were 1.3e-3 to 5.8e-3
+// off before their own rounding (a model of the roundings). Where all entries of A are alike, the rounding of
+// 11-bit products has one direction and shows: 1024 equal rows 4.0e-3 off, matrices of one number up to 6.3e-3 (the
+// model).
 //
 // Layout in the scratch: X, A and P in blocks of 128 rows x 64 columns, 16 KB each, row by row with their
 // 16-byte pieces permuted as the tensor cores want them in shared memory. So every copy is one run of 8 or
@@ -30,11 +35,11 @@
 //
 // Measured on a B200 (cuBLAS bf16 1637 TFLOP/s in bursts, 1370 sustained): products of 4096 x 4096 and 8192 x 2048
 // bf16 matrices 1338 to 1420 TFLOP/s as issued, launches timed one by one; the three products of a 4096 x 4096 matrix
-// 58 + 62 + 107 us in bf16 and 164 + 166 + 290 us in f32; a step over 8 bf16 matrices of 16M elements 7.9 ms, over 24
-// f32 ones of 1 to 4M 3.37 ms, over 5 of up to 80 x 64 33 us. In that first step the products run at 1.07 PFLOP/s as
+// 58 + 62 + 107 us in bf16 and 164 + 166 + 290 us in f32; a step over 8 bf16 matrices of 16M elements 8.3 ms, over 24
+// f32 ones of 1 to 4M 3.35 ms, over 5 of up to 80 x 64 33 us. In that first step the products run at some 1.03 PFLOP/s as
 // issued, at 1365 MHz under the power limit (cuBLAS: 1.40 at 1335 MHz): a phase waits for its longest unit, and what
-// else it waits for is not known. Middle sizes lose 20 us and more of a phase so (4 matrices of up to 4M in 0.70 ms
-// at 1807 MHz), small ones are bound by 15 rounds' latency.
+// else it waits for is not known. Middle sizes lose 20 us and more of a phase so (4 matrices of up to 4M in 0.76 ms
+// at some 1800 MHz), small ones are bound by 15 rounds' latency.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -55,7 +60,6 @@
 namespace arcqml {
 namespace {
 
-constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
 // Scales of the stored values: the largest powers of two that keep them in f16.
 constexpr float kScaleX = 32768.0f; // of X and A; P has half of it
 constexpr int kThreads = 256;
@@ -88,7 +92,7 @@ struct Group {
     uint32_t *fault;   // set by a wait that ran out
     uint32_t *arrived; // parts of a tile that are done, for each warp of the units that begin one
     float *partial;
-    int *shift;      // of each matrix: X is stored 2^shift times as large at first
+    double *inverse; // of each matrix: what X is times, stored as it is at first
     double *sums;
     double eps;
 };
@@ -176,18 +180,41 @@ __device__ __forceinline__ void new_update8(float (&u)[8], const Matrix &a, uint
     for (int e = 0; e < 8; ++e) u[e] = a.nesterov ? a.beta * m[e] + a.keep * u[e] : m[e];
 }
 
-// |X| 2^shift lies in (1/4, 1]: exponents are compared, not their numbers; a norm of zero, infinity or NaN has no shift.
-__device__ __forceinline__ int shift_of(double norm, double whole) {
-    return norm > 0.0 && norm < whole && whole < INFINITY ? max(0, ilogb(whole) - ilogb(norm) - 1) : 0;
+// X is stored kScaleX / inverse times as large as it is. At first that is u times a power of two, with a norm of
+// kScaleX / 2 to kScaleX: 16-bit numbers and their low parts are exact, and none of their roundings has one direction
+// (u / |u| of 4 x 1000 bf16 numbers was rounded downwards throughout where |u| is just above a power of two, and 1e-3 off
+// for that). X grows by at most 3.4445 a step, so 1 / inverse falls by 4 until it is 1.
+struct Start {
+    double factor, inverse; // X as stored is u factor
+};
+// Zeros stay zeros without an epsilon too, where X is 0 / 0; infinities become NaN.
+__device__ __forceinline__ Start start_of(double norm, double whole) {
+    if (!(norm > 0.0 && norm < INFINITY)) return {norm * 0.0, 1.0};
+    const double factor = ldexp(double(kScaleX) / 2, -ilogb(norm));
+    return {factor, double(kScaleX) / factor / whole};
 }
-// X as it is stored is u times this. Zeros stay zeros without an epsilon too, where X is 0 / 0.
-__device__ __forceinline__ double factor_of(double whole, int shift) {
-    return whole == 0.0 ? 0.0 : ldexp(double(kScaleX) / whole, shift);
+__device__ __forceinline__ double inverse_at(double first, uint32_t step) {
+    return step == 0 ? first : fmin(1.0, first * double(uint64_t(1) << 2 * step));
 }
-
-// 2^-n; 0 below f32's normal range, where what it scales is nothing beside what it joins. (ldexpf takes some
-// 300 cycles, in every phase.)
-__device__ __forceinline__ float power(int n) { return n > 126 ? 0.0f : __int_as_float((127 - n) << 23); }
+// What a phase's sums, and what they are added to, are times; and the result, as stored, of the last phase. Of P's
+// diagonal d of A and the sum of products s make a + (b d + c (s + d^2)): it is formed in f64, since a is nearly lost
+// in it (a 2 x 2 matrix of f32 was 1.8e-6 off with the f32 operations of the entries beside it).
+struct Scales {
+    float sum, old, result;
+    double b, c;
+    __device__ __forceinline__ float diagonal(float d, float s) const {
+        return float(3.4445 + (b * double(d) + c * (double(s) + double(d) * double(d))));
+    }
+};
+template <int PHASE> __device__ __forceinline__ Scales scales_of(double inverse) {
+    const double square = inverse * inverse, next = fmin(1.0, 4.0 * inverse);
+    const float ratio = float(next < 1.0 ? 0.25 : inverse); // of inverse and next
+    if constexpr (PHASE == 0) return {1.0f / kScaleX, 0.0f, 0.0f, 0.0, 0.0};
+    else if constexpr (PHASE == 1) {
+        const double b = -4.7750 * square, c = 2.0315 * square * square / kScaleX;
+        return {float(0.5 * c), float(0.5 * b), 0.0f, b / kScaleX, c / kScaleX};
+    } else return {2.0f / kScaleX * ratio, ratio, float(next / kScaleX), 0.0, 0.0};
+}
 
 // ------------------------------------------------------------------ the update and its norm
 
@@ -232,6 +259,18 @@ __device__ __forceinline__ uint64_t place_of(uint32_t row, uint32_t column, uint
            ((column % kDepth / 8) ^ (row % 8)) * 16;
 }
 __host__ __device__ inline uint64_t bytes_of(uint32_t down, uint32_t across) { return uint64_t(down) * across * kBlock; }
+
+// How far behind 8 of X's high parts their low ones lie. Where products take them, both buffers have their own, laid
+// out alike; else one set lies behind both buffers (who writes an entry's new low part is who has read the old one), in
+// runs of 512 bytes for 32 rows, as warps take sums out: laid out alike they would cost as much again as the high parts
+// (4 matrices 810 us instead of 755).
+template <bool SPLIT>
+__device__ __forceinline__ uint64_t low_of_x(uint64_t bytes, uint32_t buffer, uint32_t row, uint32_t column) {
+    if constexpr (SPLIT) return bytes;
+    const uint32_t piece = column % kDepth / 8;
+    return bytes * (2 - buffer) + ((row % kRows / 32 * 8 + piece) * 512 + row % 32 * 16) -
+           (row % kRows * 128 + (piece ^ row % 8) * 16);
+}
 
 // 8 values as f16, and with SPLIT what that leaves behind them.
 template <bool SPLIT> __device__ __forceinline__ void store_operand(char *at, uint64_t low, const float (&v)[8]) {
@@ -292,11 +331,10 @@ template <bool SPLIT> __global__ void __launch_bounds__(kThreads) k_spread(const
     double sum = 0.0;
     for (uint32_t b = sums.first[k] + threadIdx.x; b < sums.first[k + 1]; b += kThreads) sum += g.sums[b];
     const double norm = sqrt(block_sum(sum)), whole = norm + g.eps;
-    const int shift = shift_of(norm, whole);
-    if (block == 0 && threadIdx.x == 0) g.shift[k] = shift;
-    const double factor = factor_of(whole, shift);
+    const Start start = start_of(norm, whole);
+    if (block == 0 && threadIdx.x == 0) g.inverse[k] = start.inverse;
     const uint32_t row0 = block / a.x_blocks * kRows, column0 = block % a.x_blocks * kDepth;
-    const uint64_t low = bytes_of(a.down_blocks, a.x_blocks);
+    const uint64_t bytes = bytes_of(a.down_blocks, a.x_blocks);
     char *to = g.scratch + a.x[0];
     if (a.flip) { // X's rows are the matrix's columns
         for (uint32_t t = threadIdx.x; t < kDepth * (kRows / 8); t += kThreads) {
@@ -326,8 +364,8 @@ template <bool SPLIT> __global__ void __launch_bounds__(kThreads) k_spread(const
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) // 0 behind the edges also where the factor is not finite
-            u[e] = row0 + r < a.m && column0 + c + e < a.n ? float(double(u[e]) * factor) : 0.0f;
-        store_operand<SPLIT>(to + place_of(row0 + r, column0 + c, a.x_blocks), low, u);
+            u[e] = row0 + r < a.m && column0 + c + e < a.n ? float(double(u[e]) * start.factor) : 0.0f;
+        store_operand<true>(to + place_of(row0 + r, column0 + c, a.x_blocks), low_of_x<SPLIT>(bytes, 0, r, c), u);
     }
 }
 
@@ -415,14 +453,13 @@ __device__ __forceinline__ void finish(T *at, uint64_t pitch, uint32_t count, co
         if (q < count) at[q * pitch] = to_element<T>(fmaf(a.down, to_wide(p[q]), v[q] * rate));
 }
 
-// N neighbouring values of X's row for each thread of a warp, stored 2^shift kScaleX times as large as they
-// are, go out. Rows of the matrix are turned in shared memory (`square`), so that neighbouring lanes have
+// N neighbouring values of X's row for each thread of a warp, `times` what they are stored as, go out. Rows of the matrix are turned in shared memory (`square`), so that neighbouring lanes have
 // neighbouring elements; X's rows are the columns of a flipped matrix and lie that way already.
 template <int N>
-__device__ __forceinline__ void give_result(const Matrix &a, float (&v)[N], uint32_t row, uint32_t column, int shift,
+__device__ __forceinline__ void give_result(const Matrix &a, float (&v)[N], uint32_t row, uint32_t column, float times,
                                             float *square) {
     constexpr uint32_t ROWS = 32 / N; // of the matrix side by side
-    const float rate = ldexpf(a.momentum ? -a.rate / kScaleX : 1.0f / kScaleX, -shift);
+    const float rate = a.momentum ? -a.rate * times : times;
     const uint32_t lane = threadIdx.x & 31;
     uint32_t along, mine, step; // v[q] belongs to place (along + q step, mine) of rows of `pitch`
     const uint32_t pitch = a.flip ? a.m : a.n, rows = a.flip ? a.n : a.m;
@@ -451,42 +488,42 @@ __device__ __forceinline__ void give_result(const Matrix &a, float (&v)[N], uint
     __syncwarp();
 }
 
-// An entry of P from that of A off its diagonal (x), the sum of products off the diagonal, and the diagonal's
+// An entry of P beside the diagonal from that of A (x), the sum of products beside the diagonals, and the diagonal's
 // entries of its row and column.
-__device__ __forceinline__ float combine(float x, float sum, float row, float column, bool diagonal, float of_old, float of_sum) {
-    return diagonal ? of_old * row + of_sum * (sum + row * row) : of_old * x + of_sum * (sum + (row + column) * x);
+__device__ __forceinline__ float combine(float x, float sum, float row, float column, float of_old, float of_sum) {
+    return of_old * x + of_sum * (sum + (row + column) * x);
 }
 
 // 32 neighbouring sums of a row, for each thread of a warp, become what the phase stores.
 template <int PHASE, bool SPLIT>
 __device__ __forceinline__ void take_sums(const Group &g, const Matrix &a, float (&v)[32], uint32_t row, uint32_t column,
-                                          bool mirrored, int shift, uint32_t current, bool last, float *square) {
+                                          bool mirrored, const Scales &scales, uint32_t current, bool last, float *square) {
     // rows and columns up to the end of their block: behind the matrix they are zero
     const uint32_t across = PHASE == APPLY ? a.x_blocks : a.a_blocks;
     if (row >= a.down_blocks * kRows || column >= across * kDepth) return; // the same for the whole warp
     const uint32_t lane = threadIdx.x & 31;
-    const int next = max(0, shift - 2);
-    // of the sum and of what is added to it
-    const float of_sum = PHASE == GRAM         ? 1.0f / kScaleX
-                         : PHASE == POLYNOMIAL ? 0.5f * kC / kScaleX * power(4 * shift)
-                                               : 2.0f / kScaleX * power(shift - next);
-    const float of_old = PHASE == POLYNOMIAL ? 0.5f * kB * power(2 * shift) : kA * power(shift - next);
-    const uint64_t low = bytes_of(a.down_blocks, across);
+    const float of_sum = scales.sum, of_old = scales.old;
+    const uint64_t bytes = bytes_of(a.down_blocks, across);
+    const auto low = [&](uint32_t buffer, uint32_t at) {
+        return PHASE == APPLY ? low_of_x<SPLIT>(bytes, buffer, row, at) : bytes;
+    };
     const char *old = g.scratch + (PHASE == APPLY ? a.x[current] : a.a);
     char *to = g.scratch + (PHASE == APPLY ? a.x[current ^ 1] : PHASE == GRAM ? a.a : a.p);
     float *of_a = reinterpret_cast<float *>(g.scratch + a.diagonal), *of_p = of_a + a.down_blocks * kRows;
-    const float mine = PHASE == GRAM ? 0.0f : PHASE == POLYNOMIAL ? of_a[row] : of_old + of_p[row] * of_sum;
+    const float mine = PHASE == GRAM ? 0.0f : PHASE == POLYNOMIAL ? of_a[row] : of_old * of_p[row];
     const uint32_t own = row - column; // the diagonal's place among the 32, if below that
+    float on_diagonal = 0.0f;
     // what is read is read before the first store, which it might otherwise have to wait for: a round trip to L2
     // for 32 columns, or 16 where registers are short
+    constexpr bool BOTH = SPLIT || PHASE == APPLY; // X keeps its low parts
     constexpr uint32_t BATCH = SPLIT ? 16 : 32;
 #pragma unroll
     for (uint32_t q0 = 0; q0 < 32; q0 += BATCH) {
-        OperandWords<SPLIT> was[BATCH / 8];
+        OperandWords<BOTH> was[BATCH / 8];
         float4 other[BATCH / 4];
 #pragma unroll
         for (uint32_t q = 0; q < BATCH; q += 8) {
-            if constexpr (PHASE != GRAM) was[q / 8].load(old + place_of(row, column + q0 + q, across), low);
+            if constexpr (PHASE != GRAM) was[q / 8].load(old + place_of(row, column + q0 + q, across), low(current, column + q0 + q));
             if constexpr (PHASE == POLYNOMIAL) {
                 other[q / 4] = *reinterpret_cast<const float4 *>(of_a + column + q0 + q);
                 other[q / 4 + 1] = *reinterpret_cast<const float4 *>(of_a + column + q0 + q + 4);
@@ -499,20 +536,21 @@ __device__ __forceinline__ void take_sums(const Group &g, const Matrix &a, float
             if constexpr (PHASE != GRAM) was[i / 8].unpack(x);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
+                if (PHASE == POLYNOMIAL && q + e == own) on_diagonal = v[q + e];
                 if constexpr (PHASE == GRAM) v[q + e] *= of_sum;
                 else if constexpr (PHASE == APPLY) v[q + e] = mine * x[e] + v[q + e] * of_sum;
                 else
-                    v[q + e] = combine(x[e], v[q + e], mine, reinterpret_cast<const float *>(other)[i + e], q + e == own, of_old,
-                                       of_sum);
+                    v[q + e] = combine(x[e], v[q + e], mine, reinterpret_cast<const float *>(other)[i + e], of_old, of_sum);
                 if (PHASE != APPLY && q + e == own) {
-                    (PHASE == GRAM ? of_a : of_p)[row] = v[q + e];
+                    if constexpr (PHASE == GRAM) of_a[row] = v[q + e];
                     v[q + e] = 0.0f;
                 }
                 x[e] = v[q + e];
             }
-            if (PHASE != APPLY || !last) store_operand<SPLIT>(to + place_of(row, column + q, across), low, x);
+            if (PHASE != APPLY || !last) store_operand<BOTH>(to + place_of(row, column + q, across), low(current ^ 1, column + q), x);
         }
     }
+    if (PHASE == POLYNOMIAL && own < 32) of_p[row] = scales.diagonal(mine, on_diagonal);
     if (PHASE != APPLY && mirrored) { // lanes in pairs, each with two rows of one column
 #pragma unroll
         for (uint32_t q = 0; q < 32; q += 2) {
@@ -524,11 +562,11 @@ __device__ __forceinline__ void take_sums(const Group &g, const Matrix &a, float
             *reinterpret_cast<__half2 *>(at) = h;
             if constexpr (SPLIT) {
                 const float2 y = __half22float2(h);
-                *reinterpret_cast<__half2 *>(at + low) = __floats2half2_rn(one - y.x, two - y.y);
+                *reinterpret_cast<__half2 *>(at + bytes) = __floats2half2_rn(one - y.x, two - y.y);
             }
         }
     }
-    if (PHASE == APPLY && last) give_result(a, v, row, column, next, square);
+    if (PHASE == APPLY && last) give_result(a, v, row, column, scales.result, square);
 }
 
 // One phase for all matrices of a group: D = L R^T in tiles of 128 CG x 128 CG, a pair of blocks a tile with
@@ -575,7 +613,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
     if (more) {
         const Matrix &a = *tile_of<PHASE, SIZE>(g, part.tile).a;
         asm volatile("" ::"l"(a.x[current]), "l"(a.x[current ^ 1]), "l"(a.a), "l"(a.p), "l"(a.diagonal), "l"(a.out), "r"(a.m),
-                     "r"(a.n), "r"(a.down_blocks), "r"(a.x_blocks), "r"(a.a_blocks), "f"(a.rate), "l"(g.scratch), "l"(g.shift),
+                     "r"(a.n), "r"(a.down_blocks), "r"(a.x_blocks), "r"(a.a_blocks), "f"(a.rate), "l"(g.scratch), "l"(g.inverse),
                      "l"(g.fault), "l"(g.partial));
     }
     cudaGridDependencySynchronize();
@@ -705,9 +743,9 @@ __global__ void __launch_bounds__(kProductThreads, 1)
             const Matrix &a = *tile.a;
             const uint32_t row = tile.i * SIZE + rank * kRows + quarter * 32 + lane;
             const uint32_t lanes = quarter * 32 << 16;
-            const int shift = max(0, g.shift[tile.index] - 2 * int(step));
+            const Scales scales = scales_of<PHASE>(inverse_at(g.inverse[tile.index], step));
             const auto take = [&](float (&v)[32], uint32_t c) {
-                take_sums<PHASE, SPLIT>(g, a, v, row, tile.j * SIZE + first + c, tile.i != tile.j, shift, current, last != 0,
+                take_sums<PHASE, SPLIT>(g, a, v, row, tile.j * SIZE + first + c, tile.i != tile.j, scales, current, last != 0,
                                         square);
             };
             const bool whole = part.whole();
@@ -813,14 +851,13 @@ __global__ void __launch_bounds__(kThreads) k_check_fault(const __grid_constant_
 
 // ------------------------------------------------------------------ small matrices
 
-// A matrix of at most 128 rows of X whose operands fit into a block's shared memory is orthogonalised by
+// A matrix of at most 128 rows of X whose 22-bit operands fit into a block's shared memory is orthogonalised by
 // that block from its update to its result: one launch for a list, 15 rounds of some 2900 cycles each.
 constexpr uint32_t kSmallThreads = 256;
 static_assert(kSmallThreads == 2 * kRows, "a thread for each diagonal entry of A and P");
-template <bool SPLIT> constexpr uint32_t kSmallBlocks = SPLIT ? 4 : 8; // of X: 256 or 512 columns
-template <bool SPLIT> constexpr uint32_t kSmallShared =
-    1024 + (kSmallBlocks<SPLIT> + 2) * (SPLIT ? 2 : 1) * kBlock + 256 + kSmallThreads / 32 * 32 * 17 * sizeof(float) +
-    2 * kRows * sizeof(float);
+constexpr uint32_t kSmallBlocks = 4; // of X: 256 columns
+constexpr uint32_t kSmallShared =
+    1024 + (kSmallBlocks + 2) * 2 * kBlock + 256 + kSmallThreads / 32 * 32 * 17 * sizeof(float) + 2 * kRows * sizeof(float);
 
 struct SmallState {
     uint64_t done;
@@ -865,13 +902,12 @@ __device__ __forceinline__ void take_row(const Matrix &a, double eps, int steps)
     }
 }
 
-template <bool SPLIT> __global__ void __launch_bounds__(kSmallThreads, 1)
-    k_small(const __grid_constant__ Group g, int steps) {
-    constexpr uint32_t LOW = kSmallBlocks<SPLIT> * kBlock; // X's low parts behind its high ones
+__global__ void __launch_bounds__(kSmallThreads, 1) k_small(const __grid_constant__ Group g, int steps) {
+    constexpr uint32_t LOW = kSmallBlocks * kBlock; // X's low parts behind its high ones
     extern __shared__ char raw[];
     char *x = raw + (1024 - (tc::shared_address(raw) & 1023)) % 1024;
-    char *p = x + LOW * (SPLIT ? 2 : 1); // A, then P; low parts 2 blocks behind
-    SmallState &st = *reinterpret_cast<SmallState *>(p + 2 * kBlock * (SPLIT ? 2 : 1));
+    char *p = x + LOW * 2; // A, then P; low parts 2 blocks behind
+    SmallState &st = *reinterpret_cast<SmallState *>(p + 2 * kBlock * 2);
     const Matrix &a = g.matrix[blockIdx.x];
     if (a.m == 1) return take_row(a, g.eps, steps);
     const uint32_t thread = threadIdx.x, warp = thread / 32, lane = thread % 32;
@@ -901,11 +937,10 @@ template <bool SPLIT> __global__ void __launch_bounds__(kSmallThreads, 1)
     const uint32_t m16 = (a.m + 15) / 16 * 16, n16 = (a.n + 15) / 16 * 16, used = (a.n + kDepth - 1) / kDepth * kBlock;
     for (uint32_t i = thread * 16; i < used; i += kSmallThreads * 16) {
         *reinterpret_cast<uint4 *>(x + i) = make_uint4(0, 0, 0, 0);
-        if constexpr (SPLIT) *reinterpret_cast<uint4 *>(x + LOW + i) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4 *>(x + LOW + i) = make_uint4(0, 0, 0, 0);
     }
     const double norm = sqrt(block_sum(sum)), whole = norm + g.eps; // (and a barrier)
-    int shift = shift_of(norm, whole);
-    const double factor = factor_of(whole, shift);
+    const Start start = start_of(norm, whole);
     const uint32_t pitch = a.flip ? a.m : a.n;
     for (uint32_t i = thread * 8; i < all; i += kSmallThreads * 8) {
         const uint32_t count = min(8u, all - i);
@@ -916,11 +951,11 @@ template <bool SPLIT> __global__ void __launch_bounds__(kSmallThreads, 1)
         for (int e = 0; e < 8; ++e) {
             if (uint32_t(e) < count) {
                 const uint32_t row = a.flip ? c : r, column = a.flip ? r : c;
-                char *at = x + place_of(row, column, kSmallBlocks<SPLIT>) + column % 8 * 2;
-                const float v = float(double(u[e]) * factor);
+                char *at = x + place_of(row, column, kSmallBlocks) + column % 8 * 2;
+                const float v = float(double(u[e]) * start.factor);
                 const __half h = __float2half_rn(v);
                 *reinterpret_cast<__half *>(at) = h;
-                if constexpr (SPLIT) *reinterpret_cast<__half *>(at + LOW) = __float2half_rn(v - __half2float(h));
+                *reinterpret_cast<__half *>(at + LOW) = __float2half_rn(v - __half2float(h));
             }
             if (++c == pitch) c = 0, ++r;
         }
@@ -942,10 +977,8 @@ template <bool SPLIT> __global__ void __launch_bounds__(kSmallThreads, 1)
             const uint32_t by_depth = k / 4 * kBlock + k % 4 * 32, along = by_width ? k * 2048 : by_depth;
             const uint32_t apart = by_width ? kBlock : 16;
             tc::mma<1>(sums, tc::descriptor(left + by_depth, 16), tc::descriptor(right + along, apart), instr, k != 0);
-            if constexpr (SPLIT) {
-                tc::mma<1>(sums + CROSS, tc::descriptor(left + by_depth, 16), tc::descriptor(right_low + along, apart), instr, k != 0);
-                tc::mma<1>(sums + CROSS, tc::descriptor(left_low + by_depth, 16), tc::descriptor(right + along, apart), instr, true);
-            }
+            tc::mma<1>(sums + CROSS, tc::descriptor(left + by_depth, 16), tc::descriptor(right_low + along, apart), instr, k != 0);
+            tc::mma<1>(sums + CROSS, tc::descriptor(left_low + by_depth, 16), tc::descriptor(right + along, apart), instr, true);
         }
     };
     const auto sums_ready = [&] {
@@ -964,57 +997,48 @@ template <bool SPLIT> __global__ void __launch_bounds__(kSmallThreads, 1)
     int step = 0;
     const auto run_phase = [&](auto which) {
         constexpr int PHASE = which;
-        const int next = max(0, shift - 2);
         const uint32_t columns = PHASE == APPLY ? n16 : m16;
         if (thread == 0) {
             if (PHASE == GRAM) multiply(tmem, x_at, x_at + LOW, x_at, x_at + LOW, n16, m16, false);
             else if (PHASE == POLYNOMIAL) multiply(tmem, p_at, p_at + 2 * kBlock, p_at, p_at + 2 * kBlock, m16, m16, false);
-            else
-                for (uint32_t c = 0; c < n16; c += 256)
-                    multiply(tmem + c, p_at, p_at + 2 * kBlock, x_at + c / kDepth * kBlock, x_at + LOW + c / kDepth * kBlock,
-                             m16, min(256u, n16 - c), true);
+            else multiply(tmem, p_at, p_at + 2 * kBlock, x_at, x_at + LOW, m16, n16, true);
             tc::commit<1>(&st.done);
         }
-        const float of_sum = PHASE == GRAM         ? 1.0f / kScaleX
-                             : PHASE == POLYNOMIAL ? 0.5f * kC / kScaleX * power(4 * shift)
-                                                   : 2.0f / kScaleX * power(shift - next);
-        const float of_old = PHASE == GRAM ? 0.0f : PHASE == POLYNOMIAL ? 0.5f * kB * power(2 * shift) : kA * power(shift - next);
-        const float diagonal = PHASE == GRAM ? 0.0f : PHASE == POLYNOMIAL ? of_a[row] : of_old + of_p[row] * of_sum;
+        const Scales scales = scales_of<PHASE>(inverse_at(start.inverse, step));
+        const float of_sum = scales.sum, of_old = scales.old;
+        const float diagonal = PHASE == GRAM ? 0.0f : PHASE == POLYNOMIAL ? of_a[row] : of_old * of_p[row];
         char *to = PHASE == APPLY ? x : p;
         constexpr uint64_t low = PHASE == APPLY ? LOW : 2 * kBlock;
-        constexpr uint32_t across = PHASE == APPLY ? kSmallBlocks<SPLIT> : 2;
+        constexpr uint32_t across = PHASE == APPLY ? kSmallBlocks : 2;
         if (!sums_ready()) return;
 #pragma unroll 1
         for (uint32_t c = warp / 4 * 16; c < columns; c += 32) {
             float v[16];
-            if constexpr (SPLIT) {
-                tc::tmem_load2(v, mine + c, mine + CROSS + c);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) v[e] = 0.0f;
-                tc::tmem_add(v, mine + c);
-            }
+            tc::tmem_load2(v, mine + c, mine + CROSS + c);
             const uint32_t own = row - c;
+            float on_diagonal = 0.0f;
 #pragma unroll
             for (uint32_t q = 0; q < 16; q += 8) {
                 char *at = to + place_of(row, c + q, across);
                 float y[8];
-                if constexpr (PHASE != GRAM) load_operand<SPLIT>(y, at, low);
+                if constexpr (PHASE != GRAM) load_operand<true>(y, at, low);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     float &z = v[q + e];
+                    if (PHASE == POLYNOMIAL && q + e == own) on_diagonal = z;
                     if constexpr (PHASE == GRAM) z *= of_sum;
                     else if constexpr (PHASE == APPLY) z = diagonal * y[e] + z * of_sum;
-                    else z = combine(y[e], z, diagonal, of_a[c + q + e], q + e == own, of_old, of_sum);
+                    else z = combine(y[e], z, diagonal, of_a[c + q + e], of_old, of_sum);
                     if (PHASE != APPLY && q + e == own) {
-                        (PHASE == GRAM ? of_a : of_p)[row] = z;
+                        if constexpr (PHASE == GRAM) of_a[row] = z;
                         z = 0.0f;
                     }
                     y[e] = z;
                 }
-                store_operand<SPLIT>(at, low, y);
+                store_operand<true>(at, low, y);
             }
-            if (PHASE == APPLY && step + 1 == steps) give_result(a, v, row, c, next, square);
+            if (PHASE == POLYNOMIAL && own < 16) of_p[row] = scales.diagonal(diagonal, on_diagonal);
+            if (PHASE == APPLY && step + 1 == steps) give_result(a, v, row, c, scales.result, square);
         }
         operands_ready();
     };
@@ -1022,7 +1046,6 @@ template <bool SPLIT> __global__ void __launch_bounds__(kSmallThreads, 1)
         run_phase(std::integral_constant<int, GRAM>{});
         if (!broken) run_phase(std::integral_constant<int, POLYNOMIAL>{});
         if (!broken) run_phase(std::integral_constant<int, APPLY>{});
-        shift = max(0, shift - 2);
     }
     if (broken)
         for (uint32_t i = thread; i < all; i += kSmallThreads) store1(a.out, a.out_type, i, __int_as_float(0x7fffffff));
@@ -1089,26 +1112,27 @@ void start(void (*kernel)(P...), uint32_t blocks, uint32_t threads, uint32_t clu
     prof_end(tok, s, bytes);
 }
 
-// Types of 11 bits and more take operands of 22.
-bool is_split(uint32_t type) { return type != ARCQML_BF16; }
+// Types of 11 bits and more take operands of 22 bits; so do bf16 matrices of up to 128 rows (of X), whose few singular
+// values do not even out what 11 bits do to one of them (and whose products are short).
+bool is_split(const ArcqmlMatrix &a, uint32_t type) { return type != ARCQML_BF16 || std::min(a.rows, a.columns) <= kRows; }
 
-// The scratch: the fault, the shifts, the parts that arrived, sums of squares, parts of tiles, then operands.
-constexpr size_t kShiftsAt = 256, kArrivedAt = 512, kSumsAt = kArrivedAt + kSMs * kTakers * 2 * sizeof(uint32_t);
+// The scratch: the fault, the scales, the parts that arrived, sums of squares, parts of tiles, then operands.
+constexpr size_t kScalesAt = 256, kArrivedAt = kScalesAt + kMatrices * sizeof(double), kSumsAt = kArrivedAt + kSMs * kTakers * 2 * sizeof(uint32_t);
 constexpr size_t kPartialAt = (kSumsAt + size_t(kMatrices) * kSumBlocks * sizeof(double) + 1023) / 1024 * 1024;
 // two tiles for each pair of blocks (single blocks: half as much)
 constexpr size_t kOperandsAt = kPartialAt + size_t(kSMs / 2) * 2 * (2 * kRows) * (2 * kRows) * sizeof(float);
 
 // Matrices that one block takes whole; rows and columns of any length.
-bool is_small(const ArcqmlMatrix &a, bool split) {
+bool is_small(const ArcqmlMatrix &a) {
     const uint64_t m = std::min(a.rows, a.columns), n = std::max(a.rows, a.columns);
-    return m == 1 || (m <= kRows && n <= (split ? kSmallBlocks<true> : kSmallBlocks<false>) * kDepth);
+    return m == 1 || (m <= kRows && n <= kSmallBlocks * kDepth);
 }
 
 // Scratch bytes of a matrix's X (twice), A, P and their diagonals.
 uint64_t operand_bytes(const ArcqmlMatrix &a, bool split) {
     const uint64_t m = std::min(a.rows, a.columns), n = std::max(a.rows, a.columns);
     const uint32_t down = uint32_t((m + kRows - 1) / kRows), across = 2 * uint32_t((n + kRows - 1) / kRows);
-    return (2 * bytes_of(down, across) + 2 * bytes_of(down, 2 * down)) * (split ? 2 : 1) + uint64_t(down) * kRows * 8;
+    return bytes_of(down, across) * (split ? 4 : 3) + bytes_of(down, 2 * down) * (split ? 4 : 2) + uint64_t(down) * kRows * 8;
 }
 
 // The scratch of a launch's matrices: what one needs, and more of them while that stays below 2 GB.
@@ -1123,8 +1147,8 @@ struct Members {
 template <class F>
 void for_groups(const ArcqmlMatrix *list, const ArcqmlMatrix *kinds, size_t count, uint64_t most, F &&f) {
     Members members;
-    for (int kind = 0; kind < 4; ++kind) {
-        const bool split = kind & 1, small = kind & 2;
+    for (int kind = 0; kind < 3; ++kind) {
+        const bool split = kind == 1, small = kind == 2;
         uint64_t bytes = 0;
         const auto flush = [&] {
             if (members.count) f(members, bytes, split, small);
@@ -1132,7 +1156,7 @@ void for_groups(const ArcqmlMatrix *list, const ArcqmlMatrix *kinds, size_t coun
             bytes = 0;
         };
         for (size_t i = 0; i < count; ++i) {
-            if (!present(list[i]) || is_split(kinds[i].dtype) != split || is_small(list[i], split) != small) continue;
+            if (!present(list[i]) || is_small(list[i]) != small || (!small && is_split(list[i], kinds[i].dtype) != split)) continue;
             const uint64_t need = small ? 0 : operand_bytes(list[i], split);
             if (members.count == kMatrices || (bytes && bytes + need > most)) flush();
             members.at[members.count++] = i;
@@ -1216,11 +1240,11 @@ template <bool SPLIT> void run_group(Group &g, int steps, cudaStream_t s) {
         a.down_blocks = (a.m + kRows - 1) / kRows;
         a.x_blocks = 2 * ((a.n + kRows - 1) / kRows);
         a.a_blocks = 2 * a.down_blocks;
-        const uint64_t x = bytes_of(a.down_blocks, a.x_blocks) * (SPLIT ? 2 : 1);
+        const uint64_t x = bytes_of(a.down_blocks, a.x_blocks);
         const uint64_t square = bytes_of(a.down_blocks, a.a_blocks) * (SPLIT ? 2 : 1);
         a.x[0] = at;
-        a.x[1] = at + x;
-        a.a = at + 2 * x;
+        a.x[1] = at + (SPLIT ? 2 : 1) * x;
+        a.a = at + (SPLIT ? 4 : 3) * x;
         a.p = a.a + square;
         a.diagonal = a.p + square;
         at = a.diagonal + uint64_t(a.down_blocks) * kRows * 8;
@@ -1238,7 +1262,7 @@ template <bool SPLIT> void run_group(Group &g, int steps, cudaStream_t s) {
     tiles.count = g.count;
     tiles.scratch = g.scratch;
     tiles.fault = g.fault;
-    tiles.shift = g.shift;
+    tiles.inverse = g.inverse;
     tiles.sums = g.sums;
     tiles.eps = g.eps;
     start(k_spread<SPLIT>, spread, kThreads, 1, 0, true, 8.0 * elements, s, tiles, g);
@@ -1250,9 +1274,9 @@ template <bool SPLIT> void run_group(Group &g, int steps, cudaStream_t s) {
     start(k_check_fault, 8, kThreads, 1, 0, true, 0.0, s, g);
 }
 
-template <bool SPLIT> void run_small(Group &g, int steps, cudaStream_t s) {
-    allow_shared<k_small<SPLIT>>(kSmallShared<SPLIT>);
-    start(k_small<SPLIT>, g.count, kSmallThreads, 1, kSmallShared<SPLIT>, false, 0.0, s, g, steps);
+void run_small(Group &g, int steps, cudaStream_t s) {
+    allow_shared<k_small>(kSmallShared);
+    start(k_small, g.count, kSmallThreads, 1, kSmallShared, false, 0.0, s, g, steps);
 }
 
 // fill(matrix, place) sets what the call does to a place of the list.
@@ -1265,7 +1289,7 @@ void run(const ArcqmlMatrix *list, const ArcqmlMatrix *kinds, size_t count, int 
         g.count = members.count;
         g.scratch = reinterpret_cast<char *>(ws);
         g.fault = reinterpret_cast<uint32_t *>(ws);
-        g.shift = reinterpret_cast<int *>(g.scratch + kShiftsAt);
+        g.inverse = reinterpret_cast<double *>(g.scratch + kScalesAt);
         g.arrived = reinterpret_cast<uint32_t *>(g.scratch + kArrivedAt);
         g.sums = reinterpret_cast<double *>(g.scratch + kSumsAt);
         g.partial = reinterpret_cast<float *>(g.scratch + kPartialAt);
@@ -1279,8 +1303,7 @@ void run(const ArcqmlMatrix *list, const ArcqmlMatrix *kinds, size_t count, int 
             m.n = uint32_t(std::max(a.rows, a.columns));
             fill(m, members.at[i]);
         }
-        if (small && split) run_small<true>(g, steps, s);
-        else if (small) run_small<false>(g, steps, s);
+        if (small) run_small(g, steps, s);
         else if (split) run_group<true>(g, steps, s);
         else run_group<false>(g, steps, s);
     });

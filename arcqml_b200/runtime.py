@@ -993,8 +993,9 @@ def orthogonalize_device(matrices, steps: int = 5, eps: float = 1e-7, out=None, 
     """`matrices` (a TensorList or a sequence of row-major float32, bfloat16 or float16 CUDA matrices, or
     None) with their singular values pushed towards 1 (arcqml_rt_v2_orthogonalize): X = u / (|u| + eps),
     then `steps` times X <- a X + (b A + c A^2) X with A = X X^T. The results are new matrices of the same
-    types, or `out` (`matrices` themselves, or others that share no memory with them). Products carry 22 bits of float32 and float16 matrices and 11
-    of bfloat16 ones, summed in float32. A matrix of zeros stays zero."""
+    types, or `out` (`matrices` themselves, or others that share no memory with them). X keeps 22 bits, products
+    carry 22 (11 of bfloat16 matrices of more than 128 rows and columns), summed in float32. A matrix of zeros
+    stays zero."""
     import torch
     x = _tensor_list(matrices)
     device = torch.cuda.current_device()

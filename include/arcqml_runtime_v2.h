@@ -338,8 +338,8 @@ size_t arcqml_rt_v2_orthogonalize_workspace(const ArcqmlMatrix *matrices, size_t
  * polynomial X <- a X + (b A + c A^2) X, A = X X^T (X^T X for more rows than columns),
  * (a, b, c) = (3.4445, -4.7750, 2.0315), from X = matrix / (its Frobenius norm + epsilon); a matrix of
  * zeros stays zero, with an epsilon of 0 too. Products of
- * f32 and f16 matrices are formed from operands of 22 bits, those of bf16 matrices from operands of 11,
- * sums in f32. outputs have the matrices' shapes and types; they are the matrices
+ * f32 and f16 matrices, and of bf16 ones of up to 128 rows or columns, are formed from operands of 22 bits, those of
+ * larger bf16 matrices from operands of 11; sums are f32, and X has 22 bits. outputs have the matrices' shapes and types; they are the matrices
  * themselves, place by place, or overlap none of them, nor one another. A NaN or infinity in a matrix makes that
  * output NaN. A matrix has less than 2^24 rows and columns, 2^36 elements, and 2^17 on its shorter side; a row or
  * column is formed in f64. A list and its scratch give equal bits whenever they come; in another list, or with more
