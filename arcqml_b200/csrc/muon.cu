@@ -34,9 +34,9 @@
 //   k_small                      small matrices, and rows and columns, from the update to the result
 //
 // Measured on a B200 (cuBLAS bf16 1637 TFLOP/s in bursts, 1370 sustained): products of 4096 x 4096 and 8192 x 2048
-// bf16 matrices 1338 to 1420 TFLOP/s as issued, launches timed one by one; the three products of a 4096 x 4096 matrix
-// 58 + 62 + 107 us in bf16 and 164 + 166 + 290 us in f32; a step over 8 bf16 matrices of 16M elements 8.3 ms, over 24
-// f32 ones of 1 to 4M 3.35 ms, over 5 of up to 80 x 64 33 us. In that first step the products run at some 1.03 PFLOP/s as
+// bf16 matrices 1300, 1240 and 1170 TFLOP/s as issued, launches timed one by one (the last phase moves X's low parts
+// beside them; 1370 without); the three products of a 4096 x 4096 f32 matrix 164 + 166 + 290 us; a step over 8 bf16 matrices of 16M elements 8.3 ms, over 24
+// f32 ones of 1 to 4M 3.35 ms, over 5 of up to 80 x 64 33 us. In that first step the products run at some 1.01 PFLOP/s as
 // issued, at 1365 MHz under the power limit (cuBLAS: 1.40 at 1335 MHz): a phase waits for its longest unit, and what
 // else it waits for is not known. Middle sizes lose 20 us and more of a phase so (4 matrices of up to 4M in 0.76 ms
 // at some 1800 MHz), small ones are bound by 15 rounds' latency.
