@@ -35,11 +35,11 @@
 //
 // Measured on a B200 (cuBLAS bf16 1637 TFLOP/s in bursts, 1370 sustained): products of 4096 x 4096 and 8192 x 2048
 // bf16 matrices 1300, 1240 and 1170 TFLOP/s as issued, launches timed one by one (the last phase moves X's low parts
-// beside them; 1370 without); the three products of a 4096 x 4096 f32 matrix 164 + 166 + 290 us; a step over 8 bf16 matrices of 16M elements 8.3 ms, over 24
-// f32 ones of 1 to 4M 3.35 ms, over 5 of up to 80 x 64 33 us. In that first step the products run at some 1.01 PFLOP/s as
-// issued, at 1365 MHz under the power limit (cuBLAS: 1.40 at 1335 MHz): a phase waits for its longest unit, and what
-// else it waits for is not known. Middle sizes lose 20 us and more of a phase so (4 matrices of up to 4M in 0.76 ms
-// at some 1800 MHz), small ones are bound by 15 rounds' latency.
+// beside them; 1370 without); the three products of a 4096 x 4096 f32 matrix 164 + 166 + 290 us; a step over 8 bf16
+// matrices of 16M elements 8.3 ms, over 24 f32 ones of 1 to 4M 3.35 ms, over 5 of up to 80 x 64 33 us. In that first
+// step the products run at some 1.01 PFLOP/s as issued, at 1365 MHz under the power limit (cuBLAS: 1.40 at 1335 MHz): a
+// phase waits for its longest unit, and what else it waits for is not known. Middle sizes lose 20 us and more of a
+// phase so (4 matrices of up to 4M in 0.76 ms at some 1800 MHz), small ones are bound by 15 rounds' latency.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -453,8 +453,9 @@ __device__ __forceinline__ void finish(T *at, uint64_t pitch, uint32_t count, co
         if (q < count) at[q * pitch] = to_element<T>(fmaf(a.down, to_wide(p[q]), v[q] * rate));
 }
 
-// N neighbouring values of X's row for each thread of a warp, `times` what they are stored as, go out. Rows of the matrix are turned in shared memory (`square`), so that neighbouring lanes have
-// neighbouring elements; X's rows are the columns of a flipped matrix and lie that way already.
+// N neighbouring values of X's row for each thread of a warp, `times` what they are stored as, go out. Rows of the
+// matrix are turned in shared memory (`square`), so that neighbouring lanes have neighbouring elements; X's rows are the
+// columns of a flipped matrix and lie that way already.
 template <int N>
 __device__ __forceinline__ void give_result(const Matrix &a, float (&v)[N], uint32_t row, uint32_t column, float times,
                                             float *square) {
